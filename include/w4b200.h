@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define W4B200_VERSION 110 /* 1.1.0 */
+#define W4B200_VERSION 120 /* 1.2.0 */
 #define W4B200_GROUP_SIZE 128
 #define W4B200_MAX_M 16
 
@@ -41,7 +41,8 @@ typedef enum {
   W4_ERR_DEVICE = 5       /* a kernel reported a timed-out wait        */
 } w4_status;
 
-typedef enum { W4_F16 = 0, W4_BF16 = 1 } w4_dtype;
+/* W4_F32 is accepted for rotation tables only. */
+typedef enum { W4_F16 = 0, W4_BF16 = 1, W4_F32 = 2 } w4_dtype;
 
 /* Tile configuration of the fused GEMV. Zero fields mean "choose". */
 typedef struct {
@@ -216,6 +217,25 @@ int w4_gemm(const void* x, int x_dtype, const int32_t* packed, const void* scale
  * order: results do not depend on scheduling. */
 int w4_gemm_ex(const void* x, int x_dtype, const int32_t* packed, const void* scales,
                void* y, int y_dtype, int M, int K, int N, int split_k, void* stream);
+
+/* w4_gemm with an epilogue, in fp32 and rounded once:
+ *   y[m, n] = residual[m, n] + act(sum_k x[m, k] W[k, n] + bias[n]).
+ * With W4_ACT_SWIGLU the columns of W (and of bias) hold gate and up in
+ * alternating blocks of 32 (gate 0..31, up 0..31, gate 32..63, ...), and y and
+ * residual are [M, N/2]: y = residual + silu(gate + bias) * (up + bias).
+ * bias [N] and residual have y's type, are 16-byte aligned and may be NULL;
+ * residual may be y itself. The reference's W4Linear adds a bias in a separate
+ * op (scripts/decode_loop.py:56-57); it has no counterpart of the rest. */
+typedef enum { W4_ACT_NONE = 0, W4_ACT_SILU = 1, W4_ACT_GELU = 2, W4_ACT_SWIGLU = 3 } w4_act;
+#define W4B200_SWIGLU_BLOCK 32
+typedef struct {
+  int act;              /* w4_act; W4_ACT_GELU is x * Phi(x), by erf */
+  const void* bias;     /* [N] */
+  const void* residual; /* [M, N] ([M, N/2] for W4_ACT_SWIGLU), row-major */
+} w4_gemm_ops;
+int w4_gemm_fused(const void* x, int x_dtype, const int32_t* packed, const void* scales,
+                  void* y, int y_dtype, int M, int K, int N, const w4_gemm_ops* ops,
+                  int split_k, void* stream);
 
 /* Calibrated int4 packing (GPTQ), the step the reference lists after its
  * round-to-nearest packer (devto_article.md:71), in the same packed format
@@ -402,8 +422,106 @@ int w4_decode_step_scratch_bytes(const w4_decode_model* model, size_t* bytes);
 int w4_decode_step(const w4_decode_model* model, void* scratch, size_t scratch_bytes,
                    void* stream);
 
+/* ---------------------------------------------------------------------
+ * A decoder layer's attention for batches: ragged rows of several sequences
+ * against a paged KV cache in 8 bits. The reference decodes one sequence over
+ * a dynamic 16-bit cache (scripts/decode_loop.py:106-124); these stand beside
+ * w4_decode_attention, which does that in one launch.
+ *
+ * None of them allocates, synchronises or keeps anything between calls. Page
+ * numbers, lengths and positions are read on the device: one out of range is
+ * never followed; what it belongs to is left out and the device error word is
+ * set to W4B200_ERR_KV_RANGE (w4_device_error). */
+#define W4B200_ERR_KV_RANGE 8
+
+/* Rows of heads: element (row, head, d) at ptr + row * row_stride +
+ * head * head_stride + d, 16-bit elements. ptr is 16-byte aligned and both
+ * strides are multiples of 8. */
+typedef struct {
+  void* ptr;
+  int64_t row_stride, head_stride;
+  int heads;
+} w4_heads;
+
+/* Norm and rotation of heads. cos_table/sin_table [max_pos, head_dim]
+ * (table_dtype W4_F16, W4_BF16 or W4_F32, 16-byte aligned) or both NULL for no
+ * rotation; q_norm/k_norm [head_dim], of the rows' type, or NULL for no norm. */
+typedef struct {
+  const void* cos_table;
+  const void* sin_table;
+  int table_dtype;
+  int max_pos;
+  const void* q_norm;
+  const void* k_norm;
+  float eps;
+} w4_rope;
+
+/* RMS norm of every head and the rotate-half rotation, in one pass:
+ *   x' = x * rsqrt(mean(x^2) + eps) * w  (where there is a weight)
+ *   y[d] = x'[d] cos[d] - x'[d + D/2] sin[d], d < D/2
+ *   y[d] = x'[d] cos[d] + x'[d - D/2] sin[d], d >= D/2
+ * in fp32, rounded once. positions [rows] picks each row's table row (may be
+ * NULL without tables). q_out/k_out may be q/k themselves (the same pointer
+ * and strides) and must not overlap them otherwise. head_dim 64 or 128; q or k
+ * may have no heads. */
+int w4_qk_norm_rope(const w4_heads* q, const w4_heads* k, const w4_heads* q_out,
+                    const w4_heads* k_out, int dtype, int rows, int head_dim,
+                    const w4_rope* rope, const int64_t* positions, void* stream);
+
+/* The cache: e4m3 codes [pages, kv_heads, page_size, head_dim], 16-byte
+ * aligned, and one positive fp32 scale a page and head; a stored value is
+ * code * scale. page_size 16, 32, 64 or 128; head_dim 64 or 128. */
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale; /* [pages, kv_heads] */
+  float* v_scale;
+  int pages, kv_heads, page_size, head_dim;
+} w4_kv8_cache;
+
+/* One step's rows: those of sequence b are row_starts[b] .. row_starts[b + 1]
+ * - 1 (row_starts [seqs + 1], not decreasing) and take the positions behind the
+ * lengths[b] tokens that the sequence held before the step. Token t of
+ * sequence b lives in page page_table[b, t / page_size]. Rows behind the last
+ * sequence are left alone. */
+typedef struct {
+  const int32_t* page_table; /* row b at page_table + b * table_stride */
+  int64_t table_stride;
+  int max_pages;             /* entries of a row */
+  const int32_t* lengths;    /* [seqs] */
+  const int32_t* row_starts; /* [seqs + 1] */
+  int seqs;
+  int rows;                  /* rows of q, k and v, padding included */
+} w4_kv_batch;
+
+/* Writes a step's keys (normed and rotated) and values into the cache, and its
+ * queries (normed and rotated) to q_out; q->heads may be 0. The scale of a
+ * block (one page of one head, K and V apart) becomes the least power of two s
+ * in 2^-32 .. 2^120 with max|x| <= 448 s over the block's new rows; a block
+ * that held rows of the sequence already keeps its scale where that is larger,
+ * and where it is smaller those rows are rounded again in the new one. Codes
+ * round to nearest even; infinities are stored as +-448 s, NaN as NaN, and
+ * neither sets a scale. No page may belong to two sequences that the call
+ * writes. */
+int w4_kv8_append(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_heads* k,
+                  const w4_heads* v, const w4_heads* q, const w4_heads* q_out, int dtype,
+                  const w4_rope* rope, void* stream);
+
+/* Attention of a step's queries over the cache, which holds the step's own
+ * keys and values already: row i of sequence b sees the tokens 0 ..
+ * lengths[b] + i. Query head h reads cache head h / (heads / kv_heads);
+ * heads / kv_heads is 1 .. 16. out = softmax(scale * q K^T) V, the softmax and
+ * all sums in fp32; a row that sees no token (all its pages out of range) is
+ * zero. workspace: w4_kv8_attention_workspace_bytes(head_dim) bytes, 16-byte
+ * aligned, of any content, used by one call at a time. */
+size_t w4_kv8_attention_workspace_bytes(int head_dim);
+int w4_kv8_attention(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_heads* q,
+                     const w4_heads* out, int dtype, float scale, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 /* Reads and clears the device-side error word that kernels set when a
- * bounded wait gives up (0 = no error). Synchronises the device. */
+ * bounded wait gives up, or a page or position is out of range (0 = no
+ * error). Synchronises the device. */
 int w4_device_error(int device, int* code);
 
 #ifdef __cplusplus

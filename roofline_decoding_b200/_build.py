@@ -18,7 +18,8 @@ BUILD_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "libw4b200.so"
 SOURCES = ["w4_api.cu", "w4_pack.cu", "w4_gemv.cu", "w4_gemv_ops.cu", "w4_gemv_fused.cu",
            "w4_decode.cu", "w4_mega.cu",
-           "w4_gemm.cu", "w4_gptq.cu", "w4_tune.cu"]
+           "w4_gemm.cu", "w4_gptq.cu", "w4_tune.cu",
+           "w4_kv8.cu", "w4_kv8_attn.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

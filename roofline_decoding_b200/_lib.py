@@ -12,7 +12,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libw4b200.so")
 HEADER_PATH = Path(__file__).resolve().parent.parent / "include" / "w4b200.h"
 
 W4_OK, W4_ERR_INVALID_ARG, W4_ERR_ALIGNMENT, W4_ERR_UNSUPPORTED, W4_ERR_CUDA, W4_ERR_DEVICE = range(6)
-W4_F16, W4_BF16 = 0, 1
+W4_F16, W4_BF16, W4_F32 = 0, 1, 2  # W4_F32: rotation tables only
 # w4_pack input dtypes (the reference packer accepts any float tensor and
 # works on its fp32 value).
 W4_PACK_F16, W4_PACK_BF16, W4_PACK_F32 = 0, 1, 2
@@ -86,6 +86,42 @@ class DecodeModel(ctypes.Structure):
             "token", "pos", "logits")]
 
 
+W4_ACT_NONE, W4_ACT_SILU, W4_ACT_GELU, W4_ACT_SWIGLU = 0, 1, 2, 3
+SWIGLU_BLOCK = 32
+ERR_KV_RANGE = 8  # device error: a page, length or position out of range
+
+
+class GemmOps(ctypes.Structure):
+    """w4_gemm_ops: the GEMM's epilogue (include/w4b200.h)."""
+    _fields_ = [("act", ctypes.c_int), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p)]
+
+
+class Heads(ctypes.Structure):
+    """w4_heads: rows of heads by pointer and strides in elements."""
+    _fields_ = [("ptr", ctypes.c_void_p), ("row_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int)]
+
+
+class Rope(ctypes.Structure):
+    """w4_rope: rotation tables, norm weights and epsilon."""
+    _fields_ = [("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
+                ("table_dtype", ctypes.c_int), ("max_pos", ctypes.c_int),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
+class Kv8CacheDesc(ctypes.Structure):
+    """w4_kv8_cache: the 8-bit pages and their scales."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, ctypes.c_int) for n in ("pages", "kv_heads", "page_size", "head_dim")]
+
+
+class KvBatch(ctypes.Structure):
+    """w4_kv_batch: a step's rows, sequence by sequence."""
+    _fields_ = [("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("max_pages", ctypes.c_int), ("lengths", ctypes.c_void_p),
+                ("row_starts", ctypes.c_void_p), ("seqs", ctypes.c_int), ("rows", ctypes.c_int)]
+
+
 MAX_PEERS = 8
 IPC_HANDLE_BYTES = 64
 
@@ -141,6 +177,16 @@ SIGNATURES = {
                          _c_int, _c_int, _c_void_p]),
     "w4_gemm_ex": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
                             _c_int, _c_int, _c_int, _c_void_p]),
+    "w4_gemm_fused": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
+                               _c_int, _c_int, ctypes.POINTER(GemmOps), _c_int, _c_void_p]),
+    "w4_qk_norm_rope": (_c_int, [ctypes.POINTER(Heads)] * 4 + [
+        _c_int, _c_int, _c_int, ctypes.POINTER(Rope), _c_void_p, _c_void_p]),
+    "w4_kv8_append": (_c_int, [ctypes.POINTER(Kv8CacheDesc), ctypes.POINTER(KvBatch)] +
+                      [ctypes.POINTER(Heads)] * 4 + [_c_int, ctypes.POINTER(Rope), _c_void_p]),
+    "w4_kv8_attention_workspace_bytes": (_c_size_t, [_c_int]),
+    "w4_kv8_attention": (_c_int, [ctypes.POINTER(Kv8CacheDesc), ctypes.POINTER(KvBatch),
+                                  ctypes.POINTER(Heads), ctypes.POINTER(Heads), _c_int,
+                                  ctypes.c_float, _c_void_p, _c_size_t, _c_void_p]),
     "w4_gptq_block": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p,
                                _c_void_p]),
     "w4_gemv_tune": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,

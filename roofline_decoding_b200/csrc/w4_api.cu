@@ -8,6 +8,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -96,6 +97,7 @@ int init_locked(int device) {
     if (st == W4_OK) st = mega_init_device(di);
     if (st == W4_OK) st = gemm_init_device(di);
     if (st == W4_OK) st = gptq_init_device(di);
+    if (st == W4_OK) st = kv8_init_device(di);
   } while (false);
   if (prev != device) cudaSetDevice(prev);
   if (st == W4_OK) {
@@ -330,6 +332,13 @@ int w4_gemm(const void* x, int x_dtype, const int32_t* packed, const void* scale
 
 int w4_gemm_ex(const void* x, int x_dtype, const int32_t* packed, const void* scales, void* y,
                int y_dtype, int M, int K, int N, int split_k, void* stream) {
+  const w4_gemm_ops none{};
+  return w4_gemm_fused(x, x_dtype, packed, scales, y, y_dtype, M, K, N, &none, split_k, stream);
+}
+
+int w4_gemm_fused(const void* x, int x_dtype, const int32_t* packed, const void* scales, void* y,
+                  int y_dtype, int M, int K, int N, const w4_gemm_ops* ops, int split_k,
+                  void* stream) {
   if (!x || !packed || !scales || !y) return fail(W4_ERR_INVALID_ARG, "w4_gemm: null pointer");
   if (split_k < 0 || split_k > 8 || (split_k > 0 && split_k > K / 64))
     return fail(W4_ERR_INVALID_ARG, "w4_gemm: split_k=%d (0 = choose, else 1..8 and <= K/64)",
@@ -342,8 +351,150 @@ int w4_gemm_ex(const void* x, int x_dtype, const int32_t* packed, const void* sc
                 "w4_gemm: M=%d K=%d N=%d (M >= 1, K and N multiples of 128)", M, K, N);
   if (!aligned16(x) || !aligned16(packed) || !aligned16(scales) || !aligned16(y))
     return fail(W4_ERR_ALIGNMENT, "w4_gemm: pointers must be 16-byte aligned");
-  return launch_gemm(x, x_dtype == W4_BF16, packed, scales, y, y_dtype == W4_BF16, M, K, N,
+  if (!ops) return fail(W4_ERR_INVALID_ARG, "w4_gemm: null ops");
+  if (ops->act < W4_ACT_NONE || ops->act > W4_ACT_SWIGLU)
+    return fail(W4_ERR_INVALID_ARG, "w4_gemm: activation %d unknown", ops->act);
+  if ((ops->bias && !aligned16(ops->bias)) || (ops->residual && !aligned16(ops->residual)))
+    return fail(W4_ERR_ALIGNMENT, "w4_gemm: bias and residual must be 16-byte aligned");
+  return launch_gemm(x, x_dtype == W4_BF16, packed, scales, y, y_dtype == W4_BF16, M, K, N, *ops,
                      split_k, (cudaStream_t)stream);
+}
+
+// ---------------------------------------------------------------- batched attention
+
+// An empty tensor's pointer may be null: only rows that exist need one.
+static int check_heads(const w4_heads* x, int rows, int head_dim, const char* what) {
+  if (!x || x->heads < 0 || x->heads > 4096)
+    return fail(W4_ERR_INVALID_ARG, "%s: heads missing or outside 0..4096", what);
+  if (x->heads == 0 || rows == 0) return W4_OK;
+  if (!x->ptr) return fail(W4_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!aligned16(x->ptr) || x->row_stride % 8 != 0 || x->head_stride % 8 != 0)
+    return fail(W4_ERR_ALIGNMENT,
+                "%s: 16-byte aligned rows needed (pointer, and strides in multiples of 8)", what);
+  if (x->row_stride < 0 || x->head_stride < 0 || (x->heads > 1 && x->head_stride < head_dim))
+    return fail(W4_ERR_INVALID_ARG, "%s: row stride %lld, head stride %lld", what,
+                (long long)x->row_stride, (long long)x->head_stride);
+  return W4_OK;
+}
+
+static int check_head_dim(int head_dim, const char* what) {
+  if (head_dim != 64 && head_dim != 128)
+    return fail(W4_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", what, head_dim);
+  return W4_OK;
+}
+
+static int check_rope(const w4_rope* r, const char* what) {
+  if (!r) return fail(W4_ERR_INVALID_ARG, "%s: null rope", what);
+  if (!r->cos_table != !r->sin_table)
+    return fail(W4_ERR_INVALID_ARG, "%s: one of the two rotation tables is missing", what);
+  if (r->cos_table) {
+    if (r->table_dtype != W4_F16 && r->table_dtype != W4_BF16 && r->table_dtype != W4_F32)
+      return fail(W4_ERR_INVALID_ARG, "%s: table dtype %d unknown", what, r->table_dtype);
+    if (r->max_pos <= 0) return fail(W4_ERR_INVALID_ARG, "%s: max_pos=%d", what, r->max_pos);
+  }
+  if (!aligned16(r->cos_table) || !aligned16(r->sin_table) || !aligned16(r->q_norm) ||
+      !aligned16(r->k_norm))
+    return fail(W4_ERR_ALIGNMENT, "%s: tables and norm weights must be 16-byte aligned", what);
+  return W4_OK;
+}
+
+static int check_cache(const w4_kv8_cache* c, const char* what) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale)
+    return fail(W4_ERR_INVALID_ARG, "%s: null cache pointer", what);
+  if (c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 4096)
+    return fail(W4_ERR_INVALID_ARG, "%s: pages=%d kv_heads=%d", what, c->pages, c->kv_heads);
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+    return fail(W4_ERR_UNSUPPORTED, "%s: page_size %d (16, 32, 64 or 128)", what, c->page_size);
+  int st = check_head_dim(c->head_dim, what);
+  if (st != W4_OK) return st;
+  if (!aligned16(c->k) || !aligned16(c->v))
+    return fail(W4_ERR_ALIGNMENT, "%s: the cache must be 16-byte aligned", what);
+  return W4_OK;
+}
+
+static int check_batch(const w4_kv_batch* b, const char* what) {
+  if (!b) return fail(W4_ERR_INVALID_ARG, "%s: null batch", what);
+  if (b->seqs < 0 || b->rows < 0 || b->rows > (1 << 26) || b->max_pages <= 0 ||
+      b->table_stride < 0)
+    return fail(W4_ERR_INVALID_ARG, "%s: seqs=%d rows=%d max_pages=%d", what, b->seqs, b->rows,
+                b->max_pages);
+  if (b->seqs > 0 && b->rows > 0 && (!b->page_table || !b->lengths || !b->row_starts))
+    return fail(W4_ERR_INVALID_ARG, "%s: null batch pointer", what);
+  return W4_OK;
+}
+
+int w4_qk_norm_rope(const w4_heads* q, const w4_heads* k, const w4_heads* q_out,
+                    const w4_heads* k_out, int dtype, int rows, int head_dim,
+                    const w4_rope* rope, const int64_t* positions, void* stream) {
+  const char* what = "w4_qk_norm_rope";
+  int st = check_dtype(dtype, what);
+  if (st != W4_OK || (st = check_head_dim(head_dim, what)) != W4_OK) return st;
+  if (rows < 0) return fail(W4_ERR_INVALID_ARG, "%s: rows=%d", what, rows);
+  for (const w4_heads* x : {q, k, q_out, k_out})
+    if ((st = check_heads(x, rows, head_dim, what)) != W4_OK) return st;
+  if (q->heads != q_out->heads || k->heads != k_out->heads)
+    return fail(W4_ERR_INVALID_ARG, "%s: inputs and outputs differ in heads", what);
+  if ((st = check_rope(rope, what)) != W4_OK) return st;
+  if (rows == 0 || q->heads + k->heads == 0) return W4_OK;
+  if (rope->cos_table && !positions) return fail(W4_ERR_INVALID_ARG, "%s: null positions", what);
+  int dev;
+  if ((st = current_device(&dev)) != W4_OK) return st;
+  return launch_norm_rope(*q, *k, *q_out, *k_out, dtype == W4_BF16, rows, head_dim, *rope,
+                          positions, device_info(dev), (cudaStream_t)stream);
+}
+
+int w4_kv8_append(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_heads* k,
+                  const w4_heads* v, const w4_heads* q, const w4_heads* q_out, int dtype,
+                  const w4_rope* rope, void* stream) {
+  const char* what = "w4_kv8_append";
+  int st = check_dtype(dtype, what);
+  if (st != W4_OK || (st = check_cache(cache, what)) != W4_OK ||
+      (st = check_batch(batch, what)) != W4_OK)
+    return st;
+  for (const w4_heads* x : {k, v, q, q_out})
+    if ((st = check_heads(x, batch->rows, cache->head_dim, what)) != W4_OK) return st;
+  if (k->heads != cache->kv_heads || v->heads != cache->kv_heads)
+    return fail(W4_ERR_INVALID_ARG, "%s: k has %d heads, v %d, the cache %d", what, k->heads,
+                v->heads, cache->kv_heads);
+  if (q->heads != q_out->heads)
+    return fail(W4_ERR_INVALID_ARG, "%s: q and q_out differ in heads", what);
+  if ((st = check_rope(rope, what)) != W4_OK) return st;
+  if (batch->rows == 0 || batch->seqs == 0) return W4_OK;
+  int dev;
+  if ((st = current_device(&dev)) != W4_OK) return st;
+  return launch_kv8_append(*cache, *batch, *k, *v, *q, *q_out, dtype == W4_BF16, *rope,
+                           device_info(dev), (cudaStream_t)stream);
+}
+
+size_t w4_kv8_attention_workspace_bytes(int head_dim) {
+  return kv8_attention_workspace_bytes(head_dim);
+}
+
+int w4_kv8_attention(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_heads* q,
+                     const w4_heads* out, int dtype, float scale, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  const char* what = "w4_kv8_attention";
+  int st = check_dtype(dtype, what);
+  if (st != W4_OK || (st = check_cache(cache, what)) != W4_OK ||
+      (st = check_batch(batch, what)) != W4_OK ||
+      (st = check_heads(q, batch->rows, cache->head_dim, what)) != W4_OK ||
+      (st = check_heads(out, batch->rows, cache->head_dim, what)) != W4_OK)
+    return st;
+  if (q->heads != out->heads || q->heads <= 0 || q->heads % cache->kv_heads != 0 ||
+      q->heads / cache->kv_heads > 16)
+    return fail(W4_ERR_INVALID_ARG,
+                "%s: %d query heads (out %d) over %d cache heads (1 to 16 each)", what, q->heads,
+                out->heads, cache->kv_heads);
+  if (!workspace || workspace_bytes < kv8_attention_workspace_bytes(cache->head_dim))
+    return fail(W4_ERR_INVALID_ARG, "%s: workspace of %zu bytes < %zu", what, workspace_bytes,
+                kv8_attention_workspace_bytes(cache->head_dim));
+  if (!aligned16(workspace))
+    return fail(W4_ERR_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);
+  if (batch->rows == 0 || batch->seqs == 0) return W4_OK;
+  int dev;
+  if ((st = current_device(&dev)) != W4_OK) return st;
+  return launch_kv8_attention(*cache, *batch, *q, *out, dtype == W4_BF16, scale, workspace,
+                              device_info(dev), (cudaStream_t)stream);
 }
 
 int w4_gptq_block(const float* w, const float* hinv, int N, int32_t* packed, void* scales,

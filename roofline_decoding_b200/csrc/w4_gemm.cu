@@ -18,8 +18,10 @@
 //                  stage for each of the tile's one or two 128-row halves
 //                  (both halves share one dequantised B tile), and commits to
 //                  the ring's mbarriers;
-//   epilogue     : the dequant warps read the accumulators with tcgen05.ld
-//                  and store Y (fp16 or bf16).
+//   epilogue     : the dequant warps read the accumulators with tcgen05.ld,
+//                  apply bias, activation (or the gated pair of interleaved
+//                  gate and up columns) and residual in fp32 where the call
+//                  asks for them, and store Y (fp16 or bf16) with one rounding.
 // bf16 activations use bf16 weights bf16((q - 8) * s) (one rounding of the
 // fp32 product; the reference has no bf16 path). Every wait is bounded; a
 // CTA that gives up sets the device error word, drains its copies and
@@ -65,6 +67,9 @@ struct GemmParams {
   // n_tile0 + t % ntx) in units of the instance's rows and columns
   int m_tile0, n_tile0, ntx;
   int ksplit;       // K slices (gridDim.z, one cluster per tile when > 1)
+  int act;               // w4_act
+  const void* bias;      // [N] of y's type, or null
+  const void* residual;  // like y, or null
   int wait_at_end;  // a launch overlapping the previous one on the stream
                     // completes only after it (griddepcontrol.wait at exit)
 };
@@ -215,6 +220,93 @@ __device__ __forceinline__ uint4 dequant_word(uint32_t w, uint32_t s2, float sf)
     }
   }
   return out;
+}
+
+// ---------------------------------------------------------------- epilogue
+
+// Four 16-bit elements (8 bytes) or eight (16 bytes) to fp32.
+template <int NV>
+__device__ __forceinline__ void load_row(const void* p, size_t at, int bf16, float (&f)[NV]) {
+  uint32_t w[NV / 2];
+  const uint16_t* src = static_cast<const uint16_t*>(p) + at;
+  if constexpr (NV == 8)
+    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src);
+  else
+    *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(src);
+#pragma unroll
+  for (int i = 0; i < NV / 2; ++i) {
+    if (bf16) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  }
+}
+
+template <int NV>
+__device__ __forceinline__ void store_row(void* p, size_t at, int bf16, const float (&f)[NV]) {
+  uint32_t w[NV / 2];
+#pragma unroll
+  for (int i = 0; i < NV / 2; ++i) {
+    if (bf16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  uint16_t* dst = static_cast<uint16_t*>(p) + at;
+  if constexpr (NV == 8)
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(w);
+  else
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(w);
+}
+
+__device__ __forceinline__ float silu(float a) { return __fdividef(a, 1.0f + __expf(-a)); }
+
+// NV accumulators of columns n.. of one row (u: the up columns, 32 further, of
+// a gated pair) to NV outputs.
+template <int NV>
+__device__ __forceinline__ void finish(const GemmParams& p, int row, int n, float (&a)[NV],
+                                       float (&u)[NV]) {
+  const bool gated = p.act == W4_ACT_SWIGLU;
+  if (p.bias) {
+    float b[NV];
+    load_row(p.bias, (size_t)n, p.y_bf16, b);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) a[i] += b[i];
+    if (gated) {
+      load_row(p.bias, (size_t)n + W4B200_SWIGLU_BLOCK, p.y_bf16, b);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) u[i] += b[i];
+    }
+  }
+  if (gated) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) a[i] = silu(a[i]) * u[i];
+  } else if (p.act == W4_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) a[i] = silu(a[i]);
+  } else if (p.act == W4_ACT_GELU) {
+    // x Phi(x) by the complementary error function: 1 + erf would cancel in
+    // the left tail
+#pragma unroll
+    for (int i = 0; i < NV; ++i) a[i] = 0.5f * a[i] * erfcf(a[i] * -0.70710678118654752f);
+  }
+  // gate column 64 j + i is output column 32 j + i
+  const int col = gated ? (n >> 6) * W4B200_SWIGLU_BLOCK + (n & (W4B200_SWIGLU_BLOCK - 1)) : n;
+  const size_t at = (size_t)row * (gated ? p.N / 2 : p.N) + col;
+  if (p.residual) {
+    float r[NV];
+    load_row(p.residual, at, p.y_bf16, r);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) a[i] += r[i];
+  }
+  store_row(p.y, at, p.y_bf16, a);
 }
 
 template <bool kBF16, int BN, int NACC>
@@ -385,30 +477,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int half = (warp - 1) / 4;   // which accumulator (rows 0..127 or 128..255)
       if (half >= NACC) goto epilogue_done;
       const int row = m0 + half * kUM + 32 * q + lane;
+const uint32_t acc = tmem_d + ((uint32_t)(32 * q) << 16) + half * BN;
+      const int step = p.act == W4_ACT_SWIGLU ? 2 : 1;  // 32-column blocks a turn
 #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(tmem_d + ((uint32_t)(32 * q) << 16) + half * BN + 32 * c, r);
+      for (int c = 0; c < BN / 32; c += step) {
+        uint32_t r[32], ru[32];
+        tmem_ld32(acc + 32 * c, r);
+        if (step == 2) tmem_ld32(acc + 32 * c + 32, ru);
         if (row < p.M && n0 + 32 * c < p.N) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) +
-                                                (size_t)row * p.N + n0 + 32 * c);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            uint4 o;
-            uint32_t* oi = reinterpret_cast<uint32_t*>(&o);
+            float a[8], u[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = __uint_as_float(r[8 * v + 2 * e]);
-              const float b = __uint_as_float(r[8 * v + 2 * e + 1]);
-              if (p.y_bf16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-                oi[e] = *reinterpret_cast<const uint32_t*>(&h);
-              } else {
-                const __half2 h = __floats2half2_rn(a, b);
-                oi[e] = *reinterpret_cast<const uint32_t*>(&h);
-              }
+            for (int e = 0; e < 8; ++e) {
+              a[e] = __uint_as_float(r[8 * v + e]);
+              u[e] = __uint_as_float(ru[8 * v + e]);
             }
-            dst[v] = o;
+            finish(p, row, n0 + 32 * c + 8 * v, a, u);
           }
         }
       }
@@ -425,35 +510,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       cluster.sync();
       const int rank = (int)blockIdx.z;
       const int r0 = rank * S::kBM / p.ksplit, r1 = (rank + 1) * S::kBM / p.ksplit;
-      constexpr int kC4 = BN / 4;
+      const bool gated = p.act == W4_ACT_SWIGLU;
+      const int c4s = gated ? BN / 8 : BN / 4;  // groups of four output columns
       const float* part = reinterpret_cast<const float*>(base);
-      for (int i = threadIdx.x; i < (r1 - r0) * kC4; i += kGemmThreads) {
-        const int row = r0 + i / kC4, c4 = i - (i / kC4) * kC4;
-        const int at = row * S::kPitch + 4 * c4;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = threadIdx.x; i < (r1 - r0) * c4s; i += kGemmThreads) {
+        const int row = r0 + i / c4s;
+        int col = 4 * (i - (i / c4s) * c4s);
+        if (gated) col = (col >> 5) * 64 + (col & 31);  // the gate column
+        const int at = row * S::kPitch + col;
+        float a[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
         for (int rr = 0; rr < p.ksplit; ++rr) {
           const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + at, rr));
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
-        }
-        const int grow = m0 + row, gcol = n0 + 4 * c4;
-        if (grow < p.M && gcol < p.N) {
-          uint2 o;
-          if (p.y_bf16) {
-            const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x, acc.y);
-            const __nv_bfloat162 b = __floats2bfloat162_rn(acc.z, acc.w);
-            o = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
-                           *reinterpret_cast<const uint32_t*>(&b));
-          } else {
-            const __half2 a = __floats2half2_rn(acc.x, acc.y);
-            const __half2 b = __floats2half2_rn(acc.z, acc.w);
-            o = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
-                           *reinterpret_cast<const uint32_t*>(&b));
+          a[0] += v.x, a[1] += v.y, a[2] += v.z, a[3] += v.w;
+          if (gated) {
+            const float4 w = *reinterpret_cast<const float4*>(
+                cluster.map_shared_rank(part + at + W4B200_SWIGLU_BLOCK, rr));
+            u[0] += w.x, u[1] += w.y, u[2] += w.z, u[3] += w.w;
           }
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + (size_t)grow * p.N + gcol) = o;
         }
+        if (m0 + row < p.M && n0 + col < p.N) finish(p, m0 + row, n0 + col, a, u);
       }
       cluster.sync();  // the other ranks' reads of this CTA's partial are done
     }
@@ -596,7 +671,8 @@ int gemm_plan(int M, int K, int N, int sms, int split_k, GemmLaunch* out) {
 }  // namespace
 
 int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* scales, void* y,
-                int y_bf16, int M, int K, int N, int split_k, cudaStream_t stream) {
+                int y_bf16, int M, int K, int N, const w4_gemm_ops& ops, int split_k,
+                cudaStream_t stream) {
   int dev = 0;
   int st = current_device(&dev);
   if (st != W4_OK) return st;
@@ -623,6 +699,9 @@ int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* sc
     p.N = N;
     p.x_bf16 = x_bf16;
     p.y_bf16 = y_bf16;
+    p.act = ops.act;
+    p.bias = ops.bias;
+    p.residual = ops.residual;
     p.err = di.err_word;
     p.m_tile0 = L.m_tile0;
     p.n_tile0 = L.n_tile0;

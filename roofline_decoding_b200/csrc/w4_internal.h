@@ -86,7 +86,21 @@ inline bool lm_head_hidden_supported(int hidden) {
 // tcgen05 W4A16 GEMM (w4_gemm.cu).
 int gemm_init_device(const DeviceInfo& di);
 int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* scales, void* y,
-                int y_bf16, int M, int K, int N, int split_k, cudaStream_t stream);
+                int y_bf16, int M, int K, int N, const w4_gemm_ops& ops, int split_k,
+                cudaStream_t stream);
+
+// Head norms, rotation and the paged 8-bit KV cache (w4_kv8.cu, w4_kv8_attn.cu).
+int launch_norm_rope(const w4_heads& q, const w4_heads& k, const w4_heads& q_out,
+                     const w4_heads& k_out, int bf16, int rows, int head_dim, const w4_rope& rope,
+                     const int64_t* positions, const DeviceInfo& di, cudaStream_t stream);
+int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_heads& k,
+                      const w4_heads& v, const w4_heads& q, const w4_heads& q_out, int bf16,
+                      const w4_rope& rope, const DeviceInfo& di, cudaStream_t stream);
+int kv8_init_device(const DeviceInfo& di);
+size_t kv8_attention_workspace_bytes(int head_dim);
+int launch_kv8_attention(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_heads& q,
+                         const w4_heads& out, int bf16, float scale, void* workspace,
+                         const DeviceInfo& di, cudaStream_t stream);
 
 // Calibrated (GPTQ) packing, one 128-row block (w4_gptq.cu).
 int gptq_init_device(const DeviceInfo& di);

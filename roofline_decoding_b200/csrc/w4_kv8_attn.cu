@@ -1,0 +1,838 @@
+// w4_kv8_attn.cu - attention of a step's queries over the paged 8-bit KV cache.
+//
+//   o_r = sum_j softmax_j(scale q_r . (sk_j k_j)) sv_j v_j,  j < limit(r)
+//
+// with e4m3 codes k_j, v_j, and sk_j, sv_j the scales of their page and head.
+// The query rows of one cache head (G query heads times the sequence's new
+// tokens) form 16-row tiles; an item is (sequence, cache head, row tile), and
+// its work is its 32-token tiles of the cache.
+//
+// Bound by the cache's bytes at the small row counts of decoding (2 D bytes a
+// token and cache head against 4 D operations a query row), so the design is
+// about streaming: every warp runs alone on its own ring of tiles (cp.async,
+// 16 bytes a lane, no barrier between warps in the loop) and holds its own
+// running maximum, sum and output; the CTA's warps merge once an item.
+//
+// Work split: the tiles of all items are numbered in one line and every CTA
+// takes an equal, contiguous share, found on the device from the lengths: no
+// length is needed on the host, a captured launch follows new lengths, and
+// ragged sequences balance. An item cut by the border of two shares leaves
+// fp32 partials that a second, programmatically dependent launch joins in
+// order; nothing is atomic, so results repeat bit for bit.
+//
+// Arithmetic: mma.sync m16n8k16 in fp16 with fp32 sums. e4m3 widens to fp16
+// exactly. Queries enter scaled by a power of two a row that brings their
+// largest element to 2^14 (bf16 to fp16 is then exact but for elements 2^-28
+// below the row's largest). The page's value scale is folded into the
+// exponent: P' = exp2(s + log2 sv - m + 14) with m the running maximum of
+// s + log2 sv, so P' is at most 2^14, its rounding to fp16 (11 bits) stays
+// relative down to 2^-28 of the largest weight, and the fp32 sum adds
+// P' / sv, unrounded.
+#include "w4_internal.h"
+#include "w4_ptx.cuh"
+
+#include <algorithm>
+
+namespace w4 {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 32;        // tokens of one ring stage of a warp
+constexpr int kRows = 16;        // query rows of an item
+constexpr int kCtasPerSm = 2;
+constexpr float kShift = 14.0f;  // P' is at most 2^kShift
+// Tiles a CTA takes at least (one a warp): below that more CTAs only add
+// partials to join.
+constexpr int kMinTiles = kWarps;
+
+template <int D>
+struct AttnShape {
+  static constexpr int kStageBytes = 2 * kTile * D;  // K, then V
+  static constexpr int kStages = D == 128 ? 3 : 5;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kScales = kWarps * kStages * 16;  // per stage: K, V scale of two halves
+  static constexpr int kPitch = D + 4;                   // floats; the 4 hold maximum and sum
+  static constexpr int kMerge = 2 * kRows * kPitch * 4;  // two warps' outputs
+  static constexpr int kSmem = kRing + kScales + kMerge;
+  static constexpr int kKSteps = D / 16;   // 16-dim steps of Q K^T
+  static constexpr int kNTiles = D / 8;    // 8-dim tiles of P V
+  static constexpr int kWords = D / 32;    // 32-bit words of a lane's V chunk
+};
+
+struct AttnP {
+  const uint8_t *k, *v;
+  const float *k_scale, *v_scale;
+  const int32_t *page_table, *lengths, *row_starts;
+  int64_t table_stride;
+  int capacity;  // tokens that a row of the page table holds
+  int pages, page, page_shift, max_pages, kv_heads, seqs, rows, group;
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  uint16_t* out;
+  int64_t out_row, out_head;
+  int bf16;
+  float scale_log2;
+  float* parts;       // [CTAs][2][kRows][D + 4]
+  struct Join* join;  // [CTAs]
+  int* err;
+};
+
+// What the second launch needs to join an item: written by the CTA whose share
+// begins at the item's first inner border, empty (count 0) by every other.
+struct Join {
+  int count;       // partials, CTAs cta .. cta + count - 1
+  int cta, slot;   // the first partial's CTA and slot; the others are in slot 0
+  int row0, head0; // first output row of the sequence, first query head
+  int r0, rows;    // the tile's first query row, and all query rows of the item's head
+  int pad;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two e4m3 codes (the low half of w, or the high) to fp16, exactly.
+__device__ __forceinline__ uint32_t e4m3_lo(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
+      : "=r"(d)
+      : "r"(w));
+  return d;
+}
+__device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+      : "=r"(d)
+      : "r"(w));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(real ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
+               "r"(real ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile. Chunks are XOR-ed with
+// the 128-byte line's number, so that neither the K reads (8 lanes: two rows,
+// every second chunk) nor, at D = 128, the V reads (four rows, two chunks) of a
+// quarter warp share a bank.
+template <int D>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  if constexpr (D == 128) {
+    return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
+  } else {
+    const int line = r >> 1, cc = ((r & 1) << 2) | c;
+    return (uint32_t)(line * 128 + ((cc ^ (line & 7)) << 4));
+  }
+}
+
+// A sequence's rows and tokens. A length that the page table cannot hold is cut
+// to what it holds.
+struct Seq {
+  int first, n;  // rows
+  int past;
+};
+__device__ __forceinline__ Seq load_seq(const AttnP& p, int b) {
+  Seq s;
+  s.first = min(max(p.row_starts[b], 0), p.rows);
+  s.n = min(max(p.row_starts[b + 1], s.first), p.rows) - s.first;
+  s.past = min(max(p.lengths[b], 0), p.capacity);
+  return s;
+}
+// Tokens that query row r (of n * group) of the sequence sees.
+__device__ __forceinline__ int seen(const AttnP& p, const Seq& s, int r) {
+  return min(s.past + r / p.group + 1, p.capacity);
+}
+__device__ __forceinline__ int row_tiles(const AttnP& p, const Seq& s) {
+  return (s.n * p.group + kRows - 1) / kRows;
+}
+// Tiles of a row tile of the sequence; the shares count every row tile at the
+// length of the last (the tiles above a row tile's own limit are passed over).
+__device__ __forceinline__ int token_tiles(const AttnP& p, const Seq& s) {
+  return (min(s.past + s.n, p.capacity) + kTile - 1) / kTile;
+}
+__device__ __forceinline__ int64_t seq_work(const AttnP& p, const Seq& s) {
+  return s.n > 0 ? (int64_t)p.kv_heads * row_tiles(p, s) * token_tiles(p, s) : 0;
+}
+
+// The line of all tiles: its length, and where tile x lies. Every thread of
+// the CTA calls it.
+struct Place {
+  int b;
+  int64_t off;  // tiles of sequence b before x
+};
+
+__device__ void find_place(const AttnP& p, int64_t* total, int64_t* share0, int64_t* share1,
+                           int* ctas, Place* place) {
+  __shared__ int64_t warp_sum[kWarps];
+  __shared__ Place found;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.seqs + kThreads - 1) / kThreads;
+  const int b0 = min(p.seqs, tid * per), b1 = min(p.seqs, b0 + per);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Seq s = load_seq(p, b);
+    mine += seq_work(p, s);
+    if (s.n > 0 && (p.lengths[b] < 0 || p.lengths[b] > p.capacity - s.n))
+      atomicCAS(p.err, 0, kErrKvRange);
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += up;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int64_t all = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_sum[w];
+    all += warp_sum[w];
+  }
+  const int64_t c = min((int64_t)gridDim.x, (all + kMinTiles - 1) / kMinTiles);
+  *ctas = (int)c;
+  *total = all;
+  if ((int64_t)blockIdx.x >= c) {
+    *share0 = *share1 = all;
+    return;
+  }
+  *share0 = all * blockIdx.x / c;
+  *share1 = all * (blockIdx.x + 1) / c;
+  int64_t at = before + incl - mine;
+  if (*share0 >= at && *share0 < at + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const int64_t w = seq_work(p, load_seq(p, b));
+      if (*share0 < at + w) {
+        found.b = b;
+        found.off = *share0 - at;
+        break;
+      }
+      at += w;
+    }
+  }
+  __syncthreads();
+  *place = found;
+}
+
+// Walks a CTA's share item by item.
+struct Walk {
+  int64_t x, end;  // next tile of the line, end of the share
+  int b;           // sequence of x
+  int64_t off;     // x's place in it
+  // the item
+  Seq s;
+  int h, rt;
+  int64_t item0;   // first tile of the item in the line
+  int nt;          // its tiles (as the shares count them)
+  int t0, t1;      // the share's part of them, cut at the row tile's own limit
+  int t1_full;     // not cut
+  int limit;       // tokens that the row tile's last row sees
+
+  __device__ __forceinline__ bool next(const AttnP& p) {
+    if (x >= end) return false;
+    s = load_seq(p, b);
+    for (int64_t w; off >= (w = seq_work(p, s));) {  // sequences without rows, or just done
+      off -= w;
+      if (++b >= p.seqs) return false;
+      s = load_seq(p, b);
+    }
+    nt = token_tiles(p, s);
+    const int nrt = row_tiles(p, s);
+    const int64_t item = off / nt;
+    h = (int)(item / nrt);
+    rt = (int)(item - (int64_t)h * nrt);
+    t0 = (int)(off - item * nt);
+    t1_full = (int)min((int64_t)nt, t0 + (end - x));
+    item0 = x - t0;
+    x += t1_full - t0;
+    off += t1_full - t0;
+    limit = seen(p, s, min(s.n * p.group, (rt + 1) * kRows) - 1);
+    t1 = min(t1_full, (limit + kTile - 1) / kTile);
+    return true;
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(const AttnP p) {
+  using S = AttnShape<D>;
+  extern __shared__ __align__(128) uint8_t smem_kv8[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(smem_kv8) + warp * S::kStages * S::kStageBytes;
+  float* scales = reinterpret_cast<float*>(smem_kv8 + S::kRing) + warp * S::kStages * 4;
+  float* merge = reinterpret_cast<float*>(smem_kv8 + S::kRing + S::kScales);
+
+  grid_launch_dependents();
+  int64_t total, share0, share1;
+  int ctas;
+  Place place;
+  find_place(p, &total, &share0, &share1, &ctas, &place);
+  if (tid == 0) p.join[blockIdx.x].count = 0;
+  if (share0 >= share1) return;
+
+  // ---- the load side: this warp's tiles, kStages - 1 ahead of the compute side
+  Walk lw;
+  lw.x = share0, lw.end = share1, lw.b = place.b, lw.off = place.off;
+  Walk cw = lw;
+  bool more = lw.next(p);
+  int lt = more ? lw.t0 + warp : 0;
+  int issue_slot = 0;
+  auto issue = [&]() {
+    while (more && lt >= lw.t1) {
+      more = lw.next(p);
+      lt = lw.t0 + warp;
+    }
+    if (more) {
+      const int tok0 = lt * kTile;
+      // the (one or two) pages of the tile: halves of 16 tokens
+      int id = -1;
+      if (lane < 2) {
+        const int at = tok0 + 16 * lane;
+        const int pi = at >> p.page_shift;
+        if (at < lw.limit) {
+          id = pi < p.max_pages ? p.page_table[lw.b * p.table_stride + pi] : -1;
+          if (id < 0 || id >= p.pages) {
+            id = -1;
+            atomicCAS(p.err, 0, kErrKvRange);
+          }
+        }
+        const size_t blk = (size_t)max(id, 0) * p.kv_heads + lw.h;
+        const uint32_t dst = smem_u32(scales + issue_slot * 4 + lane);
+        cp4(dst, p.k_scale + blk, id >= 0);  // zero marks a half that is left out
+        cp4(dst + 8, p.v_scale + blk, id >= 0);
+      }
+      const int id0 = __shfl_sync(0xffffffffu, id, 0), id1 = __shfl_sync(0xffffffffu, id, 1);
+      const uint32_t st = ring + issue_slot * S::kStageBytes;
+      constexpr int CPR = D / 16, RPI = 32 / CPR;  // chunks a row, rows a pass
+      const int c = lane % CPR, rr = lane / CPR;
+      const int in_page = p.page - 1;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int idh = half ? id1 : id0;
+        const int tok = tok0 + 16 * half;
+        const size_t base =
+            (((size_t)max(idh, 0) * p.kv_heads + lw.h) * p.page + (tok & in_page)) * D + 16 * c;
+        const int valid = idh >= 0 ? min(16, lw.limit - tok) : 0;
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) {
+          const int r = i * RPI + rr;
+          const uint32_t dst = st + chunk_at<D>(16 * half + r, c);
+          const size_t src = base + (size_t)(r < valid ? r : 0) * D;
+          cp16(dst, p.k + src, r < valid);
+          cp16(dst + kTile * D, p.v + src, r < valid);
+        }
+      }
+      lt += kWarps;
+    }
+    cp_commit();
+    issue_slot = issue_slot + 1 == S::kStages ? 0 : issue_slot + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < S::kStages - 1; ++i) issue();
+
+  int slot = 0;
+  bool first_segment = true;
+  while (cw.next(p)) {
+    // ---- queries of this item: rows g and g + 8 of the tile
+    const int n_rows = cw.s.n * p.group;
+    const int r0 = cw.rt * kRows;
+    uint32_t qf[S::kKSteps][4];
+    float q_mul[2];  // turns a sum into log2 units, but for the key scale
+    int lim[2];      // tokens that the row sees
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = r0 + g + 8 * j;
+      const int i = r / p.group;
+      const bool in = r < n_rows;
+      lim[j] = in ? seen(p, cw.s, r) : 0;
+      uint4 raw[D / 32];
+      const uint16_t* src = p.q + (int64_t)(cw.s.first + i) * p.q_row +
+                            (int64_t)(cw.h * p.group + r - i * p.group) * p.q_head + (D / 4) * t;
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w)
+        raw[w] = in ? __ldg(reinterpret_cast<const uint4*>(src) + w) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t* rw = reinterpret_cast<const uint32_t*>(raw);
+      float f[D / 4];
+      float amax = 0.f;
+#pragma unroll
+      for (int w = 0; w < D / 8; ++w) {
+        float2 v;
+        if (p.bf16)
+          v = make_float2(__uint_as_float(rw[w] << 16), __uint_as_float(rw[w] & 0xffff0000u));
+        else
+          v = __half22float2(*reinterpret_cast<const __half2*>(&rw[w]));
+        f[2 * w] = v.x;
+        f[2 * w + 1] = v.y;
+        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // 2^(14 - exponent of amax), within what fp32 holds
+      const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
+      const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+      q_mul[j] = p.scale_log2 * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+      // step s of this lane: dims D/4 t + 4 s .. + 3, the order of the K words
+#pragma unroll
+      for (int s = 0; s < S::kKSteps; ++s) {
+        qf[s][j] = half2_bits(f[4 * s] * up, f[4 * s + 1] * up);
+        qf[s][j + 2] = half2_bits(f[4 * s + 2] * up, f[4 * s + 3] * up);
+      }
+    }
+    const int low = __reduce_min_sync(0xffffffffu,
+                                      min(lim[0] > 0 ? lim[0] : 0x7fffffff,
+                                          lim[1] > 0 ? lim[1] : 0x7fffffff));
+
+    float o[S::kNTiles][4];
+#pragma unroll
+    for (int j = 0; j < S::kNTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+#pragma unroll 1
+    for (int tile = cw.t0 + warp; tile < cw.t1; tile += kWarps) {
+      cp_wait<S::kStages - 2>();
+      __syncwarp();  // this stage has landed, and the stage before it is read
+      issue();
+      const uint32_t st = ring + slot * S::kStageBytes;
+      const float* sc = scales + slot * 4;
+      // ---- S = Q K^T: a lane's K words are dims D/4 t .. of token 8 j + g
+      float s[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint4 kw = lds128(st + chunk_at<D>(8 * j + g, (D / 64) * t + c));
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&kw);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t(&a)[4] = qf[4 * c + i];
+            mma_16816<false>(s[j], a[0], a[1], a[2], a[3], e4m3_lo(w[i]), e4m3_hi(w[i]));
+          }
+        }
+      }
+      // ---- scores in log2 units with the value scale, masked
+      float t_max[2] = {-INFINITY, -INFINITY};
+      float inv_vs[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float ks = sc[half], vs = sc[2 + half];
+        const float lv = vs > 0.f ? log2f(vs) : -INFINITY;
+        inv_vs[half] = vs > 0.f ? 1.0f / vs : 0.f;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          float(&x)[4] = s[2 * half + jj];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = fmaf(x[i], q_mul[i >> 1] * ks, lv);
+        }
+      }
+      const int tok0 = tile * kTile;
+      if (tok0 + kTile > low) {  // some row ends inside the tile, or before it
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (tok0 + 8 * j + 2 * t + (i & 1) >= lim[i >> 1]) s[j][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t_max[i >> 1] = fmaxf(t_max[i >> 1], s[j][i]);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        t_max[r] = fmaxf(t_max[r], __shfl_xor_sync(0xffffffffu, t_max[r], 1));
+        t_max[r] = fmaxf(t_max[r], __shfl_xor_sync(0xffffffffu, t_max[r], 2));
+      }
+      if (__any_sync(0xffffffffu, t_max[0] > m[0] || t_max[1] > m[1])) {
+        float al[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float nm = fmaxf(m[r], t_max[r]);
+          al[r] = nm == m[r] ? 1.f : ex2(m[r] - nm);
+          m[r] = nm;
+          l[r] *= al[r];
+        }
+#pragma unroll
+        for (int j = 0; j < S::kNTiles; ++j) {
+          o[j][0] *= al[0];
+          o[j][1] *= al[0];
+          o[j][2] *= al[1];
+          o[j][3] *= al[1];
+        }
+      }
+      const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0] - kShift,
+                            m[1] == -INFINITY ? 0.f : m[1] - kShift};
+      uint32_t pf[2][4];  // P as the A operand: 16 tokens a step
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          float(&x)[4] = s[2 * half + jj];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - sub[i >> 1]);
+          sum[0] += x[0] + x[1];
+          sum[1] += x[2] + x[3];
+          pf[half][2 * jj] = half2_bits(x[0], x[1]);
+          pf[half][2 * jj + 1] = half2_bits(x[2], x[3]);
+        }
+        l[0] = fmaf(sum[0], inv_vs[half], l[0]);
+        l[1] = fmaf(sum[1], inv_vs[half], l[1]);
+      }
+      // ---- O += P V: a lane's V chunks are dims D/8 g .. of tokens 2t, 2t+1,
+      // 2t+8, 2t+9 of each 16; byte pairs of two tokens make the B operand
+      const uint32_t vst = st + kTile * D;
+      const bool mixed = tok0 + kTile > low && low < cw.limit;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t vw[4][S::kWords];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = 16 * half + 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (D == 128) {
+            const uint4 w = lds128(vst + chunk_at<D>(tok, g));
+            vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
+          } else {
+            const uint32_t at = vst + chunk_at<D>(tok, g >> 1) + 8 * (g & 1);
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                         : "=r"(vw[i][0]), "=r"(vw[i][1])
+                         : "r"(at));
+          }
+        }
+        if (mixed) {
+          // Rows of this item end at different tokens here, and a NaN in a
+          // value that one row sees must not reach a row that does not (0 *
+          // NaN): NaN codes leave V, and come back as a product of "row sees
+          // token" with "value is NaN".
+          uint32_t nan_any = 0u;
+          uint32_t nm[4][S::kWords];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < S::kWords; ++w) {
+              nm[i][w] = __vcmpeq4(vw[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              vw[i][w] &= ~nm[i][w];
+              nan_any |= nm[i][w];
+            }
+          if (__any_sync(0xffffffffu, nan_any != 0u)) {
+            uint32_t see[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+              const int tok = tok0 + 16 * half + 2 * t + 8 * (a >> 1);
+              const int lr = lim[a & 1];
+              see[a] = (tok < lr ? 0x3c00u : 0u) | (tok + 1 < lr ? 0x3c000000u : 0u);
+            }
+#pragma unroll
+            for (int w = 0; w < S::kWords; ++w)
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                const uint32_t sh = 8 * d;
+                const uint32_t b0 = ((nm[0][w] >> sh) & 1u) * 0x3c00u | ((nm[1][w] >> sh) & 1u) * 0x3c000000u;
+                const uint32_t b1 = ((nm[2][w] >> sh) & 1u) * 0x3c00u | ((nm[3][w] >> sh) & 1u) * 0x3c000000u;
+                float cnt[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_16816<false>(cnt, see[0], see[1], see[2], see[3], b0, b1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (cnt[i] > 0.f) o[4 * w + d][i] = __int_as_float(0x7fffffff);
+              }
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < S::kWords; ++w) {
+          const uint32_t x0 = __byte_perm(vw[0][w], vw[1][w], 0x5140);
+          const uint32_t y0 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+          const uint32_t x1 = __byte_perm(vw[2][w], vw[3][w], 0x5140);
+          const uint32_t y1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+          const uint32_t* a = pf[half];
+          mma_16816<false>(o[4 * w + 0], a[0], a[1], a[2], a[3], e4m3_lo(x0), e4m3_lo(x1));
+          mma_16816<false>(o[4 * w + 1], a[0], a[1], a[2], a[3], e4m3_hi(x0), e4m3_hi(x1));
+          mma_16816<false>(o[4 * w + 2], a[0], a[1], a[2], a[3], e4m3_lo(y0), e4m3_lo(y1));
+          mma_16816<false>(o[4 * w + 3], a[0], a[1], a[2], a[3], e4m3_hi(y0), e4m3_hi(y1));
+        }
+      }
+      slot = slot + 1 == S::kStages ? 0 : slot + 1;
+    }
+
+    // ---- merge the warps: 2 and 3 into 0 and 1, then 1 into 0. Column 2t of
+    // o[j] is dim D/8 (2t) + j, column 2t + 1 is D/8 (2t + 1) + j.
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+    auto give = [&](float* buf) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float* row = buf + (g + 8 * r) * S::kPitch;
+        if (t == 0) row[D] = m[r], row[D + 1] = l[r];
+#pragma unroll
+        for (int j = 0; j < S::kNTiles; j += 4)
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc)
+            *reinterpret_cast<float4*>(row + (D / 8) * (2 * t + cc) + j) =
+                make_float4(o[j][2 * r + cc], o[j + 1][2 * r + cc], o[j + 2][2 * r + cc],
+                            o[j + 3][2 * r + cc]);
+      }
+    };
+    auto take = [&](const float* buf) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float* row = buf + (g + 8 * r) * S::kPitch;
+        const float om = row[D], ol = row[D + 1];
+        const float nm = fmaxf(m[r], om);
+        const float fa = m[r] == -INFINITY ? 0.f : ex2(m[r] - nm);
+        const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
+        m[r] = nm;
+        l[r] = l[r] * fa + ol * fb;
+#pragma unroll
+        for (int j = 0; j < S::kNTiles; j += 4)
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const float4 v = *reinterpret_cast<const float4*>(row + (D / 8) * (2 * t + cc) + j);
+            o[j][2 * r + cc] = o[j][2 * r + cc] * fa + v.x * fb;
+            o[j + 1][2 * r + cc] = o[j + 1][2 * r + cc] * fa + v.y * fb;
+            o[j + 2][2 * r + cc] = o[j + 2][2 * r + cc] * fa + v.z * fb;
+            o[j + 3][2 * r + cc] = o[j + 3][2 * r + cc] * fa + v.w * fb;
+          }
+      }
+    };
+    __syncthreads();  // the last item's buffers are read
+    if (warp >= 2) give(merge + (warp - 2) * kRows * S::kPitch);
+    __syncthreads();
+    if (warp < 2) take(merge + warp * kRows * S::kPitch);
+    if (warp == 1) {
+      __syncwarp();  // its own buffer is read
+      give(merge + kRows * S::kPitch);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      take(merge + kRows * S::kPitch);
+      if (cw.t0 == 0 && cw.t1_full == cw.nt) {  // the whole item: the output
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = r0 + g + 8 * r;
+          if (row >= n_rows) continue;
+          const int i = row / p.group;
+          const float inv = l[r] > 0.f || l[r] != l[r] ? 1.0f / l[r] : 0.f;
+          uint16_t* dst = p.out + (int64_t)(cw.s.first + i) * p.out_row +
+                          (int64_t)(cw.h * p.group + row - i * p.group) * p.out_head;
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+            for (int j = 0; j < S::kNTiles; j += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float a = o[j + 2 * k][2 * r + cc] * inv, b = o[j + 2 * k + 1][2 * r + cc] * inv;
+                if (p.bf16) {
+                  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+                  w[k] = *reinterpret_cast<const uint32_t*>(&v);
+                } else {
+                  w[k] = half2_bits(a, b);
+                }
+              }
+              *reinterpret_cast<uint4*>(dst + (D / 8) * (2 * t + cc) + j) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+      } else {  // a part: left for the second launch
+        float* part = p.parts + ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * kRows * S::kPitch;
+        give(part);
+        // The join is described by the CTA whose share begins at the item's
+        // first inner border: its own share starts inside the item and the
+        // share before does not.
+        if (lane == 0 && cw.t0 > 0) {
+          const int64_t before = total * (blockIdx.x - 1) / ctas;
+          if (before <= cw.item0) {
+            const int64_t end = cw.item0 + cw.nt;
+            int last = blockIdx.x;
+            while (last + 1 < ctas && total * (last + 1) / ctas < end) ++last;
+            Join jn;
+            jn.count = last - (int)blockIdx.x + 2;
+            jn.cta = (int)blockIdx.x - 1;
+            jn.slot = before == cw.item0 ? 0 : 1;
+            jn.row0 = cw.s.first;
+            jn.head0 = cw.h * p.group;
+            jn.r0 = r0;
+            jn.rows = n_rows;
+            jn.pad = 0;
+            p.join[blockIdx.x] = jn;
+          }
+        }
+      }
+    }
+    first_segment = false;
+  }
+}
+
+constexpr int kJoinWarps = 8;
+
+// Joins the partials of one row of an item: blockIdx.x the border, blockIdx.y
+// the row. The warps take the partials in turn, a lane D/32 dims, and warp 0
+// adds the warps in order.
+template <int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(const AttnP p) {
+  constexpr int V = D / 32, kPitch = AttnShape<D>::kPitch;
+  __shared__ float sm[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][D];
+  grid_dependency_wait();
+  const Join jn = p.join[blockIdx.x];
+  const int row = jn.r0 + blockIdx.y;
+  if (jn.count == 0 || row >= jn.rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = 0.f;
+#pragma unroll 4
+  for (int c = warp; c < jn.count; c += kJoinWarps) {
+    const float* part = p.parts + (((size_t)(jn.cta + c) * 2 + (c == 0 ? jn.slot : 0)) * kRows +
+                                   blockIdx.y) * kPitch;
+    const float om = part[D], ol = part[D + 1];
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = part[V * lane + i];
+    const float nm = fmaxf(m, om);
+    const float fa = m == -INFINITY ? 0.f : ex2(m - nm);
+    const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
+    m = nm;
+    l = l * fa + ol * fb;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = o[i] * fa + v[i] * fb;
+  }
+  if (lane == 0) sm[warp] = m, sl[warp] = l;
+#pragma unroll
+  for (int i = 0; i < V; ++i) so[warp][V * lane + i] = o[i];
+  __syncthreads();
+  if (warp != 0) return;
+  m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sm[w]);
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float f = sm[w] == -INFINITY ? 0.f : ex2(sm[w] - m);
+    l += sl[w] * f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] += so[w][V * lane + i] * f;
+  }
+  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+  const int i = row / p.group;
+  uint16_t* dst = p.out + (int64_t)(jn.row0 + i) * p.out_row +
+                  (int64_t)(jn.head0 + row - i * p.group) * p.out_head + V * lane;
+#pragma unroll
+  for (int k = 0; k < V; k += 2) {
+    uint32_t w;
+    if (p.bf16) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(o[k] * inv, o[k + 1] * inv);
+      w = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      w = half2_bits(o[k] * inv, o[k + 1] * inv);
+    }
+    *reinterpret_cast<uint32_t*>(dst + k) = w;
+  }
+}
+
+// CTAs that the workspace has room for: two an SM on the largest sm_100 part.
+constexpr int kMaxCtas = 160 * kCtasPerSm;
+
+template <int D>
+int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
+  using S = AttnShape<D>;
+  p.join = reinterpret_cast<Join*>(p.parts + (size_t)kMaxCtas * 2 * kRows * S::kPitch);
+  const int ctas = std::min(kMaxCtas, kCtasPerSm * di.sm_count);
+  kv8_attention_kernel<D><<<ctas, kThreads, S::kSmem, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "w4_kv8_attention launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)max_rows);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kv8_join_kernel<D>, (const AttnP)p);
+  return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_kv8_attention join launch");
+}
+
+}  // namespace
+
+size_t kv8_attention_workspace_bytes(int head_dim) {
+  return (size_t)kMaxCtas * (2 * kRows * (head_dim + 4) * 4 + sizeof(Join));
+}
+
+int kv8_init_device(const DeviceInfo& di) {
+  const void* fns[] = {(const void*)kv8_attention_kernel<64>, (const void*)kv8_attention_kernel<128>};
+  const int smem[] = {AttnShape<64>::kSmem, AttnShape<128>::kSmem};
+  for (int i = 0; i < 2; ++i) {
+    if (smem[i] > di.max_smem_optin)
+      return fail(W4_ERR_UNSUPPORTED, "w4_kv8_attention needs %d B of shared memory", smem[i]);
+    cudaError_t e = cudaFuncSetAttribute(fns[i], cudaFuncAttributeMaxDynamicSharedMemorySize, smem[i]);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(fns[i], cudaFuncAttributePreferredSharedMemoryCarveout,
+                               cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(kv8 attention)");
+  }
+  return W4_OK;
+}
+
+int launch_kv8_attention(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_heads& q,
+                         const w4_heads& out, int bf16, float scale, void* workspace,
+                         const DeviceInfo& di, cudaStream_t stream) {
+  AttnP p = {};
+  p.k = static_cast<const uint8_t*>(c.k);
+  p.v = static_cast<const uint8_t*>(c.v);
+  p.k_scale = c.k_scale;
+  p.v_scale = c.v_scale;
+  p.page_table = bt.page_table;
+  p.lengths = bt.lengths;
+  p.row_starts = bt.row_starts;
+  p.table_stride = bt.table_stride;
+  p.pages = c.pages;
+  p.page = c.page_size;
+  p.page_shift = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : c.page_size == 64 ? 6 : 7;
+  p.max_pages = bt.max_pages;
+  // below 2^31 with room for a step's rows and a tile's rounding
+  p.capacity = (int)std::min<int64_t>((int64_t)bt.max_pages * c.page_size, 0x70000000);
+  p.kv_heads = c.kv_heads;
+  p.seqs = bt.seqs;
+  p.rows = bt.rows;
+  p.group = q.heads / c.kv_heads;
+  p.q = static_cast<const uint16_t*>(q.ptr);
+  p.q_row = q.row_stride;
+  p.q_head = q.head_stride;
+  p.out = static_cast<uint16_t*>(out.ptr);
+  p.out_row = out.row_stride;
+  p.out_head = out.head_stride;
+  p.bf16 = bf16;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.parts = static_cast<float*>(workspace);
+  p.err = di.err_word;
+  const int max_rows = (int)std::min<int64_t>(kRows, (int64_t)bt.rows * p.group);
+  return c.head_dim == 128 ? launch<128>(p, max_rows, di, stream)
+                           : launch<64>(p, max_rows, di, stream);
+}
+
+}  // namespace w4

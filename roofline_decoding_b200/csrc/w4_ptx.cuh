@@ -19,6 +19,10 @@ constexpr uint32_t kSuspendHintNs = 20000;  // 20 us
 
 // Device-side error word; kernels set it when a bounded wait gives up.
 enum : int { kErrNone = 0, kErrFullWait = 1, kErrEmptyWait = 2, kErrDrainWait = 3 };
+// (codes 4 to 7 belong to the kernels that set them)
+// A page, a row's position or a rotation table's row was out of range; what it
+// belonged to was left out.
+constexpr int kErrKvRange = 8;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
