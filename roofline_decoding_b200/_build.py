@@ -2,12 +2,15 @@
 
 The shared object lands next to this file so that it ships with the source
 tree; object files go to ``_build/`` beside it. Only sm_100a is targeted.
+_w4torch.so, the small extension module that passes torch tensors to that
+library, is built beside it with the host compiler against torch's headers.
 """
 from __future__ import annotations
 
 import os
 import shutil
 import subprocess
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -16,6 +19,7 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "libw4b200.so"
+TORCH_MODULE_PATH = PKG_DIR / "_w4torch.so"
 SOURCES = ["w4_api.cu", "w4_pack.cu", "w4_gemv.cu", "w4_gemv_ops.cu", "w4_gemv_fused.cu",
            "w4_decode.cu", "w4_mega.cu",
            "w4_gemm.cu", "w4_gptq.cu", "w4_tune.cu",
@@ -79,8 +83,34 @@ def build_library(verbose: bool = False, force: bool = False, ptxas_verbose: boo
     return LIB_PATH
 
 
+def build_torch_module(verbose: bool = False, force: bool = False) -> Path:
+    """Compiles and links _w4torch.so; returns its path. Needs libw4b200.so."""
+    src = CSRC / "w4_torch.cpp"
+    if not force and not _stale(TORCH_MODULE_PATH, [src, REPO_DIR / "include" / "w4b200.h"]):
+        return TORCH_MODULE_PATH
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in cpp_extension.include_paths()),
+           f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{cuda / 'include'}", str(src),
+           "-o", str(TORCH_MODULE_PATH), f"-L{PKG_DIR}", "-l:libw4b200.so", f"-L{torch_lib}",
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({' '.join(cmd)}):\n{r.stdout}\n{r.stderr}")
+    return TORCH_MODULE_PATH
+
+
 if __name__ == "__main__":
     import sys
 
     print(build_library(verbose=True, force="--force" in sys.argv,
                         ptxas_verbose="-v" in sys.argv))
+    print(build_torch_module(verbose=True, force="--force" in sys.argv))

@@ -5,6 +5,8 @@ Loading fails loudly: there is no fallback implementation behind this module.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from pathlib import Path
 
@@ -204,6 +206,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_torch_module = None
 
 
 def load() -> ctypes.CDLL:
@@ -224,6 +227,29 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def torch_module():
+    """Returns _w4torch, which passes torch tensors to the library; raises if it is missing."""
+    global _torch_module
+    if _torch_module is None:
+        load()
+        with _lock:
+            if _torch_module is None:
+                path = LIB_PATH.with_name("_w4torch.so")
+                if not path.exists():
+                    raise ImportError(
+                        f"{path.name} is not built; run `python -c 'import __graft_entry__ as g; "
+                        f"g.build()'` (or roofline_decoding_b200/_build.py) first")
+                import torch
+
+                loader = importlib.machinery.ExtensionFileLoader("_w4torch", str(path))
+                spec = importlib.util.spec_from_loader("_w4torch", loader)
+                module = importlib.util.module_from_spec(spec)
+                loader.exec_module(module)
+                module.set_errors(check, torch.OutOfMemoryError)
+                _torch_module = module
+    return _torch_module
 
 
 def check(status: int, what: str) -> None:

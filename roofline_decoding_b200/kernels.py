@@ -16,7 +16,6 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import json
-import math
 import os
 import threading
 from pathlib import Path
@@ -472,55 +471,10 @@ def w4_gemm_fused(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     residual have N // 2 columns: residual + silu(gate) * up. bias is [N],
     residual has y's shape; both have y's type. out may be residual itself.
     """
-    K, N = _check_packed(packed, scales)
-    if N % 128:
-        raise ValueError(f"w4_gemm_fused needs N % 128 == 0, got N={N}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")
-    if x.device != packed.device or x.dtype not in _DTYPE_CODE:
-        raise ValueError(f"x must be float16 or bfloat16 on {packed.device}, got {x.dtype} on "
-                         f"{x.device}")
-    x2, squeeze = _prep_x_any_rows(x, K, packed.device)
-    M, wide = x2.shape[0], N // 2 if activation == "swiglu" else N
-    y_dtype = out_dtype or x2.dtype
-    if y_dtype not in _DTYPE_CODE:
-        raise ValueError(f"out_dtype must be float16 or bfloat16, got {y_dtype}")
-    for name, t, shape in (("bias", bias, (N,)), ("residual", residual, (M, wide))):
-        if t is None:
-            continue
-        if t.dtype != y_dtype or t.device != packed.device or t.numel() != math.prod(shape) \
-                or t.shape[-1] != shape[-1]:
-            raise ValueError(f"{name} must be {y_dtype} {list(shape)} on {packed.device}, got "
-                             f"{t.dtype} {list(t.shape)} on {t.device}")
-    bias, residual = _dense16(bias), _dense16(residual)
-    if out is None:
-        y = torch.empty((M, wide), dtype=y_dtype, device=packed.device)
-    else:
-        if out.dtype != y_dtype or out.numel() != M * wide or not out.is_contiguous() \
-                or out.device != packed.device:
-            raise ValueError(f"out must be a contiguous {y_dtype} tensor of {M}x{wide} elements "
-                             f"on {packed.device}")
-        y = out
-    if M == 0:
-        return y
-    ops = _lib.GemmOps(_ACTIVATIONS[activation], bias.data_ptr() if bias is not None else None,
-                       residual.data_ptr() if residual is not None else None)
-    packed, scales = packed.contiguous(), scales.contiguous()
-    with _on_device(packed.device):
-        check(_lib.load().w4_gemm_fused(x2.data_ptr(), _DTYPE_CODE[x2.dtype], packed.data_ptr(),
-                                        scales.data_ptr(), y.data_ptr(), _DTYPE_CODE[y_dtype], M, K,
-                                        N, ops, int(split_k or 0), _stream_ptr(packed.device)),
-              "w4_gemm_fused")
-    if out is not None:
-        return out
-    return y[0] if squeeze else y
-
-
-def _dense16(t: torch.Tensor | None) -> torch.Tensor | None:
-    """t, or a copy of it that is contiguous and 16-byte aligned."""
-    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    return _lib.torch_module().w4_gemm_fused(x, packed, scales, bias, _ACTIVATIONS[activation],
+                                             residual, out, out_dtype, int(split_k or 0))
 
 
 def _prep_x_any_rows(x: torch.Tensor, K: int, device: torch.device) -> tuple[torch.Tensor, bool]:
