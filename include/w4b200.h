@@ -491,7 +491,7 @@ typedef struct {
   const int32_t* lengths;    /* [seqs] */
   const int32_t* row_starts; /* [seqs + 1] */
   int seqs;
-  int rows;                  /* rows of q, k and v, padding included */
+  int rows;                  /* rows of q, k and v, padding included; at most 2^24 */
 } w4_kv_batch;
 
 /* Writes a step's keys (normed and rotated) and values into the cache, and its

@@ -414,7 +414,7 @@ static int check_cache(const w4_kv8_cache* c, const char* what) {
 
 static int check_batch(const w4_kv_batch* b, const char* what) {
   if (!b) return fail(W4_ERR_INVALID_ARG, "%s: null batch", what);
-  if (b->seqs < 0 || b->rows < 0 || b->rows > (1 << 26) || b->max_pages <= 0 ||
+  if (b->seqs < 0 || b->rows < 0 || b->rows > (1 << 24) || b->max_pages <= 0 ||
       b->table_stride < 0)
     return fail(W4_ERR_INVALID_ARG, "%s: seqs=%d rows=%d max_pages=%d", what, b->seqs, b->rows,
                 b->max_pages);

@@ -55,7 +55,8 @@ struct AttnShape {
   static constexpr int kScales = kWarps * kStages * 16;  // per stage: K, V scale of two halves
   static constexpr int kPitch = D + 4;                   // floats; the 4 hold maximum and sum
   static constexpr int kMerge = 2 * kRows * kPitch * 4;  // two warps' outputs
-  static constexpr int kSmem = kRing + kScales + kMerge;
+  static constexpr int kMarks = kRows * D / 8;  // one bit an output: a NaN value reached it
+  static constexpr int kSmem = kRing + kScales + kMerge + kMarks;
   static constexpr int kKSteps = D / 16;   // 16-dim steps of Q K^T
   static constexpr int kNTiles = D / 8;    // 8-dim tiles of P V
   static constexpr int kWords = D / 32;    // 32-bit words of a lane's V chunk
@@ -68,6 +69,7 @@ struct AttnP {
   int64_t table_stride;
   int capacity;  // tokens that a row of the page table holds
   int pages, page, page_shift, max_pages, kv_heads, seqs, rows, group;
+  uint32_t group_mul;  // ceil(2^32 / group), 0 for group 1
   const uint16_t* q;
   int64_t q_row, q_head;
   uint16_t* out;
@@ -159,9 +161,18 @@ __device__ __forceinline__ Seq load_seq(const AttnP& p, int b) {
   s.past = min(max(p.lengths[b], 0), p.capacity);
   return s;
 }
+// r / group, for r < 2^28: group_mul * group exceeds 2^32 by less than 16.
+__device__ __forceinline__ int by_group(const AttnP& p, int r) {
+  return p.group_mul ? (int)__umulhi((uint32_t)r, p.group_mul) : r;
+}
+// a / b, in 32 bits where a fits them (the 64-bit division is a long call).
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (((uint64_t)a | (uint64_t)b) < (1ull << 32)) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
 // Tokens that query row r (of n * group) of the sequence sees.
 __device__ __forceinline__ int seen(const AttnP& p, const Seq& s, int r) {
-  return min(s.past + r / p.group + 1, p.capacity);
+  return min(s.past + by_group(p, r) + 1, p.capacity);
 }
 __device__ __forceinline__ int row_tiles(const AttnP& p, const Seq& s) {
   return (s.n * p.group + kRows - 1) / kRows;
@@ -175,64 +186,61 @@ __device__ __forceinline__ int64_t seq_work(const AttnP& p, const Seq& s) {
   return s.n > 0 ? (int64_t)p.kv_heads * row_tiles(p, s) * token_tiles(p, s) : 0;
 }
 
-// The line of all tiles: its length, and where tile x lies. Every thread of
-// the CTA calls it.
-struct Place {
-  int b;
-  int64_t off;  // tiles of sequence b before x
+// The CTAs' shares of the line of all tiles: `per` tiles each, the last ones
+// less or none. Every warp works it out by itself, 32 sequences at a time.
+struct Share {
+  int64_t x, end;  // this CTA's tiles
+  int64_t per;     // tiles of a share
+  int b;           // the sequence of tile x
+  int64_t off;     // x's place among the sequence's tiles
 };
 
-__device__ void find_place(const AttnP& p, int64_t* total, int64_t* share0, int64_t* share1,
-                           int* ctas, Place* place) {
-  __shared__ int64_t warp_sum[kWarps];
-  __shared__ Place found;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (p.seqs + kThreads - 1) / kThreads;
-  const int b0 = min(p.seqs, tid * per), b1 = min(p.seqs, b0 + per);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Seq s = load_seq(p, b);
-    mine += seq_work(p, s);
-    if (s.n > 0 && (p.lengths[b] < 0 || p.lengths[b] > p.capacity - s.n))
-      atomicCAS(p.err, 0, kErrKvRange);
-  }
-  int64_t incl = mine;
+__device__ __forceinline__ int64_t scan32(int64_t v, int lane) {
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, incl, off);
-    if (lane >= off) incl += up;
+    const int64_t up = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += up;
   }
-  if (lane == 31) warp_sum[warp] = incl;
-  __syncthreads();
-  int64_t all = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += warp_sum[w];
-    all += warp_sum[w];
-  }
-  const int64_t c = min((int64_t)gridDim.x, (all + kMinTiles - 1) / kMinTiles);
-  *ctas = (int)c;
-  *total = all;
-  if ((int64_t)blockIdx.x >= c) {
-    *share0 = *share1 = all;
-    return;
-  }
-  *share0 = all * blockIdx.x / c;
-  *share1 = all * (blockIdx.x + 1) / c;
-  int64_t at = before + incl - mine;
-  if (*share0 >= at && *share0 < at + mine) {
-    for (int b = b0; b < b1; ++b) {
-      const int64_t w = seq_work(p, load_seq(p, b));
-      if (*share0 < at + w) {
-        found.b = b;
-        found.off = *share0 - at;
-        break;
-      }
-      at += w;
+  return v;
+}
+
+__device__ __forceinline__ Share find_share(const AttnP& p) {
+  const int lane = threadIdx.x & 31;
+  Share f;
+  int64_t all = 0, w = 0;
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.seqs; b0 += 32) {
+    w = 0;
+    if (b0 + lane < p.seqs) {
+      const Seq s = load_seq(p, b0 + lane);
+      w = seq_work(p, s);
+      const int told = p.lengths[b0 + lane];
+      if (s.n > 0 && (told < 0 || told > p.capacity - s.n)) atomicCAS(p.err, 0, kErrKvRange);
     }
+    w = scan32(w, lane);
+    all += __shfl_sync(0xffffffffu, w, 31);
   }
-  __syncthreads();
-  *place = found;
+  f.per = max((int64_t)kMinTiles, divide(all + gridDim.x - 1, gridDim.x));
+  f.x = min(all, f.per * blockIdx.x);
+  f.end = min(all, f.x + f.per);
+  f.b = 0;
+  f.off = 0;
+  if (f.x >= f.end) return f;
+  int64_t before = 0;
+#pragma unroll 1
+  for (int b0 = 0;; b0 += 32) {
+    if (p.seqs > 32)  // else the first pass has left them
+      w = scan32(b0 + lane < p.seqs ? seq_work(p, load_seq(p, b0 + lane)) : 0, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + w > f.x);
+    if (hit || b0 + 32 >= p.seqs) {
+      const int src = hit ? __ffs(hit) - 1 : 31;
+      const int64_t prev = __shfl_sync(0xffffffffu, w, max(src - 1, 0));
+      f.b = min(b0 + src, p.seqs - 1);
+      f.off = f.x - before - (src ? prev : 0);
+      return f;
+    }
+    before += __shfl_sync(0xffffffffu, w, 31);
+  }
 }
 
 // Walks a CTA's share item by item.
@@ -259,8 +267,8 @@ struct Walk {
     }
     nt = token_tiles(p, s);
     const int nrt = row_tiles(p, s);
-    const int64_t item = off / nt;
-    h = (int)(item / nrt);
+    const int64_t item = divide(off, nt);
+    h = (int)divide(item, nrt);
     rt = (int)(item - (int64_t)h * nrt);
     t0 = (int)(off - item * nt);
     t1_full = (int)min((int64_t)nt, t0 + (end - x));
@@ -283,17 +291,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   float* scales = reinterpret_cast<float*>(smem_kv8 + S::kRing) + warp * S::kStages * 4;
   float* merge = reinterpret_cast<float*>(smem_kv8 + S::kRing + S::kScales);
 
+  uint32_t* marks = reinterpret_cast<uint32_t*>(merge + S::kMerge / 4);
+
   grid_launch_dependents();
-  int64_t total, share0, share1;
-  int ctas;
-  Place place;
-  find_place(p, &total, &share0, &share1, &ctas, &place);
+  const Share share = find_share(p);
   if (tid == 0) p.join[blockIdx.x].count = 0;
-  if (share0 >= share1) return;
+  if (share.x >= share.end) return;
+  for (int i = tid; i < S::kMarks / 4; i += kThreads) marks[i] = 0u;
+  __syncthreads();
 
   // ---- the load side: this warp's tiles, kStages - 1 ahead of the compute side
   Walk lw;
-  lw.x = share0, lw.end = share1, lw.b = place.b, lw.off = place.off;
+  lw.x = share.x, lw.end = share.end, lw.b = share.b, lw.off = share.off;
   Walk cw = lw;
   bool more = lw.next(p);
   int lt = more ? lw.t0 + warp : 0;
@@ -363,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int r = r0 + g + 8 * j;
-      const int i = r / p.group;
+      const int i = by_group(p, r);
       const bool in = r < n_rows;
       lim[j] = in ? seen(p, cw.s, r) : 0;
       uint4 raw[D / 32];
@@ -502,7 +511,29 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       // ---- O += P V: a lane's V chunks are dims D/8 g .. of tokens 2t, 2t+1,
       // 2t+8, 2t+9 of each 16; byte pairs of two tokens make the B operand
       const uint32_t vst = st + kTile * D;
-      const bool mixed = tok0 + kTile > low && low < cw.limit;
+      if (tok0 + kTile > low && low < cw.limit) {
+        // Rows of this item end at different tokens here, and a NaN that one row
+        // sees must not reach a row that does not (0 * NaN): NaN codes leave the
+        // tile, and the outputs that they belong to are marked.
+#pragma unroll 1
+        for (int i = lane; i < kTile * D / 16; i += 32) {
+          const int tok = tok0 + i / (D / 16), c = i % (D / 16);
+          const uint32_t at = vst + chunk_at<D>(i / (D / 16), c);
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t v = lds32(at + 4 * w);
+            const uint32_t nan = __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            if (nan == 0u) continue;
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4 * w), "r"(v & ~nan) : "memory");
+            const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) |
+                                   (nan >> 21 & 8u)) << (16 * (c & 1) + 4 * w);
+#pragma unroll 1
+            for (int r = r0; r < min(n_rows, r0 + kRows); ++r)
+              if (tok < seen(p, cw.s, r)) atomicOr(marks + (r - r0) * (D / 32) + (c >> 1), bits);
+          }
+        }
+        __syncwarp();
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t vw[4][S::kWords];
@@ -517,44 +548,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
             asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
                          : "=r"(vw[i][0]), "=r"(vw[i][1])
                          : "r"(at));
-          }
-        }
-        if (mixed) {
-          // Rows of this item end at different tokens here, and a NaN in a
-          // value that one row sees must not reach a row that does not (0 *
-          // NaN): NaN codes leave V, and come back as a product of "row sees
-          // token" with "value is NaN".
-          uint32_t nan_any = 0u;
-          uint32_t nm[4][S::kWords];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int w = 0; w < S::kWords; ++w) {
-              nm[i][w] = __vcmpeq4(vw[i][w] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              vw[i][w] &= ~nm[i][w];
-              nan_any |= nm[i][w];
-            }
-          if (__any_sync(0xffffffffu, nan_any != 0u)) {
-            uint32_t see[4];
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-              const int tok = tok0 + 16 * half + 2 * t + 8 * (a >> 1);
-              const int lr = lim[a & 1];
-              see[a] = (tok < lr ? 0x3c00u : 0u) | (tok + 1 < lr ? 0x3c000000u : 0u);
-            }
-#pragma unroll
-            for (int w = 0; w < S::kWords; ++w)
-#pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                const uint32_t sh = 8 * d;
-                const uint32_t b0 = ((nm[0][w] >> sh) & 1u) * 0x3c00u | ((nm[1][w] >> sh) & 1u) * 0x3c000000u;
-                const uint32_t b1 = ((nm[2][w] >> sh) & 1u) * 0x3c00u | ((nm[3][w] >> sh) & 1u) * 0x3c000000u;
-                float cnt[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_16816<false>(cnt, see[0], see[1], see[2], see[3], b0, b1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (cnt[i] > 0.f) o[4 * w + d][i] = __int_as_float(0x7fffffff);
-              }
           }
         }
 #pragma unroll
@@ -580,176 +573,190 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
-    auto give = [&](float* buf) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float* row = buf + (g + 8 * r) * S::kPitch;
-        if (t == 0) row[D] = m[r], row[D + 1] = l[r];
-#pragma unroll
-        for (int j = 0; j < S::kNTiles; j += 4)
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc)
-            *reinterpret_cast<float4*>(row + (D / 8) * (2 * t + cc) + j) =
-                make_float4(o[j][2 * r + cc], o[j + 1][2 * r + cc], o[j + 2][2 * r + cc],
-                            o[j + 3][2 * r + cc]);
-      }
-    };
-    auto take = [&](const float* buf) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float* row = buf + (g + 8 * r) * S::kPitch;
-        const float om = row[D], ol = row[D + 1];
-        const float nm = fmaxf(m[r], om);
-        const float fa = m[r] == -INFINITY ? 0.f : ex2(m[r] - nm);
-        const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
-        m[r] = nm;
-        l[r] = l[r] * fa + ol * fb;
-#pragma unroll
-        for (int j = 0; j < S::kNTiles; j += 4)
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const float4 v = *reinterpret_cast<const float4*>(row + (D / 8) * (2 * t + cc) + j);
-            o[j][2 * r + cc] = o[j][2 * r + cc] * fa + v.x * fb;
-            o[j + 1][2 * r + cc] = o[j + 1][2 * r + cc] * fa + v.y * fb;
-            o[j + 2][2 * r + cc] = o[j + 2][2 * r + cc] * fa + v.z * fb;
-            o[j + 3][2 * r + cc] = o[j + 3][2 * r + cc] * fa + v.w * fb;
-          }
-      }
-    };
-    __syncthreads();  // the last item's buffers are read
-    if (warp >= 2) give(merge + (warp - 2) * kRows * S::kPitch);
-    __syncthreads();
-    if (warp < 2) take(merge + warp * kRows * S::kPitch);
-    if (warp == 1) {
-      __syncwarp();  // its own buffer is read
-      give(merge + kRows * S::kPitch);
-    }
-    __syncthreads();
-    if (warp == 0) {
-      take(merge + kRows * S::kPitch);
-      if (cw.t0 == 0 && cw.t1_full == cw.nt) {  // the whole item: the output
+    // Two rounds and a last one in which warp 0 leaves the sum: one copy of the
+    // code for all, since code that runs once an item costs its fetch.
+#pragma unroll 1
+    for (int step = 2;; step >>= 1) {
+      __syncthreads();  // the buffers are free
+      if (warp >= step && warp < max(2 * step, 1)) {
+        float* buf = merge + (warp - step) * kRows * S::kPitch;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int row = r0 + g + 8 * r;
-          if (row >= n_rows) continue;
-          const int i = row / p.group;
-          const float inv = l[r] > 0.f || l[r] != l[r] ? 1.0f / l[r] : 0.f;
-          uint16_t* dst = p.out + (int64_t)(cw.s.first + i) * p.out_row +
-                          (int64_t)(cw.h * p.group + row - i * p.group) * p.out_head;
+          float* row = buf + (g + 8 * r) * S::kPitch;
+          if (t == 0) row[D] = m[r], row[D + 1] = l[r];
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc)
+          for (int j = 0; j < S::kNTiles; j += 4)
 #pragma unroll
-            for (int j = 0; j < S::kNTiles; j += 8) {
-              uint32_t w[4];
+            for (int cc = 0; cc < 2; ++cc)
+              *reinterpret_cast<float4*>(row + (D / 8) * (2 * t + cc) + j) =
+                  make_float4(o[j][2 * r + cc], o[j + 1][2 * r + cc], o[j + 2][2 * r + cc],
+                              o[j + 3][2 * r + cc]);
+        }
+      }
+      __syncthreads();
+      if (step == 0) break;
+      if (warp < step) {
+        const float* buf = merge + warp * kRows * S::kPitch;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float a = o[j + 2 * k][2 * r + cc] * inv, b = o[j + 2 * k + 1][2 * r + cc] * inv;
-                if (p.bf16) {
-                  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-                  w[k] = *reinterpret_cast<const uint32_t*>(&v);
-                } else {
-                  w[k] = half2_bits(a, b);
-                }
-              }
-              *reinterpret_cast<uint4*>(dst + (D / 8) * (2 * t + cc) + j) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
+        for (int r = 0; r < 2; ++r) {
+          const float* row = buf + (g + 8 * r) * S::kPitch;
+          const float om = row[D], ol = row[D + 1];
+          const float nm = fmaxf(m[r], om);
+          const float fa = m[r] == -INFINITY ? 0.f : ex2(m[r] - nm);
+          const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
+          m[r] = nm;
+          l[r] = l[r] * fa + ol * fb;
+#pragma unroll
+          for (int j = 0; j < S::kNTiles; j += 4)
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) {
+              const float4 v = *reinterpret_cast<const float4*>(row + (D / 8) * (2 * t + cc) + j);
+              o[j][2 * r + cc] = o[j][2 * r + cc] * fa + v.x * fb;
+              o[j + 1][2 * r + cc] = o[j + 1][2 * r + cc] * fa + v.y * fb;
+              o[j + 2][2 * r + cc] = o[j + 2][2 * r + cc] * fa + v.z * fb;
+              o[j + 3][2 * r + cc] = o[j + 3][2 * r + cc] * fa + v.w * fb;
             }
         }
-      } else {  // a part: left for the second launch
-        float* part = p.parts + ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * kRows * S::kPitch;
-        give(part);
-        // The join is described by the CTA whose share begins at the item's
-        // first inner border: its own share starts inside the item and the
-        // share before does not.
-        if (lane == 0 && cw.t0 > 0) {
-          const int64_t before = total * (blockIdx.x - 1) / ctas;
-          if (before <= cw.item0) {
-            const int64_t end = cw.item0 + cw.nt;
-            int last = blockIdx.x;
-            while (last + 1 < ctas && total * (last + 1) / ctas < end) ++last;
-            Join jn;
-            jn.count = last - (int)blockIdx.x + 2;
-            jn.cta = (int)blockIdx.x - 1;
-            jn.slot = before == cw.item0 ? 0 : 1;
-            jn.row0 = cw.s.first;
-            jn.head0 = cw.h * p.group;
-            jn.r0 = r0;
-            jn.rows = n_rows;
-            jn.pad = 0;
-            p.join[blockIdx.x] = jn;
+      }
+    }
+    // Eight dims of a row a thread: the output of a whole item, or a part that is
+    // left for the second launch.
+    const bool whole = cw.t0 == 0 && cw.t1_full == cw.nt;
+    float* part =
+        p.parts + ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * kRows * S::kPitch;
+#pragma unroll 1
+    for (int e = tid; e < kRows * (D / 8); e += kThreads) {
+      const int rr = e / (D / 8), d = 8 * (e % (D / 8));
+      if (r0 + rr >= n_rows) break;
+      const float* src = merge + rr * S::kPitch;
+      float v[8];
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src + d);
+      *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(src + d + 4);
+      uint8_t* mark = reinterpret_cast<uint8_t*>(marks) + e;  // this thread's alone
+      if (*mark) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (*mark >> k & 1) v[k] = __int_as_float(0x7fffffff);
+        *mark = 0;
+      }
+      if (whole) {
+        const float sum = src[D + 1];
+        const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
+        const int i = by_group(p, r0 + rr);
+        uint16_t* dst = p.out + (int64_t)(cw.s.first + i) * p.out_row +
+                        (int64_t)(cw.h * p.group + r0 + rr - i * p.group) * p.out_head + d;
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = v[2 * k] * inv, b = v[2 * k + 1] * inv;
+          if (p.bf16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            w[k] = *reinterpret_cast<const uint32_t*>(&h);
+          } else {
+            w[k] = half2_bits(a, b);
           }
         }
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+        float* dst = part + rr * S::kPitch;
+        *reinterpret_cast<float4*>(dst + d) = *reinterpret_cast<const float4*>(v);
+        *reinterpret_cast<float4*>(dst + d + 4) = *reinterpret_cast<const float4*>(v + 4);
+        if (d == 0) *reinterpret_cast<float2*>(dst + D) = *reinterpret_cast<const float2*>(src + D);
+      }
+    }
+    if (!whole) {
+      // The join is described by the CTA whose share begins at the item's first
+      // inner border: it starts inside the item and the share before does not.
+      if (tid == 0 && cw.t0 > 0 && share.x - share.per <= cw.item0) {
+        const int last = (int)divide(cw.item0 + cw.nt - 1, share.per);
+        Join jn;
+        jn.count = last - (int)blockIdx.x + 2;
+        jn.cta = (int)blockIdx.x - 1;
+        jn.slot = share.x - share.per == cw.item0 ? 0 : 1;
+        jn.row0 = cw.s.first;
+        jn.head0 = cw.h * p.group;
+        jn.r0 = r0;
+        jn.rows = n_rows;
+        jn.pad = 0;
+        p.join[blockIdx.x] = jn;
       }
     }
     first_segment = false;
+    __syncthreads();  // marks are read before the next item sets any
   }
 }
 
 constexpr int kJoinWarps = 8;
 
-// Joins the partials of one row of an item: blockIdx.x the border, blockIdx.y
-// the row. The warps take the partials in turn, a lane D/32 dims, and warp 0
-// adds the warps in order.
+constexpr int kJoinRows = 4;  // blocks an item (each takes every fourth row)
+
+// Joins the partials of an item: blockIdx.x the border, blockIdx.y the rows.
+// The warps take a row's partials in turn, a lane D/32 dims, and warp 0 adds
+// the warps in order.
 template <int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(const AttnP p) {
   constexpr int V = D / 32, kPitch = AttnShape<D>::kPitch;
   __shared__ float sm[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][D];
   grid_dependency_wait();
   const Join jn = p.join[blockIdx.x];
-  const int row = jn.r0 + blockIdx.y;
-  if (jn.count == 0 || row >= jn.rows) return;
+  if (jn.count == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll 1
+  for (int ri = blockIdx.y; ri < kRows && jn.r0 + ri < jn.rows; ri += kJoinRows) {
+    float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = 0.f;
+    for (int i = 0; i < V; ++i) o[i] = 0.f;
 #pragma unroll 4
-  for (int c = warp; c < jn.count; c += kJoinWarps) {
-    const float* part = p.parts + (((size_t)(jn.cta + c) * 2 + (c == 0 ? jn.slot : 0)) * kRows +
-                                   blockIdx.y) * kPitch;
-    const float om = part[D], ol = part[D + 1];
-    float v[V];
+    for (int c = warp; c < jn.count; c += kJoinWarps) {
+      const float* part =
+          p.parts + (((size_t)(jn.cta + c) * 2 + (c == 0 ? jn.slot : 0)) * kRows + ri) * kPitch;
+      const float om = part[D], ol = part[D + 1];
+      float v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = part[V * lane + i];
-    const float nm = fmaxf(m, om);
-    const float fa = m == -INFINITY ? 0.f : ex2(m - nm);
-    const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
-    m = nm;
-    l = l * fa + ol * fb;
+      for (int i = 0; i < V; ++i) v[i] = part[V * lane + i];
+      const float nm = fmaxf(m, om);
+      const float fa = m == -INFINITY ? 0.f : ex2(m - nm);
+      const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
+      m = nm;
+      l = l * fa + ol * fb;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = o[i] * fa + v[i] * fb;
-  }
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-  for (int i = 0; i < V; ++i) so[warp][V * lane + i] = o[i];
-  __syncthreads();
-  if (warp != 0) return;
-  m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sm[w]);
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = 0.f;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    const float f = sm[w] == -INFINITY ? 0.f : ex2(sm[w] - m);
-    l += sl[w] * f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] += so[w][V * lane + i] * f;
-  }
-  const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-  const int i = row / p.group;
-  uint16_t* dst = p.out + (int64_t)(jn.row0 + i) * p.out_row +
-                  (int64_t)(jn.head0 + row - i * p.group) * p.out_head + V * lane;
-#pragma unroll
-  for (int k = 0; k < V; k += 2) {
-    uint32_t w;
-    if (p.bf16) {
-      const __nv_bfloat162 v = __floats2bfloat162_rn(o[k] * inv, o[k + 1] * inv);
-      w = *reinterpret_cast<const uint32_t*>(&v);
-    } else {
-      w = half2_bits(o[k] * inv, o[k + 1] * inv);
+      for (int i = 0; i < V; ++i) o[i] = o[i] * fa + v[i] * fb;
     }
-    *reinterpret_cast<uint32_t*>(dst + k) = w;
+    if (lane == 0) sm[warp] = m, sl[warp] = l;
+#pragma unroll
+    for (int i = 0; i < V; ++i) so[warp][V * lane + i] = o[i];
+    __syncthreads();
+    if (warp == 0) {
+      m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sm[w]);
+      l = 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = sm[w] == -INFINITY ? 0.f : ex2(sm[w] - m);
+        l += sl[w] * f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] += so[w][V * lane + i] * f;
+      }
+      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+      const int row = jn.r0 + ri, i = by_group(p, row);
+      uint16_t* dst = p.out + (int64_t)(jn.row0 + i) * p.out_row +
+                      (int64_t)(jn.head0 + row - i * p.group) * p.out_head + V * lane;
+#pragma unroll
+      for (int k = 0; k < V; k += 2) {
+        uint32_t w;
+        if (p.bf16) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(o[k] * inv, o[k + 1] * inv);
+          w = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          w = half2_bits(o[k] * inv, o[k + 1] * inv);
+        }
+        *reinterpret_cast<uint32_t*>(dst + k) = w;
+      }
+    }
+    __syncthreads();  // the shared sums are read
   }
 }
 
@@ -765,7 +772,7 @@ int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "w4_kv8_attention launch");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)max_rows);
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)std::min(max_rows, kJoinRows));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute at;
@@ -820,6 +827,7 @@ int launch_kv8_attention(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_
   p.seqs = bt.seqs;
   p.rows = bt.rows;
   p.group = q.heads / c.kv_heads;
+  p.group_mul = p.group > 1 ? (uint32_t)(((1ull << 32) + p.group - 1) / p.group) : 0u;
   p.q = static_cast<const uint16_t*>(q.ptr);
   p.q_row = q.row_stride;
   p.q_head = q.head_stride;

@@ -223,8 +223,8 @@ w4_kv_batch batch_desc(const Tensor& table, const Tensor& lengths, const Tensor&
       (lengths.size(0) > 1 && lengths.stride(0) != 1) ||
       (row_starts.size(0) > 1 && row_starts.stride(0) != 1))
     refuse("page_table's rows, lengths and row_starts must be contiguous");
-  if (lengths.size(0) > 0x7ffffffe || table.size(1) > 0x7fffffff || rows > (1 << 26))
-    refuse("a step takes at most 2^26 rows, got ", rows);
+  if (lengths.size(0) > 0x7ffffffe || table.size(1) > 0x7fffffff || rows > (1 << 24))
+    refuse("a step takes at most 2^24 rows, got ", rows);
   return w4_kv_batch{static_cast<const int32_t*>(ptr(table)), table.stride(0), (int)table.size(1),
                      static_cast<const int32_t*>(ptr(lengths)),
                      static_cast<const int32_t*>(ptr(row_starts)), (int)lengths.size(0), (int)rows};

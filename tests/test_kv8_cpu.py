@@ -44,7 +44,7 @@ BAD_CACHE = [(cache(k=None), 1), (cache(v_scale=None), 1), (cache(pages=0), 1), 
              (cache(page_size=48), 3), (cache(page_size=256), 3), (cache(head_dim=96), 3),
              (cache(v=FAKE + 8), 2)]
 BAD_BATCH = [(batch(page_table=None), 1), (batch(lengths=None), 1), (batch(row_starts=None), 1),
-             (batch(seqs=-1), 1), (batch(rows=-1), 1), (batch(rows=(1 << 26) + 1), 1),
+             (batch(seqs=-1), 1), (batch(rows=-1), 1), (batch(rows=(1 << 24) + 1), 1),
              (batch(max_pages=0), 1), (batch(table_stride=-1), 1)]
 
 
