@@ -330,15 +330,9 @@ int w4_gemm(const void* x, int x_dtype, const int32_t* packed, const void* scale
   return w4_gemm_ex(x, x_dtype, packed, scales, y, y_dtype, M, K, N, 0, stream);
 }
 
-int w4_gemm_ex(const void* x, int x_dtype, const int32_t* packed, const void* scales, void* y,
-               int y_dtype, int M, int K, int N, int split_k, void* stream) {
-  const w4_gemm_ops none{};
-  return w4_gemm_fused(x, x_dtype, packed, scales, y, y_dtype, M, K, N, &none, split_k, stream);
-}
-
-int w4_gemm_fused(const void* x, int x_dtype, const int32_t* packed, const void* scales, void* y,
-                  int y_dtype, int M, int K, int N, const w4_gemm_ops* ops, int split_k,
-                  void* stream) {
+static int gemm_call(const void* x, int x_dtype, const int32_t* packed, const void* scales, void* y,
+                     int y_dtype, int M, int K, int N, const w4_gemm_ops& ops, int split_k,
+                     bool few_tiles, void* stream) {
   if (!x || !packed || !scales || !y) return fail(W4_ERR_INVALID_ARG, "w4_gemm: null pointer");
   if (split_k < 0 || split_k > 8 || (split_k > 0 && split_k > K / 64))
     return fail(W4_ERR_INVALID_ARG, "w4_gemm: split_k=%d (0 = choose, else 1..8 and <= K/64)",
@@ -351,13 +345,25 @@ int w4_gemm_fused(const void* x, int x_dtype, const int32_t* packed, const void*
                 "w4_gemm: M=%d K=%d N=%d (M >= 1, K and N multiples of 128)", M, K, N);
   if (!aligned16(x) || !aligned16(packed) || !aligned16(scales) || !aligned16(y))
     return fail(W4_ERR_ALIGNMENT, "w4_gemm: pointers must be 16-byte aligned");
-  if (!ops) return fail(W4_ERR_INVALID_ARG, "w4_gemm: null ops");
-  if (ops->act < W4_ACT_NONE || ops->act > W4_ACT_SWIGLU)
-    return fail(W4_ERR_INVALID_ARG, "w4_gemm: activation %d unknown", ops->act);
-  if ((ops->bias && !aligned16(ops->bias)) || (ops->residual && !aligned16(ops->residual)))
+  if (ops.act < W4_ACT_NONE || ops.act > W4_ACT_SWIGLU)
+    return fail(W4_ERR_INVALID_ARG, "w4_gemm: activation %d unknown", ops.act);
+  if ((ops.bias && !aligned16(ops.bias)) || (ops.residual && !aligned16(ops.residual)))
     return fail(W4_ERR_ALIGNMENT, "w4_gemm: bias and residual must be 16-byte aligned");
-  return launch_gemm(x, x_dtype == W4_BF16, packed, scales, y, y_dtype == W4_BF16, M, K, N, *ops,
-                     split_k, (cudaStream_t)stream);
+  return launch_gemm(x, x_dtype == W4_BF16, packed, scales, y, y_dtype == W4_BF16, M, K, N, ops,
+                     split_k, few_tiles, (cudaStream_t)stream);
+}
+
+int w4_gemm_ex(const void* x, int x_dtype, const int32_t* packed, const void* scales, void* y,
+               int y_dtype, int M, int K, int N, int split_k, void* stream) {
+  return gemm_call(x, x_dtype, packed, scales, y, y_dtype, M, K, N, w4_gemm_ops{}, split_k, false,
+                   stream);
+}
+
+int w4_gemm_fused(const void* x, int x_dtype, const int32_t* packed, const void* scales, void* y,
+                  int y_dtype, int M, int K, int N, const w4_gemm_ops* ops, int split_k,
+                  void* stream) {
+  if (!ops) return fail(W4_ERR_INVALID_ARG, "w4_gemm_fused: null ops");
+  return gemm_call(x, x_dtype, packed, scales, y, y_dtype, M, K, N, *ops, split_k, true, stream);
 }
 
 // ---------------------------------------------------------------- batched attention

@@ -6,13 +6,14 @@
 // fp16 [K, N] copy of the weights, roofline/kernels.py:77-90) followed by an
 // fp32 matmul (scripts/decode_loop.py:51-55). Here the dequantised tile never
 // leaves shared memory:
-//   TMA warp     : X tiles [up to 256 rows x 64 k] (128B swizzle, the
-//                  canonical K-major layout the MMA reads) and the packed
-//                  words and scales of the W tile (128 or 256 columns),
-//                  through a 3-slot ring;
+//   TMA warps    : one brings X tiles [up to 256 rows x 64 k] (128B swizzle,
+//                  the canonical K-major layout the MMA reads), the other the
+//                  packed words of the W tile (128 or 256 columns), each through a ring of its own: words leave as soon as they
+//                  are unpacked, so the dequantisation runs ahead of the MMA
+//                  and no load's latency waits for an MMA's;
 //   8 dequant warps: expand each packed word into 8 fp16 (q - 8) * s values
 //                  - bit-identical to dequantize_v1 - and write them K-major,
-//                  128B-swizzled, into one of three B buffers;
+//                  128B-swizzled, into one of the B buffers;
 //   MMA warp     : one thread issues tcgen05.mma (M = 128, N = 128 or 256,
 //                  K = 16, fp32 accumulate in tensor memory), four per 64-k
 //                  stage for each of the tile's one or two 128-row halves
@@ -28,7 +29,7 @@
 // frees its tensor memory.
 //
 // Work split: a launch covers a region of output tiles in row-major order
-// (blockIdx.x) and may cut K into up to 16 slices (blockIdx.z), the slices of
+// (blockIdx.x) and may cut K into up to 8 slices (blockIdx.z), the slices of
 // a tile forming a thread-block cluster. A sliced CTA leaves its fp32
 // accumulators in shared memory (the freed operand rings) and every rank then
 // sums a band of the tile's rows over all ranks in rank order (DSMEM), so the
@@ -52,10 +53,10 @@ namespace {
 constexpr int kUM = 128;          // MMA M (rows of one accumulator)
 constexpr int kBMMax = 2 * kUM;   // rows of Y per CTA: up to two accumulators share a W tile
 constexpr int kBK = 64;           // k per ring stage (one 128-byte swizzle row of fp16)
-constexpr int kBStages = 3;       // dequantised W buffers
 constexpr int kDqWarps = 8;       // dequant (and epilogue) warps
 constexpr int kMmaWarp = 1 + kDqWarps;
-constexpr int kGemmThreads = 32 * (kMmaWarp + 1);  // warp 0 TMA, 1..8 dequant, 9 MMA
+constexpr int kPackedWarp = kMmaWarp + 1;
+constexpr int kGemmThreads = 32 * (kPackedWarp + 1);  // warp 0 X, 1..8 dequant, 9 MMA, 10 W
 constexpr int kErrGemmWait = 7;
 
 struct GemmParams {
@@ -67,6 +68,7 @@ struct GemmParams {
   // n_tile0 + t % ntx) in units of the instance's rows and columns
   int m_tile0, n_tile0, ntx;
   int ksplit;       // K slices (gridDim.z, one cluster per tile when > 1)
+  const uint16_t* scales;  // fp16 [K/128, N]
   int act;               // w4_act
   const void* bias;      // [N] of y's type, or null
   const void* residual;  // like y, or null
@@ -75,35 +77,42 @@ struct GemmParams {
 };
 
 // Tile of BN columns (MMA N = BN, 128 or 256) and its shared memory layout
-// (base 1024-aligned): X ring, B buffers, packed ring, scale ring, then the
-// barriers and the tensor-memory address.
+// (base 1024-aligned): X ring, B buffers, packed ring, then the barriers and the tensor-memory address. The rings take what the 227 KB hold.
 template <int BN, int NACC>
 struct GemmShape {
-  // TMA ring: 3 slots of 32 KB X tiles with two accumulators; 4 slots of
-  // 16 KB with one (the same bytes in flight, one more stage of latency cover)
-  static constexpr int kStages = NACC == 1 ? 4 : 3;
-  static constexpr int kNumBars = 2 * kStages + 2 * kBStages + 1;
+  // A stage: an X tile and a dequantised W tile. One barrier says that both
+  // are there (the X copy's bytes and the dequant warps' arrivals), one that
+  // the MMA has read both: the issuing thread's own instructions bound a stage
+  // of few MMAs (each wait costs it about 130 clocks, each commit 70).
+  static constexpr int kStages = BN == 128 ? (NACC == 1 ? 6 : 4) : (NACC == 1 ? 4 : 3);
+  // The dequant warps work as two groups that take the stages in turn: a
+  // stage's chain (wait, shared loads, unpack, shared stores, proxy fence,
+  // arrival) is latency, not issue slots. The rings are then even, so that a
+  // slot belongs to one group, which sees its phases one after another (a
+  // parity wait cannot tell a phase from the next but one); three stages of the
+  // largest tile are left to all warps together.
+  static constexpr int kGroups = kStages % 2 == 0 ? 2 : 1;
+  static constexpr int kGroupWarps = kDqWarps / kGroups;
+  static constexpr int kPkStages = BN == 128 ? 6 : 4;
+  static constexpr int kNumBars = 2 * kStages + 2 * kPkStages + 1;
   static constexpr int kBM = NACC * kUM;                 // rows of Y per CTA
   static constexpr int kXBytes = kBM * kBK * 2;          // 16 or 32 KB
   static constexpr int kBBytes = BN * kBK * 2;           // 16 or 32 KB
   static constexpr int kPkBytes = (kBK / 8) * BN * 4;    // packed words of a stage
-  static constexpr int kScBytes = BN * 2;                // scales of a stage
   static constexpr int kTmemCols = NACC * BN;            // fp32 accumulators
   static constexpr int kOffX = 0;
   static constexpr int kOffB = kOffX + kStages * kXBytes;
-  static constexpr int kOffPk = kOffB + kBStages * kBBytes;
-  static constexpr int kOffSc = kOffPk + kStages * kPkBytes;
-  static constexpr int kOffBar = kOffSc + kStages * kScBytes;
+  static constexpr int kOffPk = kOffB + kStages * kBBytes;
+  static constexpr int kOffBar = kOffPk + kPkStages * kPkBytes;
   static constexpr int kOffTmem = kOffBar + kNumBars * 8;
   static constexpr int kSmem = 1024 + kOffTmem + 16;
-  static constexpr int kThreadsPerCol = kDqWarps * 32 / BN;  // dequant threads per column
-  static constexpr int kWordsPerThread = (kBK / 8) / kThreadsPerCol;
+  static constexpr int kColsPerThread = BN / (kGroupWarps * 32);  // of a group's stage
+  static_assert(kSmem <= 227 * 1024 && kPkStages % kGroups == 0, "rings");
   static_assert(kOffB % 1024 == 0 && kXBytes % 1024 == 0 && kBBytes % 1024 == 0,
                 "swizzled operand tiles start on 1024-byte boundaries");
-  static_assert(kOffPk % 128 == 0 && kOffSc % 128 == 0 && kPkBytes % 128 == 0 &&
-                    kScBytes % 128 == 0,
+  static_assert(kOffPk % 128 == 0 && kPkBytes % 128 == 0,
                 "tensor-copy destinations are 128-byte aligned");
-  static_assert(kTmemCols <= 512 && kWordsPerThread * kThreadsPerCol == kBK / 8, "tile");
+  static_assert(kTmemCols <= 512 && kColsPerThread * kGroupWarps * 32 == BN, "tile");
   // K slices: the fp32 partial tile (rows padded by 4 floats against bank
   // conflicts) reuses the X and B rings, free once the accumulators are final
   static constexpr int kPitch = BN + 4;
@@ -126,6 +135,11 @@ __device__ __forceinline__ uint64_t kmajor_sw128_desc(uint32_t smem_addr) {
   d |= (uint64_t)2u << 61;
   return d;
 }
+// The descriptor of the operand `bytes` further (shared addresses stay below
+// 2^18, so the 14-bit field does not overflow).
+__device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t bytes) {
+  return d + (bytes >> 4);
+}
 
 // Instruction descriptor of kind::f16: fp32 accumulate, A and B of one type
 // (0 fp16, 1 bf16), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
@@ -139,10 +153,9 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a, uint64_t b
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :
-      : "r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u),
-        "r"(0u)
+      : "r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -268,11 +281,11 @@ __device__ __forceinline__ void store_row(void* p, size_t at, int bf16, const fl
 
 __device__ __forceinline__ float silu(float a) { return __fdividef(a, 1.0f + __expf(-a)); }
 
-// NV accumulators of columns n.. of one row (u: the up columns, 32 further, of
-// a gated pair) to NV outputs.
+// Bias and activation of NV accumulators of columns n.. of a row (u: the up
+// columns, 32 further, of a gated pair).
 template <int NV>
-__device__ __forceinline__ void finish(const GemmParams& p, int row, int n, float (&a)[NV],
-                                       float (&u)[NV]) {
+__device__ __forceinline__ void activate(const GemmParams& p, int n, float (&a)[NV],
+                                         float (&u)[NV]) {
   const bool gated = p.act == W4_ACT_SWIGLU;
   if (p.bias) {
     float b[NV];
@@ -297,32 +310,36 @@ __device__ __forceinline__ void finish(const GemmParams& p, int row, int n, floa
 #pragma unroll
     for (int i = 0; i < NV; ++i) a[i] = 0.5f * a[i] * erfcf(a[i] * -0.70710678118654752f);
   }
-  // gate column 64 j + i is output column 32 j + i
+}
+
+// Where column n of a row goes: gate column 64 j + i is output column 32 j + i.
+__device__ __forceinline__ size_t out_at(const GemmParams& p, int row, int n) {
+  const bool gated = p.act == W4_ACT_SWIGLU;
   const int col = gated ? (n >> 6) * W4B200_SWIGLU_BLOCK + (n & (W4B200_SWIGLU_BLOCK - 1)) : n;
-  const size_t at = (size_t)row * (gated ? p.N / 2 : p.N) + col;
-  if (p.residual) {
-    float r[NV];
-    load_row(p.residual, at, p.y_bf16, r);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) a[i] += r[i];
-  }
-  store_row(p.y, at, p.y_bf16, a);
+  return (size_t)row * (gated ? p.N / 2 : p.N) + col;
+}
+
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
 template <bool kBF16, int BN, int NACC>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     w4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                   const __grid_constant__ CUtensorMap tm_s, const GemmParams p) {
+                   const GemmParams p) {
   using S = GemmShape<BN, NACC>;
   extern __shared__ uint8_t smem_gemm[];
   uint8_t* base = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_gemm) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar);
-  uint64_t* full_tma = bars;                       // X + packed + scales landed
-  uint64_t* empty_tma = full_tma + S::kStages;        // dequant read the words, MMA read X
-  uint64_t* full_b = empty_tma + S::kStages;          // B buffer written
-  uint64_t* empty_b = full_b + kBStages;           // MMA read the B buffer
-  uint64_t* acc_full = empty_b + kBStages;         // accumulator final
+  uint64_t* full = bars;                           // X landed, W dequantised
+  uint64_t* empty = full + S::kStages;             // the MMA has read both
+  uint64_t* full_pk = empty + S::kStages;          // packed words landed
+  uint64_t* empty_pk = full_pk + S::kPkStages;     // unpacked
+  uint64_t* acc_full = empty_pk + S::kPkStages;    // accumulator final
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + S::kOffTmem);
   int* abort_flag = reinterpret_cast<int*>(base + S::kOffTmem + 4);
 
@@ -335,18 +352,31 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int KT = (int)((long long)(blockIdx.z + 1) * KT_all / p.ksplit) - kt0;
   grid_launch_dependents();  // a dependent launch may fill the SMs this grid frees
 
+  auto load_x = [&](int kt) {
+    const int s = kt % S::kStages;
+    mbar_arrive_expect_tx(&full[s], S::kXBytes);
+    tma_load_2d(base + S::kOffX + s * S::kXBytes, &tm_x, &full[s], (kt0 + kt) * kBK, m0);
+  };
+  auto load_w = [&](int kt) {
+    const int s = kt % S::kPkStages;
+    mbar_arrive_expect_tx(&full_pk[s], S::kPkBytes);
+    tma_load_2d(base + S::kOffPk + s * S::kPkBytes, &tm_w, &full_pk[s], n0, (kt0 + kt) * (kBK / 8));
+  };
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&full_tma[i], 1);
-      mbar_init(&empty_tma[i], kDqWarps + 1);  // the dequant warps + the MMA commit
+      mbar_init(&full[i], S::kGroupWarps + 1);
+      mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < kBStages; ++i) {
-      mbar_init(&full_b[i], kDqWarps);
-      mbar_init(&empty_b[i], 1);
+    for (int i = 0; i < S::kPkStages; ++i) {
+      mbar_init(&full_pk[i], 1);
+      mbar_init(&empty_pk[i], S::kGroupWarps);
     }
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     fence_mbar_init();
+    // the first copies go out while the other warps still set up
+    for (int kt = 0; kt < min(S::kPkStages, KT); ++kt) load_w(kt);
+    for (int kt = 0; kt < min(S::kStages, KT); ++kt) load_x(kt);
   }
   if (warp == kMmaWarp) {  // tensor memory for the two 128 x 128 fp32 accumulators
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -366,139 +396,189 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   auto stopped = [&]() { return *reinterpret_cast<volatile int*>(abort_flag) != 0; };
 
   if (warp == 0) {
-    // ------------------------------------------------------------ TMA
+    // ------------------------------------------------------------ X
     if (lane == 0) {
-      tma_prefetch_desc(&tm_x);
-      tma_prefetch_desc(&tm_w);
-      tma_prefetch_desc(&tm_s);
-      int issued = 0;
-      for (int kt = 0; kt < KT; ++kt) {
-        const int s = kt % S::kStages;
-        if (kt >= S::kStages && !mbar_wait(&empty_tma[s], ((kt / S::kStages) & 1) ^ 1u)) {
+      int issued = min(S::kStages, KT);
+      for (int kt = issued; kt < KT; ++kt) {
+        if (!mbar_wait(&empty[kt % S::kStages], ((kt / S::kStages) & 1) ^ 1u)) {
           give_up(kErrGemmWait);
           break;
         }
         if (stopped()) break;
-        mbar_arrive_expect_tx(&full_tma[s], S::kXBytes + S::kPkBytes + S::kScBytes);
-        const int kg = kt0 + kt;  // stage of the whole K
-        tma_load_2d(base + S::kOffX + s * S::kXBytes, &tm_x, &full_tma[s], kg * kBK, m0);
-        tma_load_2d(base + S::kOffPk + s * S::kPkBytes, &tm_w, &full_tma[s], n0, kg * (kBK / 8));
-        tma_load_2d(base + S::kOffSc + s * S::kScBytes, &tm_s, &full_tma[s], n0, (kg * kBK) / 128);
+        load_x(kt);
         ++issued;
       }
-      for (int j = issued - S::kStages > 0 ? issued - S::kStages : 0; j < issued; ++j)
-        if (!mbar_wait(&full_tma[j % S::kStages], (j / S::kStages) & 1)) give_up(kErrDrainWait);
+      for (int j = max(issued - S::kStages, 0); j < issued; ++j)  // no copy left in flight
+        if (!mbar_wait(&full[j % S::kStages], (j / S::kStages) & 1)) give_up(kErrDrainWait);
+    }
+  } else if (warp == kPackedWarp) {
+    // ------------------------------------------------------------ W
+    if (lane == 0) {
+      int issued = min(S::kPkStages, KT);  // thread 0 issued these
+      for (int kt = issued; kt < KT; ++kt) {
+        if (!mbar_wait(&empty_pk[kt % S::kPkStages], ((kt / S::kPkStages) & 1) ^ 1u)) {
+          give_up(kErrGemmWait);
+          break;
+        }
+        if (stopped()) break;
+        load_w(kt);
+        ++issued;
+      }
+      for (int j = max(issued - S::kPkStages, 0); j < issued; ++j)
+        if (!mbar_wait(&full_pk[j % S::kPkStages], (j / S::kPkStages) & 1)) give_up(kErrDrainWait);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA
     if (lane == 0) {
       constexpr uint32_t idesc = f16_idesc(kBF16 ? 1 : 0, kUM, BN);
-      int done = 0;
-      for (int kt = 0; kt < KT && !stopped(); ++kt) {
-        const int s = kt % S::kStages, sb = kt % kBStages;
-        if (!mbar_wait(&full_tma[s], (kt / S::kStages) & 1) ||
-            !mbar_wait(&full_b[sb], (kt / kBStages) & 1)) {
+      const uint64_t xd0 = kmajor_sw128_desc(smem_u32(base + S::kOffX));
+      const uint64_t bd0 = kmajor_sw128_desc(smem_u32(base + S::kOffB));
+      for (int kt = 0; kt < KT; ++kt) {
+        const int s = kt % S::kStages;
+        if (!mbar_wait(&full[s], (kt / S::kStages) & 1)) {
           give_up(kErrGemmWait);
           break;
         }
         tc_fence_after();
-        const uint32_t xa = smem_u32(base + S::kOffX + s * S::kXBytes);
-        const uint32_t ba = smem_u32(base + S::kOffB + sb * S::kBBytes);
+        const uint64_t xd = desc_at(xd0, s * S::kXBytes), bd = desc_at(bd0, s * S::kBBytes);
 #pragma unroll
-        for (int kk = 0; kk < kBK / 16; ++kk) {  // 16 k = 32 bytes along the swizzled row
-          const uint64_t bd = kmajor_sw128_desc(ba + kk * 32);
-          const uint32_t acc = (kt > 0 || kk > 0) ? 1u : 0u;
+        for (int kk = 0; kk < kBK / 16; ++kk)  // 16 k = 32 bytes along the swizzled row
           // accumulator a: rows 128a.. (16 KB further per 128 rows), columns a*BN..
 #pragma unroll
           for (int a = 0; a < NACC; ++a)
-            umma_f16(tmem_d + a * BN, kmajor_sw128_desc(xa + a * kUM * 128 + kk * 32), bd, idesc,
-                     acc);
-        }
-        umma_commit(&empty_tma[s]);
-        umma_commit(&empty_b[sb]);
-        ++done;
+            umma_f16(tmem_d + a * BN, desc_at(xd, a * kUM * 128 + kk * 32), desc_at(bd, kk * 32),
+                     idesc, kk > 0 ? 1u : (uint32_t)(kt > 0));
+        umma_commit(&empty[s]);
       }
       umma_commit(acc_full);  // after every issued MMA (also when none was issued)
-      (void)done;
     }
   } else {
     // ------------------------------------------------------------ dequant
-    const int dt = threadIdx.x - 32;
-    const int n = dt % BN;                                  // column of the tile
-    const int jh = (dt / BN) * S::kWordsPerThread;          // this thread's words of the column
-    for (int kt = 0; kt < KT && !stopped(); ++kt) {
-      const int s = kt % S::kStages, sb = kt % kBStages;
-      if (!mbar_wait(&full_tma[s], (kt / S::kStages) & 1) ||
-          (kt >= kBStages && !mbar_wait(&empty_b[sb], ((kt / kBStages) & 1) ^ 1u))) {
+    constexpr int kGroupThreads = S::kGroupWarps * 32;
+    const int group = (warp - 1) / S::kGroupWarps;
+    const int dt = threadIdx.x - 32 - group * kGroupThreads;
+    // this thread's scales come straight from global memory, a stage ahead
+    uint16_t next[S::kColsPerThread];
+    auto load_scales = [&](int kt) {
+#pragma unroll
+      for (int c = 0; c < S::kColsPerThread; ++c) {
+        const int n = n0 + dt + c * kGroupThreads;
+        next[c] = kt < KT && n < p.N
+                      ? __ldg(p.scales + (size_t)((kt0 + kt) * kBK / 128) * p.N + n)
+                      : (uint16_t)0;
+      }
+    };
+    load_scales(group);
+    // the epilogue's bias and residual on their way into the caches
+    const int q = warp & 3;           // this warp's 32-lane slice of tensor memory
+    const int half = (warp - 1) / 4;  // which accumulator (rows 0..127 or 128..255)
+    const int tile_row = half * kUM + 32 * q + lane, row = m0 + tile_row;
+    const bool has_row = half < NACC && row < p.M;
+    if (p.bias && dt < BN / 64 && n0 + 64 * dt < p.N)
+      prefetch_l1(static_cast<const uint16_t*>(p.bias) + n0 + 64 * dt);
+    if (p.residual && has_row)
+      for (int c = 0; c < BN && n0 + c < p.N; c += p.act == W4_ACT_SWIGLU ? 128 : 64)
+        prefetch_l2(static_cast<const uint16_t*>(p.residual) + out_at(p, row, n0 + c));
+    for (int kt = group; kt < KT; kt += S::kGroups) {
+      const int s = kt % S::kPkStages, sb = kt % S::kStages;
+      if (!mbar_wait(&full_pk[s], (kt / S::kPkStages) & 1) ||
+          (kt >= S::kStages && !mbar_wait(&empty[sb], ((kt / S::kStages) & 1) ^ 1u))) {
         give_up(kErrGemmWait);
         break;
       }
       const uint32_t* pk = reinterpret_cast<const uint32_t*>(base + S::kOffPk + s * S::kPkBytes);
-      const uint16_t sbits = reinterpret_cast<const uint16_t*>(base + S::kOffSc + s * S::kScBytes)[n];
-      const uint32_t s2 = (uint32_t)sbits | ((uint32_t)sbits << 16);
-      const float sf = __half2float(__ushort_as_half(sbits));
-      uint8_t* brow = base + S::kOffB + sb * S::kBBytes + n * 128;  // row n: 64 k of column n
-      uint32_t wv[S::kWordsPerThread];
+      uint16_t now[S::kColsPerThread];
 #pragma unroll
-      for (int j = 0; j < S::kWordsPerThread; ++j) wv[j] = pk[(jh + j) * BN + n];
+      for (int c = 0; c < S::kColsPerThread; ++c) now[c] = next[c];
+      load_scales(kt + S::kGroups);
 #pragma unroll
-      for (int j = 0; j < S::kWordsPerThread; ++j)  // chunk j lands at chunk j ^ (row % 8)
-        *reinterpret_cast<uint4*>(brow + (((jh + j) ^ (n & 7)) << 4)) =
-            dequant_word<kBF16>(wv[j], s2, sf);
+      for (int c = 0; c < S::kColsPerThread; ++c) {
+        const int n = dt + c * kGroupThreads;  // column of the tile
+        const uint16_t sbits = now[c];
+        const uint32_t s2 = (uint32_t)sbits | ((uint32_t)sbits << 16);
+        const float sf = __half2float(__ushort_as_half(sbits));
+        uint8_t* brow = base + S::kOffB + sb * S::kBBytes + n * 128;  // row n: 64 k of column n
+        uint32_t wv[kBK / 8];
+#pragma unroll
+        for (int j = 0; j < kBK / 8; ++j) wv[j] = pk[j * BN + n];
+#pragma unroll
+        for (int j = 0; j < kBK / 8; ++j)  // chunk j lands at chunk j ^ (row % 8)
+          *reinterpret_cast<uint4*>(brow + ((j ^ (n & 7)) << 4)) =
+              dequant_word<kBF16>(wv[j], s2, sf);
+      }
       fence_async_shared();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&full_b[sb]);
-        mbar_arrive(&empty_tma[s]);
+        mbar_arrive(&full[sb]);
+        mbar_arrive(&empty_pk[s]);
       }
     }
     // ------------------------------------------------------------ epilogue
+    const bool gated = p.act == W4_ACT_SWIGLU;
+    const int step = gated ? 2 : 1;  // 32-column blocks a turn
+    uint4 res[4];                    // the next turn's residual, a turn ahead of its use
+    auto load_residual = [&](int c) {
+      if (c < BN / 32 && p.residual && has_row && n0 + 32 * c < p.N) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            static_cast<const uint16_t*>(p.residual) + out_at(p, row, n0 + 32 * c));
+#pragma unroll
+        for (int v = 0; v < 4; ++v) res[v] = src[v];
+      }
+    };
+    if (p.ksplit == 1) load_residual(0);
     if (!mbar_wait(acc_full, 0)) give_up(kErrGemmWait);
     tc_fence_after();
+    const uint32_t acc = tmem_d + ((uint32_t)(32 * q) << 16) + half * BN;
     if (p.ksplit > 1) {
       // K slice: this warp's 32 rows of its accumulator -> the fp32 partial tile
       if constexpr (S::kCanSplit) {
-        const int q = warp & 3, half = (warp - 1) / 4;
-        if (!stopped() && half < NACC) {
-          float* prow = reinterpret_cast<float*>(base) + (size_t)(half * kUM + 32 * q + lane) * S::kPitch;
+        if (!stopped() && half < NACC && m0 + tile_row - lane < p.M) {
+          float* prow = reinterpret_cast<float*>(base) + (size_t)tile_row * S::kPitch;
 #pragma unroll 1
           for (int c = 0; c < BN / 32; ++c) {
             uint32_t r[32];
-            tmem_ld32(tmem_d + ((uint32_t)(32 * q) << 16) + half * BN + 32 * c, r);
+            tmem_ld32(acc + 32 * c, r);
+            if (has_row) {
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<uint4*>(prow + 32 * c + 4 * v) =
-                  make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+              for (int v = 0; v < 8; ++v)
+                *reinterpret_cast<uint4*>(prow + 32 * c + 4 * v) =
+                    make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
+            }
           }
         }
       }
-    } else if (!stopped()) {
-      const int q = warp & 3;            // this warp's 32-lane slice of tensor memory
-      const int half = (warp - 1) / 4;   // which accumulator (rows 0..127 or 128..255)
-      if (half >= NACC) goto epilogue_done;
-      const int row = m0 + half * kUM + 32 * q + lane;
-const uint32_t acc = tmem_d + ((uint32_t)(32 * q) << 16) + half * BN;
-      const int step = p.act == W4_ACT_SWIGLU ? 2 : 1;  // 32-column blocks a turn
+    } else if (!stopped() && half < NACC && m0 + tile_row - lane < p.M) {
 #pragma unroll 1
       for (int c = 0; c < BN / 32; c += step) {
         uint32_t r[32], ru[32];
         tmem_ld32(acc + 32 * c, r);
-        if (step == 2) tmem_ld32(acc + 32 * c + 32, ru);
-        if (row < p.M && n0 + 32 * c < p.N) {
+        if (gated) tmem_ld32(acc + 32 * c + 32, ru);
+        uint4 now[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) now[v] = res[v];
+        load_residual(c + step);
+        if (has_row && n0 + 32 * c < p.N) {
+          const size_t at = out_at(p, row, n0 + 32 * c);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             float a[8], u[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               a[e] = __uint_as_float(r[8 * v + e]);
-              u[e] = __uint_as_float(ru[8 * v + e]);
+              u[e] = gated ? __uint_as_float(ru[8 * v + e]) : 0.f;
             }
-            finish(p, row, n0 + 32 * c + 8 * v, a, u);
+            activate(p, n0 + 32 * c + 8 * v, a, u);
+            if (p.residual) {
+              float f[8];
+              load_row(&now[v], 0, p.y_bf16, f);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) a[e] += f[e];
+            }
+            store_row(p.y, at + 8 * v, p.y_bf16, a);
           }
         }
       }
     }
-  epilogue_done:
     tc_fence_before();
   }
   __syncthreads();
@@ -509,7 +589,8 @@ const uint32_t acc = tmem_d + ((uint32_t)(32 * q) << 16) + half * BN;
       cg::cluster_group cluster = cg::this_cluster();
       cluster.sync();
       const int rank = (int)blockIdx.z;
-      const int r0 = rank * S::kBM / p.ksplit, r1 = (rank + 1) * S::kBM / p.ksplit;
+      const int rows = min(S::kBM, p.M - m0);  // of the tile, cut into bands
+      const int r0 = rank * rows / p.ksplit, r1 = (rank + 1) * rows / p.ksplit;
       const bool gated = p.act == W4_ACT_SWIGLU;
       const int c4s = gated ? BN / 8 : BN / 4;  // groups of four output columns
       const float* part = reinterpret_cast<const float*>(base);
@@ -517,18 +598,34 @@ const uint32_t acc = tmem_d + ((uint32_t)(32 * q) << 16) + half * BN;
         const int row = r0 + i / c4s;
         int col = 4 * (i - (i / c4s) * c4s);
         if (gated) col = (col >> 5) * 64 + (col & 31);  // the gate column
+        if (n0 + col >= p.N) continue;
         const int at = row * S::kPitch + col;
-        float a[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int rr = 0; rr < p.ksplit; ++rr) {
-          const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + at, rr));
-          a[0] += v.x, a[1] += v.y, a[2] += v.z, a[3] += v.w;
-          if (gated) {
-            const float4 w = *reinterpret_cast<const float4*>(
-                cluster.map_shared_rank(part + at + W4B200_SWIGLU_BLOCK, rr));
-            u[0] += w.x, u[1] += w.y, u[2] += w.z, u[3] += w.w;
+        float4 v[8], w[8];  // every rank's part, all on their way at once
+#pragma unroll
+        for (int rr = 0; rr < 8; ++rr) {
+          v[rr] = w[rr] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (rr < p.ksplit) {
+            v[rr] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + at, rr));
+            if (gated)
+              w[rr] = *reinterpret_cast<const float4*>(
+                  cluster.map_shared_rank(part + at + W4B200_SWIGLU_BLOCK, rr));
           }
         }
-        if (m0 + row < p.M && n0 + col < p.N) finish(p, m0 + row, n0 + col, a, u);
+        float a[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int rr = 0; rr < 8; ++rr) {
+          a[0] += v[rr].x, a[1] += v[rr].y, a[2] += v[rr].z, a[3] += v[rr].w;
+          u[0] += w[rr].x, u[1] += w[rr].y, u[2] += w[rr].z, u[3] += w[rr].w;
+        }
+        activate(p, n0 + col, a, u);
+        const size_t to = out_at(p, m0 + row, n0 + col);
+        if (p.residual) {
+          float f[4];
+          load_row(p.residual, to, p.y_bf16, f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] += f[e];
+        }
+        store_row(p.y, to, p.y_bf16, a);
       }
       cluster.sync();  // the other ranks' reads of this CTA's partial are done
     }
@@ -566,6 +663,32 @@ void* gemm_fn() {
   return reinterpret_cast<void*>(&w4_gemm_kernel<B, BN, NACC>);
 }
 
+// Clusters of s CTAs of the 128-column instances that the device holds at once
+// (a cluster needs its SMs within one GPC), by device, accumulators and s.
+static int g_clusters[64][3][9];
+
+static int count_clusters() {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  for (int nacc = 1; nacc <= 2 && e == cudaSuccess; ++nacc)
+    for (int s = 2; s <= 8 && e == cudaSuccess; ++s) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1, 1, (unsigned)s);
+      cfg.blockDim = dim3(kGemmThreads);
+      cfg.dynamicSmemBytes = nacc == 1 ? GemmShape<128, 1>::kSmem : GemmShape<128, 2>::kSmem;
+      cudaLaunchAttribute at;
+      at.id = cudaLaunchAttributeClusterDimension;
+      at.val.clusterDim.x = at.val.clusterDim.y = 1;
+      at.val.clusterDim.z = (unsigned)s;
+      cfg.attrs = &at;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(
+          &g_clusters[dev & 63][nacc][s],
+          nacc == 1 ? gemm_fn<true, 128, 1>() : gemm_fn<true, 128, 2>(), &cfg);
+    }
+  return e == cudaSuccess ? W4_OK : cuda_fail(e, "cudaOccupancyMaxActiveClusters(w4_gemm)");
+}
+
 int gemm_init_device(const DeviceInfo& di) {
   struct K {
     void* fn;
@@ -587,7 +710,7 @@ int gemm_init_device(const DeviceInfo& di) {
                              cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(w4_gemm carveout)");
   }
-  return W4_OK;
+  return count_clusters();
 }
 
 // Tile width: 256 columns halve the re-reads of X per FLOP; 128 when a
@@ -630,8 +753,11 @@ void* gemm_instance(int bf16, int bn, int nacc, size_t* smem) {
 }
 
 // The launches of one GEMM (at most two). split_k > 0 forces one launch of
-// 128 x 256 tiles (one accumulator) cut into that many K slices.
-int gemm_plan(int M, int K, int N, int sms, int split_k, GemmLaunch* out) {
+// 128 x 256 tiles (one accumulator) cut into that many K slices. few_tiles lets
+// grids that leave SMs idle be cut along K, which w4_gemm's own calls are not
+// (their sums keep their order).
+int gemm_plan(int M, int K, int N, int sms, int split_k, bool few_tiles, int dev,
+              GemmLaunch* out) {
   const int kt = K / kBK;
   const int nt128 = (N + 127) / 128;
   // the K-sliced tile: 128 rows x 256 columns (its partial tile fits the
@@ -646,6 +772,15 @@ int gemm_plan(int M, int K, int N, int sms, int split_k, GemmLaunch* out) {
   const int bm = nacc * kUM;
   const int ntx = (N + bn - 1) / bn, mtx = (M + bm - 1) / bm;
   const int tiles = ntx * mtx;
+  if (few_tiles && tiles * 2 <= sms) {
+    // Half the SMs or more would have no tile: as many K slices as are resident
+    // at once, of three stages at least.
+    for (int s = std::min(8, kt / 3); s >= 2; --s)
+      if (tiles <= g_clusters[dev & 63][nacc][s]) {
+        out[0] = GemmLaunch{128, nacc, 0, 0, nt128, tiles, s, false};
+        return 1;
+      }
+  }
   // A grid of fewer tiles than SMs is not cut along K: measured on 2048 x
   // 8960 x 1536 (96 tiles), three K slices over 288 CTAs took 118-128 us
   // against 96 us for the 96 whole tiles (each slice's stages ran at half the
@@ -672,24 +807,23 @@ int gemm_plan(int M, int K, int N, int sms, int split_k, GemmLaunch* out) {
 
 int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* scales, void* y,
                 int y_bf16, int M, int K, int N, const w4_gemm_ops& ops, int split_k,
-                cudaStream_t stream) {
+                bool few_tiles, cudaStream_t stream) {
   int dev = 0;
   int st = current_device(&dev);
   if (st != W4_OK) return st;
   const DeviceInfo& di = device_info(dev);
   GemmLaunch plan[2];
-  const int n = gemm_plan(M, K, N, di.sm_count > 0 ? di.sm_count : 148, split_k, plan);
+  const int n = gemm_plan(M, K, N, di.sm_count > 0 ? di.sm_count : 148, split_k, few_tiles, dev,
+                          plan);
   for (int i = 0; i < n; ++i) {
     const GemmLaunch& L = plan[i];
     const int BM = L.nacc * kUM;
-    CUtensorMap tm_x, tm_w, tm_s;
+    CUtensorMap tm_x, tm_w;
     if (!encode_2d(&tm_x,
                    x_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
                    x, (uint64_t)K, (uint64_t)M, kBK, (uint32_t)BM, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, packed, (uint64_t)N,
-                   (uint64_t)(K / 8), (uint32_t)L.bn, kBK / 8, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-        !encode_2d(&tm_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, scales, (uint64_t)N,
-                   (uint64_t)(K / 128), (uint32_t)L.bn, 1, CU_TENSOR_MAP_SWIZZLE_NONE))
+                   (uint64_t)(K / 8), (uint32_t)L.bn, kBK / 8, CU_TENSOR_MAP_SWIZZLE_NONE))
       return fail(W4_ERR_CUDA, "cuTensorMapEncodeTiled failed for w4_gemm M=%d K=%d N=%d", M, K,
                   N);
     GemmParams p;
@@ -699,6 +833,7 @@ int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* sc
     p.N = N;
     p.x_bf16 = x_bf16;
     p.y_bf16 = y_bf16;
+    p.scales = static_cast<const uint16_t*>(scales);
     p.act = ops.act;
     p.bias = ops.bias;
     p.residual = ops.residual;
@@ -731,7 +866,7 @@ int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* sc
     }
     cfg.attrs = attrs;
     cfg.numAttrs = na;
-    void* args[] = {&tm_x, &tm_w, &tm_s, &p};
+    void* args[] = {&tm_x, &tm_w, &p};
     cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
     if (e != cudaSuccess) return cuda_fail(e, "w4_gemm launch");
   }

@@ -87,7 +87,7 @@ inline bool lm_head_hidden_supported(int hidden) {
 int gemm_init_device(const DeviceInfo& di);
 int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* scales, void* y,
                 int y_bf16, int M, int K, int N, const w4_gemm_ops& ops, int split_k,
-                cudaStream_t stream);
+                bool few_tiles, cudaStream_t stream);
 
 // Head norms, rotation and the paged 8-bit KV cache (w4_kv8.cu, w4_kv8_attn.cu).
 int launch_norm_rope(const w4_heads& q, const w4_heads& k, const w4_heads& q_out,

@@ -79,6 +79,8 @@ def test_epilogues(M, K, N, dtype, activation, bias, residual):
 @pytest.mark.parametrize("activation", [None, "gelu", "swiglu"])
 @pytest.mark.parametrize("M,K,N,split_k", [
     (40, 512, 384, 1), (40, 512, 384, 3), (200, 1024, 640, 8), (128, 128, 256, 2),  # K slices
+    (17, 1536, 2048, None), (128, 2304, 256, None), (511, 8960, 1536, None),  # few tiles: slices
+    (140, 384, 128, None), (33, 256, 1152, None),
     (4000, 256, 2432, None),  # 256-column tiles, the last one half filled
     (2048, 1024, 5120, None),  # 160 of them: the last wave's tiles run as K slices
     (600, 2048, 1536, None)])
@@ -93,8 +95,9 @@ def test_residual_in_place_and_shared_rows():
 
 
 def test_no_epilogue_is_w4_gemm_bit_for_bit():
-    for M, K, N in ((50, 256, 384), (2048, 1024, 5120)):
-        x, w, _, _, y = run(M, K, N, torch.float16, False, None, False)
+    """Where both cut K alike: one slice, and grids that fill the SMs."""
+    for M, K, N, split_k in ((50, 256, 384, 1), (2048, 1024, 5120, None)):
+        x, w, _, _, y = run(M, K, N, torch.float16, False, None, False, split_k=split_k)
         assert torch.equal(y, rd.w4_gemm(x, *w))
 
 
