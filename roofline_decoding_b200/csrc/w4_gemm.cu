@@ -223,12 +223,14 @@ __device__ __forceinline__ uint4 dequant_word(uint32_t w, uint32_t s2, float sf)
       o[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
   } else {
+    const float off = -136.0f * sf;  // exact: 11 + 5 bits
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t v = lop3_and_or(h[i], 0x000F000Fu, 0x43004300u);  // 128 + q
-      const float lo = __uint_as_float(v << 16) - 136.0f;                // q - 8, exact
-      const float hi = __uint_as_float(v & 0xFFFF0000u) - 136.0f;
-      const __nv_bfloat162 d = __floats2bfloat162_rn(lo * sf, hi * sf);  // one rounding
+      // (128 + q) s - 136 s = (q - 8) s: exact, it has 15 bits
+      const float lo = fmaf(__uint_as_float(v << 16), sf, off);
+      const float hi = fmaf(__uint_as_float(v & 0xFFFF0000u), sf, off);
+      const __nv_bfloat162 d = __floats2bfloat162_rn(lo, hi);  // one rounding
       o[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
   }

@@ -166,45 +166,55 @@ struct RopeParams {
   int* err;
 };
 
-// Heads [h_first, h_last) of one row, 32 / (D/16) at a time.
-template <int D>
+// Heads [h_first, h_last) of one row, 32 / (D/16) at a time; the loads of U
+// turns go out together.
+template <int D, int U>
 __device__ __forceinline__ void rope_heads(const RopeParams& p, int64_t row, int64_t pos,
                                            int h_first, int h_last, int lane) {
   constexpr int L = D / 16, HPW = 32 / L;
   const int l = lane % L;
   Turn r;
   if (p.cos_t) load_turn<D>(p.cos_t, p.sin_t, p.table_type, pos, l, r);
-#pragma unroll 2
-  for (int h0 = h_first; h0 < h_last; h0 += HPW) {
-    const int h = h0 + lane / L;
-    const bool in = h < h_last, is_q = h < p.heads;
-    const HeadsIn& x = is_q ? p.q : p.k;
-    const int hh = is_q ? h : h - p.heads;
-    float a[8], b[8];
-    uint4 va = make_uint4(0u, 0u, 0u, 0u), vb = va;
-    if (in) {
-      const uint16_t* src = x.p + row * x.row + hh * x.head + 8 * l;
-      va = *reinterpret_cast<const uint4*>(src);
-      vb = *reinterpret_cast<const uint4*>(src + D / 2);
+#pragma unroll 1
+  for (int h0 = h_first; h0 < h_last; h0 += U * HPW) {
+    uint4 va[U], vb[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * HPW + lane / L;
+      va[u] = vb[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (h < h_last) {
+        const uint16_t* src = (h < p.heads ? p.q.p + row * p.q.row + h * p.q.head
+                                           : p.k.p + row * p.k.row + (h - p.heads) * p.k.head) +
+                              8 * l;
+        va[u] = *reinterpret_cast<const uint4*>(src);
+        vb[u] = *reinterpret_cast<const uint4*>(src + D / 2);
+      }
     }
-    unpack8(va, p.bf16, a);
-    unpack8(vb, p.bf16, b);
-    // a pass may hold the last query heads and the first key heads: each lane
-    // takes its own head's weight
-    norm_turn<D>(a, b, p.q_norm || p.k_norm, is_q ? p.q_norm : p.k_norm, p.bf16, p.eps, l,
-                 p.cos_t != nullptr, r);
-    if (in) {
-      uint16_t* dst = is_q ? p.q_out + row * p.q_out_row + hh * p.q_out_head
-                           : p.k_out + row * p.k_out_row + hh * p.k_out_head;
-      *reinterpret_cast<uint4*>(dst + 8 * l) = pack8(a, p.bf16);
-      *reinterpret_cast<uint4*>(dst + D / 2 + 8 * l) = pack8(b, p.bf16);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * HPW + lane / L;
+      const bool is_q = h < p.heads;
+      float a[8], b[8];
+      unpack8(va[u], p.bf16, a);
+      unpack8(vb[u], p.bf16, b);
+      // a turn may hold the last query heads and the first key heads: each lane
+      // takes its own head's weight
+      norm_turn<D>(a, b, p.q_norm || p.k_norm, is_q ? p.q_norm : p.k_norm, p.bf16, p.eps, l,
+                   p.cos_t != nullptr, r);
+      if (h < h_last) {
+        uint16_t* dst = (is_q ? p.q_out + row * p.q_out_row + h * p.q_out_head
+                              : p.k_out + row * p.k_out_row + (h - p.heads) * p.k_out_head) +
+                        8 * l;
+        *reinterpret_cast<uint4*>(dst) = pack8(a, p.bf16);
+        *reinterpret_cast<uint4*>(dst + D / 2) = pack8(b, p.bf16);
+      }
     }
   }
 }
 
 constexpr int kRopeThreads = 128;
 
-template <int D>
+template <int D, int U>
 __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const RopeParams p) {
   constexpr int HPW = 32 / (D / 16);
   const int lane = threadIdx.x & 31;
@@ -219,7 +229,7 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const RopeParam
     if (lane == 0) atomicCAS(p.err, 0, kErrKvRange);
     return;
   }
-  rope_heads<D>(p, row, pos, h0, min(all, h0 + p.groups_per_warp * HPW), lane);
+  rope_heads<D, U>(p, row, pos, h0, min(all, h0 + p.groups_per_warp * HPW), lane);
 }
 
 // ------------------------------------------------------------ append
@@ -232,8 +242,8 @@ struct AppendParams {
   const int32_t *page_table, *lengths, *row_starts;
   int64_t table_stride;
   int pages, page, max_pages, seqs, rows, kv_heads;
-  int kv_blocks;  // blocks of the cache part; those after them turn queries
-  int groups;     // bound on the (sequence, page) pairs that the call touches
+  int kv_units;   // K and V blocks of the (sequence, page) pairs that it may touch
+  int kv_blocks;  // CTAs of the cache part; those after them turn queries
 };
 
 // First row and number of rows of sequence b, kept inside the buffers.
@@ -251,18 +261,20 @@ __device__ __forceinline__ int touched(int past, int n, int page) {
 
 constexpr int kAppendThreads = 256;
 
-// One block of the cache: K or V of one head of one page.
-template <int D, int NP>
-__device__ void append_block(const AppendParams& p, int unit) {
-  constexpr int L = D / 16, RPP = kAppendThreads / L;  // rows a pass
-  __shared__ float red[kAppendThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, l = tid % L;
+// One block of the cache, K or V of one head of one page, by W warps. Each
+// pass holds NP rows a lane group in registers; a block of more rows is loaded
+// twice, for its largest value and for its codes.
+template <int D, int W, int NP>
+__device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
+  constexpr int L = D / 16, kThreads = W * 32, RPP = kThreads / L;  // rows a turn
+  const int tid = threadIdx.x % kThreads, lane = tid & 31, l = tid % L;
   const bool is_v = unit & 1;
   const int h = (unit >> 1) % p.kv_heads;
   int g = (unit >> 1) / p.kv_heads;  // which (sequence, page) pair
 
   // every warp finds the pair by a scan over the sequences, 32 at a time
   int b = -1, past = 0, n = 0, first = 0;
+#pragma unroll 1
   for (int b0 = 0; b0 < p.seqs; b0 += 32) {
     const int bb = b0 + lane;
     int f = 0, m = 0, ps = 0;
@@ -290,7 +302,7 @@ __device__ void append_block(const AppendParams& p, int unit) {
     g -= __shfl_sync(0xffffffffu, incl, 31);
   }
   if (b < 0) return;  // fewer pairs than the bound
-  const int64_t slot_page = past / p.page + g;               // page of the sequence
+  const int64_t slot_page = past / p.page + g;                  // page of the sequence
   const int64_t tok0 = max((int64_t)past, slot_page * p.page);  // its first new token
   const int cnt = (int)(min((int64_t)past + n, (slot_page + 1) * p.page) - tok0);
   const int slot0 = (int)(tok0 - slot_page * p.page);
@@ -309,39 +321,48 @@ __device__ void append_block(const AppendParams& p, int unit) {
   const float old = slot0 > 0 ? *scale_at : 0.f;
 
   float a[NP][8], c[NP][8];
+  auto load = [&](int base) {  // rows base + i RPP + tid / L, normed and turned
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int r = base + i * RPP + tid / L;
+      uint4 va = make_uint4(0u, 0u, 0u, 0u), vb = va;
+      if (r < cnt) {
+        const uint16_t* src = x.p + (row0 + r) * x.row + h * x.head + 8 * l;
+        va = *reinterpret_cast<const uint4*>(src);
+        vb = *reinterpret_cast<const uint4*>(src + D / 2);
+      }
+      unpack8(va, p.rope.bf16, a[i]);
+      unpack8(vb, p.rope.bf16, c[i]);
+      if (!is_v) {
+        Turn t;
+        if (turned && r < cnt)
+          load_turn<D>(p.rope.cos_t, p.rope.sin_t, p.rope.table_type, tok0 + r, l, t);
+        norm_turn<D>(a[i], c[i], p.rope.k_norm != nullptr, p.rope.k_norm, p.rope.bf16, p.rope.eps,
+                     l, turned && r < cnt, t);
+      }
+    }
+  };
   float amax = 0.f;
+#pragma unroll 1
+  for (int base = 0; base < cnt; base += NP * RPP) {
+    load(base);
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int r = i * RPP + tid / L;
-    uint4 va = make_uint4(0u, 0u, 0u, 0u), vb = va;
-    if (r < cnt) {
-      const uint16_t* src = x.p + (row0 + r) * x.row + h * x.head + 8 * l;
-      va = *reinterpret_cast<const uint4*>(src);
-      vb = *reinterpret_cast<const uint4*>(src + D / 2);
-    }
-    unpack8(va, p.rope.bf16, a[i]);
-    unpack8(vb, p.rope.bf16, c[i]);
-    if (!is_v) {
-      Turn t;
-      if (turned && r < cnt)
-        load_turn<D>(p.rope.cos_t, p.rope.sin_t, p.rope.table_type, tok0 + r, l, t);
-      norm_turn<D>(a[i], c[i], p.rope.k_norm != nullptr, p.rope.k_norm, p.rope.bf16, p.rope.eps, l,
-                   turned && r < cnt, t);
-    }
-    if (r < cnt) {
+    for (int i = 0; i < NP; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {  // infinities and NaN do not set the scale
+      for (int j = 0; j < 8; ++j) {  // infinities and NaN do not set the scale (rows past cnt: 0)
         const float u = fabsf(a[i][j]), w = fabsf(c[i][j]);
         amax = fmaxf(amax, fmaxf(u <= 3.4028234e38f ? u : 0.f, w <= 3.4028234e38f ? w : 0.f));
       }
-    }
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  if (lane == 0) red[tid >> 5] = amax;
-  __syncthreads();
+  if constexpr (W > 1) {
+    __shared__ float red[W];
+    if (lane == 0) red[tid >> 5] = amax;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, red[w]);
+    for (int w = 0; w < W; ++w) amax = fmaxf(amax, red[w]);
+  }
   // amax = m 2^e with 1 <= m < 2, and 448 = 1.75 * 2^8: the least power of
   // two is 2^(e - 8), or twice that when m > 1.75
   const uint32_t bits = __float_as_uint(amax);
@@ -349,19 +370,24 @@ __device__ void append_block(const AppendParams& p, int unit) {
   e = min(max(e, kMinScaleExp), kMaxScaleExp);
   const float scale = fmaxf(__uint_as_float((uint32_t)(e + 127) << 23), old);
   const float inv = 1.0f / scale;  // a power of two, unless the block's own scale was none
+#pragma unroll 1
+  for (int base = 0; base < cnt; base += NP * RPP) {
+    if (cnt > NP * RPP) load(base);
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int r = i * RPP + tid / L;
-    if (r < cnt) {
-      uint8_t* dst = codes + (size_t)(slot0 + r) * D + 8 * l;
-      *reinterpret_cast<uint2*>(dst) = to_e4m3x8(a[i], inv);
-      *reinterpret_cast<uint2*>(dst + D / 2) = to_e4m3x8(c[i], inv);
+    for (int i = 0; i < NP; ++i) {
+      const int r = base + i * RPP + tid / L;
+      if (r < cnt) {
+        uint8_t* dst = codes + (size_t)(slot0 + r) * D + 8 * l;
+        *reinterpret_cast<uint2*>(dst) = to_e4m3x8(a[i], inv);
+        *reinterpret_cast<uint2*>(dst + D / 2) = to_e4m3x8(c[i], inv);
+      }
     }
   }
   if (scale != old) {
     if (tid == 0) *scale_at = scale;
     const float ratio = old * inv;  // the rows in use, rounded again in the larger scale
-    for (int i = tid; i < slot0 * (D / 8); i += kAppendThreads) {
+#pragma unroll 1
+    for (int i = tid; i < slot0 * (D / 8); i += kThreads) {
       uint2* at = reinterpret_cast<uint2*>(codes) + i;
       const uint2 v = *at;
       float f[8];
@@ -379,10 +405,13 @@ __device__ void append_block(const AppendParams& p, int unit) {
   }
 }
 
-template <int D, int NP>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+template <int D, int W, int NP>
+__global__ void __launch_bounds__(kAppendThreads, W == 1 ? 3 : NP == 4 ? 2 : 3)
+    append_kernel(const AppendParams p) {
   if ((int)blockIdx.x < p.kv_blocks) {
-    append_block<D, NP>(p, blockIdx.x);
+    const int unit = W == 1 ? (int)blockIdx.x * (kAppendThreads / 32) + (int)(threadIdx.x >> 5)
+                            : (int)blockIdx.x;
+    if (unit < p.kv_units) append_block<D, W, NP>(p, unit);
     return;
   }
   // queries: a warp takes a row's heads, or a part of them
@@ -396,6 +425,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   const int64_t row = unit / per_row;
   if (row >= p.rows) return;
   int b = 0;  // the sequence: as many as end at or before this row
+#pragma unroll 1
   for (int b0 = 0; b0 < p.seqs; b0 += 32) {
     const int bb = b0 + lane;
     b += __popc(__ballot_sync(0xffffffffu, bb < p.seqs && p.row_starts[bb + 1] <= row));
@@ -407,7 +437,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
     return;
   }
   const int h0 = (int)(unit - row * per_row) * r.groups_per_warp * HPW;
-  rope_heads<D>(r, row, pos, h0, min(r.heads, h0 + r.groups_per_warp * HPW), lane);
+  rope_heads<D, 1>(r, row, pos, h0, min(r.heads, h0 + r.groups_per_warp * HPW), lane);
 }
 
 HeadsIn heads_in(const w4_heads& x) {
@@ -463,10 +493,8 @@ int launch_norm_rope(const w4_heads& q, const w4_heads& k, const w4_heads& q_out
   const int64_t units = (int64_t)rows * ((groups + p.groups_per_warp - 1) / p.groups_per_warp);
   const int64_t blocks = (units + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
   if (blocks > 0x7fffffff) return fail(W4_ERR_UNSUPPORTED, "w4_qk_norm_rope: %d rows", rows);
-  if (head_dim == 128)
-    norm_rope_kernel<128><<<(unsigned)blocks, kRopeThreads, 0, stream>>>(p);
-  else
-    norm_rope_kernel<64><<<(unsigned)blocks, kRopeThreads, 0, stream>>>(p);
+  void (*fn)(RopeParams) = head_dim == 128 ? norm_rope_kernel<128, 2> : norm_rope_kernel<64, 2>;
+  fn<<<(unsigned)blocks, kRopeThreads, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_qk_norm_rope launch");
 }
@@ -498,21 +526,33 @@ int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_hea
   // n rows of a sequence touch at most (n - 1) / page + 2 pages, and no more than n
   const int64_t pairs =
       std::min<int64_t>(bt.rows, (int64_t)bt.rows / c.page_size + 2 * (int64_t)bt.seqs);
-  const int64_t kv_blocks = pairs * c.kv_heads * 2;
+  const int64_t kv_units = pairs * c.kv_heads * 2;
+  // A warp a block of the cache while sequences bring a few rows each: most
+  // threads of a CTA would idle on one row. A CTA a block for prompts.
+  const bool by_warp = bt.rows <= 4 * (int64_t)bt.seqs;
+  const int64_t kv_blocks =
+      by_warp ? (kv_units + kAppendThreads / 32 - 1) / (kAppendThreads / 32) : kv_units;
   const int hpw = 32 / (c.head_dim / 16);
   const int groups = (q.heads + hpw - 1) / hpw;
   p.rope.groups_per_warp = groups_per_warp(bt.rows, groups, di.sm_count);
   const int64_t units =
       (int64_t)bt.rows * ((groups + p.rope.groups_per_warp - 1) / p.rope.groups_per_warp);
   const int64_t blocks = kv_blocks + (units + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-  if (blocks > 0x7fffffff) return fail(W4_ERR_UNSUPPORTED, "w4_kv8_append: %d rows", bt.rows);
+  if (blocks > 0x7fffffff || kv_units > 0x7fffffff)
+    return fail(W4_ERR_UNSUPPORTED, "w4_kv8_append: %d rows", bt.rows);
+  p.kv_units = (int)kv_units;
   p.kv_blocks = (int)kv_blocks;
   const int np = std::max(1, c.page_size * (c.head_dim / 16) / kAppendThreads);
-  void (*fn)(AppendParams) = c.head_dim == 128
-                                 ? (np == 4   ? append_kernel<128, 4>
-                                    : np == 2 ? append_kernel<128, 2>
-                                              : append_kernel<128, 1>)
-                                 : (np == 2 ? append_kernel<64, 2> : append_kernel<64, 1>);
+  void (*fn)(AppendParams);
+  if (c.head_dim == 128)
+    fn = by_warp   ? append_kernel<128, 1, 1>
+         : np == 4 ? append_kernel<128, 8, 4>
+         : np == 2 ? append_kernel<128, 8, 2>
+                   : append_kernel<128, 8, 1>;
+  else
+    fn = by_warp   ? append_kernel<64, 1, 1>
+         : np == 2 ? append_kernel<64, 8, 2>
+                   : append_kernel<64, 8, 1>;
   fn<<<(unsigned)blocks, kAppendThreads, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_kv8_append launch");
