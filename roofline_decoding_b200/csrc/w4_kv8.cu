@@ -36,32 +36,40 @@ constexpr int kMinScaleExp = -32, kMaxScaleExp = 120;
 
 // ------------------------------------------------------------ element types
 
-// Eight 16-bit elements (16 bytes) to fp32.
-__device__ __forceinline__ void unpack8(const uint4& v, int bf16, float (&f)[8]) {
+struct F8 {
+  float f[8];
+};
+
+// Eight 16-bit elements (16 bytes) to fp32, and back with one rounding.
+template <bool BF16>
+__device__ __forceinline__ F8 unpack8(const uint4& v) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+  F8 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (bf16) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    if constexpr (BF16) {
+      r.f[2 * i] = __uint_as_float(w[i] << 16);
+      r.f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     } else {
-      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      r.f[2 * i] = h.x;
+      r.f[2 * i + 1] = h.y;
     }
   }
+  return r;
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&f)[8], int bf16) {
+template <bool BF16>
+__device__ __forceinline__ uint4 pack8(const F8& r) {
   uint4 v;
   uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (bf16) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    if constexpr (BF16) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(r.f[2 * i], r.f[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     } else {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      const __half2 h = __floats2half2_rn(r.f[2 * i], r.f[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
@@ -69,28 +77,26 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8], int bf16) {
 }
 
 // Eight elements at index i (a multiple of 8) of a table or weight.
-__device__ __forceinline__ void load8(const void* p, int type, size_t i, float (&f)[8]) {
+__device__ __forceinline__ F8 load8(const void* p, int type, size_t i) {
   if (type == W4_F32) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
     const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i) + 1);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-    f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i)),
-            type == W4_BF16, f);
+    return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
   }
+  const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+  return type == W4_BF16 ? unpack8<true>(v) : unpack8<false>(v);
 }
 
-// Eight fp32 values to e4m3: round to nearest even, +-448 beyond the range
-// (infinities too), NaN kept.
-__device__ __forceinline__ uint2 to_e4m3x8(const float (&f)[8], float mul) {
+// Eight fp32 values times mul to e4m3: round to nearest even, +-448 beyond the
+// range (infinities too), NaN kept.
+__device__ __forceinline__ uint2 to_e4m3x8(const F8& r, float mul) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(
-        make_float2(f[4 * i] * mul, f[4 * i + 1] * mul), __NV_SATFINITE, __NV_E4M3);
+        make_float2(r.f[4 * i] * mul, r.f[4 * i + 1] * mul), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-        make_float2(f[4 * i + 2] * mul, f[4 * i + 3] * mul), __NV_SATFINITE, __NV_E4M3);
+        make_float2(r.f[4 * i + 2] * mul, r.f[4 * i + 3] * mul), __NV_SATFINITE, __NV_E4M3);
     w[i] = lo | (hi << 16);
   }
   return make_uint2(w[0], w[1]);
@@ -98,52 +104,72 @@ __device__ __forceinline__ uint2 to_e4m3x8(const float (&f)[8], float mul) {
 
 // ------------------------------------------------------------ one head
 
-// The rotation of one position: this lane's chunks of its cos and sin rows.
+// What a lane multiplies its two chunks a (dims 8l..) and b (D/2 + 8l..) of a
+// normed head by: norm weight and rotation in one,
+//   a' = a ac - b bs,  b' = b bc + a as.
 struct Turn {
-  float c0[8], c1[8], s0[8], s1[8];
+  F8 ac, bs, bc, as;
 };
 
 template <int D>
 __device__ __forceinline__ void load_turn(const void* cos_t, const void* sin_t, int type,
                                           int64_t pos, int l, Turn& r) {
   const size_t at = (size_t)pos * D + 8 * l;
-  load8(cos_t, type, at, r.c0);
-  load8(cos_t, type, at + D / 2, r.c1);
-  load8(sin_t, type, at, r.s0);
-  load8(sin_t, type, at + D / 2, r.s1);
+  r.ac = load8(cos_t, type, at);
+  r.bc = load8(cos_t, type, at + D / 2);
+  r.bs = load8(sin_t, type, at);
+  r.as = load8(sin_t, type, at + D / 2);
 }
 
-// Norm (where the lane's head has a weight) and rotation of a head spread over
-// D / 16 neighbouring lanes. `normed` is the same for the whole warp: every
-// lane takes part in the sum's exchange.
+// Brings the norm's weight into r (r holds cos and sin where `turned`).
+template <int D, bool BF16>
+__device__ __forceinline__ void weigh(const void* weight, int l, bool turned, Turn& r) {
+  const F8 wa = load8(weight, BF16 ? W4_BF16 : W4_F16, 8 * l);
+  const F8 wb = load8(weight, BF16 ? W4_BF16 : W4_F16, D / 2 + 8 * l);
+  if (!turned) {
+    r.ac = wa;
+    r.bc = wb;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    r.ac.f[i] *= wa.f[i];
+    r.bs.f[i] *= wb.f[i];
+    r.bc.f[i] *= wb.f[i];
+    r.as.f[i] *= wa.f[i];
+  }
+}
+
+// A head spread over D / 16 neighbouring lanes: normed, then multiplied out.
+// All lanes of the warp take part in the sum's exchange.
 template <int D>
-__device__ __forceinline__ void norm_turn(float (&a)[8], float (&b)[8], bool normed,
-                                          const void* weight, int bf16, float eps, int l,
-                                          bool turned, const Turn& r) {
+__device__ __forceinline__ void norm_turn(F8& a, F8& b, bool normed, float eps, bool turned,
+                                          const Turn& r) {
   if (normed) {
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+    for (int i = 0; i < 8; ++i) ss = fmaf(a.f[i], a.f[i], fmaf(b.f[i], b.f[i], ss));
 #pragma unroll
     for (int off = D / 32; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-    if (weight) {
-      const float inv = rsqrtf(ss / (float)D + eps);
-      float w0[8], w1[8];
-      load8(weight, bf16 ? W4_BF16 : W4_F16, 8 * l, w0);
-      load8(weight, bf16 ? W4_BF16 : W4_F16, D / 2 + 8 * l, w1);
+    const float inv = rsqrtf(ss * (1.0f / D) + eps);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] = a[i] * inv * w0[i];
-        b[i] = b[i] * inv * w1[i];
-      }
+    for (int i = 0; i < 8; ++i) {
+      a.f[i] *= inv;
+      b.f[i] *= inv;
     }
   }
   if (turned) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = fmaf(x, r.c0[i], -(y * r.s0[i]));
-      b[i] = fmaf(y, r.c1[i], x * r.s1[i]);
+      const float x = a.f[i], y = b.f[i];
+      a.f[i] = fmaf(x, r.ac.f[i], -(y * r.bs.f[i]));
+      b.f[i] = fmaf(y, r.bc.f[i], x * r.as.f[i]);
+    }
+  } else if (normed) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a.f[i] *= r.ac.f[i];
+      b.f[i] *= r.bc.f[i];
     }
   }
 }
@@ -160,76 +186,80 @@ struct RopeParams {
   const void *q_norm, *k_norm, *cos_t, *sin_t;
   const int64_t* positions;
   int heads, kv_heads, rows, max_pos;
-  int bf16, table_type;
+  int table_type;
   float eps;
   int groups_per_warp;
   int* err;
 };
 
-// Heads [h_first, h_last) of one row, 32 / (D/16) at a time; the loads of U
-// turns go out together.
-template <int D, int U>
-__device__ __forceinline__ void rope_heads(const RopeParams& p, int64_t row, int64_t pos,
-                                           int h_first, int h_last, int lane) {
+// Groups of heads that a warp holds at once, of queries and of keys.
+template <int D>
+__host__ __device__ __forceinline__ int head_groups(int heads) {
+  constexpr int HPW = 32 / (D / 16);
+  return (heads + HPW - 1) / HPW;
+}
+
+// Head groups [g0, g1) of the queries or keys of one row.
+template <int D, bool BF16>
+__device__ __forceinline__ void rope_groups(const HeadsIn& x, uint16_t* out, int64_t out_row,
+                                            int64_t out_head, int heads, const void* weight,
+                                            const RopeParams& p, int64_t row, int64_t pos, int g0,
+                                            int g1, int lane) {
   constexpr int L = D / 16, HPW = 32 / L;
   const int l = lane % L;
+  const bool turned = p.cos_t != nullptr;
   Turn r;
-  if (p.cos_t) load_turn<D>(p.cos_t, p.sin_t, p.table_type, pos, l, r);
+  if (turned) load_turn<D>(p.cos_t, p.sin_t, p.table_type, pos, l, r);
+  if (weight) weigh<D, BF16>(weight, l, turned, r);
+  const uint16_t* src = x.p + row * x.row + 8 * l;
+  uint16_t* dst = out + row * out_row + 8 * l;
 #pragma unroll 1
-  for (int h0 = h_first; h0 < h_last; h0 += U * HPW) {
-    uint4 va[U], vb[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HPW + lane / L;
-      va[u] = vb[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (h < h_last) {
-        const uint16_t* src = (h < p.heads ? p.q.p + row * p.q.row + h * p.q.head
-                                           : p.k.p + row * p.k.row + (h - p.heads) * p.k.head) +
-                              8 * l;
-        va[u] = *reinterpret_cast<const uint4*>(src);
-        vb[u] = *reinterpret_cast<const uint4*>(src + D / 2);
-      }
+  for (int g = g0; g < g1; ++g) {
+    const int h = g * HPW + lane / L;
+    uint4 va = make_uint4(0u, 0u, 0u, 0u), vb = va;
+    if (h < heads) {
+      va = *reinterpret_cast<const uint4*>(src + h * x.head);
+      vb = *reinterpret_cast<const uint4*>(src + h * x.head + D / 2);
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * HPW + lane / L;
-      const bool is_q = h < p.heads;
-      float a[8], b[8];
-      unpack8(va[u], p.bf16, a);
-      unpack8(vb[u], p.bf16, b);
-      // a turn may hold the last query heads and the first key heads: each lane
-      // takes its own head's weight
-      norm_turn<D>(a, b, p.q_norm || p.k_norm, is_q ? p.q_norm : p.k_norm, p.bf16, p.eps, l,
-                   p.cos_t != nullptr, r);
-      if (h < h_last) {
-        uint16_t* dst = (is_q ? p.q_out + row * p.q_out_row + h * p.q_out_head
-                              : p.k_out + row * p.k_out_row + (h - p.heads) * p.k_out_head) +
-                        8 * l;
-        *reinterpret_cast<uint4*>(dst) = pack8(a, p.bf16);
-        *reinterpret_cast<uint4*>(dst + D / 2) = pack8(b, p.bf16);
-      }
+    F8 a = unpack8<BF16>(va), b = unpack8<BF16>(vb);
+    norm_turn<D>(a, b, weight != nullptr, p.eps, turned, r);
+    if (h < heads) {
+      *reinterpret_cast<uint4*>(dst + h * out_head) = pack8<BF16>(a);
+      *reinterpret_cast<uint4*>(dst + h * out_head + D / 2) = pack8<BF16>(b);
     }
   }
 }
 
+// Groups [g0, g1) of a row, the queries' first.
+template <int D, bool BF16>
+__device__ __forceinline__ void rope_row(const RopeParams& p, int64_t row, int64_t pos, int g0,
+                                         int g1, int lane) {
+  const int gq = head_groups<D>(p.heads);
+  if (g0 < gq)
+    rope_groups<D, BF16>(p.q, p.q_out, p.q_out_row, p.q_out_head, p.heads, p.q_norm, p, row, pos, g0,
+                   min(g1, gq), lane);
+  if (g1 > gq)
+    rope_groups<D, BF16>(p.k, p.k_out, p.k_out_row, p.k_out_head, p.kv_heads, p.k_norm, p, row, pos,
+                   max(g0 - gq, 0), g1 - gq, lane);
+}
+
 constexpr int kRopeThreads = 128;
 
-template <int D, int U>
+template <int D, bool BF16>
 __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const RopeParams p) {
-  constexpr int HPW = 32 / (D / 16);
   const int lane = threadIdx.x & 31;
-  const int all = p.heads + p.kv_heads, groups = (all + HPW - 1) / HPW;
+  const int groups = head_groups<D>(p.heads) + head_groups<D>(p.kv_heads);
   const int per_row = (groups + p.groups_per_warp - 1) / p.groups_per_warp;
   const int64_t unit = (int64_t)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
   const int64_t row = unit / per_row;
   if (row >= p.rows) return;
-  const int h0 = (int)(unit - row * per_row) * p.groups_per_warp * HPW;
+  const int g0 = (int)(unit - row * per_row) * p.groups_per_warp;
   const int64_t pos = p.positions ? p.positions[row] : 0;
   if (p.cos_t && (pos < 0 || pos >= p.max_pos)) {  // no such table row: the row is left as it is
     if (lane == 0) atomicCAS(p.err, 0, kErrKvRange);
     return;
   }
-  rope_heads<D, U>(p, row, pos, h0, min(all, h0 + p.groups_per_warp * HPW), lane);
+  rope_row<D, BF16>(p, row, pos, g0, min(groups, g0 + p.groups_per_warp), lane);
 }
 
 // ------------------------------------------------------------ append
@@ -261,10 +291,10 @@ __device__ __forceinline__ int touched(int past, int n, int page) {
 
 constexpr int kAppendThreads = 256;
 
-// One block of the cache, K or V of one head of one page, by W warps. Each
-// pass holds NP rows a lane group in registers; a block of more rows is loaded
-// twice, for its largest value and for its codes.
-template <int D, int W, int NP>
+// One block of the cache, K or V of one head of one page, by W warps. A lane
+// group holds NP rows in registers: a whole page with eight warps; one warp
+// loads a block of more rows twice, for its largest value and for its codes.
+template <int D, bool BF16, int W, int NP>
 __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   constexpr int L = D / 16, kThreads = W * 32, RPP = kThreads / L;  // rows a turn
   const int tid = threadIdx.x % kThreads, lane = tid & 31, l = tid % L;
@@ -310,17 +340,10 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   const int page =
       slot_page < p.max_pages ? p.page_table[(int64_t)b * p.table_stride + slot_page] : -1;
   const bool turned = !is_v && p.rope.cos_t != nullptr;
-  if (page < 0 || page >= p.pages || (turned && tok0 + cnt > p.rope.max_pos)) {
-    if (tid == 0) atomicCAS(p.rope.err, 0, kErrKvRange);  // no such page or position: not stored
-    return;
-  }
   const HeadsIn& x = is_v ? p.v : p.k;
-  const size_t block = (size_t)page * p.kv_heads + h;
-  float* scale_at = (is_v ? p.v_scale : p.k_scale) + block;
-  uint8_t* codes = (is_v ? p.v_cache : p.k_cache) + block * p.page * D;
-  const float old = slot0 > 0 ? *scale_at : 0.f;
+  const bool no_turn = turned && tok0 + cnt > p.rope.max_pos;
 
-  float a[NP][8], c[NP][8];
+  F8 a[NP], c[NP];
   auto load = [&](int base) {  // rows base + i RPP + tid / L, normed and turned
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -331,26 +354,37 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
         va = *reinterpret_cast<const uint4*>(src);
         vb = *reinterpret_cast<const uint4*>(src + D / 2);
       }
-      unpack8(va, p.rope.bf16, a[i]);
-      unpack8(vb, p.rope.bf16, c[i]);
+      a[i] = unpack8<BF16>(va);
+      c[i] = unpack8<BF16>(vb);
       if (!is_v) {
         Turn t;
-        if (turned && r < cnt)
-          load_turn<D>(p.rope.cos_t, p.rope.sin_t, p.rope.table_type, tok0 + r, l, t);
-        norm_turn<D>(a[i], c[i], p.rope.k_norm != nullptr, p.rope.k_norm, p.rope.bf16, p.rope.eps,
-                     l, turned && r < cnt, t);
+        if (turned)  // a row past the block's: any table row, its zeros stay zeros
+          load_turn<D>(p.rope.cos_t, p.rope.sin_t, p.rope.table_type,
+                       no_turn ? 0 : r < cnt ? tok0 + r : tok0, l, t);
+        if (p.rope.k_norm) weigh<D, BF16>(p.rope.k_norm, l, turned, t);
+        norm_turn<D>(a[i], c[i], p.rope.k_norm != nullptr, p.rope.eps, turned, t);
       }
     }
   };
+  load(0);  // on its way beside the page's number
+  if (page < 0 || page >= p.pages || no_turn) {
+    if (tid == 0) atomicCAS(p.rope.err, 0, kErrKvRange);  // no such page or position: not stored
+    return;
+  }
+  const size_t block = (size_t)page * p.kv_heads + h;
+  float* scale_at = (is_v ? p.v_scale : p.k_scale) + block;
+  uint8_t* codes = (is_v ? p.v_cache : p.k_cache) + block * p.page * D;
+  const float old = slot0 > 0 ? *scale_at : 0.f;
   float amax = 0.f;
 #pragma unroll 1
   for (int base = 0; base < cnt; base += NP * RPP) {
-    load(base);
+    if constexpr (W == 1)
+      if (base > 0) load(base);
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {  // infinities and NaN do not set the scale (rows past cnt: 0)
-        const float u = fabsf(a[i][j]), w = fabsf(c[i][j]);
+        const float u = fabsf(a[i].f[j]), w = fabsf(c[i].f[j]);
         amax = fmaxf(amax, fmaxf(u <= 3.4028234e38f ? u : 0.f, w <= 3.4028234e38f ? w : 0.f));
       }
   }
@@ -372,7 +406,8 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   const float inv = 1.0f / scale;  // a power of two, unless the block's own scale was none
 #pragma unroll 1
   for (int base = 0; base < cnt; base += NP * RPP) {
-    if (cnt > NP * RPP) load(base);
+    if constexpr (W == 1)
+      if (cnt > NP * RPP) load(base);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int r = base + i * RPP + tid / L;
@@ -390,40 +425,48 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
     for (int i = tid; i < slot0 * (D / 8); i += kThreads) {
       uint2* at = reinterpret_cast<uint2*>(codes) + i;
       const uint2 v = *at;
-      float f[8];
       const uint32_t w[2] = {v.x, v.y};
+      F8 f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(
             (__nv_fp8x2_storage_t)((w[j >> 1] >> (16 * (j & 1))) & 0xffffu), __NV_E4M3);
         const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-        f[2 * j] = f2.x;
-        f[2 * j + 1] = f2.y;
+        f.f[2 * j] = f2.x;
+        f.f[2 * j + 1] = f2.y;
       }
       *at = to_e4m3x8(f, ratio);
     }
   }
 }
 
-template <int D, int W, int NP>
+template <int D, bool BF16, int W, int NP>
 __global__ void __launch_bounds__(kAppendThreads, W == 1 ? 3 : NP == 4 ? 2 : 3)
     append_kernel(const AppendParams p) {
   if ((int)blockIdx.x < p.kv_blocks) {
     const int unit = W == 1 ? (int)blockIdx.x * (kAppendThreads / 32) + (int)(threadIdx.x >> 5)
                             : (int)blockIdx.x;
-    if (unit < p.kv_units) append_block<D, W, NP>(p, unit);
+    if (unit < p.kv_units) append_block<D, BF16, W, NP>(p, unit);
     return;
   }
   // queries: a warp takes a row's heads, or a part of them
-  constexpr int HPW = 32 / (D / 16);
   const int lane = threadIdx.x & 31;
   const RopeParams& r = p.rope;
-  const int groups = (r.heads + HPW - 1) / HPW;
+  const int groups = head_groups<D>(r.heads);
   const int per_row = (groups + r.groups_per_warp - 1) / r.groups_per_warp;
   const int64_t unit =
       (int64_t)(blockIdx.x - p.kv_blocks) * (kAppendThreads / 32) + (threadIdx.x >> 5);
   const int64_t row = unit / per_row;
   if (row >= p.rows) return;
+  const int g0 = (int)(unit - row * per_row) * r.groups_per_warp;
+  const int g1 = min(groups, g0 + r.groups_per_warp);
+  {  // the heads on their way while the row's position is looked up
+    constexpr int kLanes = D / 64;  // lanes a head: one a 128-byte line
+    for (int h = g0 * (32 / (D / 16)) + lane / kLanes; h < min(r.heads, g1 * (32 / (D / 16)));
+         h += 32 / kLanes)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(r.q.p + row * r.q.row + h * r.q.head +
+                                                    64 * (lane % kLanes)));
+  }
   int b = 0;  // the sequence: as many as end at or before this row
 #pragma unroll 1
   for (int b0 = 0; b0 < p.seqs; b0 += 32) {
@@ -436,8 +479,14 @@ __global__ void __launch_bounds__(kAppendThreads, W == 1 ? 3 : NP == 4 ? 2 : 3)
     if (lane == 0) atomicCAS(r.err, 0, kErrKvRange);
     return;
   }
-  const int h0 = (int)(unit - row * per_row) * r.groups_per_warp * HPW;
-  rope_heads<D, 1>(r, row, pos, h0, min(r.heads, h0 + r.groups_per_warp * HPW), lane);
+  rope_row<D, BF16>(r, row, pos, g0, g1, lane);
+}
+
+template <int D, bool BF16>
+auto append_fn(bool by_warp, int np) -> void (*)(AppendParams) {
+  if (by_warp) return append_kernel<D, BF16, 1, 1>;
+  if (np == 4) return append_kernel<D, BF16, 8, D == 128 ? 4 : 2>;  // pages of 128, D = 128
+  return np == 2 ? append_kernel<D, BF16, 8, 2> : append_kernel<D, BF16, 8, 1>;
 }
 
 HeadsIn heads_in(const w4_heads& x) {
@@ -486,14 +535,15 @@ int launch_norm_rope(const w4_heads& q, const w4_heads& k, const w4_heads& q_out
   p.k_out_head = k_out.head_stride;
   p.positions = positions;
   p.rows = rows;
-  p.bf16 = bf16;
-  const int hpw = 32 / (head_dim / 16);
-  const int groups = (p.heads + p.kv_heads + hpw - 1) / hpw;
+  const int groups = head_dim == 128 ? head_groups<128>(p.heads) + head_groups<128>(p.kv_heads)
+                                     : head_groups<64>(p.heads) + head_groups<64>(p.kv_heads);
   p.groups_per_warp = groups_per_warp(rows, groups, di.sm_count);
   const int64_t units = (int64_t)rows * ((groups + p.groups_per_warp - 1) / p.groups_per_warp);
   const int64_t blocks = (units + kRopeThreads / 32 - 1) / (kRopeThreads / 32);
   if (blocks > 0x7fffffff) return fail(W4_ERR_UNSUPPORTED, "w4_qk_norm_rope: %d rows", rows);
-  void (*fn)(RopeParams) = head_dim == 128 ? norm_rope_kernel<128, 2> : norm_rope_kernel<64, 2>;
+  void (*fn)(RopeParams) = head_dim == 128
+                               ? (bf16 ? norm_rope_kernel<128, true> : norm_rope_kernel<128, false>)
+                               : (bf16 ? norm_rope_kernel<64, true> : norm_rope_kernel<64, false>);
   fn<<<(unsigned)blocks, kRopeThreads, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_qk_norm_rope launch");
@@ -506,7 +556,6 @@ int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_hea
   p.rope = rope_params(rope, di);
   set_queries(p.rope, q, q_out);
   p.rope.rows = bt.rows;
-  p.rope.bf16 = bf16;
   p.k = heads_in(k);
   p.v = heads_in(v);
   p.k_cache = static_cast<uint8_t*>(c.k);
@@ -532,8 +581,7 @@ int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_hea
   const bool by_warp = bt.rows <= 4 * (int64_t)bt.seqs;
   const int64_t kv_blocks =
       by_warp ? (kv_units + kAppendThreads / 32 - 1) / (kAppendThreads / 32) : kv_units;
-  const int hpw = 32 / (c.head_dim / 16);
-  const int groups = (q.heads + hpw - 1) / hpw;
+  const int groups = c.head_dim == 128 ? head_groups<128>(q.heads) : head_groups<64>(q.heads);
   p.rope.groups_per_warp = groups_per_warp(bt.rows, groups, di.sm_count);
   const int64_t units =
       (int64_t)bt.rows * ((groups + p.rope.groups_per_warp - 1) / p.rope.groups_per_warp);
@@ -543,16 +591,11 @@ int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_hea
   p.kv_units = (int)kv_units;
   p.kv_blocks = (int)kv_blocks;
   const int np = std::max(1, c.page_size * (c.head_dim / 16) / kAppendThreads);
-  void (*fn)(AppendParams);
-  if (c.head_dim == 128)
-    fn = by_warp   ? append_kernel<128, 1, 1>
-         : np == 4 ? append_kernel<128, 8, 4>
-         : np == 2 ? append_kernel<128, 8, 2>
-                   : append_kernel<128, 8, 1>;
-  else
-    fn = by_warp   ? append_kernel<64, 1, 1>
-         : np == 2 ? append_kernel<64, 8, 2>
-                   : append_kernel<64, 8, 1>;
+  void (*fn)(AppendParams) = c.head_dim == 128
+                                 ? (bf16 ? append_fn<128, true>(by_warp, np)
+                                         : append_fn<128, false>(by_warp, np))
+                                 : (bf16 ? append_fn<64, true>(by_warp, np)
+                                         : append_fn<64, false>(by_warp, np));
   fn<<<(unsigned)blocks, kAppendThreads, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_kv8_append launch");
