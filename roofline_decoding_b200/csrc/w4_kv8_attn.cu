@@ -4,8 +4,8 @@
 //
 // with e4m3 codes k_j, v_j, and sk_j, sv_j the scales of their page and head.
 // The query rows of one cache head (G query heads times the sequence's new
-// tokens) form 16-row tiles; an item is (sequence, cache head, row tile), and
-// its work is its 32-token tiles of the cache.
+// tokens) form tiles of 8, 16 or 32 rows; an item is (sequence, cache head, row
+// tile), and its work is its 32-token tiles of the cache.
 //
 // Bound by the cache's bytes at the small row counts of decoding (2 D bytes a
 // token and cache head against 4 D operations a query row), so the design is
@@ -20,12 +20,17 @@
 // fp32 partials that a second, programmatically dependent launch joins in
 // order; nothing is atomic, so results repeat bit for bit.
 //
-// Arithmetic: mma.sync m16n8k16 in fp16 with fp32 sums. e4m3 widens to fp16
-// exactly. Queries enter scaled by a power of two a row that brings their
-// largest element to 2^14 (bf16 to fp16 is then exact but for elements 2^-28
-// below the row's largest). The page's value scale is folded into the
-// exponent: P' = exp2(s + log2 sv - m + 14) with m the running maximum of
-// s + log2 sv, so P' is at most 2^14, its rounding to fp16 (11 bits) stays
+// Arithmetic: mma.sync m16n8k16 in fp16 with fp32 sums, transposed: the cache
+// is the 16-wide operand (S^T = K Q^T, O^T = V^T P^T) and the query rows the
+// 8-wide one, so that a decoding step's few rows leave little of a product
+// unused, every widened K or V register serves all row blocks, and softmax and
+// output take half the registers of the 16-row form (470 instead of 900
+// instructions a tile). P^T turns from result to operand by movmatrix. e4m3
+// widens to fp16 exactly. Queries enter scaled by a power of two a row that
+// brings their largest element to 2^14 (bf16 to fp16 is then exact but for
+// elements 2^-28 below the row's largest). The page's value scale is folded
+// into the exponent: P' = exp2(s + log2 sv - m + 14) with m the running maximum
+// of s + log2 sv, so P' is at most 2^14, its rounding to fp16 (11 bits) stays
 // relative down to 2^-28 of the largest weight, and the fp32 sum adds
 // P' / sv, unrounded.
 #include "w4_internal.h"
@@ -40,26 +45,32 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;        // tokens of one ring stage of a warp
-constexpr int kRows = 16;        // query rows of an item
 constexpr int kCtasPerSm = 2;
 constexpr float kShift = 14.0f;  // P' is at most 2^kShift
 // Tiles a CTA takes at least (one a warp): below that more CTAs only add
 // partials to join.
 constexpr int kMinTiles = kWarps;
 
-template <int D>
+// NT: 8-row blocks of an item (1, 2 or 4).
+template <int D, int NT>
 struct AttnShape {
+  static constexpr int kRows = 8 * NT;               // query rows of an item
   static constexpr int kStageBytes = 2 * kTile * D;  // K, then V
-  static constexpr int kStages = D == 128 ? 3 : 5;
+  static constexpr int kStages = D == 128 ? (NT == 4 ? 2 : 3) : (NT == 4 ? 4 : 5);
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kScales = kWarps * kStages * 16;  // per stage: K, V scale of two halves
   static constexpr int kPitch = D + 4;                   // floats; the 4 hold maximum and sum
   static constexpr int kMerge = 2 * kRows * kPitch * 4;  // two warps' outputs
   static constexpr int kMarks = kRows * D / 8;  // one bit an output: a NaN value reached it
-  static constexpr int kSmem = kRing + kScales + kMerge + kMarks;
-  static constexpr int kKSteps = D / 16;   // 16-dim steps of Q K^T
-  static constexpr int kNTiles = D / 8;    // 8-dim tiles of P V
-  static constexpr int kWords = D / 32;    // 32-bit words of a lane's V chunk
+  static constexpr int kKSteps = D / 16;        // 16-dim steps of K Q^T
+  static constexpr int kMTiles = D / 16;        // 16-dim tiles of V^T P^T
+  static constexpr int kWords = D / 32;         // 32-bit words of a lane's V chunk
+  // four row blocks' queries do not fit the registers: their fragments and
+  // factors stay in shared memory
+  static constexpr bool kSharedQ = NT == 4;
+  static constexpr int kQ = kSharedQ ? kKSteps * NT * 32 * 8 + kRows * 4 : 0;
+  static constexpr int kSmem = kRing + kScales + kMerge + kMarks + kQ;
+  static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 struct AttnP {
@@ -76,7 +87,7 @@ struct AttnP {
   int64_t out_row, out_head;
   int bf16;
   float scale_log2;
-  float* parts;       // [CTAs][2][kRows][D + 4]
+  float* parts;       // [CTAs][2][rows of an item][D + 4]
   struct Join* join;  // [CTAs]
   int* err;
 };
@@ -118,7 +129,11 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Zeros where it is not `real` (src is a valid address all the same).
+__device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(real ? 16 : 0)
                : "memory");
@@ -137,7 +152,8 @@ __device__ __forceinline__ void cp_wait() {
 // Byte offset of 16-byte chunk c of row r in a tile. Chunks are XOR-ed with
 // the 128-byte line's number, so that neither the K reads (8 lanes: two rows,
 // every second chunk) nor, at D = 128, the V reads (four rows, two chunks) of a
-// quarter warp share a bank.
+// quarter warp share a bank. The loops use the same map in lane constants: a
+// step of 8 rows (D = 128) or of 8 or 16 (D = 64) keeps or flips bit 6.
 template <int D>
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   if constexpr (D == 128) {
@@ -174,6 +190,7 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
 __device__ __forceinline__ int seen(const AttnP& p, const Seq& s, int r) {
   return min(s.past + by_group(p, r) + 1, p.capacity);
 }
+template <int kRows>
 __device__ __forceinline__ int row_tiles(const AttnP& p, const Seq& s) {
   return (s.n * p.group + kRows - 1) / kRows;
 }
@@ -182,8 +199,9 @@ __device__ __forceinline__ int row_tiles(const AttnP& p, const Seq& s) {
 __device__ __forceinline__ int token_tiles(const AttnP& p, const Seq& s) {
   return (min(s.past + s.n, p.capacity) + kTile - 1) / kTile;
 }
+template <int kRows>
 __device__ __forceinline__ int64_t seq_work(const AttnP& p, const Seq& s) {
-  return s.n > 0 ? (int64_t)p.kv_heads * row_tiles(p, s) * token_tiles(p, s) : 0;
+  return s.n > 0 ? (int64_t)p.kv_heads * row_tiles<kRows>(p, s) * token_tiles(p, s) : 0;
 }
 
 // The CTAs' shares of the line of all tiles: `per` tiles each, the last ones
@@ -204,6 +222,7 @@ __device__ __forceinline__ int64_t scan32(int64_t v, int lane) {
   return v;
 }
 
+template <int kRows>
 __device__ __forceinline__ Share find_share(const AttnP& p) {
   const int lane = threadIdx.x & 31;
   Share f;
@@ -213,7 +232,7 @@ __device__ __forceinline__ Share find_share(const AttnP& p) {
     w = 0;
     if (b0 + lane < p.seqs) {
       const Seq s = load_seq(p, b0 + lane);
-      w = seq_work(p, s);
+      w = seq_work<kRows>(p, s);
       const int told = p.lengths[b0 + lane];
       if (s.n > 0 && (told < 0 || told > p.capacity - s.n)) atomicCAS(p.err, 0, kErrKvRange);
     }
@@ -230,7 +249,7 @@ __device__ __forceinline__ Share find_share(const AttnP& p) {
 #pragma unroll 1
   for (int b0 = 0;; b0 += 32) {
     if (p.seqs > 32)  // else the first pass has left them
-      w = scan32(b0 + lane < p.seqs ? seq_work(p, load_seq(p, b0 + lane)) : 0, lane);
+      w = scan32(b0 + lane < p.seqs ? seq_work<kRows>(p, load_seq(p, b0 + lane)) : 0, lane);
     const unsigned hit = __ballot_sync(0xffffffffu, before + w > f.x);
     if (hit || b0 + 32 >= p.seqs) {
       const int src = hit ? __ffs(hit) - 1 : 31;
@@ -244,6 +263,7 @@ __device__ __forceinline__ Share find_share(const AttnP& p) {
 }
 
 // Walks a CTA's share item by item.
+template <int kRows>
 struct Walk {
   int64_t x, end;  // next tile of the line, end of the share
   int b;           // sequence of x
@@ -260,13 +280,13 @@ struct Walk {
   __device__ __forceinline__ bool next(const AttnP& p) {
     if (x >= end) return false;
     s = load_seq(p, b);
-    for (int64_t w; off >= (w = seq_work(p, s));) {  // sequences without rows, or just done
+    for (int64_t w; off >= (w = seq_work<kRows>(p, s));) {  // sequences without rows, or just done
       off -= w;
       if (++b >= p.seqs) return false;
       s = load_seq(p, b);
     }
     nt = token_tiles(p, s);
-    const int nrt = row_tiles(p, s);
+    const int nrt = row_tiles<kRows>(p, s);
     const int64_t item = divide(off, nt);
     h = (int)divide(item, nrt);
     rt = (int)(item - (int64_t)h * nrt);
@@ -281,75 +301,154 @@ struct Walk {
   }
 };
 
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The queries of 8 rows as the B operand: row `row` (this lane's, of n_rows) is
+// scaled to 2^14, step s of lane t is dims D/4 t + 4 s .. + 3, the order of the
+// K words. Returns the factor that turns a sum into log2 units, but for the
+// key scale.
 template <int D>
+__device__ __forceinline__ float load_queries(const AttnP& p, const Seq& s, int h, int row,
+                                              int n_rows, int t, uint32_t (&b)[D / 16][2]) {
+  const int i = by_group(p, row);
+  const bool in = row < n_rows;
+  uint4 raw[D / 32];
+  const uint16_t* src = p.q + (int64_t)(s.first + i) * p.q_row +
+                        (int64_t)(h * p.group + row - i * p.group) * p.q_head + (D / 4) * t;
+#pragma unroll
+  for (int w = 0; w < D / 32; ++w)
+    raw[w] = in ? __ldg(reinterpret_cast<const uint4*>(src) + w) : make_uint4(0u, 0u, 0u, 0u);
+  const uint32_t* rw = reinterpret_cast<const uint32_t*>(raw);
+  float f[D / 4];
+  float amax = 0.f;
+#pragma unroll
+  for (int w = 0; w < D / 8; ++w) {
+    float2 v;
+    if (p.bf16)
+      v = make_float2(__uint_as_float(rw[w] << 16), __uint_as_float(rw[w] & 0xffff0000u));
+    else
+      v = __half22float2(*reinterpret_cast<const __half2*>(&rw[w]));
+    f[2 * w] = v.x;
+    f[2 * w + 1] = v.y;
+    amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  // 2^(14 - exponent of amax), within what fp32 holds
+  const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
+  const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    b[k][0] = half2_bits(f[4 * k] * up, f[4 * k + 1] * up);
+    b[k][1] = half2_bits(f[4 * k + 2] * up, f[4 * k + 3] * up);
+  }
+  return p.scale_log2 * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+}
+
+template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(const AttnP p) {
-  using S = AttnShape<D>;
+  using S = AttnShape<D, NT>;
+  constexpr int kRows = S::kRows;
   extern __shared__ __align__(128) uint8_t smem_kv8[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem_kv8) + warp * S::kStages * S::kStageBytes;
   float* scales = reinterpret_cast<float*>(smem_kv8 + S::kRing) + warp * S::kStages * 4;
   float* merge = reinterpret_cast<float*>(smem_kv8 + S::kRing + S::kScales);
-
   uint32_t* marks = reinterpret_cast<uint32_t*>(merge + S::kMerge / 4);
+  uint2* shared_q = reinterpret_cast<uint2*>(marks + S::kMarks / 4);        // kSharedQ only
+  float* shared_mul = reinterpret_cast<float*>(shared_q + S::kKSteps * NT * 32);
 
   grid_launch_dependents();
-  const Share share = find_share(p);
+  const Share share = find_share<kRows>(p);
   if (tid == 0) p.join[blockIdx.x].count = 0;
   if (share.x >= share.end) return;
   for (int i = tid; i < S::kMarks / 4; i += kThreads) marks[i] = 0u;
   __syncthreads();
 
   // ---- the load side: this warp's tiles, kStages - 1 ahead of the compute side
-  Walk lw;
+  Walk<kRows> lw;
   lw.x = share.x, lw.end = share.end, lw.b = share.b, lw.off = share.off;
-  Walk cw = lw;
+  Walk<kRows> cw = lw;
   bool more = lw.next(p);
   int lt = more ? lw.t0 + warp : 0;
+  // Page numbers of the warp's next 16 tiles, two halves of 16 tokens each: lane
+  // 2 k + half has those of tile k.
+  int ids = -1, id_at = 16;
+  auto fetch_ids = [&]() {
+    const int tile = lt + kWarps * (lane >> 1);
+    const int tok = tile * kTile + 16 * (lane & 1);
+    ids = -1;
+    if (tile < lw.t1 && tok < lw.limit) {
+      const int pi = tok >> p.page_shift;
+      if (pi < p.max_pages) ids = p.page_table[lw.b * p.table_stride + pi];
+      if ((uint32_t)ids >= (uint32_t)p.pages) {
+        ids = -1;
+        atomicCAS(p.err, 0, kErrKvRange);
+      }
+    }
+    id_at = 0;
+  };
+  if (more) fetch_ids();
   int issue_slot = 0;
+  // this lane's 16 bytes of a 512-byte pass, in global and in shared memory
+  const uint32_t src_lane = 16 * lane;
+  const uint32_t dst_lane = chunk_at<D>(lane / (D / 16), lane % (D / 16));
+  const ptrdiff_t v_from_k = p.v - p.k;
   auto issue = [&]() {
-    while (more && lt >= lw.t1) {
-      more = lw.next(p);
-      lt = lw.t0 + warp;
+    if (more && lt >= lw.t1) {
+      do {
+        more = lw.next(p);
+        lt = lw.t0 + warp;
+      } while (more && lt >= lw.t1);
+      id_at = 16;
     }
     if (more) {
+      if (id_at == 16) fetch_ids();
       const int tok0 = lt * kTile;
-      // the (one or two) pages of the tile: halves of 16 tokens
-      int id = -1;
-      if (lane < 2) {
-        const int at = tok0 + 16 * lane;
-        const int pi = at >> p.page_shift;
-        if (at < lw.limit) {
-          id = pi < p.max_pages ? p.page_table[lw.b * p.table_stride + pi] : -1;
-          if (id < 0 || id >= p.pages) {
-            id = -1;
-            atomicCAS(p.err, 0, kErrKvRange);
-          }
-        }
+      const int id0 = __shfl_sync(0xffffffffu, ids, 2 * id_at);
+      const int id1 = __shfl_sync(0xffffffffu, ids, 2 * id_at + 1);
+      ++id_at;
+      const uint32_t st = ring + issue_slot * S::kStageBytes + dst_lane;
+      if (lane < 2) {  // the scales of the halves; zero marks one that is left out
+        const int id = lane ? id1 : id0;
         const size_t blk = (size_t)max(id, 0) * p.kv_heads + lw.h;
         const uint32_t dst = smem_u32(scales + issue_slot * 4 + lane);
-        cp4(dst, p.k_scale + blk, id >= 0);  // zero marks a half that is left out
+        cp4(dst, p.k_scale + blk, id >= 0);
         cp4(dst + 8, p.v_scale + blk, id >= 0);
       }
-      const int id0 = __shfl_sync(0xffffffffu, id, 0), id1 = __shfl_sync(0xffffffffu, id, 1);
-      const uint32_t st = ring + issue_slot * S::kStageBytes;
-      constexpr int CPR = D / 16, RPI = 32 / CPR;  // chunks a row, rows a pass
-      const int c = lane % CPR, rr = lane / CPR;
-      const int in_page = p.page - 1;
+      const bool full = tok0 + kTile <= lw.limit && (id0 | id1) >= 0;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int idh = half ? id1 : id0;
-        const int tok = tok0 + 16 * half;
-        const size_t base =
-            (((size_t)max(idh, 0) * p.kv_heads + lw.h) * p.page + (tok & in_page)) * D + 16 * c;
-        const int valid = idh >= 0 ? min(16, lw.limit - tok) : 0;
+        const int id = max(half ? id1 : id0, 0);
+        const uint8_t* src = p.k + src_lane +
+                             ((((size_t)id * p.kv_heads + lw.h) << p.page_shift) +
+                              ((tok0 + 16 * half) & (p.page - 1))) * D;
+        if (full) {
 #pragma unroll
-        for (int i = 0; i < 16 / RPI; ++i) {
-          const int r = i * RPI + rr;
-          const uint32_t dst = st + chunk_at<D>(16 * half + r, c);
-          const size_t src = base + (size_t)(r < valid ? r : 0) * D;
-          cp16(dst, p.k + src, r < valid);
-          cp16(dst + kTile * D, p.v + src, r < valid);
+          for (int i = 0; i < 16 * D / 512; ++i) {
+            const uint32_t dst = (i & 1 ? st ^ 64u : st) + half * 16 * D + i * 512;
+            cp16(dst, src + i * 512);
+            cp16(dst + kTile * D, src + v_from_k + i * 512);
+          }
+        } else {  // rows behind the limit, and those of no page, become zeros
+          const int valid = (half ? id1 : id0) >= 0 ? lw.limit - tok0 - 16 * half : 0;
+#pragma unroll
+          for (int i = 0; i < 16 * D / 512; ++i) {
+            const uint32_t dst = (i & 1 ? st ^ 64u : st) + half * 16 * D + i * 512;
+            const bool real = i * (512 / D) + lane / (D / 16) < valid;
+            cp16_if(dst, src + i * 512, real);
+            cp16_if(dst + kTile * D, src + v_from_k + i * 512, real);
+          }
         }
       }
       lt += kWarps;
@@ -360,62 +459,70 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
 #pragma unroll 1
   for (int i = 0; i < S::kStages - 1; ++i) issue();
 
+  // lane constants of the K reads (token g, chunk c; token g + 8) and V reads
+  // (tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9)
+  uint32_t k_at[D / 64], k_at8[D / 64], v_at[4];
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    k_at[c] = chunk_at<D>(g, (D / 64) * t + c);
+    k_at8[c] = chunk_at<D>(g + 8, (D / 64) * t + c);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v_at[i] = kTile * D + (D == 128 ? chunk_at<D>(2 * t + (i & 1) + 8 * (i >> 1), g)
+                                    : chunk_at<D>(2 * t + (i & 1) + 8 * (i >> 1), g >> 1) +
+                                          8 * (g & 1));
+
   int slot = 0;
   bool first_segment = true;
   while (cw.next(p)) {
-    // ---- queries of this item: rows g and g + 8 of the tile
+    // ---- queries of this item: row 8 n + g as operand, rows 8 n + 2 t and
+    // 8 n + 2 t + 1 of the results
     const int n_rows = cw.s.n * p.group;
     const int r0 = cw.rt * kRows;
-    uint32_t qf[S::kKSteps][4];
-    float q_mul[2];  // turns a sum into log2 units, but for the key scale
-    int lim[2];      // tokens that the row sees
+    uint32_t qf[S::kSharedQ ? 1 : NT][S::kKSteps][2];
+    float q_mul[NT][2];
+    if constexpr (S::kSharedQ) {
+      const float mul = load_queries<D>(p, cw.s, cw.h, r0 + 8 * warp + g, n_rows, t, qf[0]);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = r0 + g + 8 * j;
-      const int i = by_group(p, r);
-      const bool in = r < n_rows;
-      lim[j] = in ? seen(p, cw.s, r) : 0;
-      uint4 raw[D / 32];
-      const uint16_t* src = p.q + (int64_t)(cw.s.first + i) * p.q_row +
-                            (int64_t)(cw.h * p.group + r - i * p.group) * p.q_head + (D / 4) * t;
+      for (int k = 0; k < S::kKSteps; ++k)
+        shared_q[(k * NT + warp) * 32 + lane] = make_uint2(qf[0][k][0], qf[0][k][1]);
+      if (t == 0) shared_mul[8 * warp + g] = mul;
+      __syncthreads();
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w)
-        raw[w] = in ? __ldg(reinterpret_cast<const uint4*>(src) + w) : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t* rw = reinterpret_cast<const uint32_t*>(raw);
-      float f[D / 4];
-      float amax = 0.f;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int w = 0; w < D / 8; ++w) {
-        float2 v;
-        if (p.bf16)
-          v = make_float2(__uint_as_float(rw[w] << 16), __uint_as_float(rw[w] & 0xffff0000u));
-        else
-          v = __half22float2(*reinterpret_cast<const __half2*>(&rw[w]));
-        f[2 * w] = v.x;
-        f[2 * w + 1] = v.y;
-        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
-      }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // 2^(14 - exponent of amax), within what fp32 holds
-      const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
-      const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-      q_mul[j] = p.scale_log2 * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-      // step s of this lane: dims D/4 t + 4 s .. + 3, the order of the K words
+        for (int r = 0; r < 2; ++r) q_mul[n][r] = shared_mul[8 * n + 2 * t + r];
+    } else {
 #pragma unroll
-      for (int s = 0; s < S::kKSteps; ++s) {
-        qf[s][j] = half2_bits(f[4 * s] * up, f[4 * s + 1] * up);
-        qf[s][j + 2] = half2_bits(f[4 * s + 2] * up, f[4 * s + 3] * up);
+      for (int n = 0; n < NT; ++n) {
+        const float mul = load_queries<D>(p, cw.s, cw.h, r0 + 8 * n + g, n_rows, t, qf[n]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          q_mul[n][r] = __shfl_sync(0xffffffffu, mul, 4 * (2 * t + r));
       }
     }
-    const int low = __reduce_min_sync(0xffffffffu,
-                                      min(lim[0] > 0 ? lim[0] : 0x7fffffff,
-                                          lim[1] > 0 ? lim[1] : 0x7fffffff));
-
-    float o[S::kNTiles][4];
+    int lim[NT][2];  // tokens that the row sees
+    int low = 0x7fffffff;
 #pragma unroll
-    for (int j = 0; j < S::kNTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = r0 + 8 * n + 2 * t + r;
+        lim[n][r] = row < n_rows ? seen(p, cw.s, row) : 0;
+        if (lim[n][r] > 0) low = min(low, lim[n][r]);
+      }
+    low = __reduce_min_sync(0xffffffffu, low);
+
+    float o[NT][S::kMTiles][4];
+    float m[NT][2], l[NT][2], sub[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < S::kMTiles; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) m[n][r] = -INFINITY, l[n][r] = 0.f, sub[n][r] = 0.f;
+    }
 
 #pragma unroll 1
     for (int tile = cw.t0 + warp; tile < cw.t1; tile += kWarps) {
@@ -423,102 +530,114 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       __syncwarp();  // this stage has landed, and the stage before it is read
       issue();
       const uint32_t st = ring + slot * S::kStageBytes;
-      const float* sc = scales + slot * 4;
-      // ---- S = Q K^T: a lane's K words are dims D/4 t .. of token 8 j + g
-      float s[4][4];
+      // ---- S^T = K Q^T: tokens 16 i + g and + 8, a lane's K words are dims D/4 t ..
+      float s[2][NT][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          const uint4 kw = lds128(st + chunk_at<D>(8 * j + g, (D / 64) * t + c));
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&kw);
+        for (int n = 0; n < NT; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t(&a)[4] = qf[4 * c + i];
-            mma_16816<false>(s[j], a[0], a[1], a[2], a[3], e4m3_lo(w[i]), e4m3_hi(w[i]));
+      for (int c = 0; c < D / 64; ++c) {
+        uint4 ka[2], kb[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ka[i] = lds128(st + k_at[c] + i * 16 * D);
+          kb[i] = lds128(st + k_at8[c] + i * 16 * D);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int k = 4 * c + w;
+          uint32_t b[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (S::kSharedQ) {
+              const uint2 v = shared_q[(k * NT + n) * 32 + lane];
+              b[n][0] = v.x, b[n][1] = v.y;
+            } else {
+              b[n][0] = qf[n][k][0], b[n][1] = qf[n][k][1];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = reinterpret_cast<const uint32_t*>(&ka[i])[w];
+            const uint32_t y = reinterpret_cast<const uint32_t*>(&kb[i])[w];
+            const uint32_t a0 = e4m3_lo(x), a1 = e4m3_lo(y), a2 = e4m3_hi(x), a3 = e4m3_hi(y);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816<false>(s[i][n], a0, a1, a2, a3, b[n][0], b[n][1]);
           }
         }
       }
       // ---- scores in log2 units with the value scale, masked
-      float t_max[2] = {-INFINITY, -INFINITY};
-      float inv_vs[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float ks = sc[half], vs = sc[2 + half];
-        const float lv = vs > 0.f ? log2f(vs) : -INFINITY;
-        inv_vs[half] = vs > 0.f ? 1.0f / vs : 0.f;
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          float(&x)[4] = s[2 * half + jj];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = fmaf(x[i], q_mul[i >> 1] * ks, lv);
-        }
-      }
+      const float4 sc = *reinterpret_cast<const float4*>(scales + slot * 4);
+      const float ks[2] = {sc.x, sc.y};
+      const float lv[2] = {sc.z > 0.f ? lg2(sc.z) : -INFINITY, sc.w > 0.f ? lg2(sc.w) : -INFINITY};
       const int tok0 = tile * kTile;
-      if (tok0 + kTile > low) {  // some row ends inside the tile, or before it
+      const bool cut = tok0 + kTile > low;  // some row ends inside the tile, or before it
+      float top[NT][2];  // this lane's largest score of each row
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (tok0 + 8 * j + 2 * t + (i & 1) >= lim[i >> 1]) s[j][i] = -INFINITY;
-      }
+        for (int r = 0; r < 2; ++r) {  // elements r and r + 2 are row r's
+          const float f[2] = {q_mul[n][r] * ks[0], q_mul[n][r] * ks[1]};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t_max[i >> 1] = fmaxf(t_max[i >> 1], s[j][i]);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        t_max[r] = fmaxf(t_max[r], __shfl_xor_sync(0xffffffffu, t_max[r], 1));
-        t_max[r] = fmaxf(t_max[r], __shfl_xor_sync(0xffffffffu, t_max[r], 2));
-      }
-      if (__any_sync(0xffffffffu, t_max[0] > m[0] || t_max[1] > m[1])) {
-        float al[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float nm = fmaxf(m[r], t_max[r]);
-          al[r] = nm == m[r] ? 1.f : ex2(m[r] - nm);
-          m[r] = nm;
-          l[r] *= al[r];
+            for (int e = r; e < 4; e += 2) {
+              float& x = s[i][n][e];
+              x = fmaf(x, f[i], lv[i]);
+              if (cut && tok0 + 16 * i + g + 8 * (e >> 1) >= lim[n][r]) x = -INFINITY;
+            }
+          top[n][r] = fmaxf(fmaxf(s[0][n][r], s[0][n][r + 2]), fmaxf(s[1][n][r], s[1][n][r + 2]));
         }
+      bool larger = false;
 #pragma unroll
-        for (int j = 0; j < S::kNTiles; ++j) {
-          o[j][0] *= al[0];
-          o[j][1] *= al[0];
-          o[j][2] *= al[1];
-          o[j][3] *= al[1];
+      for (int n = 0; n < NT; ++n) larger |= top[n][0] > m[n][0] || top[n][1] > m[n][1];
+      if (__any_sync(0xffffffffu, larger)) {  // seldom after the first tiles
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float most = top[n][r];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1)
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+            most = fmaxf(most, m[n][r]);
+            const float al = m[n][r] == -INFINITY ? 0.f : ex2(m[n][r] - most);
+            m[n][r] = most;
+            sub[n][r] = most == -INFINITY ? 0.f : most - kShift;
+            l[n][r] *= al;
+#pragma unroll
+            for (int j = 0; j < S::kMTiles; ++j) {
+              o[n][j][r] *= al;
+              o[n][j][r + 2] *= al;
+            }
+          }
+      }
+      uint32_t pf[2][NT][2];  // P^T as the B operand: 16 tokens a step
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float inv = lv[i] == -INFINITY ? 0.f : ex2(-lv[i]);  // 1 / sv
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float(&v)[4] = s[i][n];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = ex2(v[e] - sub[n][e & 1]);
+          l[n][0] = fmaf(v[0] + v[2], inv, l[n][0]);
+          l[n][1] = fmaf(v[1] + v[3], inv, l[n][1]);
+          pf[i][n][0] = transpose8x8(half2_bits(v[0], v[1]));
+          pf[i][n][1] = transpose8x8(half2_bits(v[2], v[3]));
         }
       }
-      const float sub[2] = {m[0] == -INFINITY ? 0.f : m[0] - kShift,
-                            m[1] == -INFINITY ? 0.f : m[1] - kShift};
-      uint32_t pf[2][4];  // P as the A operand: 16 tokens a step
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          float(&x)[4] = s[2 * half + jj];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - sub[i >> 1]);
-          sum[0] += x[0] + x[1];
-          sum[1] += x[2] + x[3];
-          pf[half][2 * jj] = half2_bits(x[0], x[1]);
-          pf[half][2 * jj + 1] = half2_bits(x[2], x[3]);
-        }
-        l[0] = fmaf(sum[0], inv_vs[half], l[0]);
-        l[1] = fmaf(sum[1], inv_vs[half], l[1]);
-      }
-      // ---- O += P V: a lane's V chunks are dims D/8 g .. of tokens 2t, 2t+1,
-      // 2t+8, 2t+9 of each 16; byte pairs of two tokens make the B operand
-      const uint32_t vst = st + kTile * D;
-      if (tok0 + kTile > low && low < cw.limit) {
+      // ---- O^T += V^T P^T: a lane's V chunks are dims D/8 g .. of tokens 2t, 2t+1,
+      // 2t+8, 2t+9 of each 16; byte pairs of two tokens make the A operand
+      if (cut && low < cw.limit) {
         // Rows of this item end at different tokens here, and a NaN that one row
         // sees must not reach a row that does not (0 * NaN): NaN codes leave the
         // tile, and the outputs that they belong to are marked.
 #pragma unroll 1
         for (int i = lane; i < kTile * D / 16; i += 32) {
           const int tok = tok0 + i / (D / 16), c = i % (D / 16);
-          const uint32_t at = vst + chunk_at<D>(i / (D / 16), c);
+          const uint32_t at = st + kTile * D + chunk_at<D>(i / (D / 16), c);
 #pragma unroll 1
           for (int w = 0; w < 4; ++w) {
             const uint32_t v = lds32(at + 4 * w);
@@ -535,18 +654,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         __syncwarp();
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t vw[4][S::kWords];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = 16 * half + 2 * t + (i & 1) + 8 * (i >> 1);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t at = st + v_at[k] + i * 16 * D;
           if constexpr (D == 128) {
-            const uint4 w = lds128(vst + chunk_at<D>(tok, g));
-            vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
+            const uint4 w = lds128(at);
+            vw[k][0] = w.x, vw[k][1] = w.y, vw[k][2] = w.z, vw[k][3] = w.w;
           } else {
-            const uint32_t at = vst + chunk_at<D>(tok, g >> 1) + 8 * (g & 1);
             asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                         : "=r"(vw[i][0]), "=r"(vw[i][1])
+                         : "=r"(vw[k][0]), "=r"(vw[k][1])
                          : "r"(at));
           }
         }
@@ -556,23 +674,28 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
           const uint32_t y0 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
           const uint32_t x1 = __byte_perm(vw[2][w], vw[3][w], 0x5140);
           const uint32_t y1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
-          const uint32_t* a = pf[half];
-          mma_16816<false>(o[4 * w + 0], a[0], a[1], a[2], a[3], e4m3_lo(x0), e4m3_lo(x1));
-          mma_16816<false>(o[4 * w + 1], a[0], a[1], a[2], a[3], e4m3_hi(x0), e4m3_hi(x1));
-          mma_16816<false>(o[4 * w + 2], a[0], a[1], a[2], a[3], e4m3_lo(y0), e4m3_lo(y1));
-          mma_16816<false>(o[4 * w + 3], a[0], a[1], a[2], a[3], e4m3_hi(y0), e4m3_hi(y1));
+          uint32_t a0 = e4m3_lo(x0), a1 = e4m3_hi(x0), a2 = e4m3_lo(x1), a3 = e4m3_hi(x1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            mma_16816<false>(o[n][2 * w], a0, a1, a2, a3, pf[i][n][0], pf[i][n][1]);
+          a0 = e4m3_lo(y0), a1 = e4m3_hi(y0), a2 = e4m3_lo(y1), a3 = e4m3_hi(y1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            mma_16816<false>(o[n][2 * w + 1], a0, a1, a2, a3, pf[i][n][0], pf[i][n][1]);
         }
       }
       slot = slot + 1 == S::kStages ? 0 : slot + 1;
     }
 
-    // ---- merge the warps: 2 and 3 into 0 and 1, then 1 into 0. Column 2t of
-    // o[j] is dim D/8 (2t) + j, column 2t + 1 is D/8 (2t + 1) + j.
+    // ---- merge the warps: 2 and 3 into 0 and 1, then 1 into 0. o[n][j] holds
+    // dims D/8 g + 2 j (elements 0, 1) and + 1 (2, 3) of rows 2 t and 2 t + 1.
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1)
+          l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], off);
     // Two rounds and a last one in which warp 0 leaves the sum: one copy of the
     // code for all, since code that runs once an item costs its fetch.
 #pragma unroll 1
@@ -581,42 +704,41 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       if (warp >= step && warp < max(2 * step, 1)) {
         float* buf = merge + (warp - step) * kRows * S::kPitch;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float* row = buf + (g + 8 * r) * S::kPitch;
-          if (t == 0) row[D] = m[r], row[D + 1] = l[r];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < S::kNTiles; j += 4)
+          for (int r = 0; r < 2; ++r) {
+            float* row = buf + (8 * n + 2 * t + r) * S::kPitch;
+            if (g == 0) row[D] = m[n][r], row[D + 1] = l[n][r];
 #pragma unroll
-            for (int cc = 0; cc < 2; ++cc)
-              *reinterpret_cast<float4*>(row + (D / 8) * (2 * t + cc) + j) =
-                  make_float4(o[j][2 * r + cc], o[j + 1][2 * r + cc], o[j + 2][2 * r + cc],
-                              o[j + 3][2 * r + cc]);
-        }
+            for (int j = 0; j < S::kMTiles; j += 2)
+              *reinterpret_cast<float4*>(row + (D / 8) * g + 2 * j) = make_float4(
+                  o[n][j][r], o[n][j][r + 2], o[n][j + 1][r], o[n][j + 1][r + 2]);
+          }
       }
       __syncthreads();
       if (step == 0) break;
       if (warp < step) {
         const float* buf = merge + warp * kRows * S::kPitch;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float* row = buf + (g + 8 * r) * S::kPitch;
-          const float om = row[D], ol = row[D + 1];
-          const float nm = fmaxf(m[r], om);
-          const float fa = m[r] == -INFINITY ? 0.f : ex2(m[r] - nm);
-          const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
-          m[r] = nm;
-          l[r] = l[r] * fa + ol * fb;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < S::kNTiles; j += 4)
+          for (int r = 0; r < 2; ++r) {
+            const float* row = buf + (8 * n + 2 * t + r) * S::kPitch;
+            const float om = row[D], ol = row[D + 1];
+            const float nm = fmaxf(m[n][r], om);
+            const float fa = m[n][r] == -INFINITY ? 0.f : ex2(m[n][r] - nm);
+            const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
+            m[n][r] = nm;
+            l[n][r] = l[n][r] * fa + ol * fb;
 #pragma unroll
-            for (int cc = 0; cc < 2; ++cc) {
-              const float4 v = *reinterpret_cast<const float4*>(row + (D / 8) * (2 * t + cc) + j);
-              o[j][2 * r + cc] = o[j][2 * r + cc] * fa + v.x * fb;
-              o[j + 1][2 * r + cc] = o[j + 1][2 * r + cc] * fa + v.y * fb;
-              o[j + 2][2 * r + cc] = o[j + 2][2 * r + cc] * fa + v.z * fb;
-              o[j + 3][2 * r + cc] = o[j + 3][2 * r + cc] * fa + v.w * fb;
+            for (int j = 0; j < S::kMTiles; j += 2) {
+              const float4 v = *reinterpret_cast<const float4*>(row + (D / 8) * g + 2 * j);
+              o[n][j][r] = o[n][j][r] * fa + v.x * fb;
+              o[n][j][r + 2] = o[n][j][r + 2] * fa + v.y * fb;
+              o[n][j + 1][r] = o[n][j + 1][r] * fa + v.z * fb;
+              o[n][j + 1][r + 2] = o[n][j + 1][r + 2] * fa + v.w * fb;
             }
-        }
+          }
       }
     }
     // Eight dims of a row a thread: the output of a whole item, or a part that is
@@ -693,9 +815,9 @@ constexpr int kJoinRows = 4;  // blocks an item (each takes every fourth row)
 // Joins the partials of an item: blockIdx.x the border, blockIdx.y the rows.
 // The warps take a row's partials in turn, a lane D/32 dims, and warp 0 adds
 // the warps in order.
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(const AttnP p) {
-  constexpr int V = D / 32, kPitch = AttnShape<D>::kPitch;
+  constexpr int V = D / 32, kPitch = AttnShape<D, NT>::kPitch, kRows = AttnShape<D, NT>::kRows;
   __shared__ float sm[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][D];
   grid_dependency_wait();
   const Join jn = p.join[blockIdx.x];
@@ -763,12 +885,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(const AttnP p
 // CTAs that the workspace has room for: two an SM on the largest sm_100 part.
 constexpr int kMaxCtas = 160 * kCtasPerSm;
 
-template <int D>
+template <int D, int NT>
 int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
-  using S = AttnShape<D>;
-  p.join = reinterpret_cast<Join*>(p.parts + (size_t)kMaxCtas * 2 * kRows * S::kPitch);
+  using S = AttnShape<D, NT>;
+  p.join = reinterpret_cast<Join*>(p.parts + (size_t)kMaxCtas * 2 * S::kRows * S::kPitch);
   const int ctas = std::min(kMaxCtas, kCtasPerSm * di.sm_count);
-  kv8_attention_kernel<D><<<ctas, kThreads, S::kSmem, stream>>>(p);
+  kv8_attention_kernel<D, NT><<<ctas, kThreads, S::kSmem, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "w4_kv8_attention launch");
   cudaLaunchConfig_t cfg = {};
@@ -780,29 +902,38 @@ int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kv8_join_kernel<D>, (const AttnP)p);
+  e = cudaLaunchKernelEx(&cfg, kv8_join_kernel<D, NT>, (const AttnP)p);
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_kv8_attention join launch");
 }
 
 }  // namespace
 
 size_t kv8_attention_workspace_bytes(int head_dim) {
-  return (size_t)kMaxCtas * (2 * kRows * (head_dim + 4) * 4 + sizeof(Join));
+  return (size_t)kMaxCtas * (2 * 32 * (head_dim + 4) * 4 + sizeof(Join));  // 32-row items
+}
+
+template <int D, int NT>
+static int init_attention(const DeviceInfo& di) {
+  constexpr int smem = AttnShape<D, NT>::kSmem;
+  if (smem > di.max_smem_optin)
+    return fail(W4_ERR_UNSUPPORTED, "w4_kv8_attention needs %d B of shared memory", smem);
+  cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<D, NT>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kv8_attention_kernel<D, NT>,
+                             cudaFuncAttributePreferredSharedMemoryCarveout,
+                             cudaSharedmemCarveoutMaxShared);
+  return e == cudaSuccess ? W4_OK : cuda_fail(e, "cudaFuncSetAttribute(kv8 attention)");
 }
 
 int kv8_init_device(const DeviceInfo& di) {
-  const void* fns[] = {(const void*)kv8_attention_kernel<64>, (const void*)kv8_attention_kernel<128>};
-  const int smem[] = {AttnShape<64>::kSmem, AttnShape<128>::kSmem};
-  for (int i = 0; i < 2; ++i) {
-    if (smem[i] > di.max_smem_optin)
-      return fail(W4_ERR_UNSUPPORTED, "w4_kv8_attention needs %d B of shared memory", smem[i]);
-    cudaError_t e = cudaFuncSetAttribute(fns[i], cudaFuncAttributeMaxDynamicSharedMemorySize, smem[i]);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(fns[i], cudaFuncAttributePreferredSharedMemoryCarveout,
-                               cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(kv8 attention)");
-  }
-  return W4_OK;
+  int st = init_attention<64, 1>(di);
+  if (st == W4_OK) st = init_attention<64, 2>(di);
+  if (st == W4_OK) st = init_attention<64, 4>(di);
+  if (st == W4_OK) st = init_attention<128, 1>(di);
+  if (st == W4_OK) st = init_attention<128, 2>(di);
+  if (st == W4_OK) st = init_attention<128, 4>(di);
+  return st;
 }
 
 int launch_kv8_attention(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_heads& q,
@@ -838,9 +969,19 @@ int launch_kv8_attention(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_
   p.scale_log2 = scale * 1.4426950408889634f;
   p.parts = static_cast<float*>(workspace);
   p.err = di.err_word;
-  const int max_rows = (int)std::min<int64_t>(kRows, (int64_t)bt.rows * p.group);
-  return c.head_dim == 128 ? launch<128>(p, max_rows, di, stream)
-                           : launch<64>(p, max_rows, di, stream);
+  // Rows of an item by the rows that a sequence brings on average: wider items
+  // read and widen the cache less often, narrower ones waste less of a step of
+  // few rows.
+  const int64_t avg = ((int64_t)bt.rows + bt.seqs - 1) / bt.seqs * p.group;
+  const int nt = avg <= 8 ? 1 : avg <= 16 ? 2 : 4;
+  const int max_rows = (int)std::min<int64_t>(8 * nt, (int64_t)bt.rows * p.group);
+  if (c.head_dim == 128)
+    return nt == 1   ? launch<128, 1>(p, max_rows, di, stream)
+           : nt == 2 ? launch<128, 2>(p, max_rows, di, stream)
+                     : launch<128, 4>(p, max_rows, di, stream);
+  return nt == 1   ? launch<64, 1>(p, max_rows, di, stream)
+         : nt == 2 ? launch<64, 2>(p, max_rows, di, stream)
+                   : launch<64, 4>(p, max_rows, di, stream);
 }
 
 }  // namespace w4
