@@ -72,8 +72,9 @@ struct GemmParams {
   int act;               // w4_act
   const void* bias;      // [N] of y's type, or null
   const void* residual;  // like y, or null
-  int wait_at_end;  // a launch overlapping the previous one on the stream
-                    // completes only after it (griddepcontrol.wait at exit)
+  int wait_at_end;  // the second launch of a plan runs beside the first and
+                    // completes only after it (griddepcontrol.wait at exit);
+                    // the first waits before it touches global memory
 };
 
 // Tile of BN columns (MMA N = BN, 128 or 256) and its shared memory layout
@@ -352,7 +353,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int KT_all = p.K / kBK;
   const int kt0 = (int)((long long)blockIdx.z * KT_all / p.ksplit);
   const int KT = (int)((long long)(blockIdx.z + 1) * KT_all / p.ksplit) - kt0;
-  grid_launch_dependents();  // a dependent launch may fill the SMs this grid frees
 
   auto load_x = [&](int kt) {
     const int s = kt % S::kStages;
@@ -376,6 +376,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     fence_mbar_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+    if (!p.wait_at_end) grid_dependency_wait();  // the inputs are written
     // the first copies go out while the other warps still set up
     for (int kt = 0; kt < min(S::kPkStages, KT); ++kt) load_w(kt);
     for (int kt = 0; kt < min(S::kStages, KT); ++kt) load_x(kt);
@@ -388,6 +391,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     tc_fence_before();
   }
+  if (!p.wait_at_end) grid_dependency_wait();
+  // A dependent launch may fill the SMs that this grid frees. The second launch
+  // of a plan does not wait before it reads, so it must not start before what
+  // wrote the inputs has ended: not before this wait.
+  grid_launch_dependents();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_d = *tmem_slot;
@@ -861,7 +869,7 @@ int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* sc
       attrs[na].val.clusterDim.z = (unsigned)L.ksplit;
       ++na;
     }
-    if (L.after_previous) {
+    if (L.after_previous || few_tiles) {  // the first one waits before it reads anything
       attrs[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
       attrs[na].val.programmaticStreamSerializationAllowed = 1;
       ++na;

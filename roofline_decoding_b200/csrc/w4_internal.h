@@ -113,6 +113,28 @@ int decode_step_scratch_bytes(const w4_decode_model& m, size_t* bytes);
 int launch_decode_step(const w4_decode_model& m, void* scratch, size_t scratch_bytes,
                        cudaStream_t stream);
 
+// Launches fn with programmatic dependent launch: its CTAs may be placed while
+// the stream's previous kernel ends. fn calls griddepcontrol.wait in every
+// thread before it reads or writes global memory, so it sees all that ran
+// before, and ends after it; and only then lets its own dependents start, since
+// those of this library that read some inputs before their wait count on
+// everything but the kernel just before them being done.
+template <typename P>
+cudaError_t launch_overlapped(void (*fn)(P), dim3 grid, int threads, size_t smem,
+                              cudaStream_t stream, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, p);
+}
+
 // Tensor-map encoder resolved from the driver at init.
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

@@ -247,6 +247,8 @@ constexpr int kRopeThreads = 128;
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const RopeParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int groups = head_groups<D>(p.heads) + head_groups<D>(p.kv_heads);
   const int per_row = (groups + p.groups_per_warp - 1) / p.groups_per_warp;
@@ -443,6 +445,8 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
 template <int D, bool BF16, int W, int NP>
 __global__ void __launch_bounds__(kAppendThreads, W == 1 ? 3 : NP == 4 ? 2 : 3)
     append_kernel(const AppendParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
   if ((int)blockIdx.x < p.kv_blocks) {
     const int unit = W == 1 ? (int)blockIdx.x * (kAppendThreads / 32) + (int)(threadIdx.x >> 5)
                             : (int)blockIdx.x;
@@ -544,8 +548,8 @@ int launch_norm_rope(const w4_heads& q, const w4_heads& k, const w4_heads& q_out
   void (*fn)(RopeParams) = head_dim == 128
                                ? (bf16 ? norm_rope_kernel<128, true> : norm_rope_kernel<128, false>)
                                : (bf16 ? norm_rope_kernel<64, true> : norm_rope_kernel<64, false>);
-  fn<<<(unsigned)blocks, kRopeThreads, 0, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      launch_overlapped(fn, dim3((unsigned)blocks), kRopeThreads, 0, stream, p);
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_qk_norm_rope launch");
 }
 
@@ -596,8 +600,8 @@ int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_hea
                                          : append_fn<128, false>(by_warp, np))
                                  : (bf16 ? append_fn<64, true>(by_warp, np)
                                          : append_fn<64, false>(by_warp, np));
-  fn<<<(unsigned)blocks, kAppendThreads, 0, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      launch_overlapped(fn, dim3((unsigned)blocks), kAppendThreads, 0, stream, p);
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_kv8_append launch");
 }
 

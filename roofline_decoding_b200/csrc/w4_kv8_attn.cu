@@ -50,6 +50,10 @@ constexpr float kShift = 14.0f;  // P' is at most 2^kShift
 // Tiles a CTA takes at least (one a warp): below that more CTAs only add
 // partials to join.
 constexpr int kMinTiles = kWarps;
+// What an item costs beside its tiles (queries, merge, output), in tiles: each
+// is that much longer in the line, at its front, so that a CTA of many short
+// items does not end last.
+constexpr int kItemTiles = 12;
 
 // NT: 8-row blocks of an item (1, 2 or 4).
 template <int D, int NT>
@@ -201,7 +205,8 @@ __device__ __forceinline__ int token_tiles(const AttnP& p, const Seq& s) {
 }
 template <int kRows>
 __device__ __forceinline__ int64_t seq_work(const AttnP& p, const Seq& s) {
-  return s.n > 0 ? (int64_t)p.kv_heads * row_tiles<kRows>(p, s) * token_tiles(p, s) : 0;
+  return s.n > 0 ? (int64_t)p.kv_heads * row_tiles<kRows>(p, s) * (token_tiles(p, s) + kItemTiles)
+                 : 0;
 }
 
 // The CTAs' shares of the line of all tiles: `per` tiles each, the last ones
@@ -271,32 +276,39 @@ struct Walk {
   // the item
   Seq s;
   int h, rt;
-  int64_t item0;   // first tile of the item in the line
-  int nt;          // its tiles (as the shares count them)
-  int t0, t1;      // the share's part of them, cut at the row tile's own limit
-  int t1_full;     // not cut
-  int limit;       // tokens that the row tile's last row sees
+  int64_t item0;  // where it begins in the line
+  int nt;         // its tiles (as the shares count them)
+  int t0, t1;     // the share's part of them, cut at the row tile's own limit
+  bool whole;     // the part is all of them
+  int limit;      // tokens that the row tile's last row sees
 
+  // The next item of which the share has a tile.
   __device__ __forceinline__ bool next(const AttnP& p) {
-    if (x >= end) return false;
-    s = load_seq(p, b);
-    for (int64_t w; off >= (w = seq_work<kRows>(p, s));) {  // sequences without rows, or just done
-      off -= w;
-      if (++b >= p.seqs) return false;
+    while (true) {
+      if (x >= end) return false;
       s = load_seq(p, b);
+      for (int64_t w; off >= (w = seq_work<kRows>(p, s));) {  // no rows, or just done
+        off -= w;
+        if (++b >= p.seqs) return false;
+        s = load_seq(p, b);
+      }
+      nt = token_tiles(p, s);
+      const int nrt = row_tiles<kRows>(p, s), len = nt + kItemTiles;
+      const int64_t item = divide(off, len);
+      h = (int)divide(item, nrt);
+      rt = (int)(item - (int64_t)h * nrt);
+      const int at = (int)(off - item * len);
+      const int to = (int)min((int64_t)len, at + (end - x));
+      item0 = x - at;
+      x += to - at;
+      off += to - at;
+      t0 = max(at - kItemTiles, 0);
+      t1 = max(to - kItemTiles, 0);
+      if (t0 < t1) break;
     }
-    nt = token_tiles(p, s);
-    const int nrt = row_tiles<kRows>(p, s);
-    const int64_t item = divide(off, nt);
-    h = (int)divide(item, nrt);
-    rt = (int)(item - (int64_t)h * nrt);
-    t0 = (int)(off - item * nt);
-    t1_full = (int)min((int64_t)nt, t0 + (end - x));
-    item0 = x - t0;
-    x += t1_full - t0;
-    off += t1_full - t0;
+    whole = t1 - t0 == nt;
     limit = seen(p, s, min(s.n * p.group, (rt + 1) * kRows) - 1);
-    t1 = min(t1_full, (limit + kTile - 1) / kTile);
+    t1 = min(t1, (limit + kTile - 1) / kTile);
     return true;
   }
 };
@@ -368,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   uint2* shared_q = reinterpret_cast<uint2*>(marks + S::kMarks / 4);        // kSharedQ only
   float* shared_mul = reinterpret_cast<float*>(shared_q + S::kKSteps * NT * 32);
 
+  grid_dependency_wait();
   grid_launch_dependents();
   const Share share = find_share<kRows>(p);
   if (tid == 0) p.join[blockIdx.x].count = 0;
@@ -379,7 +392,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   Walk<kRows> lw;
   lw.x = share.x, lw.end = share.end, lw.b = share.b, lw.off = share.off;
   Walk<kRows> cw = lw;
+  // The queries of an item on their way to the L1 cache while its first tiles are.
+  auto prefetch_queries = [&]() {
+    constexpr int kLines = D / 64;  // 128-byte lines of a head
+    const int row = lw.rt * kRows + tid / kLines;
+    if (tid < kRows * kLines && row < lw.s.n * p.group) {
+      const int i = by_group(p, row);
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(
+          p.q + (int64_t)(lw.s.first + i) * p.q_row +
+          (int64_t)(lw.h * p.group + row - i * p.group) * p.q_head + 64 * (tid % kLines)));
+    }
+  };
   bool more = lw.next(p);
+  if (more) prefetch_queries();
   int lt = more ? lw.t0 + warp : 0;
   // Page numbers of the warp's next 16 tiles, two halves of 16 tokens each: lane
   // 2 k + half has those of tile k.
@@ -408,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     if (more && lt >= lw.t1) {
       do {
         more = lw.next(p);
+        if (more) prefetch_queries();
         lt = lw.t0 + warp;
       } while (more && lt >= lw.t1);
       id_at = 16;
@@ -743,7 +769,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     }
     // Eight dims of a row a thread: the output of a whole item, or a part that is
     // left for the second launch.
-    const bool whole = cw.t0 == 0 && cw.t1_full == cw.nt;
     float* part =
         p.parts + ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * kRows * S::kPitch;
 #pragma unroll 1
@@ -761,7 +786,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
           if (*mark >> k & 1) v[k] = __int_as_float(0x7fffffff);
         *mark = 0;
       }
-      if (whole) {
+      if (cw.whole) {
         const float sum = src[D + 1];
         const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
         const int i = by_group(p, r0 + rr);
@@ -786,15 +811,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         if (d == 0) *reinterpret_cast<float2*>(dst + D) = *reinterpret_cast<const float2*>(src + D);
       }
     }
-    if (!whole) {
+    if (!cw.whole) {
       // The join is described by the CTA whose share begins at the item's first
       // inner border: it starts inside the item and the share before does not.
-      if (tid == 0 && cw.t0 > 0 && share.x - share.per <= cw.item0) {
-        const int last = (int)divide(cw.item0 + cw.nt - 1, share.per);
+      if (tid == 0 && cw.t0 > 0 && share.x - share.per <= cw.item0 + kItemTiles) {
+        const int last = (int)divide(cw.item0 + kItemTiles + cw.nt - 1, share.per);
         Join jn;
         jn.count = last - (int)blockIdx.x + 2;
         jn.cta = (int)blockIdx.x - 1;
-        jn.slot = share.x - share.per == cw.item0 ? 0 : 1;
+        jn.slot = share.x - share.per >= cw.item0 ? 0 : 1;
         jn.row0 = cw.s.first;
         jn.head0 = cw.h * p.group;
         jn.r0 = r0;
@@ -808,101 +833,162 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   }
 }
 
+// CTAs that the workspace has room for: two an SM on the largest sm_100 part.
+constexpr int kMaxCtas = 160 * kCtasPerSm;
+
 constexpr int kJoinWarps = 8;
+constexpr int kJoinThreads = kJoinWarps * 32;
+constexpr int kFew = 8;  // partials that a warp joins by itself
 
-constexpr int kJoinRows = 4;  // blocks an item (each takes every fourth row)
-
-// Joins the partials of an item: blockIdx.x the border, blockIdx.y the rows.
-// The warps take a row's partials in turn, a lane D/32 dims, and warp 0 adds
-// the warps in order.
+// Joins the partials of an item: blockIdx.x the border, blockIdx.y the rows. A
+// few partials: a warp a row. Many (a long sequence over many CTAs): the block
+// takes one row at a time, first every partial's factor, then the sum of the
+// outputs, eight partials side by side and in a fixed order.
 template <int D, int NT>
-__global__ void __launch_bounds__(kJoinWarps * 32) kv8_join_kernel(const AttnP p) {
+__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const AttnP p) {
   constexpr int V = D / 32, kPitch = AttnShape<D, NT>::kPitch, kRows = AttnShape<D, NT>::kRows;
+  __shared__ float factor[kMaxCtas];
   __shared__ float sm[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][D];
   grid_dependency_wait();
+  grid_launch_dependents();
   const Join jn = p.join[blockIdx.x];
   if (jn.count == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rows = min(kRows, jn.rows - jn.r0);
+  auto part_of = [&](int c, int ri) {
+    return p.parts +
+           (((size_t)(jn.cta + c) * 2 + (c == 0 ? jn.slot : 0)) * kRows + ri) * kPitch;
+  };
+  auto store = [&](int ri, const float (&o)[V], float l) {
+    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
+    const int row = jn.r0 + ri, i = by_group(p, row);
+    uint16_t* dst = p.out + (int64_t)(jn.row0 + i) * p.out_row +
+                    (int64_t)(jn.head0 + row - i * p.group) * p.out_head + V * lane;
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      if (p.bf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(o[2 * k] * inv, o[2 * k + 1] * inv);
+        w[k] = *reinterpret_cast<const uint32_t*>(&v);
+      } else {
+        w[k] = half2_bits(o[2 * k] * inv, o[2 * k + 1] * inv);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) reinterpret_cast<uint32_t*>(dst)[k] = w[k];
+  };
+  if (jn.count <= kFew) {
 #pragma unroll 1
-  for (int ri = blockIdx.y; ri < kRows && jn.r0 + ri < jn.rows; ri += kJoinRows) {
-    float m = -INFINITY, l = 0.f, o[V];
+    for (int ri = blockIdx.y * kJoinWarps + warp; ri < rows; ri += gridDim.y * kJoinWarps) {
+      float m[kFew], l[kFew], v[kFew][V];
+      float most = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kFew; ++c) {
+        m[c] = -INFINITY, l[c] = 0.f;
+        if (c < jn.count) {
+          const float* part = part_of(c, ri);
+          m[c] = part[D], l[c] = part[D + 1];
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[c][i] = part[V * lane + i];
+        }
+        most = fmaxf(most, m[c]);
+      }
+      float sum = 0.f, o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kFew; ++c)
+        if (c < jn.count) {
+          const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - most);
+          sum += l[c] * f;
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[i] += v[c][i] * f;
+        }
+      store(ri, o, sum);
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int ri = blockIdx.y; ri < rows; ri += gridDim.y) {
+    constexpr int kMine = (kMaxCtas + kJoinThreads - 1) / kJoinThreads;
+    float m[kMine], pl[kMine], most = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int c = tid + k * kJoinThreads;
+      m[k] = -INFINITY, pl[k] = 0.f;
+      if (c < jn.count) {
+        const float2 ml = *reinterpret_cast<const float2*>(part_of(c, ri) + D);
+        m[k] = ml.x, pl[k] = ml.y;
+      }
+      most = fmaxf(most, m[k]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+    if (lane == 0) sm[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, sm[w]);
+    float l = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int c = tid + k * kJoinThreads;
+      const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - most);
+      if (c < jn.count) factor[c] = f;
+      l += pl[k] * f;
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    if (lane == 0) sl[warp] = l;
+    __syncthreads();
+    float o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int c = warp; c < jn.count; c += kJoinWarps) {
-      const float* part =
-          p.parts + (((size_t)(jn.cta + c) * 2 + (c == 0 ? jn.slot : 0)) * kRows + ri) * kPitch;
-      const float om = part[D], ol = part[D + 1];
-      float v[V];
+      const float* part = part_of(c, ri) + V * lane;
+      const float f = factor[c];
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = part[V * lane + i];
-      const float nm = fmaxf(m, om);
-      const float fa = m == -INFINITY ? 0.f : ex2(m - nm);
-      const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
-      m = nm;
-      l = l * fa + ol * fb;
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = o[i] * fa + v[i] * fb;
+      for (int i = 0; i < V; ++i) o[i] += part[i] * f;
     }
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
 #pragma unroll
     for (int i = 0; i < V; ++i) so[warp][V * lane + i] = o[i];
     __syncthreads();
     if (warp == 0) {
-      m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sm[w]);
       l = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) o[i] = 0.f;
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) {
-        const float f = sm[w] == -INFINITY ? 0.f : ex2(sm[w] - m);
-        l += sl[w] * f;
+        l += sl[w];
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] += so[w][V * lane + i] * f;
+        for (int i = 0; i < V; ++i) o[i] += so[w][V * lane + i];
       }
-      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-      const int row = jn.r0 + ri, i = by_group(p, row);
-      uint16_t* dst = p.out + (int64_t)(jn.row0 + i) * p.out_row +
-                      (int64_t)(jn.head0 + row - i * p.group) * p.out_head + V * lane;
-#pragma unroll
-      for (int k = 0; k < V; k += 2) {
-        uint32_t w;
-        if (p.bf16) {
-          const __nv_bfloat162 v = __floats2bfloat162_rn(o[k] * inv, o[k + 1] * inv);
-          w = *reinterpret_cast<const uint32_t*>(&v);
-        } else {
-          w = half2_bits(o[k] * inv, o[k + 1] * inv);
-        }
-        *reinterpret_cast<uint32_t*>(dst + k) = w;
-      }
+      store(ri, o, l);
     }
     __syncthreads();  // the shared sums are read
   }
 }
-
-// CTAs that the workspace has room for: two an SM on the largest sm_100 part.
-constexpr int kMaxCtas = 160 * kCtasPerSm;
 
 template <int D, int NT>
 int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
   using S = AttnShape<D, NT>;
   p.join = reinterpret_cast<Join*>(p.parts + (size_t)kMaxCtas * 2 * S::kRows * S::kPitch);
   const int ctas = std::min(kMaxCtas, kCtasPerSm * di.sm_count);
-  kv8_attention_kernel<D, NT><<<ctas, kThreads, S::kSmem, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_overlapped(kv8_attention_kernel<D, NT>, dim3((unsigned)ctas), kThreads,
+                                    S::kSmem, stream, p);
   if (e != cudaSuccess) return cuda_fail(e, "w4_kv8_attention launch");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, (unsigned)std::min(max_rows, kJoinRows));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kv8_join_kernel<D, NT>, (const AttnP)p);
+  // Blocks of an item's join. Where the page table has no room for more than a
+  // few partials an item, a warp a row. Else a row at a time each: eight blocks
+  // when there are few items for all the CTAs (one sequence of 32768 tokens over
+  // two heads: 13 us in all, against 16 with four), four otherwise (16 sequences
+  // of up to 2000 over four heads: 13.0 us, against 14.7 with eight).
+  const int most = ((p.capacity + kTile - 1) / kTile) / kMinTiles + 2;
+  const bool few_items = (int64_t)ctas > (int64_t)kFew * p.seqs * p.kv_heads;
+  const int by = most <= kFew ? (max_rows + kJoinWarps - 1) / kJoinWarps
+                              : std::min(max_rows, few_items ? 8 : 4);
+  e = launch_overlapped(kv8_join_kernel<D, NT>, dim3((unsigned)ctas, (unsigned)by), kJoinThreads, 0,
+                        stream, p);
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_kv8_attention join launch");
 }
 

@@ -161,3 +161,24 @@ def test_rows_behind_the_last_are_untouched_and_streams_and_graphs():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, rd.w4_gemm_fused(x, *w, activation="silu", residual=r))
+
+
+def test_inputs_written_just_before_are_seen():
+    """x from a kernel that is still running when the call is made, in plans of one launch,
+    of K slices and of two launches, and the result read by the next."""
+    g = gen(12)
+    for M, K, N in ((40, 512, 384), (300, 1024, 1152), (2048, 1024, 5120)):
+        w = weights(g, K, N)
+        xs = [randn(g, M, K) for _ in range(4)]
+        want = [rd.w4_gemm_fused(x, *w, activation="silu") for x in xs]
+        torch.cuda.synchronize()
+        buf = torch.zeros((M, K), device=DEV, dtype=torch.bfloat16)
+        big = torch.randn(4096, 4096, device=DEV)
+        got = []
+        for x in xs * 3:
+            torch.mm(big, big)  # keeps the stream behind the host
+            buf.copy_(x)
+            got.append(rd.w4_gemm_fused(buf, *w, activation="silu") + 0)
+            buf.fill_(float("nan"))
+        for i, y in enumerate(got):
+            assert torch.equal(y, want[i % 4]), (M, K, N, i)

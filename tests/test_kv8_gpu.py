@@ -659,3 +659,35 @@ def test_a_batched_decoder_layer(dtype):
         check_gemm(h2, act, w_down, residual=before)
         past = [p + n for p, n in zip(past, rows)]
     assert rd.device_error() == 0
+
+
+def test_a_chain_of_calls_sees_each_others_results():
+    """Append, attention and norms back to back with the kernels that write and reuse their inputs."""
+    g, page = gen(81), 32
+    past, rows = [300, 45, 0, 77], [1, 1, 1, 1]
+    table, pages = page_tables(g, past, rows, page)
+    cache = fresh_cache(g, pages, 2, 128, page)
+    cos, sin = tables(400, 128, torch.float32)
+    lengths, rs = i32(past), i32(starts(rows))
+    steps = [randn(g, 4, 12, 128) for _ in range(5)]
+
+    def run(behind):
+        c = rd.KV8Cache(*[t.clone() for t in cache])
+        buf, outs = torch.empty_like(steps[0]), []
+        big = torch.randn(4096, 4096, device=DEV)
+        torch.cuda.synchronize()
+        for x in steps:
+            if behind:
+                torch.mm(big, big)
+            buf.copy_(x)
+            q = rd.kv8_append(c, buf[:, 8:10], buf[:, 10:], table, lengths, rs, cos, sin, q=buf[:, :8])
+            o1 = rd.kv8_attention(q, c, table, lengths, rs)
+            n1, n2 = rd.qk_norm_rope(o1, q[:, :2], cos, sin, lengths.long())
+            outs += [q + 0, o1 + 0, n1 + n2.repeat(1, 4, 1)]
+            buf.fill_(float("nan"))
+            if not behind:
+                torch.cuda.synchronize()
+        return outs
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b) and not torch.isnan(a).any()
