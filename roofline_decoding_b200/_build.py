@@ -23,7 +23,7 @@ TORCH_MODULE_PATH = PKG_DIR / "_w4torch.so"
 SOURCES = ["w4_api.cu", "w4_pack.cu", "w4_gemv.cu", "w4_gemv_ops.cu", "w4_gemv_fused.cu",
            "w4_decode.cu", "w4_mega.cu",
            "w4_gemm.cu", "w4_gptq.cu", "w4_tune.cu",
-           "w4_kv8.cu", "w4_kv8_attn.cu"]
+           "w4_kv8.cu", "w4_kv8_attn.cu", "w4_kv8_prompt.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

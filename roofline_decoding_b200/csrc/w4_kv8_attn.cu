@@ -33,8 +33,7 @@
 // of s + log2 sv, so P' is at most 2^14, its rounding to fp16 (11 bits) stays
 // relative down to 2^-28 of the largest weight, and the fp32 sum adds
 // P' / sv, unrounded.
-#include "w4_internal.h"
-#include "w4_ptx.cuh"
+#include "w4_kv8_attn.cuh"
 
 #include <algorithm>
 
@@ -47,13 +46,38 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;        // tokens of one ring stage of a warp
 constexpr int kCtasPerSm = 2;
 constexpr float kShift = 14.0f;  // P' is at most 2^kShift
-// Tiles a CTA takes at least (one a warp): below that more CTAs only add
-// partials to join.
-constexpr int kMinTiles = kWarps;
-// What an item costs beside its tiles (queries, merge, output), in tiles: each
-// is that much longer in the line, at its front, so that a CTA of many short
-// items does not end last.
-constexpr int kItemTiles = 12;
+
+// From this many query rows of a cache head a sequence on, the other kernel.
+constexpr int kPromptRows = 64;
+
+// Every row tile of a sequence counts as long as its last (the few tiles above a
+// row tile's own limit are passed over), in tiles.
+template <int NT>
+struct Rows8 {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kTile = w4::kTile;
+  static constexpr int kUnit = 1;
+  static constexpr int kOver = 12;           // so that a CTA of many short items does not end last
+  static constexpr int kMinShare = kWarps;   // below a tile a warp, more CTAs only add partials
+  static __device__ __forceinline__ int tiles(const AttnP& p, const Seq& s, int) {
+    return (min(s.past + s.n, p.capacity) + kTile - 1) / kTile;
+  }
+  static __device__ __forceinline__ int row_tiles(const AttnP& p, const Seq& s) {
+    return (s.n * p.group + kRows - 1) / kRows;
+  }
+  static __device__ __forceinline__ int64_t seq_work(const AttnP& p, const Seq& s) {
+    return s.n > 0 ? (int64_t)p.kv_heads * row_tiles(p, s) * (tiles(p, s, 0) + kOver) : 0;
+  }
+  static __device__ __forceinline__ void locate(const AttnP& p, const Seq& s, int64_t off, int* h,
+                                                int* rt, int64_t* at, int64_t* len) {
+    const int nrt = row_tiles(p, s);
+    *len = tiles(p, s, 0) + kOver;
+    const int64_t item = divide(off, *len);
+    *h = (int)divide(item, nrt);
+    *rt = (int)(item - (int64_t)*h * nrt);
+    *at = off - item * *len;
+  }
+};
 
 // NT: 8-row blocks of an item (1, 2 or 4).
 template <int D, int NT>
@@ -76,62 +100,6 @@ struct AttnShape {
   static constexpr int kSmem = kRing + kScales + kMerge + kMarks + kQ;
   static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
-
-struct AttnP {
-  const uint8_t *k, *v;
-  const float *k_scale, *v_scale;
-  const int32_t *page_table, *lengths, *row_starts;
-  int64_t table_stride;
-  int capacity;  // tokens that a row of the page table holds
-  int pages, page, page_shift, max_pages, kv_heads, seqs, rows, group;
-  uint32_t group_mul;  // ceil(2^32 / group), 0 for group 1
-  const uint16_t* q;
-  int64_t q_row, q_head;
-  uint16_t* out;
-  int64_t out_row, out_head;
-  int bf16;
-  float scale_log2;
-  float* parts;       // [CTAs][2][rows of an item][D + 4]
-  struct Join* join;  // [CTAs]
-  int* err;
-};
-
-// What the second launch needs to join an item: written by the CTA whose share
-// begins at the item's first inner border, empty (count 0) by every other.
-struct Join {
-  int count;       // partials, CTAs cta .. cta + count - 1
-  int cta, slot;   // the first partial's CTA and slot; the others are in slot 0
-  int row0, head0; // first output row of the sequence, first query head
-  int r0, rows;    // the tile's first query row, and all query rows of the item's head
-  int pad;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two e4m3 codes (the low half of w, or the high) to fp16, exactly.
-__device__ __forceinline__ uint32_t e4m3_lo(uint32_t w) {
-  uint32_t d;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
-      : "=r"(d)
-      : "r"(w));
-  return d;
-}
-__device__ __forceinline__ uint32_t e4m3_hi(uint32_t w) {
-  uint32_t d;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
-      : "=r"(d)
-      : "r"(w));
-  return d;
-}
-
-__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -168,162 +136,11 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   }
 }
 
-// A sequence's rows and tokens. A length that the page table cannot hold is cut
-// to what it holds.
-struct Seq {
-  int first, n;  // rows
-  int past;
-};
-__device__ __forceinline__ Seq load_seq(const AttnP& p, int b) {
-  Seq s;
-  s.first = min(max(p.row_starts[b], 0), p.rows);
-  s.n = min(max(p.row_starts[b + 1], s.first), p.rows) - s.first;
-  s.past = min(max(p.lengths[b], 0), p.capacity);
-  return s;
-}
-// r / group, for r < 2^28: group_mul * group exceeds 2^32 by less than 16.
-__device__ __forceinline__ int by_group(const AttnP& p, int r) {
-  return p.group_mul ? (int)__umulhi((uint32_t)r, p.group_mul) : r;
-}
-// a / b, in 32 bits where a fits them (the 64-bit division is a long call).
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-  if (((uint64_t)a | (uint64_t)b) < (1ull << 32)) return (uint32_t)a / (uint32_t)b;
-  return a / b;
-}
-// Tokens that query row r (of n * group) of the sequence sees.
-__device__ __forceinline__ int seen(const AttnP& p, const Seq& s, int r) {
-  return min(s.past + by_group(p, r) + 1, p.capacity);
-}
-template <int kRows>
-__device__ __forceinline__ int row_tiles(const AttnP& p, const Seq& s) {
-  return (s.n * p.group + kRows - 1) / kRows;
-}
-// Tiles of a row tile of the sequence; the shares count every row tile at the
-// length of the last (the tiles above a row tile's own limit are passed over).
-__device__ __forceinline__ int token_tiles(const AttnP& p, const Seq& s) {
-  return (min(s.past + s.n, p.capacity) + kTile - 1) / kTile;
-}
-template <int kRows>
-__device__ __forceinline__ int64_t seq_work(const AttnP& p, const Seq& s) {
-  return s.n > 0 ? (int64_t)p.kv_heads * row_tiles<kRows>(p, s) * (token_tiles(p, s) + kItemTiles)
-                 : 0;
-}
-
-// The CTAs' shares of the line of all tiles: `per` tiles each, the last ones
-// less or none. Every warp works it out by itself, 32 sequences at a time.
-struct Share {
-  int64_t x, end;  // this CTA's tiles
-  int64_t per;     // tiles of a share
-  int b;           // the sequence of tile x
-  int64_t off;     // x's place among the sequence's tiles
-};
-
-__device__ __forceinline__ int64_t scan32(int64_t v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, v, off);
-    if (lane >= off) v += up;
-  }
-  return v;
-}
-
-template <int kRows>
-__device__ __forceinline__ Share find_share(const AttnP& p) {
-  const int lane = threadIdx.x & 31;
-  Share f;
-  int64_t all = 0, w = 0;
-#pragma unroll 1
-  for (int b0 = 0; b0 < p.seqs; b0 += 32) {
-    w = 0;
-    if (b0 + lane < p.seqs) {
-      const Seq s = load_seq(p, b0 + lane);
-      w = seq_work<kRows>(p, s);
-      const int told = p.lengths[b0 + lane];
-      if (s.n > 0 && (told < 0 || told > p.capacity - s.n)) atomicCAS(p.err, 0, kErrKvRange);
-    }
-    w = scan32(w, lane);
-    all += __shfl_sync(0xffffffffu, w, 31);
-  }
-  f.per = max((int64_t)kMinTiles, divide(all + gridDim.x - 1, gridDim.x));
-  f.x = min(all, f.per * blockIdx.x);
-  f.end = min(all, f.x + f.per);
-  f.b = 0;
-  f.off = 0;
-  if (f.x >= f.end) return f;
-  int64_t before = 0;
-#pragma unroll 1
-  for (int b0 = 0;; b0 += 32) {
-    if (p.seqs > 32)  // else the first pass has left them
-      w = scan32(b0 + lane < p.seqs ? seq_work<kRows>(p, load_seq(p, b0 + lane)) : 0, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, before + w > f.x);
-    if (hit || b0 + 32 >= p.seqs) {
-      const int src = hit ? __ffs(hit) - 1 : 31;
-      const int64_t prev = __shfl_sync(0xffffffffu, w, max(src - 1, 0));
-      f.b = min(b0 + src, p.seqs - 1);
-      f.off = f.x - before - (src ? prev : 0);
-      return f;
-    }
-    before += __shfl_sync(0xffffffffu, w, 31);
-  }
-}
-
-// Walks a CTA's share item by item.
-template <int kRows>
-struct Walk {
-  int64_t x, end;  // next tile of the line, end of the share
-  int b;           // sequence of x
-  int64_t off;     // x's place in it
-  // the item
-  Seq s;
-  int h, rt;
-  int64_t item0;  // where it begins in the line
-  int nt;         // its tiles (as the shares count them)
-  int t0, t1;     // the share's part of them, cut at the row tile's own limit
-  bool whole;     // the part is all of them
-  int limit;      // tokens that the row tile's last row sees
-
-  // The next item of which the share has a tile.
-  __device__ __forceinline__ bool next(const AttnP& p) {
-    while (true) {
-      if (x >= end) return false;
-      s = load_seq(p, b);
-      for (int64_t w; off >= (w = seq_work<kRows>(p, s));) {  // no rows, or just done
-        off -= w;
-        if (++b >= p.seqs) return false;
-        s = load_seq(p, b);
-      }
-      nt = token_tiles(p, s);
-      const int nrt = row_tiles<kRows>(p, s), len = nt + kItemTiles;
-      const int64_t item = divide(off, len);
-      h = (int)divide(item, nrt);
-      rt = (int)(item - (int64_t)h * nrt);
-      const int at = (int)(off - item * len);
-      const int to = (int)min((int64_t)len, at + (end - x));
-      item0 = x - at;
-      x += to - at;
-      off += to - at;
-      t0 = max(at - kItemTiles, 0);
-      t1 = max(to - kItemTiles, 0);
-      if (t0 < t1) break;
-    }
-    whole = t1 - t0 == nt;
-    limit = seen(p, s, min(s.n * p.group, (rt + 1) * kRows) - 1);
-    t1 = min(t1, (limit + kTile - 1) / kTile);
-    return true;
-  }
-};
-
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // The queries of 8 rows as the B operand: row `row` (this lane's, of n_rows) is
 // scaled to 2^14, step s of lane t is dims D/4 t + 4 s .. + 3, the order of the
 // K words. Returns the factor that turns a sum into log2 units, but for the
@@ -369,6 +186,7 @@ __device__ __forceinline__ float load_queries(const AttnP& p, const Seq& s, int 
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(const AttnP p) {
   using S = AttnShape<D, NT>;
+  using G = Rows8<NT>;
   constexpr int kRows = S::kRows;
   extern __shared__ __align__(128) uint8_t smem_kv8[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -382,16 +200,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
 
   grid_dependency_wait();
   grid_launch_dependents();
-  const Share share = find_share<kRows>(p);
+  const Share share = find_share<G>(p);
   if (tid == 0) p.join[blockIdx.x].count = 0;
   if (share.x >= share.end) return;
   for (int i = tid; i < S::kMarks / 4; i += kThreads) marks[i] = 0u;
   __syncthreads();
 
   // ---- the load side: this warp's tiles, kStages - 1 ahead of the compute side
-  Walk<kRows> lw;
-  lw.x = share.x, lw.end = share.end, lw.b = share.b, lw.off = share.off;
-  Walk<kRows> cw = lw;
+  Walk<G> lw;
+  lw.start(share);
+  Walk<G> cw = lw;
   // The queries of an item on their way to the L1 cache while its first tiles are.
   auto prefetch_queries = [&]() {
     constexpr int kLines = D / 64;  // 128-byte lines of a head
@@ -500,7 +318,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
                                           8 * (g & 1));
 
   int slot = 0;
-  bool first_segment = true;
   while (cw.next(p)) {
     // ---- queries of this item: row 8 n + g as operand, rows 8 n + 2 t and
     // 8 n + 2 t + 1 of the results
@@ -770,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     // Eight dims of a row a thread: the output of a whole item, or a part that is
     // left for the second launch.
     float* part =
-        p.parts + ((size_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * kRows * S::kPitch;
+        p.parts + ((size_t)blockIdx.x * 2 + cw.slot(share)) * kRows * S::kPitch;
 #pragma unroll 1
     for (int e = tid; e < kRows * (D / 8); e += kThreads) {
       const int rr = e / (D / 8), d = 8 * (e % (D / 8));
@@ -811,162 +628,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         if (d == 0) *reinterpret_cast<float2*>(dst + D) = *reinterpret_cast<const float2*>(src + D);
       }
     }
-    if (!cw.whole) {
-      // The join is described by the CTA whose share begins at the item's first
-      // inner border: it starts inside the item and the share before does not.
-      if (tid == 0 && cw.t0 > 0 && share.x - share.per <= cw.item0 + kItemTiles) {
-        const int last = (int)divide(cw.item0 + kItemTiles + cw.nt - 1, share.per);
-        Join jn;
-        jn.count = last - (int)blockIdx.x + 2;
-        jn.cta = (int)blockIdx.x - 1;
-        jn.slot = share.x - share.per >= cw.item0 ? 0 : 1;
-        jn.row0 = cw.s.first;
-        jn.head0 = cw.h * p.group;
-        jn.r0 = r0;
-        jn.rows = n_rows;
-        jn.pad = 0;
-        p.join[blockIdx.x] = jn;
-      }
-    }
-    first_segment = false;
+    if (!cw.whole && tid == 0) cw.describe(p, share);
     __syncthreads();  // marks are read before the next item sets any
-  }
-}
-
-// CTAs that the workspace has room for: two an SM on the largest sm_100 part.
-constexpr int kMaxCtas = 160 * kCtasPerSm;
-
-constexpr int kJoinWarps = 8;
-constexpr int kJoinThreads = kJoinWarps * 32;
-constexpr int kFew = 8;  // partials that a warp joins by itself
-
-// Joins the partials of an item: blockIdx.x the border, blockIdx.y the rows. A
-// few partials: a warp a row. Many (a long sequence over many CTAs): the block
-// takes one row at a time, first every partial's factor, then the sum of the
-// outputs, eight partials side by side and in a fixed order.
-template <int D, int NT>
-__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const AttnP p) {
-  constexpr int V = D / 32, kPitch = AttnShape<D, NT>::kPitch, kRows = AttnShape<D, NT>::kRows;
-  __shared__ float factor[kMaxCtas];
-  __shared__ float sm[kJoinWarps], sl[kJoinWarps], so[kJoinWarps][D];
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const Join jn = p.join[blockIdx.x];
-  if (jn.count == 0) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rows = min(kRows, jn.rows - jn.r0);
-  auto part_of = [&](int c, int ri) {
-    return p.parts +
-           (((size_t)(jn.cta + c) * 2 + (c == 0 ? jn.slot : 0)) * kRows + ri) * kPitch;
-  };
-  auto store = [&](int ri, const float (&o)[V], float l) {
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-    const int row = jn.r0 + ri, i = by_group(p, row);
-    uint16_t* dst = p.out + (int64_t)(jn.row0 + i) * p.out_row +
-                    (int64_t)(jn.head0 + row - i * p.group) * p.out_head + V * lane;
-    uint32_t w[V / 2];
-#pragma unroll
-    for (int k = 0; k < V / 2; ++k) {
-      if (p.bf16) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(o[2 * k] * inv, o[2 * k + 1] * inv);
-        w[k] = *reinterpret_cast<const uint32_t*>(&v);
-      } else {
-        w[k] = half2_bits(o[2 * k] * inv, o[2 * k + 1] * inv);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < V / 2; ++k) reinterpret_cast<uint32_t*>(dst)[k] = w[k];
-  };
-  if (jn.count <= kFew) {
-#pragma unroll 1
-    for (int ri = blockIdx.y * kJoinWarps + warp; ri < rows; ri += gridDim.y * kJoinWarps) {
-      float m[kFew], l[kFew], v[kFew][V];
-      float most = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < kFew; ++c) {
-        m[c] = -INFINITY, l[c] = 0.f;
-        if (c < jn.count) {
-          const float* part = part_of(c, ri);
-          m[c] = part[D], l[c] = part[D + 1];
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[c][i] = part[V * lane + i];
-        }
-        most = fmaxf(most, m[c]);
-      }
-      float sum = 0.f, o[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < kFew; ++c)
-        if (c < jn.count) {
-          const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - most);
-          sum += l[c] * f;
-#pragma unroll
-          for (int i = 0; i < V; ++i) o[i] += v[c][i] * f;
-        }
-      store(ri, o, sum);
-    }
-    return;
-  }
-#pragma unroll 1
-  for (int ri = blockIdx.y; ri < rows; ri += gridDim.y) {
-    constexpr int kMine = (kMaxCtas + kJoinThreads - 1) / kJoinThreads;
-    float m[kMine], pl[kMine], most = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      const int c = tid + k * kJoinThreads;
-      m[k] = -INFINITY, pl[k] = 0.f;
-      if (c < jn.count) {
-        const float2 ml = *reinterpret_cast<const float2*>(part_of(c, ri) + D);
-        m[k] = ml.x, pl[k] = ml.y;
-      }
-      most = fmaxf(most, m[k]);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-    if (lane == 0) sm[warp] = most;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) most = fmaxf(most, sm[w]);
-    float l = 0.f;
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      const int c = tid + k * kJoinThreads;
-      const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - most);
-      if (c < jn.count) factor[c] = f;
-      l += pl[k] * f;
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    if (lane == 0) sl[warp] = l;
-    __syncthreads();
-    float o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 0.f;
-#pragma unroll 8
-    for (int c = warp; c < jn.count; c += kJoinWarps) {
-      const float* part = part_of(c, ri) + V * lane;
-      const float f = factor[c];
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] += part[i] * f;
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) so[warp][V * lane + i] = o[i];
-    __syncthreads();
-    if (warp == 0) {
-      l = 0.f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) {
-        l += sl[w];
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] += so[w][V * lane + i];
-      }
-      store(ri, o, l);
-    }
-    __syncthreads();  // the shared sums are read
   }
 }
 
@@ -983,11 +646,11 @@ int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
   // when there are few items for all the CTAs (one sequence of 32768 tokens over
   // two heads: 13 us in all, against 16 with four), four otherwise (16 sequences
   // of up to 2000 over four heads: 13.0 us, against 14.7 with eight).
-  const int most = ((p.capacity + kTile - 1) / kTile) / kMinTiles + 2;
+  const int most = ((p.capacity + kTile - 1) / kTile) / Rows8<NT>::kMinShare + 2;
   const bool few_items = (int64_t)ctas > (int64_t)kFew * p.seqs * p.kv_heads;
   const int by = most <= kFew ? (max_rows + kJoinWarps - 1) / kJoinWarps
                               : std::min(max_rows, few_items ? 8 : 4);
-  e = launch_overlapped(kv8_join_kernel<D, NT>, dim3((unsigned)ctas, (unsigned)by), kJoinThreads, 0,
+  e = launch_overlapped(kv8_join_kernel<D, S::kRows>, dim3((unsigned)ctas, (unsigned)by), kJoinThreads, 0,
                         stream, p);
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "w4_kv8_attention join launch");
 }
@@ -995,7 +658,8 @@ int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
 }  // namespace
 
 size_t kv8_attention_workspace_bytes(int head_dim) {
-  return (size_t)kMaxCtas * (2 * 32 * (head_dim + 4) * 4 + sizeof(Join));  // 32-row items
+  return std::max((size_t)kMaxCtas * (2 * 32 * (head_dim + 4) * 4 + sizeof(Join)),  // 32-row items
+                  kv8_prompt_workspace_bytes(head_dim));
 }
 
 template <int D, int NT>
@@ -1019,6 +683,7 @@ int kv8_init_device(const DeviceInfo& di) {
   if (st == W4_OK) st = init_attention<128, 1>(di);
   if (st == W4_OK) st = init_attention<128, 2>(di);
   if (st == W4_OK) st = init_attention<128, 4>(di);
+  if (st == W4_OK) st = kv8_prompt_init_device(di);
   return st;
 }
 
@@ -1059,6 +724,7 @@ int launch_kv8_attention(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_
   // read and widen the cache less often, narrower ones waste less of a step of
   // few rows.
   const int64_t avg = ((int64_t)bt.rows + bt.seqs - 1) / bt.seqs * p.group;
+  if (avg >= kPromptRows) return launch_kv8_prompt(p, c.head_dim, di, stream);
   const int nt = avg <= 8 ? 1 : avg <= 16 ? 2 : 4;
   const int max_rows = (int)std::min<int64_t>(8 * nt, (int64_t)bt.rows * p.group);
   if (c.head_dim == 128)

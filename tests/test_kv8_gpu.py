@@ -691,3 +691,101 @@ def test_a_chain_of_calls_sees_each_others_results():
 
     for a, b in zip(run(True), run(False)):
         assert torch.equal(a, b) and not torch.isnan(a).any()
+
+
+# ------------------------------------------------------------------ many rows a sequence
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("past,rows,heads,kv,page", [
+    ([0], [128], 1, 1, 64), ([0], [127], 2, 1, 16), ([5], [129], 3, 1, 32), ([130], [64], 8, 8, 128),
+    ([0, 1000, 300], [200, 1, 77], 8, 2, 64), ([4000], [100], 10, 2, 16),
+    ([0, 0, 0, 0], [40, 300, 0, 150], 16, 1, 32), ([0], [1500], 5, 1, 64)])
+def test_attention_prompts(D, past, rows, heads, kv, page):
+    run_attention(sum(rows) + D, past, rows, heads=heads, kv=kv, D=D, page=page)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("mul", [1e-3, 1.0, 30.0, 1e4])
+def test_attention_prompts_sharp_and_flat(dtype, mul):
+    run_attention(91, [700, 33], [150, 90], heads=4, kv=2, dtype=dtype, mul=mul, lead=1, pad=2)
+
+
+def test_attention_prompts_scales_of_any_size():
+    def tune(q, cache):
+        s = torch.exp2(torch.rand(cache.v_scale.shape, generator=gen(1), device=DEV) * 40 - 20)
+        return cache._replace(v_scale=s, k_scale=torch.rand_like(s) * 0.02 + 1e-3)
+    run_attention(92, [300, 20], [70, 100], page=16, tune=tune, scale=0.31)
+
+
+def test_attention_prompts_many_short_ones():
+    """Items of one tile one after another, some of them empty."""
+    rows = [(17 * i) % 23 + 20 if i % 7 else 0 for i in range(90)]
+    run_attention(93, [(5 * i) % 40 for i in range(90)], rows, heads=8, kv=2, D=64, page=16)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_attention_prompts_nan_reaches_only_the_rows_that_see_it(D, where):
+    """NaN codes in several items' mixed tiles, of sequences one after another."""
+    g, n = gen(94), 100
+    past, bad = [36, 0, 200], [41, 63, 290]
+    table, pages = page_tables(g, past, [n] * 3, 16)
+    cache = fresh_cache(g, pages, 2, D, 16)
+    clean = rd.KV8Cache(*[t.clone() for t in cache])
+    for b in range(3):
+        pid = int(table[b, bad[b] // 16])
+        for c, code in ((cache, 0x7F), (clean, 0)):
+            (c.k if where == "k" else c.v).view(torch.uint8)[pid, 1, bad[b] % 16, 3 + b] = code
+    q = randn(g, 3 * n, 4, D)
+    lengths, rs = i32(past), i32([0, n, 2 * n, 3 * n])
+    got = rd.kv8_attention(q, cache, table, lengths, rs)
+    want = rd.kv8_attention(q, clean, table, lengths, rs)
+    check_attention(want, q, clean, table, lengths, rs)
+    for b in range(3):
+        first, rows = bad[b] - past[b], slice(b * n, (b + 1) * n)
+        a, w = got[rows], want[rows]
+        assert torch.equal(a[:, :2], w[:, :2])          # the other cache head's rows
+        assert torch.equal(a[:first, 2:], w[:first, 2:])
+        if where == "k":
+            assert torch.isnan(a[first:, 2:]).all()
+        else:
+            assert torch.isnan(a[first:, 2:, 3 + b]).all()
+            keep = [d for d in range(D) if d != 3 + b]
+            assert torch.equal(a[:, :, keep], w[:, :, keep])
+
+
+def test_attention_prompts_bad_pages_and_stale_contents():
+    g, page = gen(95), 16
+    past, rows = [50, 10], [80, 80]
+    table, pages = page_tables(g, past, rows, page)
+    cache = fresh_cache(g, pages, 2, 64, page)
+    used = torch.zeros(pages, page, dtype=torch.bool, device=DEV)
+    for b in range(2):
+        for t in range(past[b] + rows[b]):
+            used[int(table[b, t // page]), t % page] = True
+    for c in (cache.k, cache.v):
+        c.view(torch.uint8).copy_(torch.where(used[:, None, :, None], c.view(torch.uint8), 0x7F))
+    q = randn(g, 160, 4, 64)
+    lengths, rs = i32(past), i32([0, 80, 160])
+    check_attention(rd.kv8_attention(q, cache, table, lengths, rs), q, cache, table, lengths, rs)
+    bad = table.clone()
+    bad[1, :] = -5
+    got = rd.kv8_attention(q, cache, bad, lengths, rs)
+    assert rd.device_error() == _lib.ERR_KV_RANGE
+    check_attention(got, q, cache, table, lengths, rs, rows=slice(0, 80))
+    assert torch.all(got[80:] == 0)
+
+
+def test_attention_prompts_agree_with_single_rows():
+    """The same rows as one chunk and one at a time, on the two kernels."""
+    g = gen(96)
+    past, n = 77, 70
+    table, pages = page_tables(g, [past], [n], 32)
+    cache = fresh_cache(g, pages, 2, 128, 32)
+    q = randn(g, n, 8, 128)
+    many = rd.kv8_attention(q, cache, table, i32([past]), i32([0, n]))
+    for i in (0, 1, 50, n - 1):
+        one = rd.kv8_attention(q[i:i + 1], cache, table, i32([past + i]), i32([0, 1]))
+        check_attention(many[i:i + 1], q[i:i + 1], cache, table, i32([past + i]), i32([0, 1]))
+        check_attention(one, q[i:i + 1], cache, table, i32([past + i]), i32([0, 1]))
