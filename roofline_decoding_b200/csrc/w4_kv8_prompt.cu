@@ -5,24 +5,26 @@
 // The maths, the split and the join are those of w4_kv8_attn.cu; there a step's
 // few rows make the cache's bytes the bound, here 4 D operations a (row, token)
 // pair do. An item is 128 query rows of one cache head (G query heads times the
-// new tokens), worked through in tiles of 128 tokens by one CTA an SM:
-//   4 widen warps  : the tile's pages from global memory into registers, a tile
-//                    ahead; e4m3 to fp16 (exact) and into shared memory as MMA
-//                    operands, K and V alike token by token in the 128B-swizzled
+// new tokens), worked through in tiles of 128 tokens by one CTA an SM, the tiles
+// in turn by two streams that meet at the item's end:
+//   4 widen warps  : the tile's pages by cp.async into shared memory, a tile ahead
+//                    (a thread copies, waits for and reads its own chunks: no
+//                    barrier); e4m3 to fp16 (exact) and back as MMA operands, K and V alike token by token in the 128B-swizzled
 //                    layout (K is the K-major operand of Q K^T; of P V the same
 //                    rows are the MN-major operand V, so nothing is transposed);
-//   MMA warp       : one thread issues S = Q K^T (M = N = 128) of tile i + 1
-//                    before O += P V of tile i, so that the tensor cores work
-//                    while the softmax does;
-//   4 softmax warps: a thread a row. S from tensor memory, the exponent's
-//                    argument with the page's scales folded in (as in the other
-//                    kernel), P' in fp16 into shared memory. O stays in tensor
-//                    memory; it is rescaled only when the running maximum has
-//                    grown by more than 2^3 since the last time (P' may then
-//                    reach 2^14, inside fp16's range).
-// S and the widened tiles are double-buffered. The exponentials are the floor of
-// this split: 128 x 128 of them a tile at 16 a clock are 1024 clocks, as long as
-// the tile's two products together at their best rate.
+//   MMA warp       : one thread issues S = Q K^T of one stream (M = N = 128),
+//                    then O += P V of the other, so that the tensor cores work
+//                    for one while the other's softmax does;
+//   2 x 4 softmax warps: a thread a row of its stream. S from tensor memory, the
+//                    exponent's argument with the page's scales folded in (as in
+//                    the other kernel), P' in fp16 back into tensor memory over
+//                    the S that it came from. O stays in tensor memory, one a
+//                    stream with a maximum of its own, and is rescaled only when
+//                    a row's running maximum has grown by more than 2^3 since the
+//                    last time (P' may then reach 2^14, inside fp16's range).
+// Two O, two S (with P over them) fill the tensor memory: 4 x 128 columns. The
+// exponentials are the floor of this split: 128 x 128 of them a tile at 16 a clock
+// are 1024 clocks, as long as the tile's two products together at their best rate.
 #include "w4_kv8_attn.cuh"
 
 #include <algorithm>
@@ -31,8 +33,9 @@ namespace w4 {
 
 namespace {
 
-constexpr int kSoftWarps = 4, kWidenWarps = 4;
-constexpr int kMmaWarp = kSoftWarps + kWidenWarps;
+constexpr int kSoftWarps = 4, kWidenWarps = 4;  // softmax warps of a stream
+constexpr int kWidenWarp = 2 * kSoftWarps;
+constexpr int kMmaWarp = kWidenWarp + kWidenWarps;
 constexpr int kPromptThreads = 32 * (kMmaWarp + 1);
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
 constexpr float kPromptShift = 11.0f;  // P' of the maximum that O is scaled by is 2^kPromptShift
@@ -90,17 +93,20 @@ template <int D>
 struct PromptShape {
   static constexpr int kHalf = kPromptTile * 128;         // 128 rows of 64 fp16
   static constexpr int kOperand = kHalf * (D / 64);       // Q, or a K or V tile
-  static constexpr int kP = kPromptTile * kPromptTile * 2;
   static constexpr int kPitch = D + 4;
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + kOperand;          // two buffers
   static constexpr int kOffV = kOffK + 2 * kOperand;      // two buffers
-  static constexpr int kOffP = kOffV + 2 * kOperand;
-  static constexpr int kOffScale = kOffP + kP;            // four tiles of 8 x (K, log2 V, 1 / V, 0)
-  static constexpr int kOffMarks = kOffScale + 4 * 8 * 16;
+  static constexpr int kRaw = kPromptTile * D;            // a K or V tile's codes
+  static constexpr int kOffRaw = kOffV + 2 * kOperand;    // K, then V
+  static constexpr int kOffScale = kOffRaw + 2 * kRaw;  // four tiles of 8 x (K, log2 V, 1 / V, 0)
+  static constexpr int kOffMul = kOffScale + 4 * 8 * 16;  // a factor a row
+  static constexpr int kOffSums = kOffMul + kPromptTile * 4;  // second stream's maxima and sums,
+                                                              // two items in turn
+  static constexpr int kOffMarks = kOffSums + 2 * kPromptTile * 8;
   static constexpr int kMarks = kPromptTile * D / 8;      // of an item; four items
   static constexpr int kOffBar = kOffMarks + 4 * kMarks;
-  static constexpr int kBars = 2 + 2 + 2 + 2 + 2 + 2 + 1 + 1 + 1 + 1;
+  static constexpr int kBars = 7 * 2 + 3;
   static constexpr int kOffTmem = kOffBar + kBars * 8;
   static constexpr int kSmem = 1024 + kOffTmem + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -125,6 +131,17 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :
       : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in tensor memory: a lane a row, two elements a column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      :
+      : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void commit_to(uint64_t* bar) {
@@ -159,8 +176,7 @@ __device__ __forceinline__ void ld32(uint32_t addr, float* r) {
 __device__ __forceinline__ void ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void st32(uint32_t addr, const float* r) {
-  const uint32_t* u = reinterpret_cast<const uint32_t*>(r);
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t* u) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -171,6 +187,14 @@ __device__ __forceinline__ void st32(uint32_t addr, const float* r) {
       "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]),
       "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]),
       "r"(u[30]), "r"(u[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
+      "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void st_wait() {
@@ -197,16 +221,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       (reinterpret_cast<uintptr_t>(smem_prompt) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t sm = smem_u32(base);
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + S::kOffBar);
-  uint64_t* k_full = bars;          // [2] widened K tile there (widen warps)
-  uint64_t* k_empty = bars + 2;     // [2] its product is done (commit)
-  uint64_t* v_full = bars + 4;      // [2]
-  uint64_t* v_empty = bars + 6;     // [2]
-  uint64_t* s_full = bars + 8;      // [2] S of a tile is in tensor memory (commit)
-  uint64_t* s_empty = bars + 10;    // [2] the softmax threads have read it, and the tile's scales
-  uint64_t* p_full = bars + 12;     // P' is in shared memory, O is rescaled
-  uint64_t* pv_done = bars + 13;    // P V of a tile is done (commit)
-  uint64_t* q_full = bars + 14;     // an item's queries are in shared memory
-  uint64_t* o_empty = bars + 15;    // an item's output is read
+  // two of each, by stream (the parity of the tile)
+  uint64_t* k_full = bars;        // widened K tile there (widen warps)
+  uint64_t* k_empty = bars + 2;   // its product is done (commit)
+  uint64_t* v_full = bars + 4;
+  uint64_t* v_empty = bars + 6;
+  uint64_t* s_full = bars + 8;    // S is in tensor memory (commit)
+  uint64_t* p_full = bars + 10;   // P' is in its place, O is rescaled (softmax warps)
+  uint64_t* pv_done = bars + 12;  // P V is done (commit)
+  uint64_t* q_full = bars + 14;   // an item's queries are in shared memory (first stream)
+  uint64_t* b_done = bars + 15;   // the second stream is through with an item
+  uint64_t* o_empty = bars + 16;  // an item's outputs are read (first stream)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + S::kOffTmem);
   int* abort_flag = reinterpret_cast<int*>(base + S::kOffTmem + 4);
   // Marks of four items in turn: the widen warps may be two tiles ahead, that is
@@ -224,16 +249,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       mbar_init(&v_full[i], kWidenWarps);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], kSoftWarps);
+      mbar_init(&p_full[i], kSoftWarps);
+      mbar_init(&pv_done[i], 1);
     }
-    mbar_init(p_full, kSoftWarps);
-    mbar_init(pv_done, 1);
     mbar_init(q_full, kSoftWarps);
+    mbar_init(b_done, kSoftWarps);
     mbar_init(o_empty, kSoftWarps);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kMmaWarp) {  // S twice 128 columns, O: 512 is the next size that there is
+  if (warp == kMmaWarp) {  // all of it: two S, two O
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
                  "r"(512)
@@ -249,7 +274,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   __syncthreads();
   after_sync();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem_o = tmem + 256;
+  const uint32_t tmem_o = tmem + 2 * kPromptTile;  // O of stream u: + 128 u
   // A wait that gives up ends its role; the others give up in turn.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_wait(bar, parity)) return true;
@@ -269,31 +294,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
     if (lane == 0) {
       constexpr uint32_t idesc_s = prompt_idesc(kPromptTile, 0), idesc_o = prompt_idesc(D, 1);
       const uint64_t q_desc = operand_desc(sm + S::kOffQ, 16, 1024);
-      const uint64_t p_desc = operand_desc(sm + S::kOffP, 16, 1024);
-      // O += P V of tile m, the first of its item or not
+      // O += P V of tile m, the first of its item and stream or not
       auto output = [&](int m, bool first) {
         const int u = m & 1;
-        if (!wait(p_full, m & 1) || !wait(&v_full[u], (m >> 1) & 1) ||
+        if (!wait(&p_full[u], (m >> 1) & 1) || !wait(&v_full[u], (m >> 1) & 1) ||
             (first && item > 0 && !wait(o_empty, (item - 1) & 1)))
           return false;
         after_sync();
         const uint64_t v_desc = operand_desc(sm + S::kOffV + u * S::kOperand, S::kHalf, 1024);
 #pragma unroll
-        for (int k = 0; k < kPromptTile / 16; ++k)  // 16 tokens: 32 bytes of P, 16 rows of V
-          mma_f16(tmem_o, p_desc + (((k >> 2) * S::kHalf + (k & 3) * 32) >> 4),
-                  v_desc + ((k * 16 * 128) >> 4), idesc_o, first && k == 0 ? 0u : 1u);
+        for (int k = 0; k < kPromptTile / 16; ++k)  // 16 tokens: 8 columns of P, 16 rows of V
+          mma_f16_ts(tmem_o + u * kPromptTile, tmem + u * kPromptTile + 8 * k,
+                     v_desc + ((k * 16 * 128) >> 4), idesc_o, first && k == 0 ? 0u : 1u);
         __threadfence_block();  // the widen warps' marks, for those who wait for pv_done
         commit_to(&v_empty[u]);
-        commit_to(pv_done);
+        commit_to(&pv_done[u]);
         return true;
       };
       while (ok && walk.next(p)) {
         if (!(ok = wait(q_full, item & 1))) break;
-        const int tiles = walk.t1 - walk.t0;
-        for (int i = 0; i < tiles && ok; ++i, ++n) {
+        const int n0 = n;
+        for (int t = walk.t0; t < walk.t1 && ok; ++t, ++n) {
           const int u = n & 1;
+          // the stream's last P lies where this S goes
           ok = wait(&k_full[u], (n >> 1) & 1) &&
-               (n < 2 || wait(&s_empty[u], ((n >> 1) & 1) ^ 1u));
+               (n < 2 || wait(&pv_done[u], ((n >> 1) & 1) ^ 1u));
           if (!ok) break;
           after_sync();
           const uint64_t k_desc = operand_desc(sm + S::kOffK + u * S::kOperand, 16, 1024);
@@ -305,81 +330,91 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           __threadfence_block();  // the widen warps' scales, for those who wait for s_full
           commit_to(&k_empty[u]);
           commit_to(&s_full[u]);
-          if (i > 0) ok = output(n - 1, i == 1);
+          if (n > n0) ok = output(n - 1, n - 1 - n0 < 2);
         }
-        if (ok) ok = output(n - 1, tiles == 1);
+        if (ok) ok = output(n - 1, n - 1 - n0 < 2);
         ++item;
       }
     }
-  } else if (warp >= kSoftWarps) {
+  } else if (warp >= kWidenWarp) {
     // ------------------------------------------------------------ widen
     constexpr int CPR = D / 16, RPP = 128 / CPR, NP = kPromptTile / RPP;  // chunks a row, rows a pass
-    const int wt = tid - kSoftWarps * 32;
+    const int wt = tid - kWidenWarp * 32;
     const int c = wt % CPR, rr = wt / CPR;
-    uint4 kr[NP], vr[NP];
-    int ids = -1;       // lane 8 j + b: block b of tile t + j, j < 4
+    const uint32_t raw_k = sm + S::kOffRaw + 16 * wt, raw_v = raw_k + S::kRaw;  // + 2048 a pass
+    const ptrdiff_t v_from_k = p.v - p.k;
+    float sc_k = 0.f, sc_v = 0.f;  // scales of block wt of the loaded tile, threads 0 .. 7
+    int ids = -1;         // lane 8 j + b: block b of tile t + j, j < 4
     Walk<G> next = walk;  // the item of the tile that is loaded
     bool more = next.next(p);
     int lt = more ? next.t0 : 0, id_at = 4;
-    // Loads the next tile's bytes, and writes its scales to slot m & 3.
-    auto load = [&](int m) {
-      if (!more) return;
-      if (id_at == 4) {
-        const int tok = (lt + (lane >> 3)) * kPromptTile + 16 * (lane & 7);
-        ids = -1;
-        if (lt + (lane >> 3) < next.t1 && tok < next.limit) {
-          const int pi = tok >> p.page_shift;
-          if (pi < p.max_pages) ids = p.page_table[next.b * p.table_stride + pi];
-          if ((uint32_t)ids >= (uint32_t)p.pages) {
-            ids = -1;
-            atomicCAS(p.err, 0, kErrKvRange);
+    uint32_t real = 0u;   // bit i: the row of pass i has a page and is below the limit
+    int64_t offs[NP];     // where its chunk lies
+    // The next tile's K codes and its scales on their way, then (load_v) its V codes.
+    auto load_k = [&]() {
+      if (more) {
+        if (id_at == 4) {
+          const int tok = (lt + (lane >> 3)) * kPromptTile + 16 * (lane & 7);
+          ids = -1;
+          if (lt + (lane >> 3) < next.t1 && tok < next.limit) {
+            const int pi = tok >> p.page_shift;
+            if (pi < p.max_pages) ids = p.page_table[next.b * p.table_stride + pi];
+            if ((uint32_t)ids >= (uint32_t)p.pages) {
+              ids = -1;
+              atomicCAS(p.err, 0, kErrKvRange);
+            }
+          }
+          id_at = 0;
+        }
+        const int id_b = __shfl_sync(0xffffffffu, ids, 8 * id_at + (lane & 7));
+        if (wt < 8) {
+          sc_k = sc_v = 0.f;  // no page
+          if (id_b >= 0) {
+            const size_t blk = (size_t)id_b * p.kv_heads + next.h;
+            sc_k = p.k_scale[blk];
+            sc_v = p.v_scale[blk];
           }
         }
-        id_at = 0;
-      }
-      const int id_b = __shfl_sync(0xffffffffu, ids, 8 * id_at + (lane & 7));
-      if (wt < 8) {  // a block's scales; no page: a score of minus infinity
-        const int id = id_b;
-        float4 sc = make_float4(0.f, -INFINITY, 0.f, 0.f);
-        if (id >= 0) {
-          const size_t blk = (size_t)id * p.kv_heads + next.h;
-          const float vs = p.v_scale[blk];
-          sc = vs > 0.f ? make_float4(p.k_scale[blk], lg2(vs), 1.0f / vs, 0.f) : sc;
-        }
-        reinterpret_cast<float4*>(base + S::kOffScale)[(m & 3) * 8 + wt] = sc;
-      }
-      const int tok0 = lt * kPromptTile;
+        real = 0u;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int row = i * RPP + rr, tok = tok0 + row;
-        const int id = __shfl_sync(0xffffffffu, ids, 8 * id_at + (row >> 4));
-        const bool real = id >= 0 && tok < next.limit;
-        const size_t at = ((((size_t)max(id, 0) * p.kv_heads + next.h) << p.page_shift) +
-                           (tok & (p.page - 1))) * D + 16 * c;
-        kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (real) {
-          kr[i] = __ldg(reinterpret_cast<const uint4*>(p.k + at));
-          vr[i] = __ldg(reinterpret_cast<const uint4*>(p.v + at));
+        for (int i = 0; i < NP; ++i) {
+          const int row = i * RPP + rr, tok = lt * kPromptTile + row;
+          const int id = __shfl_sync(0xffffffffu, ids, 8 * id_at + (row >> 4));
+          offs[i] = ((((int64_t)max(id, 0) * p.kv_heads + next.h) << p.page_shift) +
+                     (tok & (p.page - 1))) * D + 16 * c;
+          const bool is = id >= 0 && tok < next.limit;
+          real |= (uint32_t)is << i;
+          cp16_if(raw_k + 2048 * i, p.k + offs[i], is);
         }
       }
-      ++id_at;
-      if (++lt >= next.t1) {
-        more = next.next(p);
-        lt = next.t0;
-        id_at = 4;
+      cp_commit();
+    };
+    auto load_v = [&]() {
+      if (more) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          cp16_if(raw_v + 2048 * i, p.k + offs[i] + v_from_k, (real >> i & 1u) != 0u);
+        ++id_at;
+        if (++lt >= next.t1) {
+          more = next.next(p);
+          lt = next.t0;
+          id_at = 4;
+        }
       }
+      cp_commit();
     };
     // 16 codes to two chunks of an operand row
-    auto widen = [&](uint32_t to, int row, const uint4& v) {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
-      const uint4 a = make_uint4(e4m3_lo(w[0]), e4m3_hi(w[0]), e4m3_lo(w[1]), e4m3_hi(w[1]));
-      const uint4 b = make_uint4(e4m3_lo(w[2]), e4m3_hi(w[2]), e4m3_lo(w[3]), e4m3_hi(w[3]));
+    auto widen = [&](uint32_t to, int row, uint32_t from) {
+      const uint4 v = lds128(from);
+      const uint4 a = make_uint4(e4m3_lo(v.x), e4m3_hi(v.x), e4m3_lo(v.y), e4m3_hi(v.y));
+      const uint4 b = make_uint4(e4m3_lo(v.z), e4m3_hi(v.z), e4m3_lo(v.w), e4m3_hi(v.w));
       const uint32_t half = to + (c >> 2) * S::kHalf;
       const int j = 2 * (c & 3), first = c >> 2;  // the halves' lanes write in other orders:
       sts128(half + operand_at(row, j + first), first ? b : a);  // no bank twice
       sts128(half + operand_at(row, j + 1 - first), first ? a : b);
     };
-    load(0);
+    load_k();
+    load_v();
     while (ok && walk.next(p)) {
       const int n_rows = walk.s.n * p.group;
       const int cur_r0 = walk.rt * kRows;
@@ -388,57 +423,71 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       for (int t = walk.t0; t < walk.t1 && ok; ++t, ++n) {
         const int u = n & 1;
         if (n >= 2 && !(ok = wait(&k_empty[u], ((n >> 1) & 1) ^ 1u))) break;
+        if (wt < 8)  // the block's K scale, log2 and inverse of its V scale; no page: -inf
+          reinterpret_cast<float4*>(base + S::kOffScale)[(n & 3) * 8 + wt] =
+              sc_v > 0.f ? make_float4(sc_k, lg2(sc_v), 1.0f / sc_v, 0.f)
+                         : make_float4(0.f, -INFINITY, 0.f, 0.f);
+        cp_wait<1>();  // K's copies
 #pragma unroll
-        for (int i = 0; i < NP; ++i) widen(sm + S::kOffK + u * S::kOperand, i * RPP + rr, kr[i]);
+        for (int i = 0; i < NP; ++i)
+          widen(sm + S::kOffK + u * S::kOperand, i * RPP + rr, raw_k + 2048 * i);
         to_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[u]);
+        load_k();
         if (n >= 2 && !(ok = wait(&v_empty[u], ((n >> 1) & 1) ^ 1u))) break;
-        const bool mixed = (t + 1) * kPromptTile > low && low < walk.limit;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          uint4 v = vr[i];
-          if (mixed) {
-            // A NaN that one row of the item sees must not reach a row that does
-            // not (0 * NaN): NaN codes leave V, and the outputs that they belong
-            // to are marked.
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
+        cp_wait<1>();  // V's
+        if ((t + 1) * kPromptTile > low && low < walk.limit) {
+          // Rows of the item end at different tokens here, and a NaN that one row
+          // sees must not reach a row that does not (0 * NaN): NaN codes leave V,
+          // and the outputs that they belong to are marked.
+#pragma unroll 1
+          for (int i = 0; i < NP; ++i) {
+            const int tok = t * kPromptTile + i * RPP + rr;
+#pragma unroll 1
             for (int k = 0; k < 4; ++k) {
-              const uint32_t nan = __vcmpeq4(w[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              const uint32_t at = raw_v + 2048 * i + 4 * k;
+              const uint32_t v = lds32(at);
+              const uint32_t nan = __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
               if (nan == 0u) continue;
-              w[k] &= ~nan;
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v & ~nan) : "memory");
               const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) |
                                      (nan >> 21 & 8u)) << (16 * (c & 1) + 4 * k);
-              const int tok = t * kPromptTile + i * RPP + rr;
 #pragma unroll 1
               for (int r = cur_r0; r < min(n_rows, cur_r0 + kRows); ++r)
                 if (tok < seen(p, walk.s, r))
                   atomicOr(mine + (r - cur_r0) * (D / 32) + (c >> 1), bits);
             }
           }
-          widen(sm + S::kOffV + u * S::kOperand, i * RPP + rr, v);
+          __syncwarp();
         }
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          widen(sm + S::kOffV + u * S::kOperand, i * RPP + rr, raw_v + 2048 * i);
         to_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[u]);
-        load(n + 1);
+        load_v();
       }
       ++item;
     }
   } else {
     // ------------------------------------------------------------ softmax
-    const uint32_t lanes = (uint32_t)(32 * warp) << 16;  // this warp's lanes of tensor memory
+    const int stream = warp / kSoftWarps, r = tid % kPromptTile;  // row of the item
+    const uint32_t lanes = (uint32_t)(32 * (warp % kSoftWarps)) << 16;  // its lanes of tensor memory
+    const uint32_t tmem_s = tmem + lanes + stream * kPromptTile;
+    float* mul_s = reinterpret_cast<float*>(base + S::kOffMul);
+    float2* sums_s = reinterpret_cast<float2*>(base + S::kOffSums);
     while (ok && walk.next(p)) {
       const int n_rows = walk.s.n * p.group;
-      const int row = walk.rt * kRows + tid;
+      const int row = walk.rt * kRows + r;
       const bool in = row < n_rows;
       const int qi = by_group(p, row);
       const int lim = in ? seen(p, walk.s, row) : 0;
-      // ---- this row's query, scaled to 2^14, as the A operand. The last item's
-      // products are done: its last S has been read.
       float q_mul;
-      {
+      if (stream == 0) {
+        // ---- this row's query, scaled to 2^14, as the A operand. The last item's
+        // products are done: both streams are through with it.
         const uint16_t* src = p.q + (int64_t)(walk.s.first + qi) * p.q_row +
                               (int64_t)(walk.h * p.group + row - qi * p.group) * p.q_head;
         uint4 raw[D / 8];
@@ -460,6 +509,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
         const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
         q_mul = p.scale_log2 * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+        mul_s[r] = q_mul;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) {
           uint32_t o[4];
@@ -468,102 +518,131 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             const float2 f = two(reinterpret_cast<const uint32_t*>(&raw[k])[w]);
             o[w] = half2_bits(f.x * up, f.y * up);
           }
-          sts128(sm + S::kOffQ + (k >> 3) * S::kHalf + operand_at(tid, k & 7),
+          sts128(sm + S::kOffQ + (k >> 3) * S::kHalf + operand_at(r, k & 7),
                  make_uint4(o[0], o[1], o[2], o[3]));
         }
         to_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
+      } else {
+        if (!(ok = wait(q_full, item & 1))) break;
+        q_mul = mul_s[r];
       }
-      float m = -INFINITY;  // the running maximum that O and l are scaled by
+      float m = -INFINITY;  // the running maximum that the stream's O and l are scaled by
       float l = 0.f;
-      const int n0 = n;
+      int last = -1;        // the stream's last tile
       for (int t = walk.t0; t < walk.t1 && ok; ++t, ++n) {
-        const int u = n & 1;
-        if (!(ok = wait(&s_full[u], (n >> 1) & 1))) break;
+        if ((n & 1) != stream) continue;
+        if (!(ok = wait(&s_full[stream], (n >> 1) & 1))) break;
         after_sync();
-        float x[kPromptTile];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) ld32(tmem + lanes + u * kPromptTile + 32 * c, x + 32 * c);
-        ld_wait();
         const float4* sc = scale_s + (n & 3) * 8;
         const int left = lim - t * kPromptTile;  // tokens of the tile that the row sees
-        float top = -INFINITY;
+        const bool cut = __any_sync(0xffffffffu, left < kPromptTile);
+        // Columns 32 c .. + 31 of S to log2 units with the value scale, masked. Read
+        // twice, for the maximum and for P': 128 registers a thread are what two
+        // streams leave.
+        float x[32];
+        auto scores = [&](int c) {
+          ld32(tmem_s + 32 * c, x);
+          ld_wait();
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          const float4 f = sc[b];
-          const float ks = f.x * q_mul;
+          for (int b = 0; b < 2; ++b) {
+            const float4 f = sc[2 * c + b];
+            const float ks = f.x * q_mul;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[16 * b + k] = fmaf(x[16 * b + k], ks, f.y);
+            for (int k = 0; k < 16; ++k) x[16 * b + k] = fmaf(x[16 * b + k], ks, f.y);
+          }
+          if (cut) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (32 * c + k >= left) x[k] = -INFINITY;
+          }
+        };
+        float tops[8];  // chains side by side
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tops[k] = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          scores(c);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) tops[k & 7] = fmaxf(tops[k & 7], x[k]);
         }
-        if (__any_sync(0xffffffffu, left < kPromptTile)) {
-#pragma unroll
-          for (int k = 0; k < kPromptTile; ++k)
-            if (k >= left) x[k] = -INFINITY;
-        }
-#pragma unroll
-        for (int k = 0; k < kPromptTile; ++k) top = fmaxf(top, x[k]);
-        // ---- a much larger maximum: O and l move to it
-        const bool grow = top > m + kGrowth;  // also from minus infinity
-        const bool any_grow = __any_sync(0xffffffffu, grow);
-        // P V of the tile before: P' may be overwritten, O is at rest
-        if (n > n0 && !(ok = wait(pv_done, (n - 1) & 1))) break;
-        after_sync();
-        if (any_grow) {
-          const float al = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
-          if (grow) m = top;
+        const float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
+                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+        // ---- a row's maximum much larger: all rows' O and l move to theirs (the
+        // stream's last product is done: S came after it)
+        if (__any_sync(0xffffffffu, top > m + kGrowth)) {
+          const float most = fmaxf(m, top);
+          const float al = m == -INFINITY ? 0.f : ex2(m - most);
+          m = most;
           l *= al;
-          if (n > n0) {
+          if (last >= 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
+              const uint32_t at = tmem_o + lanes + stream * kPromptTile + 32 * c;
               float o[32];
-              ld32(tmem_o + lanes + 32 * c, o);
+              ld32(at, o);
               ld_wait();
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] *= al;
-              st32(tmem_o + lanes + 32 * c, o);
+              st32(at, reinterpret_cast<const uint32_t*>(o));
             }
-            st_wait();
           }
         }
         const float sub = m == -INFINITY ? 0.f : m - kPromptShift;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          scores(c);
+          uint32_t w[16];
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          float sum = 0.f;
-          uint32_t w[8];
+          for (int b = 0; b < 2; ++b) {
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float a = ex2(x[16 * b + 2 * k] - sub), d = ex2(x[16 * b + 2 * k + 1] - sub);
-            sum += a + d;
-            w[k] = half2_bits(a, d);
+            for (int k = 0; k < 8; ++k) {
+              const float a = ex2(x[16 * b + 2 * k] - sub), d = ex2(x[16 * b + 2 * k + 1] - sub);
+              sum[k & 3] += a + d;
+              w[8 * b + k] = half2_bits(a, d);
+            }
+            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), sc[2 * c + b].z, l);
           }
-          l = fmaf(sum, sc[b].z, l);
-          const uint32_t to = sm + S::kOffP + (b >> 2) * S::kHalf;
-          sts128(to + operand_at(tid, 2 * (b & 3)), make_uint4(w[0], w[1], w[2], w[3]));
-          sts128(to + operand_at(tid, 2 * (b & 3) + 1), make_uint4(w[4], w[5], w[6], w[7]));
+          st16(tmem_s + 16 * c, w);  // over columns that have been read
         }
-        to_async_proxy();
+        st_wait();
         before_sync();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&s_empty[u]);
-          mbar_arrive(p_full);
-        }
+        if (lane == 0) mbar_arrive(&p_full[stream]);
+        last = n;
       }
-      if (!ok) break;
-      // ---- the item's output, or the part of it
-      if (!(ok = wait(pv_done, (n - 1) & 1))) break;
+      if (!ok || (last >= 0 && !(ok = wait(&pv_done[stream], (last >> 1) & 1)))) break;
+      // ---- the streams meet: the second one leaves maximum and sum
+      if (stream == 1) {
+        sums_s[(item & 1) * kPromptTile + r] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_done);
+        ++item;
+        continue;
+      }
+      if (!(ok = wait(b_done, item & 1))) break;
       after_sync();
-      uint32_t* mine = marks + (item & 3) * (S::kMarks / 4) + tid * (D / 32);  // this thread's alone
+      const float2 other = sums_s[(item & 1) * kPromptTile + r];
+      const float most = fmaxf(m, other.x);
+      const float fa = m == -INFINITY ? 0.f : ex2(m - most);
+      const float fb = other.x == -INFINITY ? 0.f : ex2(other.x - most);
+      l = l * fa + other.y * fb;
+      const bool has_a = last >= 0, has_b = walk.t1 - walk.t0 > 1 || !has_a;
+      uint32_t* mine = marks + (item & 3) * (S::kMarks / 4) + r * (D / 32);  // this thread's alone
       const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
       uint16_t* dst = p.out + (int64_t)(walk.s.first + qi) * p.out_row +
                       (int64_t)(walk.h * p.group + row - qi * p.group) * p.out_head;
-      float* part = p.parts + (((size_t)blockIdx.x * 2 + walk.slot(share)) * kRows + tid) * S::kPitch;
+      float* part = p.parts + (((size_t)blockIdx.x * 2 + walk.slot(share)) * kRows + r) * S::kPitch;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        ld32(tmem_o + lanes + 32 * c, o);
+        float o[32], o2[32];
+        if (has_a) ld32(tmem_o + lanes + 32 * c, o);
+        if (has_b) ld32(tmem_o + lanes + kPromptTile + 32 * c, o2);
         ld_wait();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = (has_a ? o[k] * fa : 0.f) + (has_b ? o2[k] * fb : 0.f);
         const uint32_t mark = mine[c];
         if (mark) {
 #pragma unroll
@@ -596,9 +675,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         }
       }
       if (!walk.whole) {
-        // in the other kernel's terms the maximum is m, with P' scaled by 2^14:
-        // only the ratio of outputs and sum counts
-        if (in) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+        if (in) *reinterpret_cast<float2*>(part + D) = make_float2(most, l);
         if (tid == 0) walk.describe(p, share);
       }
       before_sync();
