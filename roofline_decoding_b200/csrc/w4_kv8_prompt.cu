@@ -12,6 +12,8 @@
 //                    barrier); e4m3 to fp16 (exact) and back as MMA operands, K and V alike token by token in the 128B-swizzled
 //                    layout (K is the K-major operand of Q K^T; of P V the same
 //                    rows are the MN-major operand V, so nothing is transposed);
+//   item warp      : walks the CTA's share and leaves the items in a ring, so that
+//                    no other warp carries the walk in its registers and code;
 //   MMA warp       : one thread issues S = Q K^T of one stream (M = N = 128),
 //                    then O += P V of the other, so that the tensor cores work
 //                    for one while the other's softmax does;
@@ -36,7 +38,12 @@ namespace {
 constexpr int kSoftWarps = 4, kWidenWarps = 4;  // softmax warps of a stream
 constexpr int kWidenWarp = 2 * kSoftWarps;
 constexpr int kMmaWarp = kWidenWarp + kWidenWarps;
-constexpr int kPromptThreads = 32 * (kMmaWarp + 1);
+constexpr int kItemWarp = kMmaWarp + 1;
+constexpr int kPromptThreads = 32 * (kMmaWarp + 4);  // four warpgroups; two warps idle
+// Registers a thread: 128 at launch, then by warpgroup (their sum is four times
+// that, which is what the block has).
+constexpr int kSoftRegs = 152, kWidenRegs = 128, kMmaRegs = 80;
+static_assert(2 * kSoftRegs + kWidenRegs + kMmaRegs <= 4 * 128, "registers of the block");
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
 constexpr float kPromptShift = 11.0f;  // P' of the maximum that O is scaled by is 2^kPromptShift
 constexpr float kGrowth = 3.0f;        // the running maximum may exceed it by this much
@@ -89,6 +96,19 @@ struct Rows128 {
   }
 };
 
+// An item as the item warp leaves it; t0 == t1: there are no more.
+struct Item {
+  int t0, t1;        // its tiles
+  int limit;         // tokens that its last row sees
+  int past;          // tokens before the sequence's rows
+  int b, h;          // sequence, cache head
+  int first;         // the sequence's first row
+  int r0, n_rows;    // first query row, all query rows of the head
+  int whole, slot;   // all tiles of the item are here, or where the part goes
+  int pad;
+};
+constexpr int kItems = 4;  // ring
+
 template <int D>
 struct PromptShape {
   static constexpr int kHalf = kPromptTile * 128;         // 128 rows of 64 fp16
@@ -100,13 +120,14 @@ struct PromptShape {
   static constexpr int kRaw = kPromptTile * D;            // a K or V tile's codes
   static constexpr int kOffRaw = kOffV + 2 * kOperand;    // K, then V
   static constexpr int kOffScale = kOffRaw + 2 * kRaw;  // four tiles of 8 x (K, log2 V, 1 / V, 0)
-  static constexpr int kOffMul = kOffScale + 4 * 8 * 16;  // a factor a row
-  static constexpr int kOffSums = kOffMul + kPromptTile * 4;  // second stream's maxima and sums,
-                                                              // two items in turn
+  // two items in turn: a factor a row, maxima and sums of the stream that meets the other
+  static constexpr int kOffMul = kOffScale + 4 * 8 * 16;
+  static constexpr int kOffSums = kOffMul + 2 * kPromptTile * 4;
   static constexpr int kOffMarks = kOffSums + 2 * kPromptTile * 8;
   static constexpr int kMarks = kPromptTile * D / 8;      // of an item; four items
-  static constexpr int kOffBar = kOffMarks + 4 * kMarks;
-  static constexpr int kBars = 7 * 2 + 3;
+  static constexpr int kOffItems = kOffMarks + 4 * kMarks;
+  static constexpr int kOffBar = kOffItems + kItems * (int)sizeof(Item);
+  static constexpr int kBars = 8 * 2 + 2 + 2 * kItems;
   static constexpr int kOffTmem = kOffBar + kBars * 8;
   static constexpr int kSmem = 1024 + kOffTmem + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -159,22 +180,23 @@ __device__ __forceinline__ void after_sync() {
 __device__ __forceinline__ void to_async_proxy() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-// 32 columns of this warp's 32 lanes; several loads may be in flight until ld_wait.
-__device__ __forceinline__ void ld32(uint32_t addr, float* r) {
+// 32 columns of this warp's 32 lanes, landed: the wait stands in the same statement,
+// so that nothing is done with the registers before it.
+__device__ __forceinline__ void ld32(uint32_t addr, float (&r)[32]) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
-        "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
-        "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]),
-        "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]),
-        "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-      : "r"(addr));
-}
-__device__ __forceinline__ void ld_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31"
+      "}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
+        "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
+        "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr)
+      : "memory");
 }
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t* u) {
   asm volatile(
@@ -205,13 +227,36 @@ __device__ __forceinline__ void st_wait() {
 __device__ __forceinline__ uint32_t operand_at(int r, int c) {
   return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
                : "memory");
 }
 
-template <int D>
+// mbar_wait with the clock for its limit, about a second: little code, for a
+// dozen waits in each role.
+__device__ __forceinline__ bool wait_on(uint64_t* bar, uint32_t parity) {
+  const long long began = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - began > 2000000000ll) return false;
+  return true;
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int D, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const AttnP p) {
   using S = PromptShape<D>;
   using G = Rows128;
@@ -229,11 +274,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   uint64_t* s_full = bars + 8;    // S is in tensor memory (commit)
   uint64_t* p_full = bars + 10;   // P' is in its place, O is rescaled (softmax warps)
   uint64_t* pv_done = bars + 12;  // P V is done (commit)
-  uint64_t* q_full = bars + 14;   // an item's queries are in shared memory (first stream)
-  uint64_t* b_done = bars + 15;   // the second stream is through with an item
-  uint64_t* o_empty = bars + 16;  // an item's outputs are read (first stream)
+  // Two, by item: a stream that writes an item out may be at its queries when the
+  // other one prepares those of the item after. (Never two after: that takes a
+  // second S of the first stream, which has read its factors by then.)
+  uint64_t* q_full = bars + 14;   // an item's queries are in shared memory, factors in mul_s
+  uint64_t* b_done = bars + 16;   // the stream without the item's last tile is through with it
+  uint64_t* o_empty = bars + 17;  // an item's outputs are read (the other one)
+  uint64_t* item_full = bars + 18;             // an item is in the ring
+  uint64_t* item_empty = item_full + kItems;   // MMA, widen and softmax warps are through with it
+  Item* items = reinterpret_cast<Item*>(base + S::kOffItems);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + S::kOffTmem);
-  int* abort_flag = reinterpret_cast<int*>(base + S::kOffTmem + 4);
   // Marks of four items in turn: the widen warps may be two tiles ahead, that is
   // two short items, of the item whose output is read, but no more than that:
   // they have seen a product of the item before theirs but one, whose first waits
@@ -251,11 +301,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], kSoftWarps);
       mbar_init(&pv_done[i], 1);
+      mbar_init(&q_full[i], kSoftWarps);
     }
-    mbar_init(q_full, kSoftWarps);
     mbar_init(b_done, kSoftWarps);
     mbar_init(o_empty, kSoftWarps);
-    *abort_flag = 0;
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 1 + kWidenWarps + 2 * kSoftWarps);
+    }
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {  // all of it: two S, two O
@@ -269,29 +322,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   for (int i = tid; i < S::kMarks; i += kPromptThreads) marks[i] = 0u;
   grid_dependency_wait();
   grid_launch_dependents();
-  const Share share = find_share<G>(p);
-  if (tid == 0) p.join[blockIdx.x].count = 0;
   __syncthreads();
   after_sync();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem + 2 * kPromptTile;  // O of stream u: + 128 u
   // A wait that gives up ends its role; the others give up in turn.
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (mbar_wait(bar, parity)) return true;
-    if (p.err) atomicCAS(p.err, 0, kErrPromptWait);
-    *reinterpret_cast<volatile int*>(abort_flag) = 1;
-    return false;
-  };
-
-  Walk<G> walk;
-  walk.start(share);
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_on(bar, parity); };
   int n = 0;     // tiles that this CTA has begun, over all items
   int item = 0;  // items
   bool ok = true;
+  Item it;
+  // Item `item` of the ring; false when there is none.
+  auto next_item = [&]() {
+    if (!(ok = wait(&item_full[item % kItems], (item / kItems) & 1))) return false;
+    it = items[item % kItems];
+    return it.t0 < it.t1;
+  };
+  auto done_item = [&]() { mbar_arrive(&item_empty[item++ % kItems]); };  // once a warp
 
-  if (warp == kMmaWarp) {
+  if (warp >= kMmaWarp) {
     // ------------------------------------------------------------ MMA
-    if (lane == 0) {
+    fewer_registers<kMmaRegs>();
+    if (warp == kItemWarp) {
+      const Share share = find_share<G>(p);
+      if (lane == 0) p.join[blockIdx.x].count = 0;
+      Walk<G> walk;
+      walk.start(share);
+      for (;; ++item) {
+        const bool more = share.x < share.end && walk.next(p);
+        const int at = item % kItems;
+        if (item >= kItems && !(ok = wait(&item_empty[at], ((item / kItems) & 1) ^ 1u))) break;
+        if (lane == 0) {
+          it.t0 = it.t1 = 0;
+          if (more) {
+            it.t0 = walk.t0, it.t1 = walk.t1, it.limit = walk.limit, it.past = walk.s.past;
+            it.b = walk.b, it.h = walk.h, it.first = walk.s.first;
+            it.r0 = walk.rt * kRows, it.n_rows = walk.s.n * p.group;
+            it.whole = walk.whole, it.slot = walk.slot(share);
+            if (!walk.whole) walk.describe(p, share);
+          }
+          items[at] = it;
+          mbar_arrive(&item_full[at]);
+        }
+        __syncwarp();
+        if (!more) break;
+      }
+    } else if (warp == kMmaWarp && lane == 0) {
       constexpr uint32_t idesc_s = prompt_idesc(kPromptTile, 0), idesc_o = prompt_idesc(D, 1);
       const uint64_t q_desc = operand_desc(sm + S::kOffQ, 16, 1024);
       // O += P V of tile m, the first of its item and stream or not
@@ -311,10 +387,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         commit_to(&pv_done[u]);
         return true;
       };
-      while (ok && walk.next(p)) {
-        if (!(ok = wait(q_full, item & 1))) break;
+      while (ok && next_item()) {
+        if (!(ok = wait(&q_full[item & 1], (item >> 1) & 1))) break;
         const int n0 = n;
-        for (int t = walk.t0; t < walk.t1 && ok; ++t, ++n) {
+        for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
           const int u = n & 1;
           // the stream's last P lies where this S goes
           ok = wait(&k_full[u], (n >> 1) & 1) &&
@@ -333,32 +409,60 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           if (n > n0) ok = output(n - 1, n - 1 - n0 < 2);
         }
         if (ok) ok = output(n - 1, n - 1 - n0 < 2);
-        ++item;
+        done_item();
       }
     }
   } else if (warp >= kWidenWarp) {
     // ------------------------------------------------------------ widen
+    fewer_registers<kWidenRegs>();
     constexpr int CPR = D / 16, RPP = 128 / CPR, NP = kPromptTile / RPP;  // chunks a row, rows a pass
     const int wt = tid - kWidenWarp * 32;
-    const int c = wt % CPR, rr = wt / CPR;
+    // A quarter warp takes one chunk of eight rows: its 16-byte stores fall on all
+    // banks. A pass is RPP rows.
+    const int c = (lane >> 3) + (CPR == 8 ? 4 * ((wt >> 5) & 1) : 0);
+    const int rr = (lane & 7) + 8 * (CPR == 8 ? wt >> 6 : wt >> 5);
     const uint32_t raw_k = sm + S::kOffRaw + 16 * wt, raw_v = raw_k + S::kRaw;  // + 2048 a pass
-    const ptrdiff_t v_from_k = p.v - p.k;
     float sc_k = 0.f, sc_v = 0.f;  // scales of block wt of the loaded tile, threads 0 .. 7
     int ids = -1;         // lane 8 j + b: block b of tile t + j, j < 4
-    Walk<G> next = walk;  // the item of the tile that is loaded
-    bool more = next.next(p);
-    int lt = more ? next.t0 : 0, id_at = 4;
-    uint32_t real = 0u;   // bit i: the row of pass i has a page and is below the limit
-    int64_t offs[NP];     // where its chunk lies
+    // the item of the tile that is loaded: it may be the one after `it`
+    int l_item = 0, l_t1 = 0, l_limit = 0, l_b = 0, l_h = 0, lt = 0, id_at = 4;
+    bool more = true;
+    auto next_load = [&]() {
+      const int at = l_item % kItems;
+      more = (ok = wait(&item_full[at], (l_item / kItems) & 1)) && items[at].t0 < items[at].t1;
+      if (!more) return;
+      lt = items[at].t0, l_t1 = items[at].t1, l_limit = items[at].limit;
+      l_b = items[at].b, l_h = items[at].h;
+      ++l_item;
+      id_at = 4;
+    };
+    next_load();
+    int64_t block_at = 0;  // lane b: where block b & 7 of the tile begins
+    bool full = false;     // every block has a page, every token is below the limit
+    int limit_in = 0;      // tokens of the tile below the limit
+    uint32_t pages_in = 0; // bit b: block b has a page
+    // pass i of this warp lies in block (i * RPP) / 16 + own_block, at own_at
+    const int own_block = rr >> 4, own_at = (rr & 15) * D + 16 * c;
+    auto copy = [&](const uint8_t* from, uint32_t to) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int b = i * RPP / 16 + own_block;
+        const uint8_t* src = from + __shfl_sync(0xffffffffu, block_at, b) + own_at;
+        if (full)
+          cp16(to + 2048 * i, src);
+        else  // zeros for tokens behind the limit and of no page
+          cp16_if(to + 2048 * i, src, (pages_in >> b & 1u) && i * RPP + rr < limit_in);
+      }
+    };
     // The next tile's K codes and its scales on their way, then (load_v) its V codes.
     auto load_k = [&]() {
       if (more) {
         if (id_at == 4) {
           const int tok = (lt + (lane >> 3)) * kPromptTile + 16 * (lane & 7);
           ids = -1;
-          if (lt + (lane >> 3) < next.t1 && tok < next.limit) {
+          if (lt + (lane >> 3) < l_t1 && tok < l_limit) {
             const int pi = tok >> p.page_shift;
-            if (pi < p.max_pages) ids = p.page_table[next.b * p.table_stride + pi];
+            if (pi < p.max_pages) ids = p.page_table[l_b * p.table_stride + pi];
             if ((uint32_t)ids >= (uint32_t)p.pages) {
               ids = -1;
               atomicCAS(p.err, 0, kErrKvRange);
@@ -367,60 +471,56 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           id_at = 0;
         }
         const int id_b = __shfl_sync(0xffffffffu, ids, 8 * id_at + (lane & 7));
+        const int64_t blk = (int64_t)max(id_b, 0) * p.kv_heads + l_h;
         if (wt < 8) {
           sc_k = sc_v = 0.f;  // no page
           if (id_b >= 0) {
-            const size_t blk = (size_t)id_b * p.kv_heads + next.h;
             sc_k = p.k_scale[blk];
             sc_v = p.v_scale[blk];
           }
         }
-        real = 0u;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const int row = i * RPP + rr, tok = lt * kPromptTile + row;
-          const int id = __shfl_sync(0xffffffffu, ids, 8 * id_at + (row >> 4));
-          offs[i] = ((((int64_t)max(id, 0) * p.kv_heads + next.h) << p.page_shift) +
-                     (tok & (p.page - 1))) * D + 16 * c;
-          const bool is = id >= 0 && tok < next.limit;
-          real |= (uint32_t)is << i;
-          cp16_if(raw_k + 2048 * i, p.k + offs[i], is);
-        }
+        const int tok0 = lt * kPromptTile;
+        block_at = ((blk << p.page_shift) + ((tok0 + 16 * (lane & 7)) & (p.page - 1))) * D;
+        limit_in = l_limit - tok0;
+        pages_in = __ballot_sync(0xffffffffu, id_b >= 0);
+        full = limit_in >= kPromptTile && (pages_in & 0xffu) == 0xffu;
+        copy(p.k, raw_k);
       }
       cp_commit();
     };
     auto load_v = [&]() {
       if (more) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          cp16_if(raw_v + 2048 * i, p.k + offs[i] + v_from_k, (real >> i & 1u) != 0u);
+        copy(p.v, raw_v);
         ++id_at;
-        if (++lt >= next.t1) {
-          more = next.next(p);
-          lt = next.t0;
-          id_at = 4;
-        }
+        if (++lt >= l_t1) next_load();
       }
       cp_commit();
     };
-    // 16 codes to two chunks of an operand row
-    auto widen = [&](uint32_t to, int row, uint32_t from) {
-      const uint4 v = lds128(from);
-      const uint4 a = make_uint4(e4m3_lo(v.x), e4m3_hi(v.x), e4m3_lo(v.y), e4m3_hi(v.y));
-      const uint4 b = make_uint4(e4m3_lo(v.z), e4m3_hi(v.z), e4m3_lo(v.w), e4m3_hi(v.w));
-      const uint32_t half = to + (c >> 2) * S::kHalf;
-      const int j = 2 * (c & 3), first = c >> 2;  // the halves' lanes write in other orders:
-      sts128(half + operand_at(row, j + first), first ? b : a);  // no bank twice
-      sts128(half + operand_at(row, j + 1 - first), first ? a : b);
+    // A tile's codes, 16 a chunk, to two chunks of fp16 in an operand row each; the
+    // reads of four passes go out together.
+    auto widen = [&](uint32_t to, uint32_t from) {
+#pragma unroll
+      for (int i0 = 0; i0 < NP; i0 += 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lds128(from + 2048 * (i0 + i));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 a = make_uint4(e4m3_lo(v[i].x), e4m3_hi(v[i].x), e4m3_lo(v[i].y), e4m3_hi(v[i].y));
+          const uint4 b = make_uint4(e4m3_lo(v[i].z), e4m3_hi(v[i].z), e4m3_lo(v[i].w), e4m3_hi(v[i].w));
+          const int row = (i0 + i) * RPP + rr;
+          const uint32_t half = to + (c >> 2) * S::kHalf;
+          sts128(half + operand_at(row, 2 * (c & 3)), a);
+          sts128(half + operand_at(row, 2 * (c & 3) + 1), b);
+        }
+      }
     };
     load_k();
     load_v();
-    while (ok && walk.next(p)) {
-      const int n_rows = walk.s.n * p.group;
-      const int cur_r0 = walk.rt * kRows;
+    while (ok && next_item()) {
       uint32_t* mine = marks + (item & 3) * (S::kMarks / 4);
-      const int low = seen(p, walk.s, cur_r0);  // tokens that the first row sees
-      for (int t = walk.t0; t < walk.t1 && ok; ++t, ++n) {
+      const int low = min(it.past + by_group(p, it.r0) + 1, p.capacity);  // what the first row sees
+      for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
         const int u = n & 1;
         if (n >= 2 && !(ok = wait(&k_empty[u], ((n >> 1) & 1) ^ 1u))) break;
         if (wt < 8)  // the block's K scale, log2 and inverse of its V scale; no page: -inf
@@ -428,16 +528,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
               sc_v > 0.f ? make_float4(sc_k, lg2(sc_v), 1.0f / sc_v, 0.f)
                          : make_float4(0.f, -INFINITY, 0.f, 0.f);
         cp_wait<1>();  // K's copies
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          widen(sm + S::kOffK + u * S::kOperand, i * RPP + rr, raw_k + 2048 * i);
+        widen(sm + S::kOffK + u * S::kOperand, raw_k);
         to_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[u]);
         load_k();
         if (n >= 2 && !(ok = wait(&v_empty[u], ((n >> 1) & 1) ^ 1u))) break;
         cp_wait<1>();  // V's
-        if ((t + 1) * kPromptTile > low && low < walk.limit) {
+        if ((t + 1) * kPromptTile > low && low < it.limit) {
           // Rows of the item end at different tokens here, and a NaN that one row
           // sees must not reach a row that does not (0 * NaN): NaN codes leave V,
           // and the outputs that they belong to are marked.
@@ -454,50 +552,61 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
               const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) |
                                      (nan >> 21 & 8u)) << (16 * (c & 1) + 4 * k);
 #pragma unroll 1
-              for (int r = cur_r0; r < min(n_rows, cur_r0 + kRows); ++r)
-                if (tok < seen(p, walk.s, r))
-                  atomicOr(mine + (r - cur_r0) * (D / 32) + (c >> 1), bits);
+              for (int r = it.r0; r < min(it.n_rows, it.r0 + kRows); ++r)
+                if (tok < min(it.past + by_group(p, r) + 1, p.capacity))
+                  atomicOr(mine + (r - it.r0) * (D / 32) + (c >> 1), bits);
             }
           }
           __syncwarp();
         }
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          widen(sm + S::kOffV + u * S::kOperand, i * RPP + rr, raw_v + 2048 * i);
+        widen(sm + S::kOffV + u * S::kOperand, raw_v);
         to_async_proxy();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[u]);
         load_v();
       }
-      ++item;
+      __syncwarp();
+      if (lane == 0)
+        done_item();
+      else
+        ++item;
     }
   } else {
     // ------------------------------------------------------------ softmax
+    more_registers<kSoftRegs>();
     const int stream = warp / kSoftWarps, r = tid % kPromptTile;  // row of the item
     const uint32_t lanes = (uint32_t)(32 * (warp % kSoftWarps)) << 16;  // its lanes of tensor memory
     const uint32_t tmem_s = tmem + lanes + stream * kPromptTile;
     float* mul_s = reinterpret_cast<float*>(base + S::kOffMul);
     float2* sums_s = reinterpret_cast<float2*>(base + S::kOffSums);
-    while (ok && walk.next(p)) {
-      const int n_rows = walk.s.n * p.group;
-      const int row = walk.rt * kRows + r;
-      const bool in = row < n_rows;
+    auto through = [&]() {
+      __syncwarp();
+      if (lane == 0)
+        done_item();
+      else
+        ++item;
+    };
+    bool prepares = stream == 1;  // the queries of the next item
+    while (ok && next_item()) {
+      const int row = it.r0 + r;
+      const bool in = row < it.n_rows;
       const int qi = by_group(p, row);
-      const int lim = in ? seen(p, walk.s, row) : 0;
+      const int lim = in ? min(it.past + qi + 1, p.capacity) : 0;
       float q_mul;
-      if (stream == 0) {
-        // ---- this row's query, scaled to 2^14, as the A operand. The last item's
-        // products are done: both streams are through with it.
-        const uint16_t* src = p.q + (int64_t)(walk.s.first + qi) * p.q_row +
-                              (int64_t)(walk.h * p.group + row - qi * p.group) * p.q_head;
+      if (prepares) {
+        // ---- this row's query, scaled to 2^14, as the A operand
+        const uint16_t* src = p.q + (int64_t)(it.first + qi) * p.q_row +
+                              (int64_t)(it.h * p.group + row - qi * p.group) * p.q_head;
         uint4 raw[D / 8];
         float amax = 0.f;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k)
           raw[k] = in ? __ldg(reinterpret_cast<const uint4*>(src) + k) : make_uint4(0u, 0u, 0u, 0u);
         auto two = [&](uint32_t w) {
-          return p.bf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u))
-                        : __half22float2(*reinterpret_cast<const __half2*>(&w));
+          if constexpr (BF16)
+            return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+          else
+            return __half22float2(*reinterpret_cast<const __half2*>(&w));
         };
 #pragma unroll
         for (int k = 0; k < D / 8; ++k)
@@ -507,9 +616,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
         const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
-        const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-        q_mul = p.scale_log2 * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-        mul_s[r] = q_mul;
+        const float up = copysignf(__uint_as_float((uint32_t)(14 - e + 127) << 23), p.scale_log2);
+        q_mul = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+        mul_s[(item & 1) * kPromptTile + r] = q_mul;
+        // the last item's last S, which the other stream's tile was
+        if (n > 0 && !(ok = wait(&s_full[(n - 1) & 1], ((n - 1) >> 1) & 1))) break;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) {
           uint32_t o[4];
@@ -523,52 +634,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         }
         to_async_proxy();
         __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
+        if (lane == 0) mbar_arrive(&q_full[item & 1]);
       } else {
-        if (!(ok = wait(q_full, item & 1))) break;
-        q_mul = mul_s[r];
+        if (!(ok = wait(&q_full[item & 1], (item >> 1) & 1))) break;
+        q_mul = mul_s[(item & 1) * kPromptTile + r];
       }
       float m = -INFINITY;  // the running maximum that the stream's O and l are scaled by
       float l = 0.f;
       int last = -1;        // the stream's last tile
-      for (int t = walk.t0; t < walk.t1 && ok; ++t, ++n) {
+      for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
         if ((n & 1) != stream) continue;
         if (!(ok = wait(&s_full[stream], (n >> 1) & 1))) break;
         after_sync();
         const float4* sc = scale_s + (n & 3) * 8;
         const int left = lim - t * kPromptTile;  // tokens of the tile that the row sees
         const bool cut = __any_sync(0xffffffffu, left < kPromptTile);
-        // Columns 32 c .. + 31 of S to log2 units with the value scale, masked. Read
-        // twice, for the maximum and for P': 128 registers a thread are what two
-        // streams leave.
+        // S is read twice, for the maximum and for P', 32 columns at a time (the
+        // registers that two streams leave). A loop, not unrolled: eight warps that run
+        // it at eight places miss the instruction cache.
         float x[32];
-        auto scores = [&](int c) {
-          ld32(tmem_s + 32 * c, x);
-          ld_wait();
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float4 f = sc[2 * c + b];
-            const float ks = f.x * q_mul;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) x[16 * b + k] = fmaf(x[16 * b + k], ks, f.y);
-          }
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kPromptTile; c += 32) {
+          ld32(tmem_s + c, x);
           if (cut) {
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (32 * c + k >= left) x[k] = -INFINITY;
+              if (c + k >= left) x[k] = -INFINITY;
           }
-        };
-        float tops[8];  // chains side by side
 #pragma unroll
-        for (int k = 0; k < 8; ++k) tops[k] = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          scores(c);
+          for (int b = 0; b < 2; ++b) {  // the largest of a block, then its score: no factor is negative
+            float t[4];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) tops[k & 7] = fmaxf(tops[k & 7], x[k]);
+            for (int k = 0; k < 4; ++k)
+              t[k] = max3(max3(x[16 * b + k], x[16 * b + k + 4], x[16 * b + k + 8]),
+                          x[16 * b + k + 12], -INFINITY);
+            const float4 f = sc[c / 16 + b];
+            top = fmaxf(top, fmaf(max3(max3(t[0], t[1], t[2]), t[3], -INFINITY), f.x * q_mul, f.y));
+          }
         }
-        const float top = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])),
-                                fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
         // ---- a row's maximum much larger: all rows' O and l move to theirs (the
         // stream's last product is done: S came after it)
         if (__any_sync(0xffffffffu, top > m + kGrowth)) {
@@ -582,7 +686,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
               const uint32_t at = tmem_o + lanes + stream * kPromptTile + 32 * c;
               float o[32];
               ld32(at, o);
-              ld_wait();
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] *= al;
               st32(at, reinterpret_cast<const uint32_t*>(o));
@@ -591,21 +694,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         }
         const float sub = m == -INFINITY ? 0.f : m - kPromptShift;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          scores(c);
+        for (int c = 0; c < kPromptTile; c += 32) {
+          ld32(tmem_s + c, x);
           uint32_t w[16];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
+            const float4 f = sc[c / 16 + b];
+            const float ks = f.x * q_mul, less = f.y - sub;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[16 * b + k] = fmaf(x[16 * b + k], ks, less);
+            if (cut) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k)
+                if (c + 16 * b + k >= left) x[16 * b + k] = -INFINITY;
+            }
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float a = ex2(x[16 * b + 2 * k] - sub), d = ex2(x[16 * b + 2 * k + 1] - sub);
-              sum[k & 3] += a + d;
-              w[8 * b + k] = half2_bits(a, d);
+              const float a = ex2(x[16 * b + 2 * k]),
+                          e = ex2(x[16 * b + 2 * k + 1]);
+              sum[k & 3] += a + e;
+              w[8 * b + k] = half2_bits(a, e);
             }
-            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), sc[2 * c + b].z, l);
+            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), f.z, l);
           }
-          st16(tmem_s + 16 * c, w);  // over columns that have been read
+          st16(tmem_s + c / 2, w);  // over columns that have been read
         }
         st_wait();
         before_sync();
@@ -614,12 +727,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         last = n;
       }
       if (!ok || (last >= 0 && !(ok = wait(&pv_done[stream], (last >> 1) & 1)))) break;
-      // ---- the streams meet: the second one leaves maximum and sum
-      if (stream == 1) {
+      // ---- the streams meet. The one without the item's last tile leaves maximum and
+      // sum and prepares the next item's queries; the other one writes the item out.
+      prepares = ((n - 1) & 1) != stream;
+      if (prepares) {
         sums_s[(item & 1) * kPromptTile + r] = make_float2(m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(b_done);
-        ++item;
+        through();
         continue;
       }
       if (!(ok = wait(b_done, item & 1))) break;
@@ -629,20 +744,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       const float fa = m == -INFINITY ? 0.f : ex2(m - most);
       const float fb = other.x == -INFINITY ? 0.f : ex2(other.x - most);
       l = l * fa + other.y * fb;
-      const bool has_a = last >= 0, has_b = walk.t1 - walk.t0 > 1 || !has_a;
+      const bool has_b = it.t1 - it.t0 > 1;
       uint32_t* mine = marks + (item & 3) * (S::kMarks / 4) + r * (D / 32);  // this thread's alone
       const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-      uint16_t* dst = p.out + (int64_t)(walk.s.first + qi) * p.out_row +
-                      (int64_t)(walk.h * p.group + row - qi * p.group) * p.out_head;
-      float* part = p.parts + (((size_t)blockIdx.x * 2 + walk.slot(share)) * kRows + r) * S::kPitch;
+      uint16_t* dst = p.out + (int64_t)(it.first + qi) * p.out_row +
+                      (int64_t)(it.h * p.group + row - qi * p.group) * p.out_head;
+      float* part = p.parts + (((size_t)blockIdx.x * 2 + it.slot) * kRows + r) * S::kPitch;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float o[32], o2[32];
-        if (has_a) ld32(tmem_o + lanes + 32 * c, o);
-        if (has_b) ld32(tmem_o + lanes + kPromptTile + 32 * c, o2);
-        ld_wait();
+        ld32(tmem_o + lanes + stream * kPromptTile + 32 * c, o);
+        if (has_b) ld32(tmem_o + lanes + (stream ^ 1) * kPromptTile + 32 * c, o2);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = (has_a ? o[k] * fa : 0.f) + (has_b ? o2[k] * fb : 0.f);
+        for (int k = 0; k < 32; ++k) o[k] = o[k] * fa + (has_b ? o2[k] * fb : 0.f);
         const uint32_t mark = mine[c];
         if (mark) {
 #pragma unroll
@@ -651,14 +765,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           mine[c] = 0u;
         }
         if (!in) continue;
-        if (walk.whole) {
+        if (it.whole) {
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float a = o[k + 2 * j] * inv, d = o[k + 2 * j + 1] * inv;
-              if (p.bf16) {
+              if constexpr (BF16) {
                 const __nv_bfloat162 h = __floats2bfloat162_rn(a, d);
                 w[j] = *reinterpret_cast<const uint32_t*>(&h);
               } else {
@@ -674,16 +788,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
                 make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
-      if (!walk.whole) {
-        if (in) *reinterpret_cast<float2*>(part + D) = make_float2(most, l);
-        if (tid == 0) walk.describe(p, share);
-      }
+      if (!it.whole && in) *reinterpret_cast<float2*>(part + D) = make_float2(most, l);
       before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
-      ++item;
+      through();
     }
   }
+  if (!ok && p.err) atomicCAS(p.err, 0, kErrPromptWait);
   __syncthreads();
   if (warp == kMmaWarp) {
     after_sync();
@@ -697,8 +809,9 @@ int launch_prompt(AttnP p, const DeviceInfo& di, cudaStream_t stream) {
   using S = PromptShape<D>;
   p.join = reinterpret_cast<Join*>(p.parts + (size_t)(kMaxCtas / 2) * 2 * kPromptTile * S::kPitch);
   const int ctas = std::min(kMaxCtas / 2, di.sm_count);
-  cudaError_t e = launch_overlapped(kv8_prompt_kernel<D>, dim3((unsigned)ctas), kPromptThreads,
-                                    S::kSmem, stream, p);
+  cudaError_t e =
+      launch_overlapped(p.bf16 ? kv8_prompt_kernel<D, true> : kv8_prompt_kernel<D, false>,
+                        dim3((unsigned)ctas), kPromptThreads, S::kSmem, stream, p);
   if (e != cudaSuccess) return cuda_fail(e, "w4_kv8_attention prompt launch");
   e = launch_overlapped(kv8_join_kernel<D, kPromptTile>, dim3((unsigned)ctas, kPromptTile / kJoinWarps),
                         kJoinThreads, 0, stream, p);
@@ -710,8 +823,11 @@ int init_prompt(const DeviceInfo& di) {
   constexpr int smem = PromptShape<D>::kSmem;
   if (smem > di.max_smem_optin)
     return fail(W4_ERR_UNSUPPORTED, "w4_kv8_attention needs %d B of shared memory", smem);
-  const cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(kv8_prompt_kernel<D, true>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kv8_prompt_kernel<D, false>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   return e == cudaSuccess ? W4_OK : cuda_fail(e, "cudaFuncSetAttribute(kv8 prompt)");
 }
 
