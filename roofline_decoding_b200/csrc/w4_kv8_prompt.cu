@@ -38,16 +38,19 @@ namespace {
 constexpr int kSoftWarps = 4, kWidenWarps = 4;  // softmax warps of a stream
 constexpr int kWidenWarp = 2 * kSoftWarps;
 constexpr int kMmaWarp = kWidenWarp + kWidenWarps;
-constexpr int kItemWarp = kMmaWarp + 1;
-constexpr int kPromptThreads = 32 * (kMmaWarp + 4);  // four warpgroups; two warps idle
+constexpr int kItemWarp = kMmaWarp + 1, kCopyWarp = kMmaWarp + 2;
+constexpr int kPromptThreads = 32 * (kMmaWarp + 4);  // four warpgroups; one warp idles
 // Registers a thread: 128 at launch, then by warpgroup (their sum is four times
 // that, which is what the block has).
-constexpr int kSoftRegs = 152, kWidenRegs = 128, kMmaRegs = 80;
+constexpr int kSoftRegs = 192, kWidenRegs = 72, kMmaRegs = 56;
 static_assert(2 * kSoftRegs + kWidenRegs + kMmaRegs <= 4 * 128, "registers of the block");
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
 constexpr float kPromptShift = 11.0f;  // P' of the maximum that O is scaled by is 2^kPromptShift
 constexpr float kGrowth = 3.0f;        // the running maximum may exceed it by this much
 constexpr int kErrPromptWait = 9;
+// Factors of S are at least this, so that a masked -inf stays -inf under a scale of
+// zero; below it a score is none of the argument's 24 bits.
+constexpr float kLeast = 1e-37f;
 
 // Items in units of tokens: a row tile is as long as its own last row sees, near
 // enough (a step of 128 rows is ceil(128 / G) tokens), so that the triangle of a
@@ -108,6 +111,8 @@ struct Item {
   int pad;
 };
 constexpr int kItems = 4;  // ring
+constexpr int kRaws = 3;   // buffers of codes, K and V tiles in turn
+constexpr int kScales = 8;  // tiles whose scales are kept
 
 template <int D>
 struct PromptShape {
@@ -118,16 +123,18 @@ struct PromptShape {
   static constexpr int kOffK = kOffQ + kOperand;          // two buffers
   static constexpr int kOffV = kOffK + 2 * kOperand;      // two buffers
   static constexpr int kRaw = kPromptTile * D;            // a K or V tile's codes
-  static constexpr int kOffRaw = kOffV + 2 * kOperand;    // K, then V
-  static constexpr int kOffScale = kOffRaw + 2 * kRaw;  // four tiles of 8 x (K, log2 V, 1 / V, 0)
+  static constexpr int kOffRaw = kOffV + 2 * kOperand;    // kRaws buffers
+  // tiles of 8 x (K scale, log2 and inverse of the V scale, 0), their blocks with a page
+  static constexpr int kOffScale = kOffRaw + kRaws * kRaw;
+  static constexpr int kOffPages = kOffScale + kScales * 8 * 16;
   // two items in turn: a factor a row, maxima and sums of the stream that meets the other
-  static constexpr int kOffMul = kOffScale + 4 * 8 * 16;
+  static constexpr int kOffMul = kOffPages + kScales * 4;
   static constexpr int kOffSums = kOffMul + 2 * kPromptTile * 4;
   static constexpr int kOffMarks = kOffSums + 2 * kPromptTile * 8;
   static constexpr int kMarks = kPromptTile * D / 8;      // of an item; four items
   static constexpr int kOffItems = kOffMarks + 4 * kMarks;
   static constexpr int kOffBar = kOffItems + kItems * (int)sizeof(Item);
-  static constexpr int kBars = 8 * 2 + 2 + 2 * kItems;
+  static constexpr int kBars = 8 * 2 + 2 + 2 * kItems + 2 * kRaws;
   static constexpr int kOffTmem = kOffBar + kBars * 8;
   static constexpr int kSmem = 1024 + kOffTmem + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -198,6 +205,26 @@ __device__ __forceinline__ void ld32(uint32_t addr, float (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
+// The same with 64.
+__device__ __forceinline__ void ld64(uint32_t addr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+#define W4_OUT8(i)                                                                          \
+  "=r"(u[i]), "=r"(u[i + 1]), "=r"(u[i + 2]), "=r"(u[i + 3]), "=r"(u[i + 4]), "=r"(u[i + 5]), \
+      "=r"(u[i + 6]), "=r"(u[i + 7])
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63"
+      "}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : W4_OUT8(0), W4_OUT8(8), W4_OUT8(16), W4_OUT8(24), W4_OUT8(32), W4_OUT8(40), W4_OUT8(48),
+        W4_OUT8(56)
+      : "r"(addr)
+      : "memory");
+#undef W4_OUT8
+}
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t* u) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
@@ -236,6 +263,16 @@ __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
                : "memory");
+}
+
+// A run of bytes into shared memory; they count at the barrier as they land.
+__device__ __forceinline__ void bulk_load(uint32_t to, const void* from, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(to),
+      "l"(from), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
 
 // mbar_wait with the clock for its limit, about a second: little code, for a
@@ -281,7 +318,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   uint64_t* b_done = bars + 16;   // the stream without the item's last tile is through with it
   uint64_t* o_empty = bars + 17;  // an item's outputs are read (the other one)
   uint64_t* item_full = bars + 18;             // an item is in the ring
-  uint64_t* item_empty = item_full + kItems;   // MMA, widen and softmax warps are through with it
+  uint64_t* item_empty = item_full + kItems;   // MMA, copy, widen and softmax warps are through with it
+  uint64_t* raw_full = item_empty + kItems;    // a tile's codes have landed (bytes), its scales are there
+  uint64_t* raw_empty = raw_full + kRaws;      // widened
   Item* items = reinterpret_cast<Item*>(base + S::kOffItems);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + S::kOffTmem);
   // Marks of four items in turn: the widen warps may be two tiles ahead, that is
@@ -307,7 +346,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
     mbar_init(o_empty, kSoftWarps);
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 1 + kWidenWarps + 2 * kSoftWarps);
+      mbar_init(&item_empty[i], 2 + kWidenWarps + 2 * kSoftWarps);
+    }
+    for (int i = 0; i < kRaws; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], kWidenWarps);
     }
     fence_mbar_init();
   }
@@ -338,7 +381,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
     it = items[item % kItems];
     return it.t0 < it.t1;
   };
-  auto done_item = [&]() { mbar_arrive(&item_empty[item++ % kItems]); };  // once a warp
+  auto done_item = [&]() {  // by a whole warp
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[item % kItems]);
+    ++item;
+  };
 
   if (warp >= kMmaWarp) {
     // ------------------------------------------------------------ MMA
@@ -366,6 +413,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         }
         __syncwarp();
         if (!more) break;
+      }
+    } else if (warp == kCopyWarp) {
+      // Lane 8 j + b has block b (16 tokens) of tile t + j: its page and scales are
+      // read for four tiles at once, its codes are one run of 16 D bytes in K and V.
+      const int j = lane >> 3, b = lane & 7;
+      constexpr uint32_t kRun = 16 * D;
+      float4* scales = reinterpret_cast<float4*>(base + S::kOffScale);
+      uint32_t* pages = reinterpret_cast<uint32_t*>(base + S::kOffPages);
+      uint32_t stage = 0, turn = 0;
+      while (ok && next_item()) {
+        for (int t = it.t0; t < it.t1 && ok; t += 4) {
+          const int tok = (t + j) * kPromptTile + 16 * b;
+          int id = -1;
+          if (t + j < it.t1 && tok < it.limit) {
+            const int pi = tok >> p.page_shift;
+            if (pi < p.max_pages) id = p.page_table[it.b * p.table_stride + pi];
+            if ((uint32_t)id >= (uint32_t)p.pages) {
+              id = -1;
+              atomicCAS(p.err, 0, kErrKvRange);
+            }
+          }
+          const int64_t blk = (int64_t)max(id, 0) * p.kv_heads + it.h;
+          const int64_t at = ((blk << p.page_shift) + (tok & (p.page - 1))) * D;
+          float sc_k = 0.f, sc_v = 0.f;
+          if (id >= 0) {
+            sc_k = p.k_scale[blk];
+            sc_v = p.v_scale[blk];
+          }
+          const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
+          for (int jj = 0; jj < min(4, it.t1 - t) && ok; ++jj, ++n) {
+            const uint32_t blocks = there >> (8 * jj) & 0xffu;
+#pragma unroll 1
+            for (int kv = 0; kv < 2; ++kv) {
+              if (!(ok = wait(&raw_empty[stage], turn ^ 1u))) break;
+              if (kv == 0) {
+                // K scale, log2 and inverse of the V scale; no page: -inf
+                if (j == jj)
+                  scales[(n % kScales) * 8 + b] = sc_v > 0.f
+                                                      ? make_float4(sc_k, lg2(sc_v), 1.0f / sc_v, 0.f)
+                                                      : make_float4(0.f, -INFINITY, 0.f, 0.f);
+                if (lane == 0) pages[n % kScales] = blocks;
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive_expect_tx(&raw_full[stage], __popc(blocks) * kRun);
+              __syncwarp();
+              if (j == jj && id >= 0)
+                bulk_load(sm + S::kOffRaw + stage * S::kRaw + b * kRun, (kv ? p.v : p.k) + at, kRun,
+                          &raw_full[stage]);
+              if (++stage == kRaws) stage = 0, turn ^= 1u;
+            }
+          }
+        }
+        done_item();
       }
     } else if (warp == kMmaWarp && lane == 0) {
       constexpr uint32_t idesc_s = prompt_idesc(kPromptTile, 0), idesc_o = prompt_idesc(D, 1);
@@ -409,142 +509,87 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           if (n > n0) ok = output(n - 1, n - 1 - n0 < 2);
         }
         if (ok) ok = output(n - 1, n - 1 - n0 < 2);
-        done_item();
+        mbar_arrive(&item_empty[item++ % kItems]);
       }
     }
   } else if (warp >= kWidenWarp) {
     // ------------------------------------------------------------ widen
     fewer_registers<kWidenRegs>();
     constexpr int CPR = D / 16, RPP = 128 / CPR, NP = kPromptTile / RPP;  // chunks a row, rows a pass
-    const int wt = tid - kWidenWarp * 32;
-    // A quarter warp takes one chunk of eight rows: its 16-byte stores fall on all
-    // banks. A pass is RPP rows.
-    const int c = (lane >> 3) + (CPR == 8 ? 4 * ((wt >> 5) & 1) : 0);
-    const int rr = (lane & 7) + 8 * (CPR == 8 ? wt >> 6 : wt >> 5);
-    const uint32_t raw_k = sm + S::kOffRaw + 16 * wt, raw_v = raw_k + S::kRaw;  // + 2048 a pass
-    float sc_k = 0.f, sc_v = 0.f;  // scales of block wt of the loaded tile, threads 0 .. 7
-    int ids = -1;         // lane 8 j + b: block b of tile t + j, j < 4
-    // the item of the tile that is loaded: it may be the one after `it`
-    int l_item = 0, l_t1 = 0, l_limit = 0, l_b = 0, l_h = 0, lt = 0, id_at = 4;
-    bool more = true;
-    auto next_load = [&]() {
-      const int at = l_item % kItems;
-      more = (ok = wait(&item_full[at], (l_item / kItems) & 1)) && items[at].t0 < items[at].t1;
-      if (!more) return;
-      lt = items[at].t0, l_t1 = items[at].t1, l_limit = items[at].limit;
-      l_b = items[at].b, l_h = items[at].h;
-      ++l_item;
-      id_at = 4;
-    };
-    next_load();
-    int64_t block_at = 0;  // lane b: where block b & 7 of the tile begins
-    bool full = false;     // every block has a page, every token is below the limit
-    int limit_in = 0;      // tokens of the tile below the limit
-    uint32_t pages_in = 0; // bit b: block b has a page
-    // pass i of this warp lies in block (i * RPP) / 16 + own_block, at own_at
-    const int own_block = rr >> 4, own_at = (rr & 15) * D + 16 * c;
-    auto copy = [&](const uint8_t* from, uint32_t to) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int b = i * RPP / 16 + own_block;
-        const uint8_t* src = from + __shfl_sync(0xffffffffu, block_at, b) + own_at;
-        if (full)
-          cp16(to + 2048 * i, src);
-        else  // zeros for tokens behind the limit and of no page
-          cp16_if(to + 2048 * i, src, (pages_in >> b & 1u) && i * RPP + rr < limit_in);
-      }
-    };
-    // The next tile's K codes and its scales on their way, then (load_v) its V codes.
-    auto load_k = [&]() {
-      if (more) {
-        if (id_at == 4) {
-          const int tok = (lt + (lane >> 3)) * kPromptTile + 16 * (lane & 7);
-          ids = -1;
-          if (lt + (lane >> 3) < l_t1 && tok < l_limit) {
-            const int pi = tok >> p.page_shift;
-            if (pi < p.max_pages) ids = p.page_table[l_b * p.table_stride + pi];
-            if ((uint32_t)ids >= (uint32_t)p.pages) {
-              ids = -1;
-              atomicCAS(p.err, 0, kErrKvRange);
-            }
-          }
-          id_at = 0;
-        }
-        const int id_b = __shfl_sync(0xffffffffu, ids, 8 * id_at + (lane & 7));
-        const int64_t blk = (int64_t)max(id_b, 0) * p.kv_heads + l_h;
-        if (wt < 8) {
-          sc_k = sc_v = 0.f;  // no page
-          if (id_b >= 0) {
-            sc_k = p.k_scale[blk];
-            sc_v = p.v_scale[blk];
-          }
-        }
-        const int tok0 = lt * kPromptTile;
-        block_at = ((blk << p.page_shift) + ((tok0 + 16 * (lane & 7)) & (p.page - 1))) * D;
-        limit_in = l_limit - tok0;
-        pages_in = __ballot_sync(0xffffffffu, id_b >= 0);
-        full = limit_in >= kPromptTile && (pages_in & 0xffu) == 0xffu;
-        copy(p.k, raw_k);
-      }
-      cp_commit();
-    };
-    auto load_v = [&]() {
-      if (more) {
-        copy(p.v, raw_v);
-        ++id_at;
-        if (++lt >= l_t1) next_load();
-      }
-      cp_commit();
-    };
+    // A quarter warp takes one chunk of each of eight rows, by an exclusive or that
+    // gives its 16-byte reads of the plain codes and its stores of both halves of
+    // the chunk into the swizzled rows all banks alike. A pass is RPP rows.
+    const int w = warp - kWidenWarp, j = lane & 7, q = lane >> 3;
+    const int c = CPR == 8 ? j ^ (q + 4 * (w & 1)) : ((j & 2) | (((j >> 2) ^ (j >> 1)) & 1)) ^ q;
+    const int rr = j + 8 * (CPR == 8 ? w >> 1 : w);
+    const uint32_t raw0 = sm + S::kOffRaw + rr * D + 16 * c;  // + 2048 a pass
+    // where the halves go: rows a pass apart have the same swizzle
+    const uint32_t to_a = (c >> 2) * S::kHalf + operand_at(rr, 2 * (c & 3)), to_b = to_a ^ 16u;
+    uint32_t stage = 0, turn = 0;
     // A tile's codes, 16 a chunk, to two chunks of fp16 in an operand row each; the
-    // reads of four passes go out together.
-    auto widen = [&](uint32_t to, uint32_t from) {
+    // reads of four passes go out together. Zeros for tokens of no page and behind
+    // the limit (bit i of keep: pass i).
+    auto widen = [&](uint32_t to, uint32_t from, uint32_t keep) {
 #pragma unroll
       for (int i0 = 0; i0 < NP; i0 += 4) {
         uint4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = lds128(from + 2048 * (i0 + i));
+        for (int i = 0; i < 4; ++i) {
+          v[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (keep >> (i0 + i) & 1u) v[i] = lds128(from + 2048 * (i0 + i));
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint4 a = make_uint4(e4m3_lo(v[i].x), e4m3_hi(v[i].x), e4m3_lo(v[i].y), e4m3_hi(v[i].y));
-          const uint4 b = make_uint4(e4m3_lo(v[i].z), e4m3_hi(v[i].z), e4m3_lo(v[i].w), e4m3_hi(v[i].w));
-          const int row = (i0 + i) * RPP + rr;
-          const uint32_t half = to + (c >> 2) * S::kHalf;
-          sts128(half + operand_at(row, 2 * (c & 3)), a);
-          sts128(half + operand_at(row, 2 * (c & 3) + 1), b);
+          const uint32_t row = to + (i0 + i) * RPP * 128;
+          sts128(row + to_a, make_uint4(e4m3_lo(v[i].x), e4m3_hi(v[i].x), e4m3_lo(v[i].y),
+                                        e4m3_hi(v[i].y)));
+          sts128(row + to_b, make_uint4(e4m3_lo(v[i].z), e4m3_hi(v[i].z), e4m3_lo(v[i].w),
+                                        e4m3_hi(v[i].w)));
         }
       }
     };
-    load_k();
-    load_v();
+    auto widened = [&](uint64_t* full) {
+      to_async_proxy();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(full);
+        mbar_arrive(&raw_empty[stage]);
+      }
+      if (++stage == kRaws) stage = 0, turn ^= 1u;
+    };
     while (ok && next_item()) {
       uint32_t* mine = marks + (item & 3) * (S::kMarks / 4);
       const int low = min(it.past + by_group(p, it.r0) + 1, p.capacity);  // what the first row sees
       for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
         const int u = n & 1;
+        if (!(ok = wait(&raw_full[stage], turn))) break;
+        const uint32_t blocks = *reinterpret_cast<const volatile uint32_t*>(base + S::kOffPages +
+                                                                            4 * (n % kScales));
+        const int limit_in = it.limit - t * kPromptTile;
+        uint32_t keep = (1u << NP) - 1u;
+        if (blocks != 0xffu || limit_in < kPromptTile) {
+          keep = 0u;
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+            if ((blocks >> ((i * RPP + rr) >> 4) & 1u) && i * RPP + rr < limit_in) keep |= 1u << i;
+        }
         if (n >= 2 && !(ok = wait(&k_empty[u], ((n >> 1) & 1) ^ 1u))) break;
-        if (wt < 8)  // the block's K scale, log2 and inverse of its V scale; no page: -inf
-          reinterpret_cast<float4*>(base + S::kOffScale)[(n & 3) * 8 + wt] =
-              sc_v > 0.f ? make_float4(sc_k, lg2(sc_v), 1.0f / sc_v, 0.f)
-                         : make_float4(0.f, -INFINITY, 0.f, 0.f);
-        cp_wait<1>();  // K's copies
-        widen(sm + S::kOffK + u * S::kOperand, raw_k);
-        to_async_proxy();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[u]);
-        load_k();
-        if (n >= 2 && !(ok = wait(&v_empty[u], ((n >> 1) & 1) ^ 1u))) break;
-        cp_wait<1>();  // V's
+        widen(sm + S::kOffK + u * S::kOperand, raw0 + stage * S::kRaw, keep);
+        widened(&k_full[u]);
+        if (!(ok = wait(&raw_full[stage], turn)) ||
+            (n >= 2 && !(ok = wait(&v_empty[u], ((n >> 1) & 1) ^ 1u))))
+          break;
         if ((t + 1) * kPromptTile > low && low < it.limit) {
           // Rows of the item end at different tokens here, and a NaN that one row
           // sees must not reach a row that does not (0 * NaN): NaN codes leave V,
           // and the outputs that they belong to are marked.
 #pragma unroll 1
           for (int i = 0; i < NP; ++i) {
+            if (!(keep >> i & 1u)) continue;
             const int tok = t * kPromptTile + i * RPP + rr;
 #pragma unroll 1
             for (int k = 0; k < 4; ++k) {
-              const uint32_t at = raw_v + 2048 * i + 4 * k;
+              const uint32_t at = raw0 + stage * S::kRaw + 2048 * i + 4 * k;
               const uint32_t v = lds32(at);
               const uint32_t nan = __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
               if (nan == 0u) continue;
@@ -557,19 +602,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
                   atomicOr(mine + (r - it.r0) * (D / 32) + (c >> 1), bits);
             }
           }
-          __syncwarp();
         }
-        widen(sm + S::kOffV + u * S::kOperand, raw_v);
-        to_async_proxy();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[u]);
-        load_v();
+        // (to_async_proxy in widened also stands between these stores and the next copy)
+        widen(sm + S::kOffV + u * S::kOperand, raw0 + stage * S::kRaw, keep);
+        widened(&v_full[u]);
       }
-      __syncwarp();
-      if (lane == 0)
-        done_item();
-      else
-        ++item;
+      done_item();
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -579,13 +617,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
     const uint32_t tmem_s = tmem + lanes + stream * kPromptTile;
     float* mul_s = reinterpret_cast<float*>(base + S::kOffMul);
     float2* sums_s = reinterpret_cast<float2*>(base + S::kOffSums);
-    auto through = [&]() {
-      __syncwarp();
-      if (lane == 0)
-        done_item();
-      else
-        ++item;
-    };
     bool prepares = stream == 1;  // the queries of the next item
     while (ok && next_item()) {
       const int row = it.r0 + r;
@@ -646,32 +677,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         if ((n & 1) != stream) continue;
         if (!(ok = wait(&s_full[stream], (n >> 1) & 1))) break;
         after_sync();
-        const float4* sc = scale_s + (n & 3) * 8;
+        const float4* sc = scale_s + (n % kScales) * 8;
         const int left = lim - t * kPromptTile;  // tokens of the tile that the row sees
         const bool cut = __any_sync(0xffffffffu, left < kPromptTile);
-        // S is read twice, for the maximum and for P', 32 columns at a time (the
-        // registers that two streams leave). A loop, not unrolled: eight warps that run
-        // it at eight places miss the instruction cache.
-        float x[32];
+        // A row of S stays in registers from its maximum to its P'.
+        float x[kPromptTile];
+        ld64(tmem_s, x);
+        ld64(tmem_s + 64, x + 64);
+        if (cut) {
+#pragma unroll
+          for (int k = 0; k < kPromptTile; ++k)
+            if (k >= left) x[k] = -INFINITY;
+        }
         float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < kPromptTile; c += 32) {
-          ld32(tmem_s + c, x);
-          if (cut) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (c + k >= left) x[k] = -INFINITY;
-          }
+        for (int b = 0; b < 8; ++b) {  // the largest of a block, then its score: no factor is negative
+          float t[4];
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {  // the largest of a block, then its score: no factor is negative
-            float t[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              t[k] = max3(max3(x[16 * b + k], x[16 * b + k + 4], x[16 * b + k + 8]),
-                          x[16 * b + k + 12], -INFINITY);
-            const float4 f = sc[c / 16 + b];
-            top = fmaxf(top, fmaf(max3(max3(t[0], t[1], t[2]), t[3], -INFINITY), f.x * q_mul, f.y));
-          }
+          for (int k = 0; k < 4; ++k)
+            t[k] = max3(max3(x[16 * b + k], x[16 * b + k + 4], x[16 * b + k + 8]),
+                        x[16 * b + k + 12], -INFINITY);
+          const float4 f = sc[b];
+          top = fmaxf(top, fmaf(max3(max3(t[0], t[1], t[2]), t[3], -INFINITY),
+                                fmaxf(f.x * q_mul, kLeast), f.y));
         }
         // ---- a row's maximum much larger: all rows' O and l move to theirs (the
         // stream's last product is done: S came after it)
@@ -693,32 +721,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           }
         }
         const float sub = m == -INFINITY ? 0.f : m - kPromptShift;
-#pragma unroll 1
-        for (int c = 0; c < kPromptTile; c += 32) {
-          ld32(tmem_s + c, x);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
           uint32_t w[16];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const float4 f = sc[c / 16 + b];
-            const float ks = f.x * q_mul, less = f.y - sub;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) x[16 * b + k] = fmaf(x[16 * b + k], ks, less);
-            if (cut) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (c + 16 * b + k >= left) x[16 * b + k] = -INFINITY;
-            }
+            const float4 f = sc[2 * c + b];
+            const float ks = fmaxf(f.x * q_mul, kLeast), less = f.y - sub;
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float a = ex2(x[16 * b + 2 * k]),
-                          e = ex2(x[16 * b + 2 * k + 1]);
+              const float a = ex2(fmaf(x[32 * c + 16 * b + 2 * k], ks, less)),
+                          e = ex2(fmaf(x[32 * c + 16 * b + 2 * k + 1], ks, less));
               sum[k & 3] += a + e;
               w[8 * b + k] = half2_bits(a, e);
             }
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), f.z, l);
           }
-          st16(tmem_s + c / 2, w);  // over columns that have been read
+          st16(tmem_s + 16 * c, w);
         }
         st_wait();
         before_sync();
@@ -734,7 +754,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         sums_s[(item & 1) * kPromptTile + r] = make_float2(m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(b_done);
-        through();
+        done_item();
         continue;
       }
       if (!(ok = wait(b_done, item & 1))) break;
@@ -792,7 +812,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
-      through();
+      done_item();
     }
   }
   if (!ok && p.err) atomicCAS(p.err, 0, kErrPromptWait);
