@@ -47,7 +47,10 @@ constexpr int kTile = 32;        // tokens of one ring stage of a warp
 constexpr int kCtasPerSm = 2;
 constexpr float kShift = 14.0f;  // P' is at most 2^kShift
 
-// From this many query rows of a cache head a sequence on, the other kernel.
+// From this many query rows of a cache head a sequence on, the other kernel. This one
+// and the other one, 32 heads on 8 of 128: at 64 rows 82.1 and 81.7 us for 64 sequences
+// of 1000 tokens, 30.1 and 28.6 us for 8 of 2000; at 32 rows 63.5 and 83.3, 25.0 and
+// 28.2 us; at 128 rows 43.4 and 31.7 us for the 8.
 constexpr int kPromptRows = 64;
 
 // Every row tile of a sequence counts as long as its last (the few tiles above a
@@ -59,6 +62,7 @@ struct Rows8 {
   static constexpr int kUnit = 1;
   static constexpr int kOver = 12;           // so that a CTA of many short items does not end last
   static constexpr int kMinShare = kWarps;   // below a tile a warp, more CTAs only add partials
+  static constexpr int kCut = 0;             // equal shares always
   static __device__ __forceinline__ int tiles(const AttnP& p, const Seq& s, int) {
     return (min(s.past + s.n, p.capacity) + kTile - 1) / kTile;
   }

@@ -157,17 +157,58 @@ __device__ __forceinline__ int64_t scan32(int64_t v, int lane) {
   return v;
 }
 
+// Item blockIdx.x as this CTA's share.
+template <typename G>
+__device__ __forceinline__ Share item_share(const AttnP& p, int64_t per) {
+  const int lane = threadIdx.x & 31;
+  Share f;
+  f.x = f.end = f.off = 0;
+  f.per = per;
+  f.b = 0;
+  int left = (int)blockIdx.x;  // items before it, of the sequences from here
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.seqs; b0 += 32) {
+    Seq s;
+    s.n = 0;
+    if (b0 + lane < p.seqs) s = load_seq(p, b0 + lane);
+    const int mine = s.n > 0 ? p.kv_heads * G::row_tiles(p, s) : 0;
+    const int upto = (int)scan32(mine, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, upto > left);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      f.b = b0 + src;
+      left -= __shfl_sync(0xffffffffu, upto - mine, src);
+      s = load_seq(p, f.b);
+      const int nrt = G::row_tiles(p, s);
+      f.off = left / nrt * G::upto(p, s, nrt) + G::upto(p, s, left % nrt);
+      f.end = G::length(p, s, left % nrt);
+      return f;
+    }
+    left -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return f;
+}
+
 template <typename G>
 __device__ __forceinline__ Share find_share(const AttnP& p) {
   const int lane = threadIdx.x & 31;
   Share f;
   int64_t all = 0, w = 0;
+  int items = 0;          // of all sequences, and the longest (G::kCut > 0)
+  int64_t longest = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < p.seqs; b0 += 32) {
     w = 0;
     if (b0 + lane < p.seqs) {
       const Seq s = load_seq(p, b0 + lane);
       w = G::seq_work(p, s);
+      if constexpr (G::kCut > 0) {
+        if (s.n > 0) {
+          const int nrt = G::row_tiles(p, s);
+          items = (int)min(items + (int64_t)p.kv_heads * nrt, (int64_t)1 << 24);
+          longest = max(longest, G::length(p, s, nrt - 1));
+        }
+      }
       const int told = p.lengths[b0 + lane];
       if (s.n > 0 && (told < 0 || told > p.capacity - s.n)) atomicCAS(p.err, 0, kErrKvRange);
     }
@@ -175,6 +216,14 @@ __device__ __forceinline__ Share find_share(const AttnP& p) {
     all += __shfl_sync(0xffffffffu, w, 31);
   }
   f.per = max((int64_t)G::kMinShare, divide(all + gridDim.x - 1, gridDim.x));
+  if constexpr (G::kCut > 0) {
+    // No more items than CTAs and the longest little longer than a share: an item
+    // a CTA, none cut. Only the share's length counts then.
+    items = __reduce_add_sync(0xffffffffu, items);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    if (items <= (int)gridDim.x && longest <= f.per + G::kCut) return item_share<G>(p, f.per);
+  }
   f.x = min(all, f.per * blockIdx.x);
   f.end = min(all, f.x + f.per);
   f.b = 0;

@@ -7,9 +7,9 @@
 // pair do. An item is 128 query rows of one cache head (G query heads times the
 // new tokens), worked through in tiles of 128 tokens by one CTA an SM, the tiles
 // in turn by two streams that meet at the item's end:
-//   4 widen warps  : the tile's pages by cp.async into shared memory, a tile ahead
-//                    (a thread copies, waits for and reads its own chunks: no
-//                    barrier); e4m3 to fp16 (exact) and back as MMA operands, K and V alike token by token in the 128B-swizzled
+//   copy warp      : the pages' runs of 16 tokens by bulk copies into three buffers
+//                    of a K or a V tile, and the scales;
+//   4 widen warps  : e4m3 to fp16 (exact), K and V alike token by token in the 128B-swizzled
 //                    layout (K is the K-major operand of Q K^T; of P V the same
 //                    rows are the MN-major operand V, so nothing is transposed);
 //   item warp      : walks the CTA's share and leaves the items in a ring, so that
@@ -22,11 +22,14 @@
 //                    the other kernel), P' in fp16 back into tensor memory over
 //                    the S that it came from. O stays in tensor memory, one a
 //                    stream with a maximum of its own, and is rescaled only when
-//                    a row's running maximum has grown by more than 2^3 since the
+//                    a row's running maximum has grown by more than 2^6 since the
 //                    last time (P' may then reach 2^14, inside fp16's range).
-// Two O, two S (with P over them) fill the tensor memory: 4 x 128 columns. The
-// exponentials are the floor of this split: 128 x 128 of them a tile at 16 a clock
-// are 1024 clocks, as long as the tile's two products together at their best rate.
+// Two O, two S (with P over them) fill the tensor memory: 4 x 128 columns. A tile's
+// products at their best rate and its 128 x 128 exponentials at 16 a clock are 1024
+// clocks each, its traffic on shared memory 1750. A tile takes 2700: a stream's
+// S, softmax (2400), P V and next S follow one another, and two streams are all that
+// the tensor memory holds. 2 x 256 rows of 32 heads on 8 over 4096 tokens: 68 us, 501
+// TFLOP/s of the causal products; 8192 rows from nothing 912 us, 603 TFLOP/s.
 #include "w4_kv8_attn.cuh"
 
 #include <algorithm>
@@ -45,8 +48,11 @@ constexpr int kPromptThreads = 32 * (kMmaWarp + 4);  // four warpgroups; one war
 constexpr int kSoftRegs = 192, kWidenRegs = 72, kMmaRegs = 56;
 static_assert(2 * kSoftRegs + kWidenRegs + kMmaRegs <= 4 * 128, "registers of the block");
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
-constexpr float kPromptShift = 11.0f;  // P' of the maximum that O is scaled by is 2^kPromptShift
-constexpr float kGrowth = 3.0f;        // the running maximum may exceed it by this much
+// P' of the maximum that O is scaled by is 2^kPromptShift, and the running maximum may
+// exceed it by kGrowth: P' stays below fp16's 2^16. What is more than 2^22 below the
+// maximum falls under fp16's normal range, off by 2^-25 at most: 2^-33 of the maximum's.
+constexpr float kPromptShift = 8.0f;
+constexpr float kGrowth = 6.0f;
 constexpr int kErrPromptWait = 9;
 // Factors of S are at least this, so that a masked -inf stays -inf under a scale of
 // zero; below it a score is none of the argument's 24 bits.
@@ -70,9 +76,18 @@ struct Rows128 {
   static __device__ __forceinline__ int step(const AttnP& p) {
     return (kRows + p.group - 1) / p.group;
   }
-  // Length of row tile rt: above kOver + kUnit * tiles for every limit.
+  // Items are not cut if the longest CTA ends at most this much later than with equal
+  // shares: a cut costs two first tiles, the parts and their join. 2 x 256 rows of 32
+  // heads on 8, cut and not: past 1000 45.2 and 31.3 us, 4096 81.7 and 68.0, 12000 (13
+  // tiles later) 165.7 and 165.6; 512 rows of 16 heads past 3000 (17) 44.3 and 54.7.
+  static constexpr int kCut = 12 * kPromptTile;
+  // Length of the first row tile, then of row tile rt: above kOver + kUnit * tiles
+  // for every limit.
   static __device__ __forceinline__ int64_t first(const AttnP& p, const Seq& s) {
     return (int64_t)kOver + s.past + step(p) + kUnit;
+  }
+  static __device__ __forceinline__ int64_t length(const AttnP& p, const Seq& s, int64_t rt) {
+    return first(p, s) + step(p) * rt;
   }
   // Length of row tiles 0 .. rt - 1 together.
   static __device__ __forceinline__ int64_t upto(const AttnP& p, const Seq& s, int64_t rt) {
@@ -95,7 +110,7 @@ struct Rows128 {
     while (r + 1 < nrt && upto(p, s, r + 1) <= off) ++r;
     *rt = (int)r;
     *at = off - upto(p, s, r);
-    *len = first(p, s) + step(p) * r;
+    *len = length(p, s, r);
   }
 };
 
@@ -134,7 +149,7 @@ struct PromptShape {
   static constexpr int kMarks = kPromptTile * D / 8;      // of an item; four items
   static constexpr int kOffItems = kOffMarks + 4 * kMarks;
   static constexpr int kOffBar = kOffItems + kItems * (int)sizeof(Item);
-  static constexpr int kBars = 8 * 2 + 2 + 2 * kItems + 2 * kRaws;
+  static constexpr int kBars = 9 * 2 + 2 + 2 * kItems + 2 * kRaws;
   static constexpr int kOffTmem = kOffBar + kBars * 8;
   static constexpr int kSmem = 1024 + kOffTmem + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -250,6 +265,10 @@ __device__ __forceinline__ void st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// The bytes of four e4m3 codes that are NaN: all ones.
+__device__ __forceinline__ uint32_t has_nan(uint32_t v) {
+  return __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
+}
 // Byte offset of 16-byte chunk c (8 fp16) of row r in an operand half.
 __device__ __forceinline__ uint32_t operand_at(int r, int c) {
   return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
@@ -309,7 +328,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   uint64_t* v_full = bars + 4;
   uint64_t* v_empty = bars + 6;
   uint64_t* s_full = bars + 8;    // S is in tensor memory (commit)
-  uint64_t* p_full = bars + 10;   // P' is in its place, O is rescaled (softmax warps)
+  uint64_t* p_full = bars + 10;   // all of P' is in its place (softmax warps)
   uint64_t* pv_done = bars + 12;  // P V is done (commit)
   // Two, by item: a stream that writes an item out may be at its queries when the
   // other one prepares those of the item after. (Never two after: that takes a
@@ -321,6 +340,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   uint64_t* item_empty = item_full + kItems;   // MMA, copy, widen and softmax warps are through with it
   uint64_t* raw_full = item_empty + kItems;    // a tile's codes have landed (bytes), its scales are there
   uint64_t* raw_empty = raw_full + kRaws;      // widened
+  uint64_t* p_half = raw_empty + kRaws;        // O is rescaled, P' of 64 tokens is in its place
   Item* items = reinterpret_cast<Item*>(base + S::kOffItems);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + S::kOffTmem);
   // Marks of four items in turn: the widen warps may be two tiles ahead, that is
@@ -339,6 +359,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], kSoftWarps);
+      mbar_init(&p_half[i], kSoftWarps);
       mbar_init(&pv_done[i], 1);
       mbar_init(&q_full[i], kSoftWarps);
     }
@@ -473,15 +494,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       // O += P V of tile m, the first of its item and stream or not
       auto output = [&](int m, bool first) {
         const int u = m & 1;
-        if (!wait(&p_full[u], (m >> 1) & 1) || !wait(&v_full[u], (m >> 1) & 1) ||
+        if (!wait(&p_half[u], (m >> 1) & 1) || !wait(&v_full[u], (m >> 1) & 1) ||
             (first && item > 0 && !wait(o_empty, (item - 1) & 1)))
           return false;
         after_sync();
         const uint64_t v_desc = operand_desc(sm + S::kOffV + u * S::kOperand, S::kHalf, 1024);
 #pragma unroll
-        for (int k = 0; k < kPromptTile / 16; ++k)  // 16 tokens: 8 columns of P, 16 rows of V
+        for (int k = 0; k < kPromptTile / 16; ++k) {  // 16 tokens: 8 columns of P, 16 rows of V
+          if (k == kPromptTile / 32) {
+            if (!wait(&p_full[u], (m >> 1) & 1)) return false;
+            after_sync();
+          }
           mma_f16_ts(tmem_o + u * kPromptTile, tmem + u * kPromptTile + 8 * k,
                      v_desc + ((k * 16 * 128) >> 4), idesc_o, first && k == 0 ? 0u : 1u);
+        }
         __threadfence_block();  // the widen warps' marks, for those who wait for pv_done
         commit_to(&v_empty[u]);
         commit_to(&pv_done[u]);
@@ -583,15 +609,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           // Rows of the item end at different tokens here, and a NaN that one row
           // sees must not reach a row that does not (0 * NaN): NaN codes leave V,
           // and the outputs that they belong to are marked.
-#pragma unroll 1
+#pragma unroll 4
           for (int i = 0; i < NP; ++i) {
             if (!(keep >> i & 1u)) continue;
+            const uint4 codes = lds128(raw0 + stage * S::kRaw + 2048 * i);
+            if ((has_nan(codes.x) | has_nan(codes.y) | has_nan(codes.z) | has_nan(codes.w)) == 0u)
+              continue;
             const int tok = t * kPromptTile + i * RPP + rr;
 #pragma unroll 1
             for (int k = 0; k < 4; ++k) {
               const uint32_t at = raw0 + stage * S::kRaw + 2048 * i + 4 * k;
               const uint32_t v = lds32(at);
-              const uint32_t nan = __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              const uint32_t nan = has_nan(v);
               if (nan == 0u) continue;
               asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v & ~nan) : "memory");
               const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) |
@@ -739,11 +768,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), f.z, l);
           }
           st16(tmem_s + 16 * c, w);
+          if (c & 1) {
+            st_wait();
+            before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c == 1 ? &p_half[stream] : &p_full[stream]);
+          }
         }
-        st_wait();
-        before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[stream]);
         last = n;
       }
       if (!ok || (last >= 0 && !(ok = wait(&pv_done[stream], (last >> 1) & 1)))) break;
