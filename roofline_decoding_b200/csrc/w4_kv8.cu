@@ -102,6 +102,21 @@ __device__ __forceinline__ uint2 to_e4m3x8(const F8& r, float mul) {
   return make_uint2(w[0], w[1]);
 }
 
+// Eight codes times mul, rounded again.
+__device__ __forceinline__ uint2 again_e4m3x8(uint2 v, float mul) {
+  const uint32_t w[2] = {v.x, v.y};
+  F8 f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(
+        (__nv_fp8x2_storage_t)((w[j >> 1] >> (16 * (j & 1))) & 0xffffu), __NV_E4M3);
+    const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&hr));
+    f.f[2 * j] = f2.x;
+    f.f[2 * j + 1] = f2.y;
+  }
+  return to_e4m3x8(f, mul);
+}
+
 // ------------------------------------------------------------ one head
 
 // What a lane multiplies its two chunks a (dims 8l..) and b (D/2 + 8l..) of a
@@ -208,20 +223,25 @@ __device__ __forceinline__ void rope_groups(const HeadsIn& x, uint16_t* out, int
   constexpr int L = D / 16, HPW = 32 / L;
   const int l = lane % L;
   const bool turned = p.cos_t != nullptr;
-  Turn r;
-  if (turned) load_turn<D>(p.cos_t, p.sin_t, p.table_type, pos, l, r);
-  if (weight) weigh<D, BF16>(weight, l, turned, r);
   const uint16_t* src = x.p + row * x.row + 8 * l;
   uint16_t* dst = out + row * out_row + 8 * l;
-#pragma unroll 1
-  for (int g = g0; g < g1; ++g) {
-    const int h = g * HPW + lane / L;
-    uint4 va = make_uint4(0u, 0u, 0u, 0u), vb = va;
+  auto load = [&](int h, uint4& va, uint4& vb) {
+    va = vb = make_uint4(0u, 0u, 0u, 0u);
     if (h < heads) {
       va = *reinterpret_cast<const uint4*>(src + h * x.head);
       vb = *reinterpret_cast<const uint4*>(src + h * x.head + D / 2);
     }
+  };
+  uint4 va, vb;  // the next group's, on their way while a group is worked on
+  load(g0 * HPW + lane / L, va, vb);
+  Turn r;
+  if (turned) load_turn<D>(p.cos_t, p.sin_t, p.table_type, pos, l, r);
+  if (weight) weigh<D, BF16>(weight, l, turned, r);
+#pragma unroll 1
+  for (int g = g0; g < g1; ++g) {
+    const int h = g * HPW + lane / L;
     F8 a = unpack8<BF16>(va), b = unpack8<BF16>(vb);
+    if (g + 1 < g1) load(h + HPW, va, vb);
     norm_turn<D>(a, b, weight != nullptr, p.eps, turned, r);
     if (h < heads) {
       *reinterpret_cast<uint4*>(dst + h * out_head) = pack8<BF16>(a);
@@ -246,7 +266,7 @@ __device__ __forceinline__ void rope_row(const RopeParams& p, int64_t row, int64
 constexpr int kRopeThreads = 128;
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, 7) norm_rope_kernel(const RopeParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -273,7 +293,7 @@ struct AppendParams {
   float *k_scale, *v_scale;    // [pages, kv_heads]
   const int32_t *page_table, *lengths, *row_starts;
   int64_t table_stride;
-  int pages, page, max_pages, seqs, rows, kv_heads;
+  int pages, page, page_shift, max_pages, seqs, rows, kv_heads;
   int kv_units;   // K and V blocks of the (sequence, page) pairs that it may touch
   int kv_blocks;  // CTAs of the cache part; those after them turn queries
 };
@@ -287,8 +307,8 @@ __device__ __forceinline__ int seq_rows(const AppendParams& p, int b, int* first
 }
 
 // Pages that n rows behind `past` tokens touch.
-__device__ __forceinline__ int touched(int past, int n, int page) {
-  return n > 0 ? (past % page + n - 1) / page + 1 : 0;
+__device__ __forceinline__ int touched(int past, int n, int page_shift) {
+  return n > 0 ? (((past & ((1 << page_shift) - 1)) + n - 1) >> page_shift) + 1 : 0;
 }
 
 constexpr int kAppendThreads = 256;
@@ -304,18 +324,25 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   const int h = (unit >> 1) % p.kv_heads;
   int g = (unit >> 1) / p.kv_heads;  // which (sequence, page) pair
 
-  // every warp finds the pair by a scan over the sequences, 32 at a time
+  // Every warp finds the pair by a scan over the sequences, four neighbours a lane
+  // if there are many: their loads go out together.
+  const int each = p.seqs > 32 ? 4 : 1;
   int b = -1, past = 0, n = 0, first = 0;
 #pragma unroll 1
-  for (int b0 = 0; b0 < p.seqs; b0 += 32) {
-    const int bb = b0 + lane;
-    int f = 0, m = 0, ps = 0;
-    if (bb < p.seqs) {
-      m = seq_rows(p, bb, &f);
-      ps = max(p.lengths[bb], 0);
+  for (int b0 = 0; b0 < p.seqs; b0 += 32 * each) {
+    int f[4], m[4], ps[4], cnt[4], mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int bb = b0 + each * lane + i;
+      f[i] = m[i] = ps[i] = 0;
+      if (i < each && bb < p.seqs) {
+        m[i] = seq_rows(p, bb, &f[i]);
+        ps[i] = max(p.lengths[bb], 0);
+      }
     }
-    const int cnt = touched(ps, m, p.page);
-    int incl = cnt;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine += cnt[i] = touched(ps[i], m[i], p.page_shift);
+    int incl = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, incl, off);
@@ -324,17 +351,24 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
     const unsigned hit = __ballot_sync(0xffffffffu, incl > g);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      b = b0 + src;
-      g -= __shfl_sync(0xffffffffu, incl - cnt, src);
-      past = __shfl_sync(0xffffffffu, ps, src);
-      n = __shfl_sync(0xffffffffu, m, src);
-      first = __shfl_sync(0xffffffffu, f, src);
+      int left = g - (incl - mine), at = 0;  // (lane src's are used)
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (at == i && i + 1 < each && left >= cnt[i]) left -= cnt[i], at = i + 1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at == i) past = ps[i], n = m[i], first = f[i];
+      b = b0 + each * src + __shfl_sync(0xffffffffu, at, src);
+      g = __shfl_sync(0xffffffffu, left, src);
+      past = __shfl_sync(0xffffffffu, past, src);
+      n = __shfl_sync(0xffffffffu, n, src);
+      first = __shfl_sync(0xffffffffu, first, src);
       break;
     }
     g -= __shfl_sync(0xffffffffu, incl, 31);
   }
   if (b < 0) return;  // fewer pairs than the bound
-  const int64_t slot_page = past / p.page + g;                  // page of the sequence
+  const int64_t slot_page = (past >> p.page_shift) + g;                  // page of the sequence
   const int64_t tok0 = max((int64_t)past, slot_page * p.page);  // its first new token
   const int cnt = (int)(min((int64_t)past + n, (slot_page + 1) * p.page) - tok0);
   const int slot0 = (int)(tok0 - slot_page * p.page);
@@ -423,21 +457,21 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   if (scale != old) {
     if (tid == 0) *scale_at = scale;
     const float ratio = old * inv;  // the rows in use, rounded again in the larger scale
+    uint4* at = reinterpret_cast<uint4*>(codes);
+    const int chunks = slot0 * (D / 16);
 #pragma unroll 1
-    for (int i = tid; i < slot0 * (D / 8); i += kThreads) {
-      uint2* at = reinterpret_cast<uint2*>(codes) + i;
-      const uint2 v = *at;
-      const uint32_t w[2] = {v.x, v.y};
-      F8 f;
+    for (int i0 = tid; i0 < chunks; i0 += 4 * kThreads) {  // four reads on their way
+      uint4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2(
-            (__nv_fp8x2_storage_t)((w[j >> 1] >> (16 * (j & 1))) & 0xffffu), __NV_E4M3);
-        const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&hr));
-        f.f[2 * j] = f2.x;
-        f.f[2 * j + 1] = f2.y;
-      }
-      *at = to_e4m3x8(f, ratio);
+      for (int k = 0; k < 4; ++k)
+        if (i0 + k * kThreads < chunks) v[k] = at[i0 + k * kThreads];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i0 + k * kThreads < chunks) {
+          const uint2 lo = again_e4m3x8(make_uint2(v[k].x, v[k].y), ratio);
+          const uint2 hi = again_e4m3x8(make_uint2(v[k].z, v[k].w), ratio);
+          at[i0 + k * kThreads] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
     }
   }
 }
@@ -472,7 +506,7 @@ __global__ void __launch_bounds__(kAppendThreads, W == 1 ? 3 : NP == 4 ? 2 : 3)
                                                     64 * (lane % kLanes)));
   }
   int b = 0;  // the sequence: as many as end at or before this row
-#pragma unroll 1
+#pragma unroll 4
   for (int b0 = 0; b0 < p.seqs; b0 += 32) {
     const int bb = b0 + lane;
     b += __popc(__ballot_sync(0xffffffffu, bb < p.seqs && p.row_starts[bb + 1] <= row));
@@ -498,10 +532,11 @@ HeadsIn heads_in(const w4_heads& x) {
 }
 
 // Head groups a warp takes: whole rows (the position's table row is then read
-// once) when there are rows enough for about 32 warps an SM, else one group a
-// warp, so that a few rows still spread over the SMs.
+// once) when there are rows enough, else one group a warp, so that a few rows
+// still spread over the SMs. Rows of 32 and 8 heads, a group a warp and whole rows:
+// 64 rows 2.3 and 5.6 us, 512 5.3 and 5.7, 1024 7.6 and 6.4, 4096 28 and 16.
 int groups_per_warp(int64_t rows, int groups, int sms) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(groups, rows * groups / (32 * sms)));
+  return rows > 5 * (int64_t)sms ? std::max(groups, 1) : 1;
 }
 
 RopeParams rope_params(const w4_rope& r, const DeviceInfo& di) {
@@ -572,6 +607,7 @@ int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_hea
   p.table_stride = bt.table_stride;
   p.pages = c.pages;
   p.page = c.page_size;
+  p.page_shift = c.page_size == 16 ? 4 : c.page_size == 32 ? 5 : c.page_size == 64 ? 6 : 7;
   p.kv_heads = c.kv_heads;
   p.max_pages = bt.max_pages;
   p.seqs = bt.seqs;
@@ -580,9 +616,14 @@ int launch_kv8_append(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_hea
   const int64_t pairs =
       std::min<int64_t>(bt.rows, (int64_t)bt.rows / c.page_size + 2 * (int64_t)bt.seqs);
   const int64_t kv_units = pairs * c.kv_heads * 2;
-  // A warp a block of the cache while sequences bring a few rows each: most
-  // threads of a CTA would idle on one row. A CTA a block for prompts.
-  const bool by_warp = bt.rows <= 4 * (int64_t)bt.seqs;
+  // A warp a block of the cache while sequences bring a few rows each (most threads of
+  // a CTA would idle), and for more rows where there are blocks for many waves of
+  // CTAs; else a CTA a block. By warps and by CTAs, 8 heads of 128: 64 sequences of 1
+  // row 3.6 and 11.6 us, of 16 11.2 and 17.3, of 32 19.0 and 20.0, of 64 39 and 25; 32
+  // of 16 (1152 units) 11.1 and 9.4; 8 of 4 3.2 and 5.1, of 8 5.6 and 5.7, of 32 15.9
+  // and 5.7.
+  const bool by_warp = bt.rows <= 4 * (int64_t)bt.seqs ||
+                       (bt.rows <= 32 * (int64_t)bt.seqs && kv_units >= 10 * (int64_t)di.sm_count);
   const int64_t kv_blocks =
       by_warp ? (kv_units + kAppendThreads / 32 - 1) / (kAppendThreads / 32) : kv_units;
   const int groups = c.head_dim == 128 ? head_groups<128>(q.heads) : head_groups<64>(q.heads);

@@ -140,7 +140,7 @@ __device__ __forceinline__ int tile_at(int64_t v) {
 }
 
 // `per` units of the line a CTA, the last ones less or none. Every warp works it
-// out by itself, 32 sequences at a time.
+// out by itself, up to 128 sequences at a time.
 struct Share {
   int64_t x, end;  // this CTA's units
   int64_t per;     // units of a share
@@ -193,28 +193,45 @@ template <typename G>
 __device__ __forceinline__ Share find_share(const AttnP& p) {
   const int lane = threadIdx.x & 31;
   Share f;
-  int64_t all = 0, w = 0;
+  // Neighbouring sequences a lane, whose loads go out together: 512 sequences of 300
+  // tokens at most 85 us, 100 with one a lane.
+  const int each = p.seqs > 32 ? 4 : 1;
+  int64_t all = 0, w[4];
   int items = 0;          // of all sequences, and the longest (G::kCut > 0)
   int64_t longest = 0;
-#pragma unroll 1
-  for (int b0 = 0; b0 < p.seqs; b0 += 32) {
-    w = 0;
-    if (b0 + lane < p.seqs) {
-      const Seq s = load_seq(p, b0 + lane);
-      w = G::seq_work(p, s);
-      if constexpr (G::kCut > 0) {
-        if (s.n > 0) {
-          const int nrt = G::row_tiles(p, s);
-          items = (int)min(items + (int64_t)p.kv_heads * nrt, (int64_t)1 << 24);
-          longest = max(longest, G::length(p, s, nrt - 1));
-        }
+  bool bad = false;       // a length that the page table has no room for
+  auto load = [&](int b0) {
+    Seq s[4];
+    int told[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int b = b0 + each * lane + i;
+      s[i].first = s[i].n = s[i].past = told[i] = 0;
+      if (i < each && b < p.seqs) {
+        s[i] = load_seq(p, b);
+        told[i] = p.lengths[b];
       }
-      const int told = p.lengths[b0 + lane];
-      if (s.n > 0 && (told < 0 || told > p.capacity - s.n)) atomicCAS(p.err, 0, kErrKvRange);
     }
-    w = scan32(w, lane);
-    all += __shfl_sync(0xffffffffu, w, 31);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = i < each ? G::seq_work(p, s[i]) : 0;
+      if (s[i].n == 0) continue;
+      bad |= told[i] < 0 || told[i] > p.capacity - s[i].n;
+      if constexpr (G::kCut > 0) {
+        const int nrt = G::row_tiles(p, s[i]);
+        items = (int)min(items + (int64_t)p.kv_heads * nrt, (int64_t)1 << 24);
+        longest = max(longest, G::length(p, s[i], nrt - 1));
+      }
+    }
+  };
+#pragma unroll 1
+  for (int b0 = 0; b0 < p.seqs; b0 += 32 * each) {
+    load(b0);
+    all += (w[0] + w[1]) + (w[2] + w[3]);
   }
+  if (bad) atomicCAS(p.err, 0, kErrKvRange);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
   f.per = max((int64_t)G::kMinShare, divide(all + gridDim.x - 1, gridDim.x));
   if constexpr (G::kCut > 0) {
     // No more items than CTAs and the longest little longer than a share: an item
@@ -231,18 +248,22 @@ __device__ __forceinline__ Share find_share(const AttnP& p) {
   if (f.x >= f.end) return f;
   int64_t before = 0;
 #pragma unroll 1
-  for (int b0 = 0;; b0 += 32) {
-    if (p.seqs > 32)  // else the first pass has left them
-      w = scan32(b0 + lane < p.seqs ? G::seq_work(p, load_seq(p, b0 + lane)) : 0, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, before + w > f.x);
-    if (hit || b0 + 32 >= p.seqs) {
+  for (int b0 = 0;; b0 += 32 * each) {
+    if (p.seqs > 32 * each) load(b0);  // else the first pass has left them
+    const int64_t mine = (w[0] + w[1]) + (w[2] + w[3]), upto = scan32(mine, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > f.x);
+    if (hit || b0 + 32 * each >= p.seqs) {
       const int src = hit ? __ffs(hit) - 1 : 31;
-      const int64_t prev = __shfl_sync(0xffffffffu, w, max(src - 1, 0));
-      f.b = min(b0 + src, p.seqs - 1);
-      f.off = f.x - before - (src ? prev : 0);
+      int64_t left = f.x - before - (upto - mine);  // lane src's are used
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (at == i && i + 1 < each && left >= w[i]) left -= w[i], at = i + 1;
+      f.b = min(b0 + each * src + __shfl_sync(0xffffffffu, at, src), p.seqs - 1);
+      f.off = __shfl_sync(0xffffffffu, left, src);
       return f;
     }
-    before += __shfl_sync(0xffffffffu, w, 31);
+    before += __shfl_sync(0xffffffffu, upto, 31);
   }
 }
 
