@@ -144,7 +144,11 @@ void check_rows(const char* name, const Tensor& t, const Tensor& like, int64_t n
 Tensor output(const char* name, const Tensor* given, const Tensor& x) {
   if (!given) return empty(x.sizes(), x);
   check_rows(name, *given, x, x.size(1), x.size(2));
-  if (!readable(*given) || (given->size(0) > 1 && given->stride(0) < given->size(2)))
+  const int64_t rows = given->size(0), n = given->size(1), dim = given->size(2);
+  const int64_t row = given->stride(0), head = given->stride(1);
+  // rows apart by more than their heads span, or heads by more than their rows do
+  if (!readable(*given) || (rows > 1 && n > 0 && row < (n - 1) * head + dim &&
+                            (row < dim || head < (rows - 1) * row + dim)))
     refuse(name, " needs 16-byte aligned heads that do not overlap, got strides ",
            given->strides());
   return *given;

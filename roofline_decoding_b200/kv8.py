@@ -90,8 +90,8 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: to
     rows. A block that held rows already keeps its scale where that is larger;
     where it is smaller its rows are rounded again in the new one (exact, but for
     values that become subnormal in e4m3). Infinities are stored as +-448 s and
-    NaN as NaN; neither sets a scale. A page must not belong to two of the
-    sequences that the call writes.
+    NaN as NaN; neither sets a scale. A page that the call writes must stand in the
+    table once only.
     """
     return _lib.torch_module().kv8_append(*cache, k, v, page_table, lengths, row_starts, cos, sin, q,
                                           q_norm, k_norm, eps, out)

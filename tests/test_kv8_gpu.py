@@ -789,3 +789,31 @@ def test_attention_prompts_agree_with_single_rows():
         one = rd.kv8_attention(q[i:i + 1], cache, table, i32([past + i]), i32([0, 1]))
         check_attention(many[i:i + 1], q[i:i + 1], cache, table, i32([past + i]), i32([0, 1]))
         check_attention(one, q[i:i + 1], cache, table, i32([past + i]), i32([0, 1]))
+
+
+@pytest.mark.parametrize("D,page,most", [(128, 64, 30), (64, 16, 17), (128, 16, 3)])
+def test_append_hundreds_of_sequences(D, page, most):
+    """Sequences beyond one scan step (128), without rows, with a few and with many."""
+    past = [(37 * i) % 150 for i in range(301)]
+    rows = [(11 * i) % (most + 1) if i % 5 else 0 for i in range(301)]
+    run_append(D + most, past, rows, kv=2, heads=2, D=D, page=page, lead=1, pad=2)
+
+
+@pytest.mark.parametrize("seqs", [33, 128, 129, 300])
+@pytest.mark.parametrize("rows", [1, 24])
+def test_attention_hundreds_of_sequences(seqs, rows):
+    """Shares found four sequences a lane, in one step and in several."""
+    past = [(131 * i) % 500 for i in range(seqs)]
+    new = [rows - i % 2 if i % 6 else 0 for i in range(seqs)]
+    run_attention(seqs + rows, past, new, heads=8, kv=2, D=64, page=16, lead=1, pad=2)
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    q = torch.zeros(3, 4, 128, device=DEV, dtype=torch.bfloat16)
+    for strides in ((128, 128, 1), (256, 128, 1), (128, 256, 1)):
+        out = torch.zeros(2048, device=DEV, dtype=torch.bfloat16).as_strided((3, 4, 128), strides)
+        with pytest.raises(ValueError, match="overlap"):
+            rd.qk_norm_rope(q, q, q_out=out)
+    for strides in ((512, 128, 1), (1024, 136, 1), (128, 384, 1)):
+        out = torch.zeros(4096, device=DEV, dtype=torch.bfloat16).as_strided((3, 4, 128), strides)
+        rd.qk_norm_rope(q, q, q_out=out)
