@@ -461,24 +461,30 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         // Rows of this item end at different tokens here, and a NaN that one row
         // sees must not reach a row that does not (0 * NaN): NaN codes leave the
         // tile, and the outputs that they belong to are marked.
+        bool some = false;  // seldom
+#pragma unroll
+        for (int i = 0; i < kTile * D / 512; ++i)
+          some |= any_nan(lds128(st + kTile * D + 512 * i + 16 * lane));
+        if (__any_sync(0xffffffffu, some)) {
 #pragma unroll 1
-        for (int i = lane; i < kTile * D / 16; i += 32) {
-          const int tok = tok0 + i / (D / 16), c = i % (D / 16);
-          const uint32_t at = st + kTile * D + chunk_at<D>(i / (D / 16), c);
+          for (int i = lane; i < kTile * D / 16; i += 32) {
+            const int tok = tok0 + i / (D / 16), c = i % (D / 16);
+            const uint32_t at = st + kTile * D + chunk_at<D>(i / (D / 16), c);
 #pragma unroll 1
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t v = lds32(at + 4 * w);
-            const uint32_t nan = __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            if (nan == 0u) continue;
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4 * w), "r"(v & ~nan) : "memory");
-            const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) |
-                                   (nan >> 21 & 8u)) << (16 * (c & 1) + 4 * w);
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t v = lds32(at + 4 * w);
+              const uint32_t nan = nan_codes(v);
+              if (nan == 0u) continue;
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4 * w), "r"(v & ~nan) : "memory");
+              const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) |
+                                     (nan >> 21 & 8u)) << (16 * (c & 1) + 4 * w);
 #pragma unroll 1
-            for (int r = r0; r < min(n_rows, r0 + kRows); ++r)
-              if (tok < seen(p, cw.s, r)) atomicOr(marks + (r - r0) * (D / 32) + (c >> 1), bits);
+              for (int r = r0; r < min(n_rows, r0 + kRows); ++r)
+                if (tok < seen(p, cw.s, r)) atomicOr(marks + (r - r0) * (D / 32) + (c >> 1), bits);
+            }
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {

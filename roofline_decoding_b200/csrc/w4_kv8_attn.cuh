@@ -100,6 +100,16 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// The bytes of four e4m3 codes that are NaN (0x7f, 0xff): all ones.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t v) {
+  return (((v & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu;
+}
+__device__ __forceinline__ bool any_nan(const uint4& v) {
+  return ((((v.x & 0x7f7f7f7fu) + 0x01010101u) | ((v.y & 0x7f7f7f7fu) + 0x01010101u) |
+           ((v.z & 0x7f7f7f7fu) + 0x01010101u) | ((v.w & 0x7f7f7f7fu) + 0x01010101u)) &
+          0x80808080u) != 0u;
+}
+
 // A sequence's rows and tokens. A length that the page table cannot hold is cut
 // to what it holds.
 struct Seq {
@@ -332,6 +342,16 @@ struct Walk {
     p.join[blockIdx.x] = jn;
   }
 };
+
+// CTAs that a batch can use: a share has kMinShare units at least, and the host
+// knows bounds of the items and, by the page table, of their lengths.
+template <typename G>
+inline int useful_ctas(const AttnP& p, int ctas) {
+  const int64_t items = (int64_t)p.kv_heads * ((int64_t)p.rows * p.group / G::kRows + p.seqs);
+  const int64_t units = G::kOver + G::kMore +
+                        G::kUnit * (((int64_t)p.capacity + G::kTile - 1) / G::kTile);
+  return (int)std::min<int64_t>(ctas, (items * units + G::kMinShare - 1) / G::kMinShare);
+}
 
 // ------------------------------------------------------------ the join
 

@@ -81,6 +81,7 @@ struct Rows128 {
   // heads on 8, cut and not: past 1000 45.2 and 31.3 us, 4096 81.7 and 68.0, 12000 (13
   // tiles later) 165.7 and 165.6; 512 rows of 16 heads past 3000 (17) 44.3 and 54.7.
   static constexpr int kCut = 12 * kPromptTile;
+  static constexpr int kMore = 3 * kPromptTile;  // what first() and length() have beside past
   // Length of the first row tile, then of row tile rt: above kOver + kUnit * tiles
   // for every limit.
   static __device__ __forceinline__ int64_t first(const AttnP& p, const Seq& s) {
@@ -265,10 +266,6 @@ __device__ __forceinline__ void st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// The bytes of four e4m3 codes that are NaN: all ones.
-__device__ __forceinline__ uint32_t has_nan(uint32_t v) {
-  return __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
-}
 // Byte offset of 16-byte chunk c (8 fp16) of row r in an operand half.
 __device__ __forceinline__ uint32_t operand_at(int r, int c) {
   return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
@@ -612,15 +609,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
 #pragma unroll 4
           for (int i = 0; i < NP; ++i) {
             if (!(keep >> i & 1u)) continue;
-            const uint4 codes = lds128(raw0 + stage * S::kRaw + 2048 * i);
-            if ((has_nan(codes.x) | has_nan(codes.y) | has_nan(codes.z) | has_nan(codes.w)) == 0u)
-              continue;
+            if (!any_nan(lds128(raw0 + stage * S::kRaw + 2048 * i))) continue;
             const int tok = t * kPromptTile + i * RPP + rr;
 #pragma unroll 1
             for (int k = 0; k < 4; ++k) {
               const uint32_t at = raw0 + stage * S::kRaw + 2048 * i + 4 * k;
               const uint32_t v = lds32(at);
-              const uint32_t nan = has_nan(v);
+              const uint32_t nan = nan_codes(v);
               if (nan == 0u) continue;
               asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v & ~nan) : "memory");
               const uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) |
@@ -859,7 +854,9 @@ template <int D>
 int launch_prompt(AttnP p, const DeviceInfo& di, cudaStream_t stream) {
   using S = PromptShape<D>;
   p.join = reinterpret_cast<Join*>(p.parts + (size_t)(kMaxCtas / 2) * 2 * kPromptTile * S::kPitch);
-  const int ctas = std::min(kMaxCtas / 2, di.sm_count);
+  // (16 rows of 16 heads on 4 over 100 tokens: 12.9 us, with all CTAs 15.8; the other
+  // kernel's CTAs are smaller, and fewer of them gain nothing)
+  const int ctas = useful_ctas<Rows128>(p, std::min(kMaxCtas / 2, di.sm_count));
   cudaError_t e =
       launch_overlapped(p.bf16 ? kv8_prompt_kernel<D, true> : kv8_prompt_kernel<D, false>,
                         dim3((unsigned)ctas), kPromptThreads, S::kSmem, stream, p);
