@@ -8,9 +8,11 @@
 // leaves shared memory:
 //   TMA warps    : one brings X tiles [up to 256 rows x 64 k] (128B swizzle,
 //                  the canonical K-major layout the MMA reads), the other the
-//                  packed words of the W tile (128 or 256 columns), each through a ring of its own: words leave as soon as they
-//                  are unpacked, so the dequantisation runs ahead of the MMA
-//                  and no load's latency waits for an MMA's;
+//                  packed words of the W tile (128 or 256 columns), each
+//                  through a ring of its own: words leave as soon as they are
+//                  unpacked, so the dequantisation runs ahead of the MMA and
+//                  no load's latency waits for an MMA's (2048 x 8960 x 1536:
+//                  67 us, 96 with one ring for both);
 //   8 dequant warps: expand each packed word into 8 fp16 (q - 8) * s values
 //                  - bit-identical to dequantize_v1 - and write them K-major,
 //                  128B-swizzled, into one of the B buffers;
@@ -784,17 +786,19 @@ int gemm_plan(int M, int K, int N, int sms, int split_k, bool few_tiles, int dev
   const int tiles = ntx * mtx;
   if (few_tiles && tiles * 2 <= sms) {
     // Half the SMs or more would have no tile: as many K slices as are resident
-    // at once, of three stages at least.
+    // at once, of three stages at least. Whole tiles and slices: 17 x 1536 x 2048
+    // 13.7 and 6.5 us, 64 x 4096 x 4096 27 and 12, 511 x 8960 x 1536 66 and 22,
+    // 128 x 1536 x 8960 (70 tiles, 2 slices) 14.5 and 11.7.
     for (int s = std::min(8, kt / 3); s >= 2; --s)
       if (tiles <= g_clusters[dev & 63][nacc][s]) {
         out[0] = GemmLaunch{128, nacc, 0, 0, nt128, tiles, s, false};
         return 1;
       }
   }
-  // A grid of fewer tiles than SMs is not cut along K: measured on 2048 x
-  // 8960 x 1536 (96 tiles), three K slices over 288 CTAs took 118-128 us
-  // against 96 us for the 96 whole tiles (each slice's stages ran at half the
-  // rate).
+  // A grid of more tiles than that is not cut along K: slices would share SMs.
+  // Measured on 2048 x 8960 x 1536 (96 tiles) when the whole tiles took 96 us
+  // (67 by now): three slices over 288 CTAs 118-128 us, each slice's stages at
+  // half the rate.
   if (tiles >= sms && bn == 256 && nacc == 2) {
     // a last wave of a few tiles: those tiles go to a second launch as
     // 128-column tiles cut into K slices, spread over the SMs the first

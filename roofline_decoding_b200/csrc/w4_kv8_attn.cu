@@ -4,7 +4,7 @@
 //
 // with e4m3 codes k_j, v_j, and sk_j, sv_j the scales of their page and head.
 // The query rows of one cache head (G query heads times the sequence's new
-// tokens) form tiles of 8, 16 or 32 rows; an item is (sequence, cache head, row
+// tokens) form tiles of 8 or 16 rows; an item is (sequence, cache head, row
 // tile), and its work is its 32-token tiles of the cache.
 //
 // Bound by the cache's bytes at the small row counts of decoding (2 D bytes a
@@ -24,8 +24,8 @@
 // is the 16-wide operand (S^T = K Q^T, O^T = V^T P^T) and the query rows the
 // 8-wide one, so that a decoding step's few rows leave little of a product
 // unused, every widened K or V register serves all row blocks, and softmax and
-// output take half the registers of the 16-row form (470 instead of 900
-// instructions a tile). P^T turns from result to operand by movmatrix. e4m3
+// output take half the registers of the 16-row form (some 600 instead of 900
+// instructions a tile, all counted). P^T turns from result to operand by movmatrix. e4m3
 // widens to fp16 exactly. Queries enter scaled by a power of two a row that
 // brings their largest element to 2^14 (bf16 to fp16 is then exact but for
 // elements 2^-28 below the row's largest). The page's value scale is folded
@@ -33,6 +33,10 @@
 // of s + log2 sv, so P' is at most 2^14, its rounding to fp16 (11 bits) stays
 // relative down to 2^-28 of the largest weight, and the fp32 sum adds
 // P' / sv, unrounded.
+//
+// 32 sequences of up to 32768 tokens, 32 heads on 8 of 128: 174 us, 6.3 TB/s. A
+// single token over 700, 12 heads on 2: 8.5 us, the latency of two launches and of
+// length, page number, tile, products and merge.
 #include "w4_kv8_attn.cuh"
 
 #include <algorithm>
@@ -47,10 +51,11 @@ constexpr int kTile = 32;        // tokens of one ring stage of a warp
 constexpr int kCtasPerSm = 2;
 constexpr float kShift = 14.0f;  // P' is at most 2^kShift
 
-// From this many query rows of a cache head a sequence on, the other kernel. This one
-// and the other one, 32 heads on 8 of 128: at 64 rows 82.1 and 81.7 us for 64 sequences
-// of 1000 tokens, 30.1 and 28.6 us for 8 of 2000; at 32 rows 63.5 and 83.3, 25.0 and
-// 28.2 us; at 128 rows 43.4 and 31.7 us for the 8.
+// From this many query rows of a cache head a sequence (on average) on, the other
+// kernel. This one and the other one, 32 heads on 8 of 128: 64 sequences over 1000 tokens
+// with 34 rows 68.9 and 82.9 us, with 66 117 and 89; 8 over 2000 with 34 rows 25.7 and
+// 29.5, 50 31.2 and 30.5, 66 38.8 and 32.4; one over 2000 with 64 15.9 and 18.3, with 256
+// 26.6 and 24.0.
 constexpr int kPromptRows = 64;
 
 // Every row tile of a sequence counts as long as its last (the few tiles above a
@@ -61,6 +66,7 @@ struct Rows8 {
   static constexpr int kTile = w4::kTile;
   static constexpr int kUnit = 1;
   static constexpr int kOver = 12;           // so that a CTA of many short items does not end last
+                                             // (64 sequences of 1500 at most: 29 us, with 4 39)
   static constexpr int kMinShare = kWarps;   // below a tile a warp, more CTAs only add partials
   static constexpr int kCut = 0;             // equal shares always
   static __device__ __forceinline__ int tiles(const AttnP& p, const Seq& s, int) {
@@ -83,12 +89,12 @@ struct Rows8 {
   }
 };
 
-// NT: 8-row blocks of an item (1, 2 or 4).
+// NT: 8-row blocks of an item (1 or 2).
 template <int D, int NT>
 struct AttnShape {
   static constexpr int kRows = 8 * NT;               // query rows of an item
   static constexpr int kStageBytes = 2 * kTile * D;  // K, then V
-  static constexpr int kStages = D == 128 ? (NT == 4 ? 2 : 3) : (NT == 4 ? 4 : 5);
+  static constexpr int kStages = D == 128 ? 3 : 5;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kScales = kWarps * kStages * 16;  // per stage: K, V scale of two halves
   static constexpr int kPitch = D + 4;                   // floats; the 4 hold maximum and sum
@@ -97,11 +103,7 @@ struct AttnShape {
   static constexpr int kKSteps = D / 16;        // 16-dim steps of K Q^T
   static constexpr int kMTiles = D / 16;        // 16-dim tiles of V^T P^T
   static constexpr int kWords = D / 32;         // 32-bit words of a lane's V chunk
-  // four row blocks' queries do not fit the registers: their fragments and
-  // factors stay in shared memory
-  static constexpr bool kSharedQ = NT == 4;
-  static constexpr int kQ = kSharedQ ? kKSteps * NT * 32 * 8 + kRows * 4 : 0;
-  static constexpr int kSmem = kRing + kScales + kMerge + kMarks + kQ;
+  static constexpr int kSmem = kRing + kScales + kMerge + kMarks;
   static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
@@ -179,8 +181,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   float* scales = reinterpret_cast<float*>(smem_kv8 + S::kRing) + warp * S::kStages * 4;
   float* merge = reinterpret_cast<float*>(smem_kv8 + S::kRing + S::kScales);
   uint32_t* marks = reinterpret_cast<uint32_t*>(merge + S::kMerge / 4);
-  uint2* shared_q = reinterpret_cast<uint2*>(marks + S::kMarks / 4);        // kSharedQ only
-  float* shared_mul = reinterpret_cast<float*>(shared_q + S::kKSteps * NT * 32);
 
   grid_dependency_wait();
   grid_launch_dependents();
@@ -307,27 +307,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     // 8 n + 2 t + 1 of the results
     const int n_rows = cw.s.n * p.group;
     const int r0 = cw.rt * kRows;
-    uint32_t qf[S::kSharedQ ? 1 : NT][S::kKSteps][2];
+    uint32_t qf[NT][S::kKSteps][2];
     float q_mul[NT][2];
-    if constexpr (S::kSharedQ) {
-      const float mul = load_queries<D>(p, cw.s, cw.h, r0 + 8 * warp + g, n_rows, t, qf[0]);
 #pragma unroll
-      for (int k = 0; k < S::kKSteps; ++k)
-        shared_q[(k * NT + warp) * 32 + lane] = make_uint2(qf[0][k][0], qf[0][k][1]);
-      if (t == 0) shared_mul[8 * warp + g] = mul;
-      __syncthreads();
+    for (int n = 0; n < NT; ++n) {
+      const float mul = load_queries<D>(p, cw.s, cw.h, r0 + 8 * n + g, n_rows, t, qf[n]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) q_mul[n][r] = shared_mul[8 * n + 2 * t + r];
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float mul = load_queries<D>(p, cw.s, cw.h, r0 + 8 * n + g, n_rows, t, qf[n]);
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          q_mul[n][r] = __shfl_sync(0xffffffffu, mul, 4 * (2 * t + r));
-      }
+      for (int r = 0; r < 2; ++r)
+        q_mul[n][r] = __shfl_sync(0xffffffffu, mul, 4 * (2 * t + r));
     }
     int lim[NT][2];  // tokens that the row sees
     int low = 0x7fffffff;
@@ -374,23 +361,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int k = 4 * c + w;
-          uint32_t b[NT][2];
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if constexpr (S::kSharedQ) {
-              const uint2 v = shared_q[(k * NT + n) * 32 + lane];
-              b[n][0] = v.x, b[n][1] = v.y;
-            } else {
-              b[n][0] = qf[n][k][0], b[n][1] = qf[n][k][1];
-            }
-          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const uint32_t x = reinterpret_cast<const uint32_t*>(&ka[i])[w];
             const uint32_t y = reinterpret_cast<const uint32_t*>(&kb[i])[w];
             const uint32_t a0 = e4m3_lo(x), a1 = e4m3_lo(y), a2 = e4m3_hi(x), a3 = e4m3_hi(y);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_16816<false>(s[i][n], a0, a1, a2, a3, b[n][0], b[n][1]);
+            for (int n = 0; n < NT; ++n)
+              mma_16816<false>(s[i][n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
           }
         }
       }
@@ -648,7 +626,7 @@ int launch(AttnP p, int max_rows, const DeviceInfo& di, cudaStream_t stream) {
 }  // namespace
 
 size_t kv8_attention_workspace_bytes(int head_dim) {
-  return std::max((size_t)kMaxCtas * (2 * 32 * (head_dim + 4) * 4 + sizeof(Join)),  // 32-row items
+  return std::max((size_t)kMaxCtas * (2 * 16 * (head_dim + 4) * 4 + sizeof(Join)),  // 16-row items
                   kv8_prompt_workspace_bytes(head_dim));
 }
 
@@ -669,10 +647,8 @@ static int init_attention(const DeviceInfo& di) {
 int kv8_init_device(const DeviceInfo& di) {
   int st = init_attention<64, 1>(di);
   if (st == W4_OK) st = init_attention<64, 2>(di);
-  if (st == W4_OK) st = init_attention<64, 4>(di);
   if (st == W4_OK) st = init_attention<128, 1>(di);
   if (st == W4_OK) st = init_attention<128, 2>(di);
-  if (st == W4_OK) st = init_attention<128, 4>(di);
   if (st == W4_OK) st = kv8_prompt_init_device(di);
   return st;
 }
@@ -710,20 +686,19 @@ int launch_kv8_attention(const w4_kv8_cache& c, const w4_kv_batch& bt, const w4_
   p.scale_log2 = scale * 1.4426950408889634f;
   p.parts = static_cast<float*>(workspace);
   p.err = di.err_word;
-  // Rows of an item by the rows that a sequence brings on average: wider items
-  // read and widen the cache less often, narrower ones waste less of a step of
-  // few rows.
+  // Rows of an item by the rows that a sequence brings on average. Items of 8 and of 16:
+  // 64 sequences of 1500 tokens, 4 rows 28.9 and 36.3 us, 8 of 2000, 16 rows 15.9 and
+  // 16.2, 32 rows 21.9 and 20.3; 32 of 1000, 32 rows 39.6 and 33.7. (Items of 32 rows read
+  // the cache less often, but 35.1 us there: fewer tiles on their way, longer chains.)
   const int64_t avg = ((int64_t)bt.rows + bt.seqs - 1) / bt.seqs * p.group;
   if (avg >= kPromptRows) return launch_kv8_prompt(p, c.head_dim, di, stream);
-  const int nt = avg <= 8 ? 1 : avg <= 16 ? 2 : 4;
-  const int max_rows = (int)std::min<int64_t>(8 * nt, (int64_t)bt.rows * p.group);
+  const int rows = avg <= 8 ? 8 : 16;
+  const int max_rows = (int)std::min<int64_t>(rows, (int64_t)bt.rows * p.group);
   if (c.head_dim == 128)
-    return nt == 1   ? launch<128, 1>(p, max_rows, di, stream)
-           : nt == 2 ? launch<128, 2>(p, max_rows, di, stream)
-                     : launch<128, 4>(p, max_rows, di, stream);
-  return nt == 1   ? launch<64, 1>(p, max_rows, di, stream)
-         : nt == 2 ? launch<64, 2>(p, max_rows, di, stream)
-                   : launch<64, 4>(p, max_rows, di, stream);
+    return rows == 8 ? launch<128, 1>(p, max_rows, di, stream)
+                     : launch<128, 2>(p, max_rows, di, stream);
+  return rows == 8 ? launch<64, 1>(p, max_rows, di, stream)
+                   : launch<64, 2>(p, max_rows, di, stream);
 }
 
 }  // namespace w4

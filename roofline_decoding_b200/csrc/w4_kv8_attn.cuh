@@ -224,7 +224,9 @@ __device__ __forceinline__ Share find_share(const AttnP& p) {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = i < each ? G::seq_work(p, s[i]) : 0;
+      w[i] = 0;
+      if (i >= each) continue;
+      w[i] = G::seq_work(p, s[i]);
       if (s[i].n == 0) continue;
       bad |= told[i] < 0 || told[i] > p.capacity - s[i].n;
       if constexpr (G::kCut > 0) {

@@ -26,10 +26,11 @@
 //                    last time (P' may then reach 2^14, inside fp16's range).
 // Two O, two S (with P over them) fill the tensor memory: 4 x 128 columns. A tile's
 // products at their best rate and its 128 x 128 exponentials at 16 a clock are 1024
-// clocks each, its traffic on shared memory 1750. A tile takes 2700: a stream's
+// clocks each, its traffic on shared memory 1750. A tile takes 2600: a stream's
 // S, softmax (2400), P V and next S follow one another, and two streams are all that
-// the tensor memory holds. 2 x 256 rows of 32 heads on 8 over 4096 tokens: 68 us, 501
-// TFLOP/s of the causal products; 8192 rows from nothing 912 us, 603 TFLOP/s.
+// the tensor memory holds. 2 x 256 tokens of 32 heads on 8 over 4096: 68 us, 500
+// TFLOP/s of the causal products (16 us of it before the first S, after the last P V
+// and in the empty join's launch); 8192 tokens from nothing 885 us, 620 TFLOP/s.
 #include "w4_kv8_attn.cuh"
 
 #include <algorithm>
@@ -44,8 +45,8 @@ constexpr int kMmaWarp = kWidenWarp + kWidenWarps;
 constexpr int kItemWarp = kMmaWarp + 1, kCopyWarp = kMmaWarp + 2;
 constexpr int kPromptThreads = 32 * (kMmaWarp + 4);  // four warpgroups; one warp idles
 // Registers a thread: 128 at launch, then by warpgroup (their sum is four times
-// that, which is what the block has).
-constexpr int kSoftRegs = 192, kWidenRegs = 72, kMmaRegs = 56;
+// that, which is what the block has). 8192 tokens: softmax 176 922 us, 184 885, 192 905.
+constexpr int kSoftRegs = 184, kWidenRegs = 80, kMmaRegs = 64;
 static_assert(2 * kSoftRegs + kWidenRegs + kMmaRegs <= 4 * 128, "registers of the block");
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
 // P' of the maximum that O is scaled by is 2^kPromptShift, and the running maximum may
@@ -77,9 +78,9 @@ struct Rows128 {
     return (kRows + p.group - 1) / p.group;
   }
   // Items are not cut if the longest CTA ends at most this much later than with equal
-  // shares: a cut costs two first tiles, the parts and their join. 2 x 256 rows of 32
-  // heads on 8, cut and not: past 1000 45.2 and 31.3 us, 4096 81.7 and 68.0, 12000 (13
-  // tiles later) 165.7 and 165.6; 512 rows of 16 heads past 3000 (17) 44.3 and 54.7.
+  // shares: a cut costs two first tiles, the parts and their join. 2 sequences of
+  // up to 256 tokens, 32 heads on 8, cut and not: over 1000 45.2 and 31.3 us, 4096 81.7
+  // and 68.0, 12000 (13 tiles later) 165.7 and 165.6; 512 tokens of 16 heads over 3000 (17) 44.3 and 54.7.
   static constexpr int kCut = 12 * kPromptTile;
   static constexpr int kMore = 3 * kPromptTile;  // what first() and length() have beside past
   // Length of the first row tile, then of row tile rt: above kOver + kUnit * tiles
@@ -488,11 +489,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
     } else if (warp == kMmaWarp && lane == 0) {
       constexpr uint32_t idesc_s = prompt_idesc(kPromptTile, 0), idesc_o = prompt_idesc(D, 1);
       const uint64_t q_desc = operand_desc(sm + S::kOffQ, 16, 1024);
-      // O += P V of tile m, the first of its item and stream or not
-      auto output = [&](int m, bool first) {
+      // O += P V of tile m of item `of`, its first of the stream or not
+      auto output = [&](int m, bool first, int of) {
         const int u = m & 1;
         if (!wait(&p_half[u], (m >> 1) & 1) || !wait(&v_full[u], (m >> 1) & 1) ||
-            (first && item > 0 && !wait(o_empty, (item - 1) & 1)))
+            (first && of > 0 && !wait(o_empty, (of - 1) & 1)))
           return false;
         after_sync();
         const uint64_t v_desc = operand_desc(sm + S::kOffV + u * S::kOperand, S::kHalf, 1024);
@@ -510,6 +511,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         commit_to(&pv_done[u]);
         return true;
       };
+      // A tile's P V comes after the next tile's S, the next item's first too, so that
+      // there is a softmax to do while the item's last one is done.
+      bool first = false;
+      int of = 0;
       while (ok && next_item()) {
         if (!(ok = wait(&q_full[item & 1], (item >> 1) & 1))) break;
         const int n0 = n;
@@ -529,11 +534,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           __threadfence_block();  // the widen warps' scales, for those who wait for s_full
           commit_to(&k_empty[u]);
           commit_to(&s_full[u]);
-          if (n > n0) ok = output(n - 1, n - 1 - n0 < 2);
+          if (n > 0) ok = output(n - 1, first, of);
+          first = n - n0 < 2;
+          of = item;
         }
-        if (ok) ok = output(n - 1, n - 1 - n0 < 2);
         mbar_arrive(&item_empty[item++ % kItems]);
       }
+      if (ok && n > 0) ok = output(n - 1, first, of);
     }
   } else if (warp >= kWidenWarp) {
     // ------------------------------------------------------------ widen
@@ -854,7 +861,7 @@ template <int D>
 int launch_prompt(AttnP p, const DeviceInfo& di, cudaStream_t stream) {
   using S = PromptShape<D>;
   p.join = reinterpret_cast<Join*>(p.parts + (size_t)(kMaxCtas / 2) * 2 * kPromptTile * S::kPitch);
-  // (16 rows of 16 heads on 4 over 100 tokens: 12.9 us, with all CTAs 15.8; the other
+  // (16 tokens of 16 heads on 4 over 100: 12.9 us, with all CTAs 15.8; the other
   // kernel's CTAs are smaller, and fewer of them gain nothing)
   const int ctas = useful_ctas<Rows128>(p, std::min(kMaxCtas / 2, di.sm_count));
   cudaError_t e =

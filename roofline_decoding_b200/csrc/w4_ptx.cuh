@@ -19,7 +19,7 @@ constexpr uint32_t kSuspendHintNs = 20000;  // 20 us
 
 // Device-side error word; kernels set it when a bounded wait gives up.
 enum : int { kErrNone = 0, kErrFullWait = 1, kErrEmptyWait = 2, kErrDrainWait = 3 };
-// (codes 4 to 7 belong to the kernels that set them)
+// (codes 4 to 7 and 9, attention of prompts, belong to the kernels that set them)
 // A page, a row's position or a rotation table's row was out of range; what it
 // belonged to was left out.
 constexpr int kErrKvRange = 8;
