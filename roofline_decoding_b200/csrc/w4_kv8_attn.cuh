@@ -6,6 +6,8 @@
 #include "w4_internal.h"
 #include "w4_ptx.cuh"
 
+#include <algorithm>
+
 namespace w4 {
 
 struct AttnP {
@@ -349,7 +351,8 @@ struct Walk {
 // knows bounds of the items and, by the page table, of their lengths.
 template <typename G>
 inline int useful_ctas(const AttnP& p, int ctas) {
-  const int64_t items = (int64_t)p.kv_heads * ((int64_t)p.rows * p.group / G::kRows + p.seqs);
+  const int64_t items = std::min<int64_t>(  // (times 2^31 units at most)
+      (int64_t)p.kv_heads * ((int64_t)p.rows * p.group / G::kRows + p.seqs), 1 << 30);
   const int64_t units = G::kOver + G::kMore +
                         G::kUnit * (((int64_t)p.capacity + G::kTile - 1) / G::kTile);
   return (int)std::min<int64_t>(ctas, (items * units + G::kMinShare - 1) / G::kMinShare);

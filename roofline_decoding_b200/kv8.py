@@ -106,7 +106,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor,
     cache's (1 to 16 query heads each). Row i of sequence b sees the tokens
     0 .. lengths[b] + i. scale defaults to head_dim ** -0.5. Softmax and sums in
     fp32, rounded once to q's type; deterministic. Returns [rows, heads,
-    head_dim] (`out` if given); rows outside every sequence are left unwritten,
-    and a row whose pages are all out of range is zero.
+    head_dim] (`out` if given, which may be q); rows outside every sequence are
+    left unwritten, and a row whose pages are all out of range is zero.
     """
     return _lib.torch_module().kv8_attention(q, *cache, page_table, lengths, row_starts, scale, out)

@@ -817,3 +817,57 @@ def test_outputs_whose_rows_overlap_are_refused():
     for strides in ((512, 128, 1), (1024, 136, 1), (128, 384, 1)):
         out = torch.zeros(4096, device=DEV, dtype=torch.bfloat16).as_strided((3, 4, 128), strides)
         rd.qk_norm_rope(q, q, q_out=out)
+
+
+def test_prompts_on_two_streams_and_in_graphs_follow_lengths_and_rows():
+    """Captured prompt steps replayed side by side, with items that are cut and that are not."""
+    g, page = gen(31), 64
+    sides = []
+    for i in range(2):
+        table, pages = page_tables(g, [6000, 900, 300], [0] * 3, page)
+        x = dict(cache=fresh_cache(g, pages, 4, 128, page), table=table, q=randn(g, 300, 8, 128),
+                 lengths=i32([0, 0, 0]), rs=i32([0, 0, 0, 0]), stream=torch.cuda.Stream())
+        sides.append(x)
+    torch.cuda.synchronize()
+    for x in sides:
+        x["graph"] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(x["graph"], stream=x["stream"]):
+            x["out"] = rd.kv8_attention(x["q"], x["cache"], x["table"], x["lengths"], x["rs"])
+    steps = [([5700, 10, 0], [0, 300, 300, 300]), ([0, 800, 3], [0, 0, 90, 300]),
+             ([100, 64, 127], [5, 105, 205, 290]), ([5999, 899, 299], [0, 1, 2, 3]),
+             ([4000, 500, 0], [0, 128, 250, 300])]
+    for past, rs in steps:
+        for x in sides:
+            x["lengths"].copy_(i32(past))
+            x["rs"].copy_(i32(rs))
+            x["out"].fill_(9.0)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for x in sides:
+                with torch.cuda.stream(x["stream"]):
+                    x["graph"].replay()
+        torch.cuda.synchronize()
+        for x in sides:
+            check_attention(x["out"], x["q"], x["cache"], x["table"], x["lengths"], x["rs"])
+            assert torch.all(x["out"][:rs[0]] == 9.0) and torch.all(x["out"][rs[-1]:] == 9.0)
+            eager = rd.kv8_attention(x["q"], x["cache"], x["table"], x["lengths"], x["rs"])
+            assert torch.equal(eager[rs[0]:rs[-1]], x["out"][rs[0]:rs[-1]])
+    assert rd.device_error() == 0
+
+
+@pytest.mark.parametrize("past,rows", [(3000, 64), (4096, 256), (0, 40), (15000, 20)])
+def test_attention_into_its_own_queries(past, rows):
+    """The output over the queries: an item's are read before any of its rows is written."""
+    g = gen(past + rows)
+    table, pages = page_tables(g, [past], [rows], 64)
+    cache = fresh_cache(g, pages, 2, 128, 64)
+    q = randn(g, rows, 8, 128)
+    lengths, rs = i32([past]), i32([0, rows])
+    want = rd.kv8_attention(q, cache, table, lengths, rs)
+    got = rd.kv8_attention(q, cache, table, lengths, rs, out=q)
+    assert got is q and torch.equal(got, want)
+    for n in (1, 3):
+        q = randn(g, n, 8, 128)
+        rs = i32([0, n])
+        want = rd.kv8_attention(q, cache, table, lengths, rs)
+        assert torch.equal(rd.kv8_attention(q, cache, table, lengths, rs, out=q), want)
