@@ -69,6 +69,7 @@ struct GemmParams {
   // output tiles of this launch: blockIdx.x = t is tile (m_tile0 + t / ntx,
   // n_tile0 + t % ntx) in units of the instance's rows and columns
   int m_tile0, n_tile0, ntx;
+  uint32_t x_bytes;  // of an X tile's copy
   int ksplit;       // K slices (gridDim.z, one cluster per tile when > 1)
   const uint16_t* scales;  // fp16 [K/128, N]
   int act;               // w4_act
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 
   auto load_x = [&](int kt) {
     const int s = kt % S::kStages;
-    mbar_arrive_expect_tx(&full[s], S::kXBytes);
+    mbar_arrive_expect_tx(&full[s], p.x_bytes);
     tma_load_2d(base + S::kOffX + s * S::kXBytes, &tm_x, &full[s], (kt0 + kt) * kBK, m0);
   };
   auto load_w = [&](int kt) {
@@ -832,10 +833,14 @@ int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* sc
   for (int i = 0; i < n; ++i) {
     const GemmLaunch& L = plan[i];
     const int BM = L.nacc * kUM;
+    // Rows behind the last are not copied: what lies there reaches sums of its own rows
+    // alone. (Zero-filled rows of a tensor below 128 KB cost more than real ones: 1 x
+    // 4096 x 14336 39 us with whole boxes, 28 so; 1 x 1536 x 8960 10.7 and 9.0.)
+    const int box_rows = std::min(BM, (M + 7) / 8 * 8);
     CUtensorMap tm_x, tm_w;
     if (!encode_2d(&tm_x,
                    x_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                   x, (uint64_t)K, (uint64_t)M, kBK, (uint32_t)BM, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                   x, (uint64_t)K, (uint64_t)M, kBK, (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !encode_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_INT32, 4, packed, (uint64_t)N,
                    (uint64_t)(K / 8), (uint32_t)L.bn, kBK / 8, CU_TENSOR_MAP_SWIZZLE_NONE))
       return fail(W4_ERR_CUDA, "cuTensorMapEncodeTiled failed for w4_gemm M=%d K=%d N=%d", M, K,
@@ -856,6 +861,7 @@ int launch_gemm(const void* x, int x_bf16, const int32_t* packed, const void* sc
     p.n_tile0 = L.n_tile0;
     p.ntx = L.ntx;
     p.ksplit = L.ksplit;
+    p.x_bytes = (uint32_t)box_rows * kBK * 2;
     p.wait_at_end = L.after_previous ? 1 : 0;
     size_t smem = 0;
     void* fn = gemm_instance(x_bf16, L.bn, L.nacc, &smem);
