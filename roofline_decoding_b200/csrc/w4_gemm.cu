@@ -265,9 +265,9 @@ __device__ __forceinline__ void load_row(const void* p, size_t at, int bf16, flo
   }
 }
 
+// NV elements of a row to 16 bits, two a word.
 template <int NV>
-__device__ __forceinline__ void store_row(void* p, size_t at, int bf16, const float (&f)[NV]) {
-  uint32_t w[NV / 2];
+__device__ __forceinline__ void pack_row(int bf16, const float (&f)[NV], uint32_t (&w)[NV / 2]) {
 #pragma unroll
   for (int i = 0; i < NV / 2; ++i) {
     if (bf16) {
@@ -278,11 +278,30 @@ __device__ __forceinline__ void store_row(void* p, size_t at, int bf16, const fl
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
-  uint16_t* dst = static_cast<uint16_t*>(p) + at;
-  if constexpr (NV == 8)
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(w);
-  else
-    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(w);
+}
+
+__device__ __forceinline__ uint4 pick(bool first, const uint4& a, const uint4& b) {
+  return make_uint4(first ? a.x : b.x, first ? a.y : b.y, first ? a.z : b.z, first ? a.w : b.w);
+}
+__device__ __forceinline__ uint4 swap_lanes(const uint4& v, int lanes) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, lanes), __shfl_xor_sync(0xffffffffu, v.y, lanes),
+                    __shfl_xor_sync(0xffffffffu, v.z, lanes), __shfl_xor_sync(0xffffffffu, v.w, lanes));
+}
+// Four lanes with a row of four 16-byte chunks each: chunk j of row t to chunk t of
+// row j, and back. A warp then reads and writes 64 bytes of 8 rows at a time instead
+// of 16 bytes of 32, each of which costs the L1 cache a line's turn.
+__device__ __forceinline__ void transpose4(uint4 (&c)[4], int lane) {
+#pragma unroll
+  for (int s = 1; s <= 2; s <<= 1) {
+    const bool odd = lane & s;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int lo = s == 1 ? 2 * i : i, hi = lo + s;
+      const uint4 got = swap_lanes(pick(odd, c[lo], c[hi]), s);
+      c[lo] = pick(odd, got, c[lo]);
+      c[hi] = pick(odd, c[hi], got);
+    }
+  }
 }
 
 __device__ __forceinline__ float silu(float a) { return __fdividef(a, 1.0f + __expf(-a)); }
@@ -529,13 +548,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // ------------------------------------------------------------ epilogue
     const bool gated = p.act == W4_ACT_SWIGLU;
     const int step = gated ? 2 : 1;  // 32-column blocks a turn
-    uint4 res[4];                    // the next turn's residual, a turn ahead of its use
+    uint4 res[4] = {};               // the next turn's residual, a turn ahead of its use
+    // Chunk k of a lane in memory: chunk t of row k of its quad where tiles have many
+    // rows, of its own row otherwise. Turned and not: 300 x 1536 x 1536 17.0 and 18.2 us,
+    // 2048 x 8960 x 1536 65.6 and 68.6, 1709 x 128 x 7296 with a residual 35 and 41; but
+    // one accumulator, 17 x 1536 x 2048 14.6 and 13.4, 64 x 4096 x 4096 28.9 and 27.0.
+    constexpr bool kTurn = NACC == 2;
+    const int t = lane & 3;
+    auto row_of = [&](int k) { return kTurn ? row - t + k : row; };
+    auto col_of = [&](int k) { return 8 * (kTurn ? t : k); };
     auto load_residual = [&](int c) {
-      if (c < BN / 32 && p.residual && has_row && n0 + 32 * c < p.N) {
-        const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const uint16_t*>(p.residual) + out_at(p, row, n0 + 32 * c));
+      if (half < NACC && c < BN / 32 && p.residual && n0 + 32 * c < p.N) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) res[v] = src[v];
+        for (int k = 0; k < 4; ++k)
+          if (row_of(k) < p.M)
+            res[k] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) +
+                                                     out_at(p, row_of(k), n0 + 32 * c) + col_of(k));
       }
     };
     if (p.ksplit == 1) load_residual(0);
@@ -570,8 +598,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
         for (int v = 0; v < 4; ++v) now[v] = res[v];
         load_residual(c + step);
-        if (has_row && n0 + 32 * c < p.N) {
-          const size_t at = out_at(p, row, n0 + 32 * c);
+        if (n0 + 32 * c < p.N) {
+          if (kTurn && p.residual) transpose4(now, lane);
+          uint4 y[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             float a[8], u[8];
@@ -587,8 +616,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
               for (int e = 0; e < 8; ++e) a[e] += f[e];
             }
-            store_row(p.y, at + 8 * v, p.y_bf16, a);
+            uint32_t w[4];
+            pack_row(p.y_bf16, a, w);
+            y[v] = make_uint4(w[0], w[1], w[2], w[3]);
           }
+          if (kTurn) transpose4(y, lane);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (row_of(k) < p.M)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.y) +
+                                        out_at(p, row_of(k), n0 + 32 * c) + col_of(k)) = y[k];
         }
       }
     }
@@ -638,7 +675,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[e] += f[e];
         }
-        store_row(p.y, to, p.y_bf16, a);
+        uint32_t packed[2];
+        pack_row(p.y_bf16, a, packed);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + to) = make_uint2(packed[0], packed[1]);
       }
       cluster.sync();  // the other ranks' reads of this CTA's partial are done
     }
