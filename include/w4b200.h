@@ -431,7 +431,9 @@ int w4_decode_step(const w4_decode_model* model, void* scratch, size_t scratch_b
  * None of them allocates, synchronises or keeps anything between calls. Page
  * numbers, lengths and positions are read on the device: one out of range is
  * never followed; what it belongs to is left out and the device error word is
- * set to W4B200_ERR_KV_RANGE (w4_device_error). */
+ * set to W4B200_ERR_KV_RANGE (w4_device_error). A sequence of negative length is
+ * left out with all its rows (without rows it is no error); attention over a
+ * length that the page table has no room for is over the tokens that it has. */
 #define W4B200_ERR_KV_RANGE 8
 
 /* Rows of heads: element (row, head, d) at ptr + row * row_stride +

@@ -306,12 +306,17 @@ struct AppendParams {
   int kv_blocks;  // CTAs of the cache part; those after them turn queries
 };
 
-// First row and number of rows of sequence b, kept inside the buffers.
-__device__ __forceinline__ int seq_rows(const AppendParams& p, int b, int* first) {
+// First row and number of rows of sequence b, kept inside the buffers, and the tokens
+// before them. Rows behind a negative length have no place: none are counted.
+__device__ __forceinline__ int seq_rows(const AppendParams& p, int b, int* first, int* past) {
   const int a = min(max(p.row_starts[b], 0), p.rows);
   const int e = min(max(p.row_starts[b + 1], a), p.rows);
+  const int length = p.lengths[b];
   *first = a;
-  return e - a;
+  *past = max(length, 0);
+  if (length >= 0 || e == a) return e - a;
+  atomicCAS(p.rope.err, 0, kErrKvRange);
+  return 0;
 }
 
 // Pages that n rows behind `past` tokens touch.
@@ -343,10 +348,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
     for (int i = 0; i < 4; ++i) {
       const int bb = b0 + each * lane + i;
       f[i] = m[i] = ps[i] = 0;
-      if (i < each && bb < p.seqs) {
-        m[i] = seq_rows(p, bb, &f[i]);
-        ps[i] = max(p.lengths[bb], 0);
-      }
+      if (i < each && bb < p.seqs) m[i] = seq_rows(p, bb, &f[i], &ps[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) mine += cnt[i] = touched(ps[i], m[i], p.page_shift);
@@ -520,8 +522,9 @@ __global__ void __launch_bounds__(kAppendThreads, W == 1 ? 3 : NP == 4 ? 2 : 3)
     b += __popc(__ballot_sync(0xffffffffu, bb < p.seqs && p.row_starts[bb + 1] <= row));
   }
   if (b >= p.seqs || row < p.row_starts[b]) return;  // a row outside every sequence
-  const int64_t pos = (int64_t)max(p.lengths[b], 0) + row - max(p.row_starts[b], 0);
-  if (r.cos_t && pos >= r.max_pos) {
+  const int length = p.lengths[b];
+  const int64_t pos = (int64_t)length + row - max(p.row_starts[b], 0);
+  if (length < 0 || (r.cos_t && pos >= r.max_pos)) {
     if (lane == 0) atomicCAS(r.err, 0, kErrKvRange);
     return;
   }

@@ -113,16 +113,20 @@ __device__ __forceinline__ bool any_nan(const uint4& v) {
 }
 
 // A sequence's rows and tokens. A length that the page table cannot hold is cut
-// to what it holds.
+// to what it holds; rows behind a negative one see nothing, and none are counted.
 struct Seq {
   int first, n;  // rows
   int past;
+  bool bad;      // has rows, and a length that the page table has no room for
 };
 __device__ __forceinline__ Seq load_seq(const AttnP& p, int b) {
   Seq s;
+  const int length = p.lengths[b];
   s.first = min(max(p.row_starts[b], 0), p.rows);
   s.n = min(max(p.row_starts[b + 1], s.first), p.rows) - s.first;
-  s.past = min(max(p.lengths[b], 0), p.capacity);
+  s.past = min(max(length, 0), p.capacity);
+  s.bad = s.n > 0 && (length < 0 || length > p.capacity - s.n);
+  if (length < 0) s.n = 0;
   return s;
 }
 // r / group, for r < 2^28: group_mul * group exceeds 2^32 by less than 16.
@@ -214,23 +218,20 @@ __device__ __forceinline__ Share find_share(const AttnP& p) {
   bool bad = false;       // a length that the page table has no room for
   auto load = [&](int b0) {
     Seq s[4];
-    int told[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int b = b0 + each * lane + i;
-      s[i].first = s[i].n = s[i].past = told[i] = 0;
-      if (i < each && b < p.seqs) {
-        s[i] = load_seq(p, b);
-        told[i] = p.lengths[b];
-      }
+      s[i].first = s[i].n = s[i].past = 0;
+      s[i].bad = false;
+      if (i < each && b < p.seqs) s[i] = load_seq(p, b);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       w[i] = 0;
       if (i >= each) continue;
       w[i] = G::seq_work(p, s[i]);
+      bad |= s[i].bad;
       if (s[i].n == 0) continue;
-      bad |= told[i] < 0 || told[i] > p.capacity - s[i].n;
       if constexpr (G::kCut > 0) {
         const int nrt = G::row_tiles(p, s[i]);
         items = (int)min(items + (int64_t)p.kv_heads * nrt, (int64_t)1 << 24);

@@ -16,7 +16,9 @@ page_table[b, t // page_size]. Rows behind the last sequence are left alone.
 All of it is read on the device, so a step can be captured once in a CUDA graph
 and replayed as lengths and pages change. A page, length or position out of
 range is never followed: what it belongs to is left out, and device_error()
-returns _lib.ERR_KV_RANGE.
+returns _lib.ERR_KV_RANGE. A sequence of negative length is left out with all
+its rows (one without rows is a free slot and no error); attention over a length
+that the page table has no room for is over the tokens that it has room for.
 
 Every function runs on the current CUDA stream through the C ABI
 (include/w4b200.h); there is no CPU path.

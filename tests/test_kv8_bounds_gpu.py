@@ -1,0 +1,80 @@
+"""kv8_append and kv8_attention at the borders of their contract: lengths, positions, scales, values.
+
+Bars are those of test_kv8_gpu.py unless a test says otherwise.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import roofline_decoding_b200 as rd  # noqa: E402
+from oracle import kv8_oracle as o  # noqa: E402
+from roofline_decoding_b200 import _lib  # noqa: E402
+from test_kv8_gpu import (check_attention, fresh_cache, gen, i32, page_tables, randn, starts,  # noqa: E402
+                          tables)
+
+DEV = "cuda"
+
+
+def same_bytes(a, b):
+    return all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
+def copy_of(cache):
+    return rd.KV8Cache(*[t.clone() for t in cache])
+
+
+# ------------------------------------------------------------------ lengths below zero
+
+
+@pytest.mark.parametrize("length", [-1, -(2 ** 31)])
+@pytest.mark.parametrize("n", [1, 40])  # a warp a block of the cache, a CTA a block
+def test_append_leaves_out_a_sequence_of_negative_length(n, length):
+    g, page = gen(1), 32
+    past = [5, 60, 31]
+    table, pages = page_tables(g, past, [n] * 3, page)
+    cache = fresh_cache(g, pages, 2, 128, page)
+    want = copy_of(cache)
+    cos, sin = tables(128, 128, torch.float32)
+    q, k, v = randn(g, 3 * n, 4, 128), randn(g, 3 * n, 2, 128), randn(g, 3 * n, 2, 128)
+    out, want_q = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+    for b in (0, 2):
+        rows = slice(b * n, (b + 1) * n)
+        rd.kv8_append(want, k[rows], v[rows], table[b:b + 1], i32([past[b]]), i32([0, n]), cos, sin,
+                      q=q[rows], out=want_q[rows])
+    assert rd.device_error() == 0
+    rd.kv8_append(cache, k, v, table, i32([past[0], length, past[2]]), i32(starts([n] * 3)), cos, sin,
+                  q=q, out=out)
+    assert rd.device_error() == _lib.ERR_KV_RANGE
+    assert same_bytes(cache, want) and torch.equal(out, want_q)
+
+
+@pytest.mark.parametrize("length", [-1, -(2 ** 31)])
+@pytest.mark.parametrize("n", [1, 20, 80])
+def test_attention_leaves_out_a_sequence_of_negative_length(n, length):
+    g, page = gen(2), 32
+    past = [300, 60, 31]
+    table, pages = page_tables(g, past, [n] * 3, page)
+    cache = fresh_cache(g, pages, 2, 128, page)
+    q = randn(g, 3 * n, 4, 128)
+    out = torch.full_like(q, 9.0)
+    rd.kv8_attention(q, cache, table, i32([past[0], length, past[2]]), i32(starts([n] * 3)), out=out)
+    assert rd.device_error() == _lib.ERR_KV_RANGE
+    assert torch.all(out[n:2 * n] == 9.0)
+    for b in (0, 2):
+        rows = slice(b * n, (b + 1) * n)
+        check_attention(out[rows], q[rows], cache, table[b:b + 1], i32([past[b]]), i32([0, n]))
+
+
+def test_a_negative_length_without_rows_is_no_error():
+    """A slot of the batch that holds no sequence."""
+    g = gen(3)
+    table, pages = page_tables(g, [20, 0, 20], [1, 0, 1], 16)
+    cache = fresh_cache(g, pages, 2, 64, 16)
+    q, k = randn(g, 2, 2, 64), randn(g, 2, 2, 64)
+    lengths, rs = i32([20, -1, 20]), i32([0, 1, 1, 2])
+    rd.kv8_append(cache, k, k, table, lengths, rs, q=q)
+    got = rd.kv8_attention(q, cache, table, lengths, rs)
+    assert rd.device_error() == 0
+    keep = torch.tensor([0, 2], device=DEV)
+    check_attention(got, q, cache, table[keep], i32([20, 20]), i32([0, 1, 2]))
