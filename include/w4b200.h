@@ -503,8 +503,8 @@ typedef struct {
  * that held rows of the sequence already keeps its scale where that is larger,
  * and where it is smaller those rows are rounded again in the new one. Codes
  * round to nearest even; infinities are stored as +-448 s, NaN as NaN, and
- * neither sets a scale. No page may belong to two sequences that the call
- * writes. */
+ * neither sets a scale. A row whose position has no table row is left out, its
+ * value too. No page may belong to two sequences that the call writes. */
 int w4_kv8_append(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_heads* k,
                   const w4_heads* v, const w4_heads* q, const w4_heads* q_out, int dtype,
                   const w4_rope* rope, void* stream);

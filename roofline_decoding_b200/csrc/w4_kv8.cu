@@ -380,14 +380,17 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   if (b < 0) return;  // fewer pairs than the bound
   const int64_t slot_page = (past >> p.page_shift) + g;                  // page of the sequence
   const int64_t tok0 = max((int64_t)past, slot_page * p.page);  // its first new token
-  const int cnt = (int)(min((int64_t)past + n, (slot_page + 1) * p.page) - tok0);
+  // Tokens that the rotation tables have no row for end the step, for K and V alike: a
+  // page must not hold the value of a token whose key is missing.
+  const int64_t stop = min((int64_t)past + n, (slot_page + 1) * p.page);
+  const int64_t upto = p.rope.cos_t ? min(stop, (int64_t)p.rope.max_pos) : stop;
+  const int cnt = (int)max(upto - tok0, (int64_t)0);
   const int slot0 = (int)(tok0 - slot_page * p.page);
   const int64_t row0 = first + (tok0 - past);
   const int page =
       slot_page < p.max_pages ? p.page_table[(int64_t)b * p.table_stride + slot_page] : -1;
   const bool turned = !is_v && p.rope.cos_t != nullptr;
   const HeadsIn& x = is_v ? p.v : p.k;
-  const bool no_turn = turned && tok0 + cnt > p.rope.max_pos;
 
   F8 a[NP], c[NP];
   auto load = [&](int base) {  // rows base + i RPP + tid / L, normed and turned
@@ -406,17 +409,16 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
         Turn t;
         if (turned)  // a row past the block's: any table row, its zeros stay zeros
           load_turn<D>(p.rope.cos_t, p.rope.sin_t, p.rope.table_type,
-                       no_turn ? 0 : r < cnt ? tok0 + r : tok0, l, t);
+                       r < cnt ? tok0 + r : cnt > 0 ? tok0 : 0, l, t);
         if (p.rope.k_norm) weigh<D, BF16>(p.rope.k_norm, l, turned, t);
         norm_turn<D>(a[i], c[i], p.rope.k_norm != nullptr, p.rope.eps, turned, t);
       }
     }
   };
   load(0);  // on its way beside the page's number
-  if (page < 0 || page >= p.pages || no_turn) {
-    if (tid == 0) atomicCAS(p.rope.err, 0, kErrKvRange);  // no such page or position: not stored
-    return;
-  }
+  const bool no_page = page < 0 || page >= p.pages;
+  if (tid == 0 && (no_page || upto < stop)) atomicCAS(p.rope.err, 0, kErrKvRange);
+  if (no_page || cnt == 0) return;  // no such page, or no position in it: not stored
   const size_t block = (size_t)page * p.kv_heads + h;
   float* scale_at = (is_v ? p.v_scale : p.k_scale) + block;
   uint8_t* codes = (is_v ? p.v_cache : p.k_cache) + block * p.page * D;

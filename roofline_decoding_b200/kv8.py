@@ -85,7 +85,8 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: to
     are normed (k_norm) and rotated (cos, sin) as in qk_norm_rope, at their
     positions in the sequence. With q [rows, heads, head_dim] its heads are normed
     and rotated in the same launch and returned (into `out` if given, which may be
-    q); rows outside every sequence are left unwritten.
+    q); rows outside every sequence are left unwritten. A row whose position has no
+    table row is left out: neither its key nor its value is stored.
 
     The scale of a block (one page of one head, K and V apart) is the least power
     of two s, within 2^-32 .. 2^120, with max|x| <= 448 s over the block's new

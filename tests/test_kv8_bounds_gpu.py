@@ -78,3 +78,37 @@ def test_a_negative_length_without_rows_is_no_error():
     assert rd.device_error() == 0
     keep = torch.tensor([0, 2], device=DEV)
     check_attention(got, q, cache, table[keep], i32([20, 20]), i32([0, 1, 2]))
+
+
+# ------------------------------------------------------------------ positions beyond the tables
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("past,n,max_pos", [
+    ([14, 3, 40], [4, 4, 4], 16),     # a warp a block; across max_pos inside a page, before, behind
+    ([14, 3, 40], [40, 9, 40], 50),   # a CTA a block; inside the first pages and a later one
+    ([0, 45, 48], [60, 6, 20], 48)])  # at a page's end
+def test_append_across_the_end_of_the_tables(D, past, n, max_pos):
+    """What lies below max_pos is stored, K and V alike, and what lies behind is not."""
+    g, page = gen(4), 16
+    table, pages = page_tables(g, past, n, page)
+    cache = fresh_cache(g, pages, 2, D, page)
+    want = copy_of(cache)
+    cos, sin = tables(max_pos, D, torch.float32)
+    w = randn(g, D, mul=0.2, add=1.0)
+    T = sum(n)
+    q, k, v = randn(g, T, 4, D), randn(g, T, 2, D, mul=3.0), randn(g, T, 2, D, mul=3.0)
+    out, want_q = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+    first = 0
+    for b in range(3):
+        m = max(0, min(n[b], max_pos - past[b]))
+        rows = slice(first, first + m)
+        first += n[b]
+        if m:
+            rd.kv8_append(want, k[rows], v[rows], table[b:b + 1], i32([past[b]]), i32([0, m]), cos, sin,
+                          q=q[rows], q_norm=w, k_norm=w, out=want_q[rows])
+    assert rd.device_error() == 0
+    rd.kv8_append(cache, k, v, table, i32(past), i32(starts(n)), cos, sin, q=q, q_norm=w, k_norm=w,
+                  out=out)
+    assert rd.device_error() == _lib.ERR_KV_RANGE
+    assert same_bytes(cache, want) and torch.equal(out, want_q)
