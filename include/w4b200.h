@@ -224,8 +224,9 @@ int w4_gemm_ex(const void* x, int x_dtype, const int32_t* packed, const void* sc
  * alternating blocks of 32 (gate 0..31, up 0..31, gate 32..63, ...), and y and
  * residual are [M, N/2]: y = residual + silu(gate + bias) * (up + bias).
  * bias [N] and residual have y's type, are 16-byte aligned and may be NULL;
- * residual may be y itself. The reference's W4Linear adds a bias in a separate
- * op (scripts/decode_loop.py:56-57); it has no counterpart of the rest. */
+ * residual may be y itself; y must not overlap the inputs otherwise. The
+ * reference's W4Linear adds a bias in a separate op (scripts/decode_loop.py:56-57);
+ * it has no counterpart of the rest. */
 typedef enum { W4_ACT_NONE = 0, W4_ACT_SILU = 1, W4_ACT_GELU = 2, W4_ACT_SWIGLU = 3 } w4_act;
 #define W4B200_SWIGLU_BLOCK 32
 typedef struct {

@@ -104,6 +104,13 @@ Tensor empty(at::IntArrayRef shape, const Tensor& like) {
   return Tensor(at::detail::empty_cuda(shape, like.scalar_type(), like.device(), std::nullopt));
 }
 
+// An output must not overlap what a call reads: some CTAs write while others still read.
+// (Both contiguous.)
+bool meet(const Tensor& out, const Tensor& in) {
+  const auto a = reinterpret_cast<uintptr_t>(ptr(out)), b = reinterpret_cast<uintptr_t>(ptr(in));
+  return a < b + in.numel() * in.element_size() && b < a + out.numel() * out.element_size();
+}
+
 // The tensors' device current for the call, and its current stream.
 struct OnDevice {
   c10::cuda::OptionalCUDAGuard guard;
@@ -379,6 +386,9 @@ PyObject* do_gemm(const Args& a) {
   Tensor y;
   if (given) {
     y = *given;
+    if (meet(y, x2) || meet(y, pk) || meet(y, sc) || (bias && meet(y, b)) ||
+        (residual && meet(y, r) && ptr(y) != ptr(r)))
+      refuse("out must not overlap the inputs (it may be the residual itself)");
   } else {
     const int64_t two[2] = {M, wide};
     y = Tensor(at::detail::empty_cuda(x.dim() == 1 ? at::IntArrayRef(two + 1, 1)

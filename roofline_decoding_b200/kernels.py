@@ -469,8 +469,9 @@ def w4_gemm_fused(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor,
     "swiglu" the weight's columns (and bias) alternate gate and up in blocks of
     32 (W4DecodeModel.interleave_gate_up(w, 32) before packing), and y and
     residual have N // 2 columns: residual + silu(gate) * up. bias is [N],
-    residual has y's shape; both have y's type. out may be residual itself. For
-    up to 16 rows and no epilogue w4_matmul is faster.
+    residual has y's shape; both have y's type. out may be residual itself and
+    must not overlap the inputs otherwise. For up to 16 rows and no epilogue
+    w4_matmul is faster.
     """
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")
