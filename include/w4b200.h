@@ -465,8 +465,8 @@ typedef struct {
  *   y[d] = x'[d] cos[d] + x'[d - D/2] sin[d], d >= D/2
  * in fp32, rounded once. positions [rows] picks each row's table row (may be
  * NULL without tables). q_out/k_out may be q/k themselves (the same pointer
- * and strides) and must not overlap them otherwise. head_dim 64 or 128; q or k
- * may have no heads. */
+ * and strides); outputs must not overlap inputs or each other otherwise.
+ * head_dim 64 or 128; q or k may have no heads. */
 int w4_qk_norm_rope(const w4_heads* q, const w4_heads* k, const w4_heads* q_out,
                     const w4_heads* k_out, int dtype, int rows, int head_dim,
                     const w4_rope* rope, const int64_t* positions, void* stream);
@@ -498,7 +498,8 @@ typedef struct {
 } w4_kv_batch;
 
 /* Writes a step's keys (normed and rotated) and values into the cache, and its
- * queries (normed and rotated) to q_out; q->heads may be 0. The scale of a
+ * queries (normed and rotated) to q_out, which may be q and must not overlap q, k
+ * or v otherwise; q->heads may be 0. The scale of a
  * block (one page of one head, K and V apart) becomes the least power of two s
  * in 2^-32 .. 2^120 with max|x| <= 448 s over the block's new rows; a block
  * that held rows of the sequence already keeps its scale where that is larger,
@@ -515,8 +516,9 @@ int w4_kv8_append(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_
  * lengths[b] + i. Query head h reads cache head h / (heads / kv_heads);
  * heads / kv_heads is 1 .. 16. out = softmax(scale * q K^T) V, the softmax and
  * all sums in fp32; a row that sees no token (all its pages out of range) is
- * zero. workspace: w4_kv8_attention_workspace_bytes(head_dim) bytes, 16-byte
- * aligned, of any content, used by one call at a time. */
+ * zero. out may be q and must not overlap it otherwise. workspace:
+ * w4_kv8_attention_workspace_bytes(head_dim) bytes, 16-byte aligned, of any
+ * content, used by one call at a time. */
 size_t w4_kv8_attention_workspace_bytes(int head_dim);
 int w4_kv8_attention(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_heads* q,
                      const w4_heads* out, int dtype, float scale, void* workspace,

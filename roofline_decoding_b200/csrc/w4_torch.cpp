@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -161,6 +162,54 @@ Tensor output(const char* name, const Tensor* given, const Tensor& x) {
   return *given;
 }
 
+int64_t extent(const Tensor& t) {  // elements from the first to behind the last
+  return (t.size(0) - 1) * t.stride(0) + (t.size(1) - 1) * t.stride(1) + t.size(2);
+}
+
+// Whether no head of one lies over a head of the other ([rows, heads, dim] of one dim
+// and type, a head's elements together). Views into one buffer may interleave.
+bool apart(const Tensor& a, const Tensor& b) {
+  if (!a.numel() || !b.numel()) return true;
+  const int64_t dim = a.size(2), na = a.size(1), nb = b.size(1);
+  const int64_t off = (static_cast<const char*>(ptr(b)) - static_cast<const char*>(ptr(a))) /
+                      (int64_t)a.element_size();  // exact: both are 16-byte aligned
+  if (off >= extent(a) || -off >= extent(b)) return true;
+  const int64_t ra = a.stride(0) ? a.size(0) : 1, rb = b.stride(0) ? b.size(0) : 1;
+  const int64_t row = ra > 1 ? a.stride(0) : rb > 1 ? b.stride(0) : 0;
+  if (ra > 1 && rb > 1 && a.stride(0) != b.stride(0)) return false;  // cannot tell
+  const int64_t ha = a.stride(1), hb = b.stride(1), wide_a = (na - 1) * ha + dim,
+                wide_b = (nb - 1) * hb + dim;
+  if (row > 0) {  // a q|k|v buffer: each takes a part of its own of every row
+    const int64_t at = ((off % row) + row) % row;
+    if (at >= wide_a && at + wide_b <= row) return true;
+  }
+  for (int64_t i = 0; i < na; ++i)
+    for (int64_t j = 0; j < nb; ++j) {
+      // heads i of row r and j of row s are (s - r) row + d apart
+      const int64_t d = off + j * hb - i * ha;
+      // the least of it lies at the s - r next to -d / row
+      const int64_t least = std::clamp(row > 0 ? -d / row : 0, 1 - ra, rb - 1);
+      for (int64_t k = least - 1; k <= least + 1; ++k) {
+        if (k < 1 - ra || k > rb - 1) continue;
+        const int64_t gap = k * row + d;
+        if (gap < dim && -gap < dim) return false;
+      }
+    }
+  return true;
+}
+bool same(const Tensor& a, const Tensor& b) {  // of equal sizes
+  return ptr(a) == ptr(b) && (a.size(0) <= 1 || a.stride(0) == b.stride(0)) &&
+         (a.size(1) <= 1 || a.stride(1) == b.stride(1));
+}
+// An output of the call over what the call reads, or over its other output.
+void check_apart(const char* out, const Tensor& to, const char* other, const Tensor& from) {
+  if (!apart(to, from)) refuse(out, " must not overlap ", other);
+}
+void check_over(const char* out, const Tensor& to, const char* in, const Tensor& from) {
+  if (!same(to, from) && !apart(to, from))
+    refuse(out, " must not overlap ", in, ", but may be ", in, " itself");
+}
+
 // Tables, norm weights, and the copies that they may have needed.
 struct RopeArgs {
   Tensor cos, sin, qn, kn;
@@ -264,6 +313,15 @@ PyObject* do_norm_rope(const Args& a) {
   }
   const Tensor qo = output("q_out", a.maybe(8, "q_out"), q), ko = output("k_out", a.maybe(9, "k_out"), k);
   const Tensor qs = rows16(q), ks = rows16(k);
+  if (a.v[8] != Py_None) {
+    check_over("q_out", qo, "q", qs);
+    check_apart("q_out", qo, "k", ks);
+  }
+  if (a.v[9] != Py_None) {
+    check_over("k_out", ko, "k", ks);
+    check_apart("k_out", ko, "q", qs);
+    if (a.v[8] != Py_None) check_apart("q_out", qo, "k_out", ko);
+  }
   const w4_heads hq = heads(qs), hk = heads(ks), hqo = heads(qo), hko = heads(ko);
   const OnDevice on(q.device());
   check_status(w4_qk_norm_rope(&hq, &hk, &hqo, &hko, code(q.scalar_type()), (int)rows, (int)dim,
@@ -306,6 +364,11 @@ PyObject* do_append(const Args& a) {
     refuse("out is for q");
   }
   const Tensor k16 = rows16(k), v16 = rows16(v);
+  if (given) {
+    check_over("out", out, "q", qs);
+    check_apart("out", out, "k", k16);
+    check_apart("out", out, "v", v16);
+  }
   const w4_heads hk = heads(k16), hv = heads(v16);
   const OnDevice on(k.device());
   check_status(
@@ -327,8 +390,10 @@ PyObject* do_attention(const Args& a) {
   const w4_kv_batch b = batch_desc(a.tensor(5, "page_table"), a.tensor(6, "lengths"),
                                    a.tensor(7, "row_starts"), q.size(0), q.device());
   const double scale = a.v[8] == Py_None ? 1.0 / std::sqrt((double)c.head_dim) : a.real(8);
-  const Tensor out = output("out", a.maybe(9, "out"), q);
+  const Tensor* given = a.maybe(9, "out");
+  const Tensor out = output("out", given, q);
   const Tensor qs = rows16(q);
+  if (given) check_over("out", out, "q", qs);
   const size_t need = w4_kv8_attention_workspace_bytes(c.head_dim);
   // the workspace is this call's own: the allocator keeps it apart from other
   // streams' and, during capture, from other graphs'

@@ -68,7 +68,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None = No
     weight (q_norm, k_norm [head_dim]: x * rsqrt(mean(x^2) + eps) * w), then
     rotated (rotate-half) by row positions[row] of cos and sin [max_pos,
     head_dim], if given. fp32 throughout, rounded once. A row whose position has
-    no table row is left unwritten. q_out and k_out may be q and k.
+    no table row is left unwritten. q_out and k_out may be q and k; an output must
+    not overlap an input or the other output otherwise.
     """
     return _lib.torch_module().qk_norm_rope(q, k, cos, sin, positions, q_norm, k_norm, eps, q_out,
                                             k_out)
@@ -85,7 +86,7 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, page_table: to
     are normed (k_norm) and rotated (cos, sin) as in qk_norm_rope, at their
     positions in the sequence. With q [rows, heads, head_dim] its heads are normed
     and rotated in the same launch and returned (into `out` if given, which may be
-    q); rows outside every sequence are left unwritten. A row whose position has no
+    q and must not overlap q, k or v otherwise); rows outside every sequence are left unwritten. A row whose position has no
     table row is left out: neither its key nor its value is stored.
 
     The scale of a block (one page of one head, K and V apart) is the least power
@@ -109,7 +110,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor,
     cache's (1 to 16 query heads each). Row i of sequence b sees the tokens
     0 .. lengths[b] + i. scale defaults to head_dim ** -0.5. Softmax and sums in
     fp32, rounded once to q's type; deterministic. Returns [rows, heads,
-    head_dim] (`out` if given, which may be q); rows outside every sequence are
-    left unwritten, and a row whose pages are all out of range is zero.
+    head_dim] (`out` if given, which may be q and must not overlap it otherwise);
+    rows outside every sequence are left unwritten, and a row whose pages are all
+    out of range is zero.
     """
     return _lib.torch_module().kv8_attention(q, *cache, page_table, lengths, row_starts, scale, out)

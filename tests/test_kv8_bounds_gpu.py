@@ -112,3 +112,54 @@ def test_append_across_the_end_of_the_tables(D, past, n, max_pos):
                   out=out)
     assert rd.device_error() == _lib.ERR_KV_RANGE
     assert same_bytes(cache, want) and torch.equal(out, want_q)
+
+
+# ------------------------------------------------------------------ outputs over inputs
+
+
+def test_outputs_over_other_inputs_are_refused():
+    g = gen(9)
+    cos, sin = tables(32, 64, torch.float32)
+    pos = torch.arange(4, device=DEV)
+    buf = randn(g, 4, 12, 64)
+    q, k, v, rest = buf[:, :2], buf[:, 2:4], buf[:, 4:6], buf[:, 6:8]
+    was = buf.clone()
+    for bad in (dict(q_out=k), dict(k_out=q), dict(q_out=buf[:, 1:3]), dict(q_out=rest, k_out=rest),
+                dict(k_out=buf[:, 3:5]), dict(q_out=buf.view(-1)[512:1024].view(4, 2, 64))):
+        with pytest.raises(ValueError, match="overlap"):
+            rd.qk_norm_rope(q, k, cos, sin, pos, **bad)
+    table, pages = page_tables(g, [0], [4], 16)
+    cache = fresh_cache(g, pages, 2, 64, 16)
+    lengths, rs = i32([0]), i32([0, 4])
+    for bad in (k, v, buf[:, 1:3], buf[:, 5:7]):
+        with pytest.raises(ValueError, match="overlap"):
+            rd.kv8_append(cache, k, v, table, lengths, rs, cos, sin, q=q, out=bad)
+    for bad in (buf[:, 1:3], buf.view(-1)[:512].view(4, 2, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            rd.kv8_attention(q, cache, table, lengths, rs, out=bad)
+    assert torch.equal(buf, was)
+
+
+def test_outputs_beside_the_inputs_in_one_buffer_are_taken():
+    g = gen(10)
+    cos, sin = tables(32, 64, torch.float32)
+    pos = torch.arange(4, device=DEV)
+    buf = randn(g, 4, 12, 64)
+    q, k, v = buf[:, :2], buf[:, 2:4], buf[:, 4:6]
+    want = rd.qk_norm_rope(q.clone(), k.clone(), cos, sin, pos)
+    got = rd.qk_norm_rope(q, k, cos, sin, pos, q_out=buf[:, 6:8], k_out=buf[:, 8:10])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # every third head, and rows of another buffer's halves
+    thirds = randn(g, 4, 9, 64)
+    got = rd.qk_norm_rope(thirds[:, ::3], thirds[:, 1::3], cos, sin, pos, q_out=thirds[:, 2::3],
+                          k_out=thirds[:, 1::3])
+    assert got[0].data_ptr() == thirds[:, 2::3].data_ptr()
+    rows = randn(g, 8, 2, 64)
+    rd.qk_norm_rope(rows[:4], k, cos, sin, pos, q_out=rows[4:])
+    table, pages = page_tables(g, [0], [4], 16)
+    cache = fresh_cache(g, pages, 2, 64, 16)
+    lengths, rs = i32([0]), i32([0, 4])
+    assert torch.equal(rd.kv8_append(cache, k, v, table, lengths, rs, cos, sin, q=q, out=q), want[0])
+    one = rd.kv8_attention(q, cache, table, lengths, rs)
+    got = rd.kv8_attention(q, cache, table, lengths, rs, out=buf[:, 10:])
+    assert torch.equal(got, one)
