@@ -22,8 +22,8 @@
 //                    the other kernel), P' in fp16 back into tensor memory over
 //                    the S that it came from. O stays in tensor memory, one a
 //                    stream with a maximum of its own, and is rescaled only when
-//                    a row's running maximum has grown by more than 2^6 since the
-//                    last time (P' may then reach 2^14, inside fp16's range).
+//                    a row's running maximum has grown by more than 2^kGrowth since
+//                    the last time (P' may then reach 2^15, inside fp16's range).
 // Two O, two S (with P over them) fill the tensor memory: 4 x 128 columns. A tile's
 // products at their best rate and its 128 x 128 exponentials at 16 a clock are 1024
 // clocks each, its traffic on shared memory 1750. A tile takes 2600: a stream's
@@ -50,10 +50,12 @@ constexpr int kSoftRegs = 184, kWidenRegs = 80, kMmaRegs = 64;
 static_assert(2 * kSoftRegs + kWidenRegs + kMmaRegs <= 4 * 128, "registers of the block");
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
 // P' of the maximum that O is scaled by is 2^kPromptShift, and the running maximum may
-// exceed it by kGrowth: P' stays below fp16's 2^16. What is more than 2^22 below the
-// maximum falls under fp16's normal range, off by 2^-25 at most: 2^-33 of the maximum's.
-constexpr float kPromptShift = 8.0f;
-constexpr float kGrowth = 6.0f;
+// exceed it by kGrowth: P' stays below fp16's 2^16. What is more than 2^28 below the
+// maximum falls under fp16's normal range, off by 2^-25 at most: 2^-39 of the maximum's,
+// as in the other kernel. (A shift of 8 and a growth of 6 spare a few rescales, 2 x 256
+// over 4096 64.1 and 65.4 us, but weights of 2^-30 are then off by a seventh.)
+constexpr float kPromptShift = 14.0f;
+constexpr float kGrowth = 1.0f;
 constexpr int kErrPromptWait = 9;
 // Factors of S are at least this, so that a masked -inf stays -inf under a scale of
 // zero; below it a score is none of the argument's 24 bits.

@@ -163,3 +163,28 @@ def test_outputs_beside_the_inputs_in_one_buffer_are_taken():
     one = rd.kv8_attention(q, cache, table, lengths, rs)
     got = rd.kv8_attention(q, cache, table, lengths, rs, out=buf[:, 10:])
     assert torch.equal(got, one)
+# ------------------------------------------------------------------ small weights
+
+
+@pytest.mark.parametrize("past", [200, 900, 20000])  # shares of one CTA, of some, of all
+@pytest.mark.parametrize("rows", [1, 3, 64, 130])
+def test_small_weights_beside_a_large_one_count_in_both_kernels(rows, past):
+    """Weights of 2^-30.6 of the largest, whose value is nothing: P' is 2^-16.6 or more, an fp16
+    subnormal with steps of 2^-24, so half a step is 2^-8.4 of it; then the result's rounding."""
+    g = gen(5)
+    table, pages = page_tables(g, [past], [rows], 64)
+    cache = fresh_cache(g, pages, 1, 128, 64)
+    cache.k.view(torch.uint8).zero_()
+    cache.v.copy_(o.to_e4m3(torch.ones(cache.v.shape, device=DEV)))
+    cache.k_scale.fill_(1.0)
+    cache.v_scale.fill_(1.0)
+    pid = int(table[0, 0])
+    cache.k[pid, :, 0, 0] = 240.0
+    cache.v[pid, :, 0] = 0.0
+    q = torch.zeros((rows, 2, 128), device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    lengths, rs = i32([past]), i32([0, rows])
+    got = rd.kv8_attention(q, cache, table, lengths, rs)
+    want, _, _ = o.attention(q, cache, table, lengths, rs)
+    assert want.abs().min() > 0
+    assert torch.all((got.double() - want).abs() <= want.abs() * 2.0 ** -8 * 2)
