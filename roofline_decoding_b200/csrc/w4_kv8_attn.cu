@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
             most = fmaxf(most, m[n][r]);
             const float al = m[n][r] == -INFINITY ? 0.f : ex2(m[n][r] - most);
             m[n][r] = most;
-            sub[n][r] = most == -INFINITY ? 0.f : most - kShift;
+            // (rounded up: where the steps of fp32 are coarser than the shift P' stays in range)
+            sub[n][r] = most == -INFINITY ? 0.f : __fadd_ru(most, -kShift);
             l[n][r] *= al;
 #pragma unroll
             for (int j = 0; j < S::kMTiles; ++j) {

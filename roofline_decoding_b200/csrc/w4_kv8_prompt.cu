@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         }
         // ---- a row's maximum much larger: all rows' O and l move to theirs (the
         // stream's last product is done: S came after it)
-        if (__any_sync(0xffffffffu, top > m + kGrowth)) {
+        if (__any_sync(0xffffffffu, top > __fadd_rd(m, kGrowth))) {
           const float most = fmaxf(m, top);
           const float al = m == -INFINITY ? 0.f : ex2(m - most);
           m = most;
@@ -753,7 +753,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             }
           }
         }
-        const float sub = m == -INFINITY ? 0.f : m - kPromptShift;
+        const float sub = m == -INFINITY ? 0.f : __fadd_ru(m, -kPromptShift);
+        // 64 columns of P' are in their place.
+        auto stored = [&](int c) {
+          if (c & 1) {
+            st_wait();
+            before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c == 1 ? &p_half[stream] : &p_full[stream]);
+          }
+        };
+        last = n;
+        if (__any_sync(0xffffffffu, fabsf(sub) > 0x1p20f)) {
+          // Scores whose steps in fp32 are no small part of one (seldom): the argument in one
+          // rounding, with the maximum's two in `less`, could be off by several. Here they
+          // get the maximum's own rounding first. S is read again: P' lies over what is read.
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float y[32];
+            uint32_t w[16];
+            ld32(tmem_s + 32 * c, y);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const float4 f = sc[2 * c + b];
+              const float ks = fmaxf(f.x * q_mul, kLeast);
+              float sum = 0.f;
+#pragma unroll
+              for (int k = 16 * b; k < 16 * b + 16; ++k) {
+                y[k] = 32 * c + k < left ? ex2(fmaf(y[k], ks, f.y) - sub) : 0.f;
+                sum += y[k];
+              }
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[8 * b + k] = half2_bits(y[16 * b + 2 * k], y[16 * b + 2 * k + 1]);
+              l = fmaf(sum, f.z, l);
+            }
+            st16(tmem_s + 16 * c, w);
+            stored(c);
+          }
+          continue;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t w[16];
@@ -772,14 +810,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), f.z, l);
           }
           st16(tmem_s + 16 * c, w);
-          if (c & 1) {
-            st_wait();
-            before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(c == 1 ? &p_half[stream] : &p_full[stream]);
-          }
+          stored(c);
         }
-        last = n;
       }
       if (!ok || (last >= 0 && !(ok = wait(&pv_done[stream], (last >> 1) & 1)))) break;
       // ---- the streams meet. The one without the item's last tile leaves maximum and

@@ -188,3 +188,27 @@ def test_small_weights_beside_a_large_one_count_in_both_kernels(rows, past):
     want, _, _ = o.attention(q, cache, table, lengths, rs)
     assert want.abs().min() > 0
     assert torch.all((got.double() - want).abs() <= want.abs() * 2.0 ** -8 * 2)
+
+
+# ------------------------------------------------------------------ scores beyond 2^20
+
+
+@pytest.mark.parametrize("rows", [1, 3, 80])
+@pytest.mark.parametrize("mul", [1e4, 1e6, 4e6, 1e7, 2e7, 4e7, 1e8, 2e8, 1e9, 1e12, 1e20, 1e30])
+def test_the_largest_score_takes_all_however_large(mul, rows):
+    """One key's score is 448 / 240 of the next: its value is the result, whatever the steps of
+    the scores in fp32 are."""
+    g, page, D = gen(11), 16, 64
+    for past, at in ((0, 0), (40, 0), (40, 17), (700, 699), (700, 130)):
+        table, pages = page_tables(g, [past], [rows], page)
+        cache = fresh_cache(g, pages, 1, D, page)
+        cache.k.view(torch.uint8).zero_()
+        cache.k[:, :, :, 0] = 240.0
+        cache.k[int(table[0, at // page]), :, at % page, 0] = 448.0
+        cache.k_scale.fill_(1.0)
+        q = torch.zeros((rows, 2, D), device=DEV, dtype=torch.bfloat16)
+        q[..., 0] = mul
+        q[:, 1, 0] *= 0.6
+        got = rd.kv8_attention(q, cache, table, i32([past]), i32([0, rows]))
+        v = o.dense(cache.v, cache.v_scale, table[0].tolist(), past + 1)[0, at]
+        assert torch.all((got.double() - v).abs() <= v.abs() * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -19))
