@@ -473,7 +473,8 @@ int w4_qk_norm_rope(const w4_heads* q, const w4_heads* k, const w4_heads* q_out,
 
 /* The cache: e4m3 codes [pages, kv_heads, page_size, head_dim], 16-byte
  * aligned, and one positive fp32 scale a page and head; a stored value is
- * code * scale. page_size 16, 32, 64 or 128; head_dim 64 or 128. */
+ * code * scale (attention counts a V scale below 2^-80 as 2^-80). page_size 16,
+ * 32, 64 or 128; head_dim 64 or 128. */
 typedef struct {
   void* k;
   void* v;

@@ -32,7 +32,8 @@
 // into the exponent: P' = exp2(s + log2 sv - m + 14) with m the running maximum
 // of s + log2 sv, so P' is at most 2^14, its rounding to fp16 (11 bits) stays
 // relative down to 2^-28 of the largest weight, and the fp32 sum adds
-// P' / sv, unrounded.
+// P' / sv, unrounded (where scales lie so far apart that P' may vanish and
+// P' / sv not, exp2(s - m + 14) itself).
 //
 // 32 sequences of up to 32768 tokens, 32 heads on 8 of 128: 174 us, 6.3 TB/s. A
 // single token over 700, 12 heads on 2: 8.5 us, the latency of two launches and of
@@ -247,12 +248,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       const int id1 = __shfl_sync(0xffffffffu, ids, 2 * id_at + 1);
       ++id_at;
       const uint32_t st = ring + issue_slot * S::kStageBytes + dst_lane;
-      if (lane < 2) {  // the scales of the halves; zero marks one that is left out
+      if (lane < 2) {  // the scales of the halves; a V scale of -1 marks one that is left out
         const int id = lane ? id1 : id0;
         const size_t blk = (size_t)max(id, 0) * p.kv_heads + lw.h;
-        const uint32_t dst = smem_u32(scales + issue_slot * 4 + lane);
-        cp4(dst, p.k_scale + blk, id >= 0);
-        cp4(dst + 8, p.v_scale + blk, id >= 0);
+        float* dst = scales + issue_slot * 4 + lane;
+        if (id >= 0) {
+          cp4(smem_u32(dst), p.k_scale + blk);
+          cp4(smem_u32(dst + 2), p.v_scale + blk);
+        } else {
+          dst[0] = 0.f;
+          dst[2] = -1.f;
+        }
       }
       const bool full = tok0 + kTile <= lw.limit && (id0 | id1) >= 0;
 #pragma unroll
@@ -330,6 +336,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
 
     float o[NT][S::kMTiles][4];
     float m[NT][2], l[NT][2], sub[NT][2];
+    float most_lv = -100.0f;  // largest log2 of a V scale so far (of kLeastScale: -80)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -375,7 +382,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       // ---- scores in log2 units with the value scale, masked
       const float4 sc = *reinterpret_cast<const float4*>(scales + slot * 4);
       const float ks[2] = {sc.x, sc.y};
-      const float lv[2] = {sc.z > 0.f ? lg2(sc.z) : -INFINITY, sc.w > 0.f ? lg2(sc.w) : -INFINITY};
+      const float lv[2] = {sc.z < 0.f ? -INFINITY : lg2(fmaxf(sc.z, kLeastScale)),
+                           sc.w < 0.f ? -INFINITY : lg2(fmaxf(sc.w, kLeastScale))};
+      most_lv = fmaxf(most_lv, fmaxf(lv[0], lv[1]));
       const int tok0 = tile * kTile;
       const bool cut = tok0 + kTile > low;  // some row ends inside the tile, or before it
       float top[NT][2];  // this lane's largest score of each row
@@ -407,11 +416,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
             for (int off = 4; off < 32; off <<= 1)
               most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
             most = fmaxf(most, m[n][r]);
-            const float al = m[n][r] == -INFINITY ? 0.f : ex2(m[n][r] - most);
+            // (l's in two steps: between far scales it is below fp32, the product is not)
+            const float root = m[n][r] == -INFINITY ? 0.f : ex2(0.5f * (m[n][r] - most));
+            const float al = root * root;
             m[n][r] = most;
             // (rounded up: where the steps of fp32 are coarser than the shift P' stays in range)
             sub[n][r] = most == -INFINITY ? 0.f : __fadd_ru(most, -kShift);
-            l[n][r] *= al;
+            l[n][r] *= root;
+            l[n][r] *= root;
 #pragma unroll
             for (int j = 0; j < S::kMTiles; ++j) {
               o[n][j][r] *= al;
@@ -419,10 +431,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
             }
           }
       }
+      if (fminf(lv[0], lv[1]) < most_lv - kFar) {  // (seldom, but at a sequence's end)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (lv[i] < most_lv - kFar && lv[i] > -INFINITY) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                l[n][e & 1] += ex2(s[i][n][e] - sub[n][e & 1] - lv[i]);
+          }
+      }
       uint32_t pf[2][NT][2];  // P^T as the B operand: 16 tokens a step
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float inv = lv[i] == -INFINITY ? 0.f : ex2(-lv[i]);  // 1 / sv
+        // 1 / sv, or nothing: left out, or in the sum already
+        const float inv = lv[i] < most_lv - kFar ? 0.f : ex2(-lv[i]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float(&v)[4] = s[i][n];
@@ -538,10 +562,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
             const float* row = buf + (8 * n + 2 * t + r) * S::kPitch;
             const float om = row[D], ol = row[D + 1];
             const float nm = fmaxf(m[n][r], om);
-            const float fa = m[n][r] == -INFINITY ? 0.f : ex2(m[n][r] - nm);
-            const float fb = om == -INFINITY ? 0.f : ex2(om - nm);
+            const float ra = m[n][r] == -INFINITY ? 0.f : ex2(0.5f * (m[n][r] - nm)), fa = ra * ra;
+            const float rb = om == -INFINITY ? 0.f : ex2(0.5f * (om - nm)), fb = rb * rb;
             m[n][r] = nm;
-            l[n][r] = l[n][r] * fa + ol * fb;
+            l[n][r] = l[n][r] * ra * ra + ol * rb * rb;
 #pragma unroll
             for (int j = 0; j < S::kMTiles; j += 2) {
               const float4 v = *reinterpret_cast<const float4*>(row + (D / 8) * g + 2 * j);

@@ -49,6 +49,13 @@ namespace {
 // CTAs that the workspace has room for: two an SM on the largest sm_100 part.
 constexpr int kMaxCtas = 320;
 
+// A value scale below this counts as this: values of 2^-71 at most. Weights over
+// scales (the softmax's sums hold P' / sv) then stay inside fp32.
+constexpr float kLeastScale = 0x1p-80f;
+// Scales this much below the largest so far (in log2) are far: a P' that vanishes then
+// still counts in the sum, which is made without it.
+constexpr float kFar = 80.0f;
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -91,10 +98,8 @@ __device__ __forceinline__ void cp16_if(uint32_t dst, const void* src, bool real
                "r"(real ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src),
-               "r"(real ? 4 : 0)
-               : "memory");
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -405,6 +410,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const AttnP p) {
   if (jn.count <= kFew) {
 #pragma unroll 1
     for (int ri = blockIdx.y * kJoinWarps + warp; ri < rows; ri += gridDim.y * kJoinWarps) {
+      // The sums' factor in two steps: from one scale to another it may leave fp32 alone.
       float m[kFew], l[kFew], v[kFew][V];
       float most = -INFINITY;
 #pragma unroll
@@ -424,8 +430,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const AttnP p) {
 #pragma unroll
       for (int c = 0; c < kFew; ++c)
         if (c < jn.count) {
-          const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - most);
-          sum += l[c] * f;
+          const float h = m[c] == -INFINITY ? 0.f : ex2(0.5f * (m[c] - most)), f = h * h;
+          sum += l[c] * h * h;
 #pragma unroll
           for (int i = 0; i < V; ++i) o[i] += v[c][i] * f;
         }
@@ -458,9 +464,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const AttnP p) {
 #pragma unroll
     for (int k = 0; k < kMine; ++k) {
       const int c = tid + k * kJoinThreads;
-      const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - most);
-      if (c < jn.count) factor[c] = f;
-      l += pl[k] * f;
+      const float h = m[k] == -INFINITY ? 0.f : ex2(0.5f * (m[k] - most));
+      if (c < jn.count) factor[c] = h * h;
+      l += pl[k] * h * h;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);

@@ -144,6 +144,7 @@ struct PromptShape {
   static constexpr int kRaw = kPromptTile * D;            // a K or V tile's codes
   static constexpr int kOffRaw = kOffV + 2 * kOperand;    // kRaws buffers
   // tiles of 8 x (K scale, log2 and inverse of the V scale, 0), their blocks with a page
+  // (8 bits) and those whose V scale is far below another's (8 bits)
   static constexpr int kOffScale = kOffRaw + kRaws * kRaw;
   static constexpr int kOffPages = kOffScale + kScales * 8 * 16;
   // two items in turn: a factor a row, maxima and sums of the stream that meets the other
@@ -444,6 +445,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       uint32_t* pages = reinterpret_cast<uint32_t*>(base + S::kOffPages);
       uint32_t stage = 0, turn = 0;
       while (ok && next_item()) {
+        float most_lv = -INFINITY;  // largest log2 of the item's V scales so far
         for (int t = it.t0; t < it.t1 && ok; t += 4) {
           const int tok = (t + j) * kPromptTile + 16 * b;
           int id = -1;
@@ -457,12 +459,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           }
           const int64_t blk = (int64_t)max(id, 0) * p.kv_heads + it.h;
           const int64_t at = ((blk << p.page_shift) + (tok & (p.page - 1))) * D;
-          float sc_k = 0.f, sc_v = 0.f;
+          float sc_k = 0.f, sc_v = 0.f, lv = -INFINITY;
           if (id >= 0) {
             sc_k = p.k_scale[blk];
-            sc_v = p.v_scale[blk];
+            sc_v = fmaxf(p.v_scale[blk], kLeastScale);
+            lv = lg2(sc_v);
           }
+          most_lv = fmaxf(most_lv, lv);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1)
+            most_lv = fmaxf(most_lv, __shfl_xor_sync(0xffffffffu, most_lv, o));
           const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
+          const uint32_t far = __ballot_sync(0xffffffffu, id >= 0 && lv < most_lv - kFar);
           for (int jj = 0; jj < min(4, it.t1 - t) && ok; ++jj, ++n) {
             const uint32_t blocks = there >> (8 * jj) & 0xffu;
 #pragma unroll 1
@@ -471,10 +479,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
               if (kv == 0) {
                 // K scale, log2 and inverse of the V scale; no page: -inf
                 if (j == jj)
-                  scales[(n % kScales) * 8 + b] = sc_v > 0.f
-                                                      ? make_float4(sc_k, lg2(sc_v), 1.0f / sc_v, 0.f)
-                                                      : make_float4(0.f, -INFINITY, 0.f, 0.f);
-                if (lane == 0) pages[n % kScales] = blocks;
+                  scales[(n % kScales) * 8 + b] = id >= 0 ? make_float4(sc_k, lv, 1.0f / sc_v, 0.f)
+                                                          : make_float4(0.f, -INFINITY, 0.f, 0.f);
+                if (lane == 0) pages[n % kScales] = blocks | (far >> (8 * jj) & 0xffu) << 8;
               }
               __syncwarp();
               if (lane == 0) mbar_arrive_expect_tx(&raw_full[stage], __popc(blocks) * kRun);
@@ -595,8 +602,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
         const int u = n & 1;
         if (!(ok = wait(&raw_full[stage], turn))) break;
-        const uint32_t blocks = *reinterpret_cast<const volatile uint32_t*>(base + S::kOffPages +
-                                                                            4 * (n % kScales));
+        const uint32_t blocks = *reinterpret_cast<const volatile uint32_t*>(
+                                    base + S::kOffPages + 4 * (n % kScales)) & 0xffu;
         const int limit_in = it.limit - t * kPromptTile;
         uint32_t keep = (1u << NP) - 1u;
         if (blocks != 0xffu || limit_in < kPromptTile) {
@@ -738,9 +745,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         // stream's last product is done: S came after it)
         if (__any_sync(0xffffffffu, top > __fadd_rd(m, kGrowth))) {
           const float most = fmaxf(m, top);
-          const float al = m == -INFINITY ? 0.f : ex2(m - most);
+          // (l's in two steps: between far scales it is below fp32, the product is not)
+          const float root = m == -INFINITY ? 0.f : ex2(0.5f * (m - most)), al = root * root;
           m = most;
-          l *= al;
+          l *= root;
+          l *= root;
           if (last >= 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -764,10 +773,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           }
         };
         last = n;
-        if (__any_sync(0xffffffffu, fabsf(sub) > 0x1p20f)) {
-          // Scores whose steps in fp32 are no small part of one (seldom): the argument in one
-          // rounding, with the maximum's two in `less`, could be off by several. Here they
-          // get the maximum's own rounding first. S is read again: P' lies over what is read.
+        const uint32_t far = *reinterpret_cast<const volatile uint32_t*>(
+                                 base + S::kOffPages + 4 * (n % kScales)) >> 8;
+        if (__any_sync(0xffffffffu, fabsf(sub) > 0x1p20f || far != 0u)) {
+          // Seldom. Scores whose steps in fp32 are no small part of one: the argument in one
+          // rounding, with the maximum's two in `less`, could be off by several, so they get
+          // the maximum's own rounding first. And scales so far apart that P' may vanish and
+          // P' / sv not: the sum is made without it. S is read again: P' lies over what is read.
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float y[32];
@@ -777,15 +789,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             for (int b = 0; b < 2; ++b) {
               const float4 f = sc[2 * c + b];
               const float ks = fmaxf(f.x * q_mul, kLeast);
+              const bool apart = far >> (2 * c + b) & 1u;
+              const float over = apart ? f.y : 0.f;
               float sum = 0.f;
 #pragma unroll
               for (int k = 16 * b; k < 16 * b + 16; ++k) {
-                y[k] = 32 * c + k < left ? ex2(fmaf(y[k], ks, f.y) - sub) : 0.f;
-                sum += y[k];
+                const float a = 32 * c + k < left ? fmaf(y[k], ks, f.y) - sub : -INFINITY;
+                y[k] = ex2(a);
+                sum += ex2(a - over);
               }
 #pragma unroll
               for (int k = 0; k < 8; ++k) w[8 * b + k] = half2_bits(y[16 * b + 2 * k], y[16 * b + 2 * k + 1]);
-              l = fmaf(sum, f.z, l);
+              l = fmaf(sum, apart ? 1.f : f.z, l);
             }
             st16(tmem_s + 16 * c, w);
             stored(c);
@@ -828,9 +843,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       after_sync();
       const float2 other = sums_s[(item & 1) * kPromptTile + r];
       const float most = fmaxf(m, other.x);
-      const float fa = m == -INFINITY ? 0.f : ex2(m - most);
-      const float fb = other.x == -INFINITY ? 0.f : ex2(other.x - most);
-      l = l * fa + other.y * fb;
+      const float ra = m == -INFINITY ? 0.f : ex2(0.5f * (m - most)), fa = ra * ra;
+      const float rb = other.x == -INFINITY ? 0.f : ex2(0.5f * (other.x - most)), fb = rb * rb;
+      l = l * ra * ra + other.y * rb * rb;
       const bool has_b = it.t1 - it.t0 > 1;
       uint32_t* mine = marks + (item & 3) * (S::kMarks / 4) + r * (D / 32);  // this thread's alone
       const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;

@@ -38,7 +38,8 @@ class KV8Cache(NamedTuple):
     k and v are float8_e4m3fn [pages, kv_heads, page_size, head_dim], k_scale and
     v_scale float32 [pages, kv_heads]; a stored value is code * scale. page_size
     is 16, 32, 64 or 128, head_dim 64 or 128. kv8_append writes power-of-two
-    scales; kv8_attention takes any positive ones.
+    scales; kv8_attention takes any positive ones (a v_scale below 2^-80 counts as
+    2^-80: values of 2^-71 at most).
     """
     k: torch.Tensor
     v: torch.Tensor

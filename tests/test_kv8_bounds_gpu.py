@@ -212,3 +212,49 @@ def test_the_largest_score_takes_all_however_large(mul, rows):
         got = rd.kv8_attention(q, cache, table, i32([past]), i32([0, rows]))
         v = o.dense(cache.v, cache.v_scale, table[0].tolist(), past + 1)[0, at]
         assert torch.all((got.double() - v).abs() <= v.abs() * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -19))
+
+
+# ------------------------------------------------------------------ value scales
+
+
+@pytest.mark.parametrize("rows", [1, 3, 80])
+@pytest.mark.parametrize("order", ["small first", "large first", "mixed"])
+@pytest.mark.parametrize("past", [100, 3000])
+def test_value_scales_far_apart(rows, order, past):
+    """Equal weights of tokens whose values lie 2^149 apart: each counts in the sum.
+
+    The result is a mean of large values and of (next to them) zeros. A factor that
+    flushes loses half of the weights; the bar is the arithmetic's of check_attention
+    (weights rounded to fp16, exp2 and log2, the sums) and the result's rounding.
+    """
+    g, page = gen(6), 16
+    table, pages = page_tables(g, [past], [rows], page)
+    cache = fresh_cache(g, pages, 1, 64, page)
+    at = torch.arange(table.shape[1], device=DEV)
+    small = {"small first": at < table.shape[1] // 2, "large first": at >= table.shape[1] // 2,
+             "mixed": at % 3 != 1}[order]
+    cache.v_scale[table[0].long(), 0] = torch.where(small, 2.0 ** -32, 2.0 ** 117)
+    q = torch.zeros((rows, 2, 64), device=DEV, dtype=torch.bfloat16)
+    lengths, rs = i32([past]), i32([0, rows])
+    got = rd.kv8_attention(q, cache, table, lengths, rs)
+    assert rd.device_error() == 0
+    want, size, _ = o.attention(q, cache, table, lengths, rs)
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -16 + past / 8 * 2.0 ** -24) * size
+    assert torch.all((got.double() - want).abs() <= tol)
+
+
+@pytest.mark.parametrize("rows", [1, 80])
+@pytest.mark.parametrize("scale", [0.0, 1e-44, 1e-39, 2.0 ** -126, 2.0 ** -90])
+def test_value_scales_that_are_next_to_nothing(rows, scale):
+    """Tokens of a block with such a scale keep their weights; their values are nothing."""
+    g, page = gen(7), 16
+    past = 200
+    table, pages = page_tables(g, [past], [rows], page)
+    cache = fresh_cache(g, pages, 1, 64, page)
+    cache.v_scale[table[0, ::2].long()] = scale
+    q = randn(g, rows, 2, 64, mul=0.3)
+    lengths, rs = i32([past]), i32([0, rows])
+    check_attention(rd.kv8_attention(q, cache, table, lengths, rs), q, cache, table, lengths, rs)
+    cache.v_scale.fill_(scale)
+    got = rd.kv8_attention(q, cache, table, lengths, rs)
+    assert torch.all(got.double().abs() <= 448 * 2.0 ** -80) and rd.device_error() == 0
