@@ -161,7 +161,10 @@ __device__ __forceinline__ float load_queries(const AttnP& p, const Seq& s, int 
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   // 2^(14 - exponent of amax), within what fp32 holds
   const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
-  const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+  // (an infinite query has no softmax: NaN, also where its scores are all -inf and would
+  // look like a row that sees nothing)
+  const float up = amax <= 3.4028234e38f ? __uint_as_float((uint32_t)(14 - e + 127) << 23)
+                                         : __int_as_float(0x7fffffff);
 #pragma unroll
   for (int k = 0; k < D / 16; ++k) {
     b[k][0] = half2_bits(f[4 * k] * up, f[4 * k + 1] * up);

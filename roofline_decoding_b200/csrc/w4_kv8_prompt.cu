@@ -687,7 +687,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
         const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 126);
-        const float up = copysignf(__uint_as_float((uint32_t)(14 - e + 127) << 23), p.scale_log2);
+        // (an infinite query has no softmax: NaN, as in the other kernel)
+        const float up = amax <= 3.4028234e38f
+                             ? copysignf(__uint_as_float((uint32_t)(14 - e + 127) << 23), p.scale_log2)
+                             : __int_as_float(0x7fffffff);
         q_mul = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
         mul_s[(item & 1) * kPromptTile + r] = q_mul;
         // the last item's last S, which the other stream's tile was

@@ -258,3 +258,22 @@ def test_value_scales_that_are_next_to_nothing(rows, scale):
     cache.v_scale.fill_(scale)
     got = rd.kv8_attention(q, cache, table, lengths, rs)
     assert torch.all(got.double().abs() <= 448 * 2.0 ** -80) and rd.device_error() == 0
+
+
+# ------------------------------------------------------------------ infinite queries
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 80])
+@pytest.mark.parametrize("past", [0, 40])
+def test_an_infinite_query_against_keys_of_one_sign_is_nan(past, rows, dtype):
+    """Every score is -inf: the softmax has no value, and the row is not taken for an empty one."""
+    g = gen(8)
+    table, pages = page_tables(g, [past], [rows], 16)
+    cache = fresh_cache(g, pages, 1, 64, 16)
+    cache.k[..., 5] = -3.0
+    q = randn(g, rows, 2, 64, dtype=dtype)
+    q[0, 1, 5] = float("inf")
+    got = rd.kv8_attention(q, cache, table, i32([past]), i32([0, rows]))
+    nan = torch.isnan(got)
+    assert nan[0, 1].all() and int(nan.sum()) == 64
