@@ -304,7 +304,13 @@ __device__ __forceinline__ void transpose4(uint4 (&c)[4], int lane) {
   }
 }
 
-__device__ __forceinline__ float silu(float a) { return __fdividef(a, 1.0f + __expf(-a)); }
+// a / (1 + e^-a), with the exponential of -|a|: that of -a leaves fp32 below -88 (and the
+// short division is zero from 2^126 on), where a bf16 result times a large up column is
+// still far from zero.
+__device__ __forceinline__ float silu(float a) {
+  const float e = __expf(-fabsf(a));
+  return __fdividef(a < 0.f ? a * e : a, 1.0f + e);
+}
 
 // Bias and activation of NV accumulators of columns n.. of a row (u: the up
 // columns, 32 further, of a gated pair).
