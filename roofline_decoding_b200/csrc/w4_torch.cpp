@@ -413,6 +413,7 @@ PyObject* do_gemm(const Args& a) {
   if (packed.dim() != 2 || packed.scalar_type() != at::kInt)
     refuse("packed must be int32 [K/8, N], got ", packed);
   const int64_t K = packed.size(0) * 8, N = packed.size(1);
+  if (K == 0 || N == 0) refuse("packed must have K > 0 rows and N > 0 columns, got ", packed);
   if (K % 128 != 0 || scales.dim() != 2 || scales.scalar_type() != at::kHalf ||
       scales.size(0) != K / 128 || scales.size(1) != N)
     refuse("scales must be fp16 [", K / 128, ", ", N, "] for packed ", packed.sizes(),

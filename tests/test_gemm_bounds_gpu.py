@@ -63,3 +63,13 @@ def test_silu_of_gates_whose_exponential_is_out_of_range(gate, split_k):
         up = 1e30 if act == "swiglu" else 1.0
         slack = 2.0 ** -149 * abs(gate) * up + (2.0 ** -133 if act == "silu" else 0.0)
         assert torch.all((y - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -16) + slack)
+
+
+def test_weights_of_no_rows_or_columns_are_refused():
+    """y of no K would be residual + act(bias), which no kernel of the library makes."""
+    for K, N in ((0, 128), (128, 0)):
+        packed = torch.zeros((K // 8, N), dtype=torch.int32, device=DEV)
+        scales = torch.zeros((K // 128, N), dtype=torch.float16, device=DEV)
+        for M in (0, 5):
+            with pytest.raises(ValueError, match="packed must have K > 0"):
+                rd.w4_gemm_fused(torch.zeros((M, K), dtype=torch.float16, device=DEV), packed, scales)
