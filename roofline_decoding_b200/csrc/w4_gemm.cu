@@ -40,7 +40,7 @@
 // leave most SMs idle in a final wave (a second, programmatically dependent
 // launch that runs while the first one's last wave finishes).
 #include "w4_internal.h"
-#include "w4_ptx.cuh"
+#include "w4_tcgen05.cuh"
 
 #include <cooperative_groups.h>
 
@@ -122,83 +122,6 @@ struct GemmShape {
   static constexpr int kPitch = BN + 4;
   static constexpr bool kCanSplit = kBM * kPitch * 4 <= kOffPk;
 };
-
-// ---------------------------------------------------------------- tcgen05
-
-// Shared-memory matrix descriptor of a K-major operand tile in the canonical
-// 128B-swizzle layout: rows of 128 bytes (64 fp16 of k), 8-row atoms of
-// 1024 bytes stacked along M/N. Fields (16-byte units): start address,
-// leading byte offset 1 (unused by swizzled K-major), stride byte offset 64
-// (1024 bytes between atoms), version 1, layout type 2 (128B swizzle).
-__device__ __forceinline__ uint64_t kmajor_sw128_desc(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
-  d |= (uint64_t)1u << 16;
-  d |= (uint64_t)64u << 32;
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)2u << 61;
-  return d;
-}
-// The descriptor of the operand `bytes` further (shared addresses stay below
-// 2^18, so the 14-bit field does not overflow).
-__device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t bytes) {
-  return d + (bytes >> 4);
-}
-
-// Instruction descriptor of kind::f16: fp32 accumulate, A and B of one type
-// (0 fp16, 1 bf16), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
-__host__ __device__ constexpr uint32_t f16_idesc(int bf16, int m, int n) {
-  return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) |
-         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      :
-      : "r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Arrives once on the mbarrier when every tcgen05 operation this thread
-// issued before has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-// Generic-proxy shared-memory stores become visible to the tensor core's
-// (async proxy) reads.
-__device__ __forceinline__ void fence_async_shared() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 
 // ---------------------------------------------------------------- dequant
 
@@ -411,12 +334,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     for (int kt = 0; kt < min(S::kPkStages, KT); ++kt) load_w(kt);
     for (int kt = 0; kt < min(S::kStages, KT); ++kt) load_x(kt);
   }
-  if (warp == kMmaWarp) {  // tensor memory for the two 128 x 128 fp32 accumulators
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(tmem_slot)),
-                 "r"(S::kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if (warp == kMmaWarp) {  // tensor memory for the accumulators
+    tc_alloc(tmem_slot, S::kTmemCols);
     tc_fence_before();
   }
   if (!p.wait_at_end) grid_dependency_wait();
@@ -468,9 +387,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA
     if (lane == 0) {
-      constexpr uint32_t idesc = f16_idesc(kBF16 ? 1 : 0, kUM, BN);
-      const uint64_t xd0 = kmajor_sw128_desc(smem_u32(base + S::kOffX));
-      const uint64_t bd0 = kmajor_sw128_desc(smem_u32(base + S::kOffB));
+      constexpr uint32_t idesc = tc_idesc(kBF16 ? 1 : 0, 0, BN);
+      const uint64_t xd0 = tc_operand(smem_u32(base + S::kOffX), 16, 1024);
+      const uint64_t bd0 = tc_operand(smem_u32(base + S::kOffB), 16, 1024);
       for (int kt = 0; kt < KT; ++kt) {
         const int s = kt % S::kStages;
         if (!mbar_wait(&full[s], (kt / S::kStages) & 1)) {
@@ -478,17 +397,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint64_t xd = desc_at(xd0, s * S::kXBytes), bd = desc_at(bd0, s * S::kBBytes);
+        const uint64_t xd = tc_operand_at(xd0, s * S::kXBytes);
+        const uint64_t bd = tc_operand_at(bd0, s * S::kBBytes);
 #pragma unroll
         for (int kk = 0; kk < kBK / 16; ++kk)  // 16 k = 32 bytes along the swizzled row
           // accumulator a: rows 128a.. (16 KB further per 128 rows), columns a*BN..
 #pragma unroll
           for (int a = 0; a < NACC; ++a)
-            umma_f16(tmem_d + a * BN, desc_at(xd, a * kUM * 128 + kk * 32), desc_at(bd, kk * 32),
-                     idesc, kk > 0 ? 1u : (uint32_t)(kt > 0));
-        umma_commit(&empty[s]);
+            tc_mma(tmem_d + a * BN, tc_operand_at(xd, a * kUM * 128 + kk * 32),
+                   tc_operand_at(bd, kk * 32), idesc, kk > 0 ? 1u : (uint32_t)(kt > 0));
+        tc_commit(&empty[s]);
       }
-      umma_commit(acc_full);  // after every issued MMA (also when none was issued)
+      tc_commit(acc_full);  // after every issued MMA (also when none was issued)
     }
   } else {
     // ------------------------------------------------------------ dequant
@@ -593,7 +513,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll 1
           for (int c = 0; c < BN / 32; ++c) {
             uint32_t r[32];
-            tmem_ld32(acc + 32 * c, r);
+            tc_ld32(acc + 32 * c, r);
             if (has_row) {
 #pragma unroll
               for (int v = 0; v < 8; ++v)
@@ -612,7 +532,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < BN / 32; ++c) {
         uint32_t r[32];
-        tmem_ld32(acc + 32 * c, r);
+        tc_ld32(acc + 32 * c, r);
         if (n0 + 32 * c >= p.N) break;
         uint4 y[4];
 #pragma unroll
@@ -630,8 +550,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < BN / 32; c += step) {
         uint32_t r[32], ru[32];
-        tmem_ld32(acc + 32 * c, r);
-        if (gated) tmem_ld32(acc + 32 * c + 32, ru);
+        tc_ld32(acc + 32 * c, r);
+        if (gated) tc_ld32(acc + 32 * c + 32, ru);
         uint4 now[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) now[v] = res[v];
@@ -720,9 +640,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (lane == 0 && !mbar_wait(acc_full, 0)) give_up(kErrGemmWait);
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_d),
-                 "r"(S::kTmemCols)
-                 : "memory");
+    tc_dealloc(tmem_d, S::kTmemCols);
   }
   if (p.wait_at_end) grid_dependency_wait();
 }

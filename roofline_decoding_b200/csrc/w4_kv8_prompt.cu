@@ -32,6 +32,7 @@
 // TFLOP/s of the causal products (16 us of it before the first S, after the last P V
 // and in the empty join's launch); 8192 tokens from nothing 885 us, 620 TFLOP/s.
 #include "w4_kv8_attn.cuh"
+#include "w4_tcgen05.cuh"
 
 #include <algorithm>
 
@@ -160,116 +161,6 @@ struct PromptShape {
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// ------------------------------------------------------------ tcgen05
-
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  // 128B swizzle, version 1; offsets in bytes
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
-         (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1u << 46 | (uint64_t)2u << 61;
-}
-// kind::f16, fp16 operands, fp32 sums, M = 128; b_mn: B is MN-major.
-__host__ __device__ constexpr uint32_t prompt_idesc(int n, int b_mn) {
-  return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
-}
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      :
-      : "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// The same with A in tensor memory: a lane a row, two elements a column.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                           uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      :
-      : "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void commit_to(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void before_sync() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void after_sync() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void to_async_proxy() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-// 32 columns of this warp's 32 lanes, landed: the wait stands in the same statement,
-// so that nothing is done with the registers before it.
-__device__ __forceinline__ void ld32(uint32_t addr, float (&r)[32]) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-      "%30, %31"
-      "}, [%32];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
-        "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
-        "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-      : "r"(addr)
-      : "memory");
-}
-// The same with 64.
-__device__ __forceinline__ void ld64(uint32_t addr, float* r) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-#define W4_OUT8(i)                                                                          \
-  "=r"(u[i]), "=r"(u[i + 1]), "=r"(u[i + 2]), "=r"(u[i + 3]), "=r"(u[i + 4]), "=r"(u[i + 5]), \
-      "=r"(u[i + 6]), "=r"(u[i + 7])
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
-      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63"
-      "}, [%64];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : W4_OUT8(0), W4_OUT8(8), W4_OUT8(16), W4_OUT8(24), W4_OUT8(32), W4_OUT8(40), W4_OUT8(48),
-        W4_OUT8(56)
-      : "r"(addr)
-      : "memory");
-#undef W4_OUT8
-}
-__device__ __forceinline__ void st32(uint32_t addr, const uint32_t* u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(
-          u[0]),
-      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
-      "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]),
-      "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]),
-      "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]),
-      "r"(u[30]), "r"(u[31]), "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void st16(uint32_t addr, const uint32_t* u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(u[0]),
-      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]),
-      "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void st_wait() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
 // Byte offset of 16-byte chunk c (8 fp16) of row r in an operand half.
 __device__ __forceinline__ uint32_t operand_at(int r, int c) {
   return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
@@ -377,18 +268,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
     fence_mbar_init();
   }
   if (warp == kMmaWarp) {  // all of it: two S, two O
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(tmem_slot)),
-                 "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    before_sync();
+    tc_alloc(tmem_slot, 512);
+    tc_fence_before();
   }
   for (int i = tid; i < S::kMarks; i += kPromptThreads) marks[i] = 0u;
   grid_dependency_wait();
   grid_launch_dependents();
   __syncthreads();
-  after_sync();
+  tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem + 2 * kPromptTile;  // O of stream u: + 128 u
   // A wait that gives up ends its role; the others give up in turn.
@@ -496,28 +383,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         done_item();
       }
     } else if (warp == kMmaWarp && lane == 0) {
-      constexpr uint32_t idesc_s = prompt_idesc(kPromptTile, 0), idesc_o = prompt_idesc(D, 1);
-      const uint64_t q_desc = operand_desc(sm + S::kOffQ, 16, 1024);
+      constexpr uint32_t idesc_s = tc_idesc(0, 0, kPromptTile), idesc_o = tc_idesc(0, 1, D);
+      const uint64_t q_desc = tc_operand(sm + S::kOffQ, 16, 1024);
       // O += P V of tile m of item `of`, its first of the stream or not
       auto output = [&](int m, bool first, int of) {
         const int u = m & 1;
         if (!wait(&p_half[u], (m >> 1) & 1) || !wait(&v_full[u], (m >> 1) & 1) ||
             (first && of > 0 && !wait(o_empty, (of - 1) & 1)))
           return false;
-        after_sync();
-        const uint64_t v_desc = operand_desc(sm + S::kOffV + u * S::kOperand, S::kHalf, 1024);
+        tc_fence_after();
+        const uint64_t v_desc = tc_operand(sm + S::kOffV + u * S::kOperand, S::kHalf, 1024);
 #pragma unroll
         for (int k = 0; k < kPromptTile / 16; ++k) {  // 16 tokens: 8 columns of P, 16 rows of V
           if (k == kPromptTile / 32) {
             if (!wait(&p_full[u], (m >> 1) & 1)) return false;
-            after_sync();
+            tc_fence_after();
           }
-          mma_f16_ts(tmem_o + u * kPromptTile, tmem + u * kPromptTile + 8 * k,
+          tc_mma_ts(tmem_o + u * kPromptTile, tmem + u * kPromptTile + 8 * k,
                      v_desc + ((k * 16 * 128) >> 4), idesc_o, first && k == 0 ? 0u : 1u);
         }
         __threadfence_block();  // the widen warps' marks, for those who wait for pv_done
-        commit_to(&v_empty[u]);
-        commit_to(&pv_done[u]);
+        tc_commit(&v_empty[u]);
+        tc_commit(&pv_done[u]);
         return true;
       };
       // A tile's P V comes after the next tile's S, the next item's first too, so that
@@ -533,16 +420,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           ok = wait(&k_full[u], (n >> 1) & 1) &&
                (n < 2 || wait(&pv_done[u], ((n >> 1) & 1) ^ 1u));
           if (!ok) break;
-          after_sync();
-          const uint64_t k_desc = operand_desc(sm + S::kOffK + u * S::kOperand, 16, 1024);
+          tc_fence_after();
+          const uint64_t k_desc = tc_operand(sm + S::kOffK + u * S::kOperand, 16, 1024);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {  // 16 dims: 32 bytes along the swizzled rows
             const uint32_t at = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
-            mma_f16(tmem + u * kPromptTile, q_desc + at, k_desc + at, idesc_s, k > 0);
+            tc_mma(tmem + u * kPromptTile, q_desc + at, k_desc + at, idesc_s, k > 0);
           }
           __threadfence_block();  // the widen warps' scales, for those who wait for s_full
-          commit_to(&k_empty[u]);
-          commit_to(&s_full[u]);
+          tc_commit(&k_empty[u]);
+          tc_commit(&s_full[u]);
           if (n > 0) ok = output(n - 1, first, of);
           first = n - n0 < 2;
           of = item;
@@ -588,7 +475,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       }
     };
     auto widened = [&](uint64_t* full) {
-      to_async_proxy();
+      fence_async_shared();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(full);
@@ -643,7 +530,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             }
           }
         }
-        // (to_async_proxy in widened also stands between these stores and the next copy)
+        // (fence_async_shared in widened also stands between these stores and the next copy)
         widen(sm + S::kOffV + u * S::kOperand, raw0 + stage * S::kRaw, keep);
         widened(&v_full[u]);
       }
@@ -706,7 +593,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           sts128(sm + S::kOffQ + (k >> 3) * S::kHalf + operand_at(r, k & 7),
                  make_uint4(o[0], o[1], o[2], o[3]));
         }
-        to_async_proxy();
+        fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[item & 1]);
       } else {
@@ -719,14 +606,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
         if ((n & 1) != stream) continue;
         if (!(ok = wait(&s_full[stream], (n >> 1) & 1))) break;
-        after_sync();
+        tc_fence_after();
         const float4* sc = scale_s + (n % kScales) * 8;
         const int left = lim - t * kPromptTile;  // tokens of the tile that the row sees
         const bool cut = __any_sync(0xffffffffu, left < kPromptTile);
         // A row of S stays in registers from its maximum to its P'.
         float x[kPromptTile];
-        ld64(tmem_s, x);
-        ld64(tmem_s + 64, x + 64);
+        tc_ld64(tmem_s, x);
+        tc_ld64(tmem_s + 64, x + 64);
         if (cut) {
 #pragma unroll
           for (int k = 0; k < kPromptTile; ++k)
@@ -758,10 +645,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             for (int c = 0; c < D / 32; ++c) {
               const uint32_t at = tmem_o + lanes + stream * kPromptTile + 32 * c;
               float o[32];
-              ld32(at, o);
+              tc_ld32(at, o);
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] *= al;
-              st32(at, reinterpret_cast<const uint32_t*>(o));
+              tc_st32(at, reinterpret_cast<const uint32_t*>(o));
             }
           }
         }
@@ -769,8 +656,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         // 64 columns of P' are in their place.
         auto stored = [&](int c) {
           if (c & 1) {
-            st_wait();
-            before_sync();
+            tc_st_wait();
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(c == 1 ? &p_half[stream] : &p_full[stream]);
           }
@@ -787,7 +674,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           for (int c = 0; c < 4; ++c) {
             float y[32];
             uint32_t w[16];
-            ld32(tmem_s + 32 * c, y);
+            tc_ld32(tmem_s + 32 * c, y);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               const float4 f = sc[2 * c + b];
@@ -805,7 +692,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
               for (int k = 0; k < 8; ++k) w[8 * b + k] = half2_bits(y[16 * b + 2 * k], y[16 * b + 2 * k + 1]);
               l = fmaf(sum, apart ? 1.f : f.z, l);
             }
-            st16(tmem_s + 16 * c, w);
+            tc_st16(tmem_s + 16 * c, w);
             stored(c);
           }
           continue;
@@ -827,7 +714,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             }
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), f.z, l);
           }
-          st16(tmem_s + 16 * c, w);
+          tc_st16(tmem_s + 16 * c, w);
           stored(c);
         }
       }
@@ -843,7 +730,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         continue;
       }
       if (!(ok = wait(b_done, item & 1))) break;
-      after_sync();
+      tc_fence_after();
       const float2 other = sums_s[(item & 1) * kPromptTile + r];
       const float most = fmaxf(m, other.x);
       const float ra = m == -INFINITY ? 0.f : ex2(0.5f * (m - most)), fa = ra * ra;
@@ -858,8 +745,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float o[32], o2[32];
-        ld32(tmem_o + lanes + stream * kPromptTile + 32 * c, o);
-        if (has_b) ld32(tmem_o + lanes + (stream ^ 1) * kPromptTile + 32 * c, o2);
+        tc_ld32(tmem_o + lanes + stream * kPromptTile + 32 * c, o);
+        if (has_b) tc_ld32(tmem_o + lanes + (stream ^ 1) * kPromptTile + 32 * c, o2);
 #pragma unroll
         for (int k = 0; k < 32; ++k) o[k] = o[k] * fa + (has_b ? o2[k] * fb : 0.f);
         const uint32_t mark = mine[c];
@@ -894,7 +781,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         }
       }
       if (!it.whole && in) *reinterpret_cast<float2*>(part + D) = make_float2(most, l);
-      before_sync();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
       done_item();
@@ -903,9 +790,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   if (!ok && p.err) atomicCAS(p.err, 0, kErrPromptWait);
   __syncthreads();
   if (warp == kMmaWarp) {
-    after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
-                 : "memory");
+    tc_fence_after();
+    tc_dealloc(tmem, 512);
   }
 }
 
