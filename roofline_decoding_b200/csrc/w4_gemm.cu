@@ -439,8 +439,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         prefetch_l2(static_cast<const uint16_t*>(p.residual) + out_at(p, row, n0 + c));
     for (int kt = group; kt < KT; kt += S::kGroups) {
       const int s = kt % S::kPkStages, sb = kt % S::kStages;
-      if (!mbar_wait(&full_pk[s], (kt / S::kPkStages) & 1) ||
-          (kt >= S::kStages && !mbar_wait(&empty[sb], ((kt / S::kStages) & 1) ^ 1u))) {
+      const bool there =
+          mbar_wait(&full_pk[s], (kt / S::kPkStages) & 1) &&
+          (kt < S::kStages || mbar_wait(&empty[sb], ((kt / S::kStages) & 1) ^ 1u));
+      if (!__all_sync(0xffffffffu, there)) {  // a warp gives up as a whole
         give_up(kErrGemmWait);
         break;
       }
@@ -503,12 +505,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const bool plain = !p.bias && !p.residual && p.act == W4_ACT_NONE;
     if (p.ksplit == 1) load_residual(0);
     if (!mbar_wait(acc_full, 0)) give_up(kErrGemmWait);
+    const bool stop = __any_sync(0xffffffffu, stopped());
     tc_fence_after();
     const uint32_t acc = tmem_d + ((uint32_t)(32 * q) << 16) + half * BN;
     if (p.ksplit > 1) {
       // K slice: this warp's 32 rows of its accumulator -> the fp32 partial tile
       if constexpr (S::kCanSplit) {
-        if (!stopped() && half < NACC && m0 + tile_row - lane < p.M) {
+        if (!stop && half < NACC && m0 + tile_row - lane < p.M) {
           float* prow = reinterpret_cast<float*>(base) + (size_t)tile_row * S::kPitch;
 #pragma unroll 1
           for (int c = 0; c < BN / 32; ++c) {
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       }
-    } else if (stopped() || half >= NACC || m0 + tile_row - lane >= p.M) {
+    } else if (stop || half >= NACC || m0 + tile_row - lane >= p.M) {
       // no rows
     } else if (plain) {
       // Its own loop: with the activations' code between a turn's steps w4_gemm took 2 us

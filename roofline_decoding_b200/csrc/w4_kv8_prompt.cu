@@ -155,7 +155,7 @@ struct PromptShape {
   static constexpr int kMarks = kPromptTile * D / 8;      // of an item; four items
   static constexpr int kOffItems = kOffMarks + 4 * kMarks;
   static constexpr int kOffBar = kOffItems + kItems * (int)sizeof(Item);
-  static constexpr int kBars = 9 * 2 + 2 + 2 * kItems + 2 * kRaws;
+  static constexpr int kBars = 9 * 2 + 3 + 2 * kItems + 2 * kRaws;
   static constexpr int kOffTmem = kOffBar + kBars * 8;
   static constexpr int kSmem = 1024 + kOffTmem + 16;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   uint64_t* raw_full = item_empty + kItems;    // a tile's codes have landed (bytes), its scales are there
   uint64_t* raw_empty = raw_full + kRaws;      // widened
   uint64_t* p_half = raw_empty + kRaws;        // O is rescaled, P' of 64 tokens is in its place
+  uint64_t* mma_done = p_half + 2;             // all products are done (commit)
   Item* items = reinterpret_cast<Item*>(base + S::kOffItems);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + S::kOffTmem);
   // Marks of four items in turn: the widen warps may be two tiles ahead, that is
@@ -257,6 +258,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
     }
     mbar_init(b_done, kSoftWarps);
     mbar_init(o_empty, kSoftWarps);
+    mbar_init(mma_done, 1);
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
       mbar_init(&item_empty[i], 2 + kWidenWarps + 2 * kSoftWarps);
@@ -278,18 +280,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem + 2 * kPromptTile;  // O of stream u: + 128 u
-  // A wait that gives up ends its role; the others give up in turn.
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_on(bar, parity); };
+  // A wait that gives up ends its role; the others give up in turn. A warp gives up as a
+  // whole, since what follows needs all its lanes. (The MMA role is one lane: wait_on.)
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return (bool)__all_sync(0xffffffffu, wait_on(bar, parity));
+  };
   int n = 0;     // tiles that this CTA has begun, over all items
   int item = 0;  // items
   bool ok = true;
   Item it;
   // Item `item` of the ring; false when there is none.
-  auto next_item = [&]() {
+  auto next_by = [&](auto& wait) {
     if (!(ok = wait(&item_full[item % kItems], (item / kItems) & 1))) return false;
     it = items[item % kItems];
     return it.t0 < it.t1;
   };
+  auto next_item = [&]() { return next_by(wait); };
   auto done_item = [&]() {  // by a whole warp
     __syncwarp();
     if (lane == 0) mbar_arrive(&item_empty[item % kItems]);
@@ -382,21 +388,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         }
         done_item();
       }
+      // No copy stays in flight where the others no longer wait for it: each buffer's last,
+      // of this turn or of the one before.
+      for (int i = 0; i < kRaws && !ok; ++i)
+        wait(&raw_full[i], (uint32_t)i < stage ? turn : turn ^ 1u);
     } else if (warp == kMmaWarp && lane == 0) {
       constexpr uint32_t idesc_s = tc_idesc(0, 0, kPromptTile), idesc_o = tc_idesc(0, 1, D);
       const uint64_t q_desc = tc_operand(sm + S::kOffQ, 16, 1024);
       // O += P V of tile m of item `of`, its first of the stream or not
       auto output = [&](int m, bool first, int of) {
         const int u = m & 1;
-        if (!wait(&p_half[u], (m >> 1) & 1) || !wait(&v_full[u], (m >> 1) & 1) ||
-            (first && of > 0 && !wait(o_empty, (of - 1) & 1)))
+        if (!wait_on(&p_half[u], (m >> 1) & 1) || !wait_on(&v_full[u], (m >> 1) & 1) ||
+            (first && of > 0 && !wait_on(o_empty, (of - 1) & 1)))
           return false;
         tc_fence_after();
         const uint64_t v_desc = tc_operand(sm + S::kOffV + u * S::kOperand, S::kHalf, 1024);
 #pragma unroll
         for (int k = 0; k < kPromptTile / 16; ++k) {  // 16 tokens: 8 columns of P, 16 rows of V
           if (k == kPromptTile / 32) {
-            if (!wait(&p_full[u], (m >> 1) & 1)) return false;
+            if (!wait_on(&p_full[u], (m >> 1) & 1)) return false;
             tc_fence_after();
           }
           tc_mma_ts(tmem_o + u * kPromptTile, tmem + u * kPromptTile + 8 * k,
@@ -411,14 +421,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       // there is a softmax to do while the item's last one is done.
       bool first = false;
       int of = 0;
-      while (ok && next_item()) {
-        if (!(ok = wait(&q_full[item & 1], (item >> 1) & 1))) break;
+      while (ok && next_by(wait_on)) {
+        if (!(ok = wait_on(&q_full[item & 1], (item >> 1) & 1))) break;
         const int n0 = n;
         for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
           const int u = n & 1;
           // the stream's last P lies where this S goes
-          ok = wait(&k_full[u], (n >> 1) & 1) &&
-               (n < 2 || wait(&pv_done[u], ((n >> 1) & 1) ^ 1u));
+          ok = wait_on(&k_full[u], (n >> 1) & 1) &&
+               (n < 2 || wait_on(&pv_done[u], ((n >> 1) & 1) ^ 1u));
           if (!ok) break;
           tc_fence_after();
           const uint64_t k_desc = tc_operand(sm + S::kOffK + u * S::kOperand, 16, 1024);
@@ -437,6 +447,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         mbar_arrive(&item_empty[item++ % kItems]);
       }
       if (ok && n > 0) ok = output(n - 1, first, of);
+      // every product is done before the tensor memory is freed, also where a role gave up
+      tc_commit(mma_done);
+      ok = wait_on(mma_done, 0) && ok;
     }
   } else if (warp >= kWidenWarp) {
     // ------------------------------------------------------------ widen
