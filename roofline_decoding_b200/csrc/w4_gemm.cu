@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int c = 0; c < S::kColsPerThread; ++c) {
         const int n = n0 + dt + c * kGroupThreads;
         next[c] = kt < KT && n < p.N
-                      ? __ldg(p.scales + (size_t)((kt0 + kt) * kBK / 128) * p.N + n)
+                      ? p.scales[(size_t)((kt0 + kt) * kBK / 128) * p.N + n]
                       : (uint16_t)0;
       }
     };

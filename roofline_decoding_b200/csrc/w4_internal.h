@@ -118,7 +118,9 @@ int launch_decode_step(const w4_decode_model& m, void* scratch, size_t scratch_b
 // thread before it reads or writes global memory, so it sees all that ran
 // before, and ends after it; and only then lets its own dependents start, since
 // those of this library that read some inputs before their wait count on
-// everything but the kernel just before them being done.
+// everything but the kernel just before them being done. fn makes no read-only
+// (ld.global.nc, __ldg) loads: what they read must not change while the kernel is
+// there, and it may be there before the kernel that writes its inputs has ended.
 template <typename P>
 cudaError_t launch_overlapped(void (*fn)(P), dim3 grid, int threads, size_t smem,
                               cudaStream_t stream, const P& p) {

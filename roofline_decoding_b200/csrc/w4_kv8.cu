@@ -85,11 +85,11 @@ __device__ __forceinline__ uint4 pack8(const F8& r) {
 // Eight elements at index i (a multiple of 8) of a table or weight.
 __device__ __forceinline__ F8 load8(const void* p, int type, size_t i) {
   if (type == W4_F32) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i) + 1);
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 b = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i)[1];
     return F8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
   }
-  const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+  const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
   return type == W4_BF16 ? unpack8<true>(v) : unpack8<false>(v);
 }
 

@@ -142,7 +142,7 @@ __device__ __forceinline__ float load_queries(const AttnP& p, const Seq& s, int 
                         (int64_t)(h * p.group + row - i * p.group) * p.q_head + (D / 4) * t;
 #pragma unroll
   for (int w = 0; w < D / 32; ++w)
-    raw[w] = in ? __ldg(reinterpret_cast<const uint4*>(src) + w) : make_uint4(0u, 0u, 0u, 0u);
+    raw[w] = in ? reinterpret_cast<const uint4*>(src)[w] : make_uint4(0u, 0u, 0u, 0u);
   const uint32_t* rw = reinterpret_cast<const uint32_t*>(raw);
   float f[D / 4];
   float amax = 0.f;

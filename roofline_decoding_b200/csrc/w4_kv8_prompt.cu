@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
         float amax = 0.f;
 #pragma unroll
         for (int k = 0; k < D / 8; ++k)
-          raw[k] = in ? __ldg(reinterpret_cast<const uint4*>(src) + k) : make_uint4(0u, 0u, 0u, 0u);
+          raw[k] = in ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0u, 0u, 0u, 0u);
         auto two = [&](uint32_t w) {
           if constexpr (BF16)
             return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));

@@ -64,3 +64,11 @@ def test_gemm_warps_give_up_with_all_their_lanes():
     role = text[text.index("- dequant\n    constexpr"):text.index("tc_dealloc")]
     assert role.index("__all_sync") < role.index("break;")
     assert "__any_sync(0xffffffffu, stopped())" in role and role.count("stopped()") == 1
+
+
+def test_kernels_that_start_before_their_inputs_are_written_make_no_read_only_loads():
+    """ld.global.nc and __ldg ask that the memory does not change while the kernel is there; a
+    programmatic dependent is there before the kernel in front of it has written it."""
+    for path in [CSRC / "w4_gemm.cu", *CSRC.glob("w4_kv8*.cu"), *CSRC.glob("w4_kv8*.cuh")]:
+        code = re.sub(r"//[^\n]*", "", path.read_text())
+        assert not re.search(r"__ldg|ld\.global\.nc|__restrict__", code), path.name
