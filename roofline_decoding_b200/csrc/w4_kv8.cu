@@ -306,20 +306,16 @@ struct AppendParams {
   int kv_blocks;  // CTAs of the cache part; those after them turn queries
 };
 
-// First row and number of rows of sequence b, kept inside the buffers, and the tokens
-// before them. Rows behind a negative length have no place: none are counted.
-__device__ __forceinline__ int seq_rows(const AppendParams& p, int b, int* first, int* past) {
+// First row and number of rows of sequence b, kept inside the buffers.
+__device__ __forceinline__ int seq_rows(const AppendParams& p, int b, int* first) {
   const int a = min(max(p.row_starts[b], 0), p.rows);
   const int e = min(max(p.row_starts[b + 1], a), p.rows);
-  const int length = p.lengths[b];
   *first = a;
-  *past = max(length, 0);
-  if (length >= 0 || e == a) return e - a;
-  atomicCAS(p.rope.err, 0, kErrKvRange);
-  return 0;
+  return e - a;
 }
 
-// Pages that n rows behind `past` tokens touch.
+// Pages that n rows behind `past` tokens touch (behind a negative length: as many at most,
+// of which none is written).
 __device__ __forceinline__ int touched(int past, int n, int page_shift) {
   return n > 0 ? (((past & ((1 << page_shift) - 1)) + n - 1) >> page_shift) + 1 : 0;
 }
@@ -348,7 +344,10 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
     for (int i = 0; i < 4; ++i) {
       const int bb = b0 + each * lane + i;
       f[i] = m[i] = ps[i] = 0;
-      if (i < each && bb < p.seqs) m[i] = seq_rows(p, bb, &f[i], &ps[i]);
+      if (i < each && bb < p.seqs) {
+        m[i] = seq_rows(p, bb, &f[i]);
+        ps[i] = p.lengths[bb];
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) mine += cnt[i] = touched(ps[i], m[i], p.page_shift);
@@ -384,11 +383,12 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   // page must not hold the value of a token whose key is missing.
   const int64_t stop = min((int64_t)past + n, (slot_page + 1) * p.page);
   const int64_t upto = p.rope.cos_t ? min(stop, (int64_t)p.rope.max_pos) : stop;
-  const int cnt = (int)max(upto - tok0, (int64_t)0);
+  const int cnt = past < 0 ? 0 : (int)max(upto - tok0, (int64_t)0);
   const int slot0 = (int)(tok0 - slot_page * p.page);
   const int64_t row0 = first + (tok0 - past);
-  const int page =
-      slot_page < p.max_pages ? p.page_table[(int64_t)b * p.table_stride + slot_page] : -1;
+  const int page = past >= 0 && slot_page < p.max_pages
+                       ? p.page_table[(int64_t)b * p.table_stride + slot_page]
+                       : -1;
   const bool turned = !is_v && p.rope.cos_t != nullptr;
   const HeadsIn& x = is_v ? p.v : p.k;
 
@@ -418,7 +418,7 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int unit) {
   load(0);  // on its way beside the page's number
   const bool no_page = page < 0 || page >= p.pages;
   if (tid == 0 && (no_page || upto < stop)) atomicCAS(p.rope.err, 0, kErrKvRange);
-  if (no_page || cnt == 0) return;  // no such page, or no position in it: not stored
+  if (no_page || cnt == 0) return;  // no such length, page, or position in it: not stored
   const size_t block = (size_t)page * p.kv_heads + h;
   float* scale_at = (is_v ? p.v_scale : p.k_scale) + block;
   uint8_t* codes = (is_v ? p.v_cache : p.k_cache) + block * p.page * D;
