@@ -84,17 +84,26 @@ def build_library(verbose: bool = False, force: bool = False, ptxas_verbose: boo
 
 
 def build_torch_module(verbose: bool = False, force: bool = False) -> Path:
-    """Compiles and links _w4torch.so; returns its path. Needs libw4b200.so."""
-    src = CSRC / "w4_torch.cpp"
-    if not force and not _stale(TORCH_MODULE_PATH, [src, REPO_DIR / "include" / "w4b200.h"]):
-        return TORCH_MODULE_PATH
+    """Compiles and links _w4torch.so; returns its path. Needs libw4b200.so.
+
+    It is rebuilt when its sources are newer, and when it was built for another
+    torch or Python than this one (BUILD_DIR keeps what it was built for).
+    """
     import torch
     from torch.utils import cpp_extension
 
+    src = CSRC / "w4_torch.cpp"
+    built_for = BUILD_DIR / "w4torch.built_for"
+    version = f"{torch.__version__} {sysconfig.get_config_var('SOABI')}"
+    if (not force and built_for.exists() and built_for.read_text() == version and
+            not _stale(TORCH_MODULE_PATH, [src, REPO_DIR / "include" / "w4b200.h"])):
+        return TORCH_MODULE_PATH
+    BUILD_DIR.mkdir(exist_ok=True)
     cuda = Path(nvcc_path()).resolve().parent.parent
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DW4_TORCH_VERSION="{torch.__version__}"',
            *(f"-isystem{p}" for p in cpp_extension.include_paths()),
            f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{cuda / 'include'}", str(src),
            "-o", str(TORCH_MODULE_PATH), f"-L{PKG_DIR}", "-l:libw4b200.so", f"-L{torch_lib}",
@@ -105,6 +114,7 @@ def build_torch_module(verbose: bool = False, force: bool = False) -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed ({' '.join(cmd)}):\n{r.stdout}\n{r.stderr}")
+    built_for.write_text(version)
     return TORCH_MODULE_PATH
 
 

@@ -247,6 +247,10 @@ def torch_module():
                 spec = importlib.util.spec_from_loader("_w4torch", loader)
                 module = importlib.util.module_from_spec(spec)
                 loader.exec_module(module)
+                built_for = getattr(module, "torch_version", None)
+                if built_for != str(torch.__version__):
+                    raise ImportError(f"{path.name} was built for torch {built_for}, not "
+                                      f"{torch.__version__}; run roofline_decoding_b200/_build.py")
                 module.set_errors(check, torch.OutOfMemoryError)
                 _torch_module = module
     return _torch_module

@@ -523,4 +523,10 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_w4torch",
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__w4torch() { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__w4torch() {
+  PyObject* module = PyModule_Create(&g_module);
+  // The torch whose headers this was compiled against; another one's objects differ.
+  if (module && PyModule_AddStringConstant(module, "torch_version", W4_TORCH_VERSION) < 0)
+    Py_CLEAR(module);
+  return module;
+}
