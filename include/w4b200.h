@@ -515,12 +515,12 @@ int w4_kv8_append(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_
 /* Attention of a step's queries over the cache, which holds the step's own
  * keys and values already: row i of sequence b sees the tokens 0 ..
  * lengths[b] + i. Query head h reads cache head h / (heads / kv_heads);
- * heads / kv_heads is 1 .. 16. out = softmax(scale * q K^T) V: scores,
- * exponentials and all sums in fp32, the weights rounded to fp16 for the product
- * with V (by 2^-11 of each, or 2^-39 of the largest). A row that sees no token
- * (all its pages out of range) is zero. out may be q and must not overlap it otherwise. workspace:
- * w4_kv8_attention_workspace_bytes(head_dim) bytes, 16-byte aligned, of any
- * content, used by one call at a time. */
+ * heads / kv_heads is 1 .. 16. out = softmax(scale * q K^T) V with a finite
+ * scale: scores, exponentials and all sums in fp32, the weights rounded to fp16
+ * for the product with V (by 2^-11 of each, or 2^-39 of the largest). A row that
+ * sees no token (all its pages out of range) is zero. out may be q and must not
+ * overlap it otherwise. workspace: w4_kv8_attention_workspace_bytes(head_dim)
+ * bytes, 16-byte aligned, of any content, used by one call at a time. */
 size_t w4_kv8_attention_workspace_bytes(int head_dim);
 int w4_kv8_attention(const w4_kv8_cache* cache, const w4_kv_batch* batch, const w4_heads* q,
                      const w4_heads* out, int dtype, float scale, void* workspace,

@@ -6,6 +6,7 @@
 
 #include <cudaTypedefs.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <initializer_list>
@@ -491,6 +492,7 @@ int w4_kv8_attention(const w4_kv8_cache* cache, const w4_kv_batch* batch, const 
     return fail(W4_ERR_INVALID_ARG,
                 "%s: %d query heads (out %d) over %d cache heads (1 to 16 each)", what, q->heads,
                 out->heads, cache->kv_heads);
+  if (!std::isfinite(scale)) return fail(W4_ERR_INVALID_ARG, "%s: scale %f", what, scale);
   if (!workspace || workspace_bytes < kv8_attention_workspace_bytes(cache->head_dim))
     return fail(W4_ERR_INVALID_ARG, "%s: workspace of %zu bytes < %zu", what, workspace_bytes,
                 kv8_attention_workspace_bytes(cache->head_dim));

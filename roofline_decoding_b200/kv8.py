@@ -109,7 +109,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor,
 
     q [rows, heads, head_dim], float16 or bfloat16, heads a multiple of the
     cache's (1 to 16 query heads each). Row i of sequence b sees the tokens
-    0 .. lengths[b] + i. scale defaults to head_dim ** -0.5. Scores, exponentials
+    0 .. lengths[b] + i. scale (finite) defaults to head_dim ** -0.5. Scores, exponentials
     and all sums are in fp32; for their product with the values the softmax's
     weights are rounded to fp16 (by 2^-11 of each, or 2^-39 of the largest); the
     result is rounded once to q's type. Deterministic. Returns [rows, heads,
