@@ -57,6 +57,9 @@ constexpr float kShift = 14.0f;  // P' is at most 2^kShift
 // with 34 rows 68.9 and 82.9 us, with 66 117 and 89; 8 over 2000 with 34 rows 25.7 and
 // 29.5, 50 31.2 and 30.5, 66 38.8 and 32.4; one over 2000 with 64 15.9 and 18.3, with 256
 // 26.6 and 24.0.
+// The average is all that the host knows. A step that mixes is better called in two
+// parts, by sequences: 31 of one row and one of 2048 over 4096 tokens 420 us, apart 48 and
+// 260; 63 of one row and one of 512 over 1000 118, apart 33 and 34.
 constexpr int kPromptRows = 64;
 
 // Every row tile of a sequence counts as long as its last (the few tiles above a

@@ -109,12 +109,18 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, page_table: torch.Tensor,
 
     q [rows, heads, head_dim], float16 or bfloat16, heads a multiple of the
     cache's (1 to 16 query heads each). Row i of sequence b sees the tokens
-    0 .. lengths[b] + i. scale (finite) defaults to head_dim ** -0.5. Scores, exponentials
-    and all sums are in fp32; for their product with the values the softmax's
-    weights are rounded to fp16 (by 2^-11 of each, or 2^-39 of the largest); the
-    result is rounded once to q's type. Deterministic. Returns [rows, heads,
+    0 .. lengths[b] + i. scale (finite) defaults to head_dim ** -0.5. Scores,
+    exponentials and all sums are in fp32; for their product with the values the
+    softmax's weights are rounded to fp16 (by 2^-11 of each, or 2^-39 of the
+    largest); the result is rounded once to q's type. Deterministic. Returns [rows, heads,
     head_dim] (`out` if given, which may be q and must not overlap it otherwise);
     rows outside every sequence are left unwritten, and a row whose pages are all
     out of range is zero.
+
+    One of two kernels takes the whole call, by the average number of rows a
+    sequence. A step of many single rows and a prompt is faster as two calls over
+    parts of the same tensors (with the m single rows first):
+      kv8_attention(q[:m], cache, page_table[:m], lengths[:m], row_starts[:m + 1], out=o[:m])
+      kv8_attention(q, cache, page_table[m:], lengths[m:], row_starts[m:], out=o)
     """
     return _lib.torch_module().kv8_attention(q, *cache, page_table, lengths, row_starts, scale, out)

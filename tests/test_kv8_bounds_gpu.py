@@ -277,3 +277,24 @@ def test_an_infinite_query_against_keys_of_one_sign_is_nan(past, rows, dtype):
     got = rd.kv8_attention(q, cache, table, i32([past]), i32([0, rows]))
     nan = torch.isnan(got)
     assert nan[0, 1].all() and int(nan.sum()) == 64
+
+
+# ------------------------------------------------------------------ mixed steps
+
+
+def test_a_mixed_step_as_two_calls():
+    """Decoding sequences first, prompts behind: two calls over parts of one step's tensors."""
+    g, page, D = gen(12), 16, 128
+    past, rows = [300, 7, 1500, 64, 0, 90], [1, 1, 1, 1, 200, 130]
+    table, pages = page_tables(g, past, rows, page)
+    cache = fresh_cache(g, pages, 2, D, page)
+    q = randn(g, sum(rows), 8, D)
+    lengths, rs = i32(past), i32(starts(rows))
+    out = torch.full_like(q, 9.0)
+    rd.kv8_attention(q[:4], cache, table[:4], lengths[:4], rs[:5], out=out[:4])
+    assert torch.all(out[4:] == 9.0)
+    done = out[:4].clone()
+    rd.kv8_attention(q, cache, table[4:], lengths[4:], rs[4:], out=out)
+    assert torch.equal(out[:4], done) and rd.device_error() == 0
+    check_attention(out, q, cache, table, lengths, rs)
+    check_attention(rd.kv8_attention(q, cache, table, lengths, rs), q, cache, table, lengths, rs)
