@@ -51,12 +51,13 @@ constexpr int kSoftRegs = 184, kWidenRegs = 80, kMmaRegs = 64;
 static_assert(2 * kSoftRegs + kWidenRegs + kMmaRegs <= 4 * 128, "registers of the block");
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
 // P' of the maximum that O is scaled by is 2^kPromptShift, and the running maximum may
-// exceed it by kGrowth: P' stays below fp16's 2^16. What is more than 2^28 below the
-// maximum falls under fp16's normal range, off by 2^-25 at most: 2^-39 of the maximum's,
-// as in the other kernel. (A shift of 8 and a growth of 6 spare a few rescales, 2 x 256
-// over 4096 64.1 and 65.4 us, but weights of 2^-30 are then off by a seventh.)
+// exceed it by kGrowth (and by 2^-3, the roundings of scores below 2^20): P' stays below
+// fp16's 2^16. What is more than 2^28 below the maximum falls under fp16's normal range,
+// off by 2^-25 at most: 2^-39 of the maximum's, as in the other kernel. (A shift of 8 and a
+// growth of 6 spare rescales, 2 x 256 over 4096 70.4 and 71.3 us, but weights of 2^-30 are
+// then off by a seventh.)
 constexpr float kPromptShift = 14.0f;
-constexpr float kGrowth = 1.0f;
+constexpr float kGrowth = 1.75f;
 constexpr int kErrPromptWait = 9;
 // Factors of S are at least this, so that a masked -inf stays -inf under a scale of
 // zero; below it a score is none of the argument's 24 bits.
@@ -144,8 +145,8 @@ struct PromptShape {
   static constexpr int kOffV = kOffK + 2 * kOperand;      // two buffers
   static constexpr int kRaw = kPromptTile * D;            // a K or V tile's codes
   static constexpr int kOffRaw = kOffV + 2 * kOperand;    // kRaws buffers
-  // tiles of 8 x (K scale, log2 and inverse of the V scale, 0), their blocks with a page
-  // (8 bits) and those whose V scale is far below another's (8 bits)
+  // tiles of 8 x (K scale, log2 and inverse of the V scale, the tile's blocks whose V scale
+  // is far below another's: 8 bits), their blocks with a page
   static constexpr int kOffScale = kOffRaw + kRaws * kRaw;
   static constexpr int kOffPages = kOffScale + kScales * 8 * 16;
   // two items in turn: a factor a row, maxima and sums of the stream that meets the other
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       uint32_t* pages = reinterpret_cast<uint32_t*>(base + S::kOffPages);
       uint32_t stage = 0, turn = 0;
       while (ok && next_item()) {
-        float most_lv = -INFINITY;  // largest log2 of the item's V scales so far
+        int most_lv = -100;  // largest log2 of the item's V scales so far (of kLeastScale: -80)
         for (int t = it.t0; t < it.t1 && ok; t += 4) {
           const int tok = (t + j) * kPromptTile + 16 * b;
           int id = -1;
@@ -358,23 +359,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             sc_v = fmaxf(p.v_scale[blk], kLeastScale);
             lv = lg2(sc_v);
           }
-          most_lv = fmaxf(most_lv, lv);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-            most_lv = fmaxf(most_lv, __shfl_xor_sync(0xffffffffu, most_lv, o));
+          const int whole_lv = __float2int_rd(fmaxf(lv, -100.0f));
+          most_lv = max(most_lv, __reduce_max_sync(0xffffffffu, whole_lv));
           const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
-          const uint32_t far = __ballot_sync(0xffffffffu, id >= 0 && lv < most_lv - kFar);
+          const uint32_t far = __ballot_sync(0xffffffffu, id >= 0 && whole_lv < most_lv - (int)kFar);
           for (int jj = 0; jj < min(4, it.t1 - t) && ok; ++jj, ++n) {
             const uint32_t blocks = there >> (8 * jj) & 0xffu;
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv) {
               if (!(ok = wait(&raw_empty[stage], turn ^ 1u))) break;
               if (kv == 0) {
-                // K scale, log2 and inverse of the V scale; no page: -inf
-                if (j == jj)
-                  scales[(n % kScales) * 8 + b] = id >= 0 ? make_float4(sc_k, lv, 1.0f / sc_v, 0.f)
-                                                          : make_float4(0.f, -INFINITY, 0.f, 0.f);
-                if (lane == 0) pages[n % kScales] = blocks | (far >> (8 * jj) & 0xffu) << 8;
+                // K scale, log2 and inverse of the V scale, the tile's far blocks; no page: -inf
+                if (j == jj) {
+                  const float w = __uint_as_float(far >> (8 * jj) & 0xffu);
+                  scales[(n % kScales) * 8 + b] = id >= 0 ? make_float4(sc_k, lv, 1.0f / sc_v, w)
+                                                          : make_float4(0.f, -INFINITY, 0.f, w);
+                }
+                if (lane == 0) pages[n % kScales] = blocks;
               }
               __syncwarp();
               if (lane == 0) mbar_arrive_expect_tx(&raw_full[stage], __popc(blocks) * kRun);
@@ -502,8 +503,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
         const int u = n & 1;
         if (!(ok = wait(&raw_full[stage], turn))) break;
-        const uint32_t blocks = *reinterpret_cast<const volatile uint32_t*>(
-                                    base + S::kOffPages + 4 * (n % kScales)) & 0xffu;
+        const uint32_t blocks = *reinterpret_cast<const volatile uint32_t*>(base + S::kOffPages +
+                                                                            4 * (n % kScales));
         const int limit_in = it.limit - t * kPromptTile;
         uint32_t keep = (1u << NP) - 1u;
         if (blocks != 0xffu || limit_in < kPromptTile) {
@@ -615,6 +616,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
       }
       float m = -INFINITY;  // the running maximum that the stream's O and l are scaled by
       float l = 0.f;
+      bool coarse = false;  // m's steps in fp32 are no small part of one, in some row
       int last = -1;        // the stream's last tile
       for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
         if ((n & 1) != stream) continue;
@@ -633,6 +635,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
             if (k >= left) x[k] = -INFINITY;
         }
         float top = -INFINITY;
+        const uint32_t far = __float_as_uint(sc[0].w);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {  // the largest of a block, then its score: no factor is negative
           float t[4];
@@ -651,6 +654,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           // (l's in two steps: between far scales it is below fp32, the product is not)
           const float root = m == -INFINITY ? 0.f : ex2(0.5f * (m - most)), al = root * root;
           m = most;
+          coarse = __any_sync(0xffffffffu, fabsf(m) > 0x1p20f && m != -INFINITY);
           l *= root;
           l *= root;
           if (last >= 0) {
@@ -676,9 +680,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_prompt_kernel(const Att
           }
         };
         last = n;
-        const uint32_t far = *reinterpret_cast<const volatile uint32_t*>(
-                                 base + S::kOffPages + 4 * (n % kScales)) >> 8;
-        if (__any_sync(0xffffffffu, fabsf(sub) > 0x1p20f || far != 0u)) {
+        if (coarse || far != 0u) {
           // Seldom. Scores whose steps in fp32 are no small part of one: the argument in one
           // rounding, with the maximum's two in `less`, could be off by several, so they get
           // the maximum's own rounding first. And scales so far apart that P' may vanish and
