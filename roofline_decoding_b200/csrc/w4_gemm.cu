@@ -12,7 +12,7 @@
 //                  through a ring of its own: words leave as soon as they are
 //                  unpacked, so the dequantisation runs ahead of the MMA and
 //                  no load's latency waits for an MMA's (2048 x 8960 x 1536:
-//                  67 us, 96 with one ring for both);
+//                  64 us, 93 with one ring for both);
 //   8 dequant warps: expand each packed word into 8 fp16 (q - 8) * s values
 //                  - bit-identical to dequantize_v1 - and write them K-major,
 //                  128B-swizzled, into one of the B buffers;
@@ -81,7 +81,8 @@ struct GemmParams {
 };
 
 // Tile of BN columns (MMA N = BN, 128 or 256) and its shared memory layout
-// (base 1024-aligned): X ring, B buffers, packed ring, then the barriers and the tensor-memory address. The rings take what the 227 KB hold.
+// (base 1024-aligned): X ring, B buffers, packed ring, then the barriers and the
+// tensor-memory address. The rings take what the 227 KB hold.
 template <int BN, int NACC>
 struct GemmShape {
   // A stage: an X tile and a dequantised W tile. One barrier says that both
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int step = gated ? 2 : 1;  // 32-column blocks a turn
     uint4 res[4] = {};               // the next turn's residual, a turn ahead of its use
     // Chunk k of a lane in memory: chunk t of row k of its quad where tiles have many
-    // rows, of its own row otherwise. Turned and not: 300 x 1536 x 1536 17.0 and 18.2 us,
+    // rows, of its own row otherwise. Turned and not, in the fused loop: 300 x 1536 x 1536 17.0 and 18.2 us,
     // 2048 x 8960 x 1536 65.6 and 68.6, 1709 x 128 x 7296 with a residual 35 and 41; but
     // one accumulator, 17 x 1536 x 2048 14.6 and 13.4, 64 x 4096 x 4096 28.9 and 27.0.
     constexpr bool kTurn = NACC == 2;
@@ -791,7 +792,7 @@ int gemm_plan(int M, int K, int N, int sms, int split_k, bool few_tiles, int dev
   }
   // A grid of more tiles than that is not cut along K: slices would share SMs.
   // Measured on 2048 x 8960 x 1536 (96 tiles) when the whole tiles took 96 us
-  // (67 by now): three slices over 288 CTAs 118-128 us, each slice's stages at
+  // (64 by now): three slices over 288 CTAs 118-128 us, each slice's stages at
   // half the rate.
   if (tiles >= sms && bn == 256 && nacc == 2) {
     // a last wave of a few tiles: those tiles go to a second launch as

@@ -35,8 +35,8 @@
 // P' / sv, unrounded (where scales lie so far apart that P' may vanish and
 // P' / sv not, exp2(s - m + 14) itself).
 //
-// 32 sequences of up to 32768 tokens, 32 heads on 8 of 128: 174 us, 6.3 TB/s. A
-// single token over 700, 12 heads on 2: 8.5 us, the latency of two launches and of
+// 32 sequences of up to 32768 tokens, 32 heads on 8 of 128: 173 us, 6.4 TB/s. A
+// single token over 700, 12 heads on 2: 8.6 us, the latency of two launches and of
 // length, page number, tile, products and merge.
 #include "w4_kv8_attn.cuh"
 

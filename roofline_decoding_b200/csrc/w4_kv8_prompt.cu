@@ -28,9 +28,9 @@
 // products at their best rate and its 128 x 128 exponentials at 16 a clock are 1024
 // clocks each, its traffic on shared memory 1750. A tile takes 2600: a stream's
 // S, softmax (2400), P V and next S follow one another, and two streams are all that
-// the tensor memory holds. 2 x 256 tokens of 32 heads on 8 over 4096: 68 us, 500
+// the tensor memory holds. 2 x 256 tokens of 32 heads on 8 over 4096: 71 us, 480
 // TFLOP/s of the causal products (16 us of it before the first S, after the last P V
-// and in the empty join's launch); 8192 tokens from nothing 885 us, 620 TFLOP/s.
+// and in the empty join's launch); 8192 tokens from nothing 876 us, 630 TFLOP/s.
 #include "w4_kv8_attn.cuh"
 #include "w4_tcgen05.cuh"
 
@@ -46,7 +46,8 @@ constexpr int kMmaWarp = kWidenWarp + kWidenWarps;
 constexpr int kItemWarp = kMmaWarp + 1, kCopyWarp = kMmaWarp + 2;
 constexpr int kPromptThreads = 32 * (kMmaWarp + 4);  // four warpgroups; one warp idles
 // Registers a thread: 128 at launch, then by warpgroup (their sum is four times
-// that, which is what the block has). 8192 tokens: softmax 176 922 us, 184 885, 192 905.
+// that, which is what the block has). 8192 tokens, when chosen: softmax 176 922 us, 184
+// 885, 192 905.
 constexpr int kSoftRegs = 184, kWidenRegs = 80, kMmaRegs = 64;
 static_assert(2 * kSoftRegs + kWidenRegs + kMmaRegs <= 4 * 128, "registers of the block");
 constexpr int kPromptTile = 128;   // tokens of a tile, and rows of an item
@@ -83,7 +84,7 @@ struct Rows128 {
   }
   // Items are not cut if the longest CTA ends at most this much later than with equal
   // shares: a cut costs two first tiles, the parts and their join. 2 sequences of
-  // up to 256 tokens, 32 heads on 8, cut and not: over 1000 45.2 and 31.3 us, 4096 81.7
+  // up to 256 tokens, 32 heads on 8, cut and not, when chosen: over 1000 45.2 and 31.3 us, 4096 81.7
   // and 68.0, 12000 (13 tiles later) 165.7 and 165.6; 512 tokens of 16 heads over 3000 (17) 44.3 and 54.7.
   static constexpr int kCut = 12 * kPromptTile;
   static constexpr int kMore = 3 * kPromptTile;  // what first() and length() have beside past
